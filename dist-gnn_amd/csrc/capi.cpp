@@ -700,6 +700,216 @@ int dgs_feature_server_destroy(dgs_feature_server *s) {
   });
 }
 
+// ------------------------------------------------------------------ state cache
+namespace {
+StateView state_view(const dgs_state_cache *c) {
+  DGS_CHECK(c, "state cache: null");
+  DGS_CHECK(c->pages > 0 && c->heads > 0, "state cache: no pages or heads");
+  DGS_CHECK(c->page_size > 0 && (c->page_size & (c->page_size - 1)) == 0,
+            "state cache: page_size must be a power of two");
+  DGS_CHECK(c->head_dim > 0 && c->head_dim <= 256 && c->head_dim % 8 == 0,
+            "state cache: head_dim must be a multiple of 8 up to 256");
+  DGS_CHECK(c->group > 0 && c->group % 8 == 0 && c->head_dim % c->group == 0,
+            "state cache: group must be a multiple of 8 that divides head_dim");
+  DGS_CHECK(c->k_codes && c->k_scales && c->v_codes && c->v_scales, "state cache: null buffer");
+  DGS_CHECK((((uintptr_t)c->k_codes | (uintptr_t)c->k_scales | (uintptr_t)c->v_codes |
+              (uintptr_t)c->v_scales) % 16) == 0,
+            "state cache: buffers must be 16-byte aligned");
+  StateView v{};
+  v.kc = (uint8_t *)c->k_codes;
+  v.vc = (uint8_t *)c->v_codes;
+  v.ks = (uint32_t *)c->k_scales;
+  v.vs = (uint32_t *)c->v_scales;
+  v.pages = c->pages;
+  v.heads = c->heads;
+  v.dim = c->head_dim;
+  v.group = c->group;
+  while ((1 << v.pshift) < c->page_size) ++v.pshift;
+  return v;
+}
+StateType state_type(int dtype) {
+  DGS_CHECK(dtype >= DGS_STATE_F32 && dtype <= DGS_STATE_F16, "state cache: unknown dtype");
+  return (StateType)dtype;
+}
+IdArray id_array(const void *p, int bytes, const char *what) {
+  DGS_CHECK(p, std::string(what) + " is null");
+  DGS_CHECK(bytes == 4 || bytes == 8, std::string(what) + " must be int32 or int64");
+  return IdArray{p, bytes};
+}
+void check_rows16(const void *p, int64_t s0, int64_t s1, StateType t, const char *what) {
+  const int64_t e = t == kStateF32 ? 4 : 2;
+  DGS_CHECK(p, std::string(what) + " is null");
+  DGS_CHECK((((uintptr_t)p | (uintptr_t)(s0 * e) | (uintptr_t)(s1 * e)) % 16) == 0,
+            std::string(what) + ": rows must be 16-byte aligned");
+}
+}  // namespace
+
+int dgs_state_write(const dgs_state_cache *c, const void *k, const void *v, int dtype, int64_t n,
+                    int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head,
+                    const int64_t *slots, void *stream) {
+  return guard([&] {
+    const StateView view = state_view(c);
+    const StateType t = state_type(dtype);
+    DGS_CHECK(n >= 0, "state write: negative count");
+    if (n == 0) return;
+    check_rows16(k, k_token, k_head, t, "k");
+    check_rows16(v, v_token, v_head, t, "v");
+    DGS_CHECK(slots, "state write: null slots");
+    check_async_errors();
+    state_write(view, StateRows{k, v, k_token, k_head, v_token, v_head}, t, n, slots, S(stream));
+  });
+}
+
+int dgs_state_append(const dgs_state_cache *c, const void *k, const void *v, int dtype, int64_t n,
+                     int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head,
+                     const void *table, int table_bytes, int64_t width, const void *lens,
+                     int lens_bytes, int64_t *slots_out, void *stream) {
+  return guard([&] {
+    const StateView view = state_view(c);
+    const StateType t = state_type(dtype);
+    DGS_CHECK(n >= 0 && width >= 0, "state append: negative size");
+    if (n == 0) return;
+    check_rows16(k, k_token, k_head, t, "k");
+    check_rows16(v, v_token, v_head, t, "v");
+    DGS_CHECK(width > 0, "state append: the table has no columns");
+    const IdArray tab = id_array(table, table_bytes, "table");
+    const IdArray len = id_array(lens, lens_bytes, "lens");
+    DGS_CHECK(slots_out, "state append: null slots_out");
+    check_async_errors();
+    state_append(view, StateRows{k, v, k_token, k_head, v_token, v_head}, t, n, tab, width, len,
+                 slots_out, S(stream));
+  });
+}
+
+int dgs_state_read(const dgs_state_cache *c, const int64_t *slots, int64_t n, int dtype,
+                   void *k_out, void *v_out, void *stream) {
+  return guard([&] {
+    const StateView view = state_view(c);
+    const StateType t = state_type(dtype);
+    DGS_CHECK(n >= 0, "state read: negative count");
+    if (n == 0) return;
+    DGS_CHECK(slots, "state read: null slots");
+    check_rows16(k_out, 0, 0, t, "k_out");
+    check_rows16(v_out, 0, 0, t, "v_out");
+    check_async_errors();
+    state_read(view, slots, n, t, k_out, v_out, S(stream));
+  });
+}
+
+int dgs_state_attend_workspace(const dgs_state_cache *c, int64_t rows, int q_heads, int64_t width,
+                               int with_weights, int dtype, int64_t *bytes) {
+  return guard([&] {
+    const StateView view = state_view(c);
+    DGS_CHECK(rows >= 0 && width >= 0, "attend: negative size");
+    DGS_CHECK(q_heads > 0 && q_heads % view.heads == 0,
+              "attend: q_heads must be a multiple of the cache's heads");
+    AttendCall a{};
+    a.rows = rows;
+    a.q_heads = q_heads;
+    a.width = width;
+    a.type = state_type(dtype);
+    static float flag;
+    a.weights = with_weights ? &flag : nullptr;  // only whether there are any
+    *bytes = state_attend_workspace(view, a);
+  });
+}
+
+int dgs_state_attend(const dgs_state_cache *c, const void *q, int dtype, int64_t rows,
+                     int q_heads, int64_t q_row, int64_t q_head, const void *table,
+                     int table_bytes, int64_t width, const void *lens, int lens_bytes,
+                     double scale, float *weights, int64_t weights_cols, double decay, void *out,
+                     void *workspace, int64_t workspace_bytes, void *stream) {
+  return guard([&] {
+    const StateView view = state_view(c);
+    AttendCall a{};
+    a.type = state_type(dtype);
+    DGS_CHECK(rows >= 0 && width >= 0, "attend: negative size");
+    DGS_CHECK(q_heads > 0 && q_heads % view.heads == 0,
+              "attend: q_heads must be a multiple of the cache's heads");
+    if (rows == 0) return;
+    check_rows16(q, q_row, q_head, a.type, "q");
+    check_rows16(out, 0, 0, a.type, "out");
+    if (width > 0) a.table = id_array(table, table_bytes, "table");
+    a.lens = id_array(lens, lens_bytes, "lens");
+    DGS_CHECK(!weights || weights_cols >= (width << view.pshift),
+              "attend: weights need a column for every slot of the table");
+    a.q = q;
+    a.rows = rows;
+    a.q_heads = q_heads;
+    a.q_row = q_row;
+    a.q_head = q_head;
+    a.width = width;
+    a.scale = (float)scale;
+    a.weights = weights;
+    a.weights_cols = weights_cols;
+    a.decay = (float)decay;
+    a.out = out;
+    check_async_errors();
+    state_attend(view, a, workspace, workspace_bytes, S(stream));
+  });
+}
+
+int dgs_evict_workspace(int64_t rows, int heads, int64_t cols, int64_t budget, int64_t *bytes) {
+  return guard([&] {
+    DGS_CHECK(rows >= 0 && heads > 0 && cols >= 0 && budget > 0, "evict: bad sizes");
+    EvictCall e{};
+    e.rows = rows;
+    e.heads = heads;
+    e.cols = cols;
+    e.budget = budget;
+    *bytes = evict_workspace(e);
+  });
+}
+
+int dgs_evict_rows(void *const *stores, const int64_t *row_bytes, int nstores, int64_t pages,
+                   int heads, int64_t page_size, const float *weights, const int32_t *positions,
+                   float *weights_out, int32_t *positions_out, int64_t rows, int64_t cols,
+                   const void *table, int table_bytes, int64_t width, const void *lens,
+                   int lens_bytes, void *lens_out, int64_t budget, int64_t sinks, int64_t recent,
+                   void *workspace, int64_t workspace_bytes, void *stream) {
+  return guard([&] {
+    EvictCall e{};
+    DGS_CHECK(rows >= 0 && heads > 0 && cols >= 0 && width >= 0 && pages > 0 && page_size > 0,
+              "evict: bad sizes");
+    DGS_CHECK(budget > 0, "evict: budget must be positive");
+    DGS_CHECK(sinks >= 0 && recent >= 0 && sinks <= budget && recent <= budget - sinks,
+              "evict: sinks + recent must lie between 0 and budget");
+    DGS_CHECK(nstores >= 0 && nstores <= kEvictMaxStores, "evict: at most 8 stores");
+    DGS_CHECK(cols >= width * page_size,
+              "evict: weights need a column for every slot of the table");
+    if (rows == 0) return;
+    e.lens = id_array(lens, lens_bytes, "lens");
+    DGS_CHECK(lens_out, "evict: null lens_out");
+    if (cols > 0) {
+      if (width > 0) e.table = id_array(table, table_bytes, "table");
+      DGS_CHECK(weights && weights_out && positions_out, "evict: null weights or positions");
+      DGS_CHECK(weights != weights_out && positions != positions_out,
+                "evict: the outputs must be other arrays than the inputs");
+    }
+    e.nstores = nstores;
+    for (int i = 0; i < nstores; ++i) {
+      DGS_CHECK(stores[i] && row_bytes[i] > 0, "evict: empty store");
+      e.stores[i] = EvictStore{(char *)stores[i], row_bytes[i]};
+    }
+    e.weights = weights;
+    e.positions = positions;
+    e.weights_out = weights_out;
+    e.positions_out = positions_out;
+    e.rows = rows;
+    e.cols = cols;
+    e.heads = heads;
+    e.width = width;
+    e.pages = pages;
+    e.page = page_size;
+    e.lens_out = lens_out;
+    e.budget = budget;
+    e.sinks = sinks;
+    e.recent = recent;
+    check_async_errors();
+    evict_rows(e, workspace, workspace_bytes, S(stream));
+  });
+}
+
 // ------------------------------------------------------------------ profiling
 int dgs_profile_enable(int mask) {
   return guard([&] {

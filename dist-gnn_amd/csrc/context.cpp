@@ -464,6 +464,12 @@ void check_async_errors() {
   if (kind == 0) return;
   const int64_t id = w.host[1], rows = w.host[2], tag = w.host[3];
   __atomic_store_n(&w.host[0], 0, __ATOMIC_RELEASE);
+  if (kind == kAsyncErrSlot || kind == kAsyncErrLength)
+    throw Error("an earlier state cache call met " +
+                std::string(kind == kAsyncErrSlot ? "page or slot " : "length ") +
+                std::to_string(id) + ", outside [0, " + std::to_string(rows) +
+                (kind == kAsyncErrSlot ? "); its row was left out" : "); it was clamped") +
+                " (call #" + std::to_string(tag) + " of this process)");
   const char *what = kind == kAsyncErrFeature ? "feature gather (nids)"
                      : kind == kAsyncErrLabel ? "label gather (seeds)"
                                               : "index_select (nid)";

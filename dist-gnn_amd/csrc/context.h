@@ -121,8 +121,11 @@ bool is_device_pointer(const void *p);
 // kernel reads row 0 in place of the bad row and stores {kind, id, num_rows, tag} into these
 // coherent pinned host words with system-scope vector stores; no launch or synchronisation is
 // added.  The next gather entry point on the host (or dgs_check_async_errors) raises and clears
-// them.  kind: kAsyncErrFeature / kAsyncErrLabel / kAsyncErrSelect.
+// them.  kind: kAsyncErrFeature / kAsyncErrLabel / kAsyncErrSelect.  The state cache's kernels
+// report the same way: a page or slot outside the cache (kAsyncErrSlot; the row is left out) and
+// a length outside its table (kAsyncErrLength; clamped).
 constexpr int64_t kAsyncErrFeature = 1, kAsyncErrLabel = 2, kAsyncErrSelect = 3;
+constexpr int64_t kAsyncErrSlot = 4, kAsyncErrLength = 5;
 constexpr int kAsyncErrWords = 4;
 int64_t *async_err_dev();  // device-visible address of the words (allocated on first use)
 uint64_t async_err_next_tag();  // per-process call counter (the tag a launch reports)

@@ -63,6 +63,86 @@ int64_t count_uncovered(const int64_t *const *lists, const int64_t *counts, int 
 void ftab_assign(int64_t *ftab, int64_t num_rows, const int64_t *nids, int64_t n,
                  const void *base, int64_t row_bytes, hipStream_t st);
 
+// ---------------------------------------------------------------- state cache (state_*.hip)
+// Rows of K and V held in 4 bits, in pages of 2^pshift slots; a slot holds one row of every
+// head.  codes [pages, heads, page, dim / 2] (two channels a byte, the even one low), scales
+// [pages, heads, page, dim / group] words of two bfloat16 (scale low, base high); a channel's
+// value is scale * code + base.
+struct StateView {
+  uint8_t *kc, *vc;
+  uint32_t *ks, *vs;
+  int64_t pages;
+  int heads, dim, group, pshift;
+};
+enum StateType { kStateF32 = 0, kStateBF16 = 1, kStateF16 = 2 };
+// An int32 or int64 array of ids or lengths.
+struct IdArray {
+  const void *p;
+  int bytes;
+#ifdef __HIPCC__
+  __device__ __forceinline__ int64_t operator[](int64_t i) const {
+    return bytes == 8 ? ((const int64_t *)p)[i] : (int64_t)((const int32_t *)p)[i];
+  }
+#endif
+};
+// strides (in elements) of tokens and heads of k, then of v; channels are contiguous and every
+// row starts at a multiple of 16 bytes.
+struct StateRows {
+  const void *k, *v;
+  int64_t kt, kh, vt, vh;
+};
+// Writes row t to flat slot slots[t] (page << pshift | offset); a negative slot is skipped.
+void state_write(const StateView &c, const StateRows &x, StateType type, int64_t n,
+                 const int64_t *slots, hipStream_t st);
+// Writes row t to slot lens[t] of table row t; slots_out[t] = the flat slot (-1: skipped).
+void state_append(const StateView &c, const StateRows &x, StateType type, int64_t n,
+                  const IdArray &table, int64_t width, const IdArray &lens, int64_t *slots_out,
+                  hipStream_t st);
+// k_out, v_out [n, heads, dim] (16-byte aligned) = the rows' values; negative slot: zeros.
+void state_read(const StateView &c, const int64_t *slots, int64_t n, StateType type,
+                void *k_out, void *v_out, hipStream_t st);
+struct AttendCall {
+  const void *q;
+  StateType type;
+  int64_t rows, q_row, q_head;  // q's strides in elements
+  int q_heads;
+  IdArray table;
+  int64_t width;
+  IdArray lens;
+  float scale;
+  float *weights;  // [rows, heads, weights_cols] or null
+  int64_t weights_cols;
+  float decay;
+  void *out;  // [rows, q_heads, dim]
+};
+int64_t state_attend_workspace(const StateView &c, const AttendCall &a);
+void state_attend(const StateView &c, const AttendCall &a, void *ws, int64_t ws_bytes,
+                  hipStream_t st);
+
+// ---------------------------------------------------------------- eviction (evict.hip)
+struct EvictStore {
+  char *p;
+  int64_t row_bytes;
+};
+constexpr int kEvictMaxStores = 8;
+struct EvictCall {
+  const float *weights;      // [rows, heads, cols]
+  const int32_t *positions;  // [rows, heads, cols] or null (position = slot)
+  float *weights_out;
+  int32_t *positions_out;
+  int64_t rows, cols;
+  int heads;
+  IdArray table;
+  int64_t width, pages, page;
+  IdArray lens;
+  void *lens_out;  // the type of lens
+  int64_t budget, sinks, recent;
+  EvictStore stores[kEvictMaxStores];
+  int nstores;
+};
+int64_t evict_workspace(const EvictCall &e);
+void evict_rows(const EvictCall &e, void *ws, int64_t ws_bytes, hipStream_t st);
+
 // ---------------------------------------------------------------- CSR utilities (csr.hip)
 // sub_indptr[i] = sum_{j<i} deg(nids[j]), i = 0..n
 void extract_indptr(const int64_t *nids, int64_t n, const int64_t *indptr, int64_t *sub_indptr,

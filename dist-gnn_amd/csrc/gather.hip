@@ -16,6 +16,7 @@
 
 #include "context.h"
 #include "dgs_common.h"
+#include "dgs_guard.cuh"
 #include "dgs_ops.h"
 
 namespace dgs {
@@ -155,16 +156,6 @@ constexpr int kGatherUnroll = DGS_GATHER_UNROLL;
 // 0.211) and keep 4 (profiles/r05_ab_gather_unroll.txt).
 constexpr int kGatherUnrollBig = 8;
 constexpr int64_t kGatherBigChunks = int64_t(2) << 20;
-
-// Stores the first out-of-range id a launch met into the process's async error words
-// (context.h): id, row count and call tag first, then the kind with a system-scope release.
-__device__ __attribute__((noinline)) void report_bad_id(int64_t *err, int64_t kind, int64_t id,
-                                                        uint64_t rows, int64_t tag) {
-  __hip_atomic_store(err + 1, id, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-  __hip_atomic_store(err + 2, (int64_t)rows, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-  __hip_atomic_store(err + 3, tag, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-  __hip_atomic_store(err, kind, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_SYSTEM);
-}
 
 template <int V, int U, typename Src>
 __global__ __launch_bounds__(kGatherThreads) void k_gather(Src src, uint32_t nchunks,

@@ -98,6 +98,19 @@ _SIGS = {
     "dgs_feature_server_local_cache": (c_int, [c_vp, p_vp, p_i64]),
     "dgs_feature_server_layout": (c_int, [c_vp, ctypes.POINTER(c_int)]),
     "dgs_feature_server_destroy": (c_int, [c_vp]),
+    "dgs_state_write": (c_int, [c_vp, c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp,
+                                c_vp]),
+    "dgs_state_append": (c_int, [c_vp, c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp,
+                                 c_int, c_i64, c_vp, c_int, c_vp, c_vp]),
+    "dgs_state_read": (c_int, [c_vp, c_vp, c_i64, c_int, c_vp, c_vp, c_vp]),
+    "dgs_state_attend_workspace": (c_int, [c_vp, c_i64, c_int, c_i64, c_int, c_int, p_i64]),
+    "dgs_state_attend": (c_int, [c_vp, c_vp, c_int, c_i64, c_int, c_i64, c_i64, c_vp, c_int, c_i64,
+                                 c_vp, c_int, c_dbl, c_vp, c_i64, c_dbl, c_vp, c_vp, c_i64,
+                                 c_vp]),
+    "dgs_evict_workspace": (c_int, [c_i64, c_int, c_i64, c_i64, p_i64]),
+    "dgs_evict_rows": (c_int, [p_vp, p_i64, c_int, c_i64, c_int, c_i64, c_vp, c_vp, c_vp, c_vp,
+                               c_i64, c_i64, c_vp, c_int, c_i64, c_vp, c_int, c_vp, c_i64, c_i64,
+                               c_i64, c_vp, c_i64, c_vp]),
     "dgs_profile_enable": (c_int, [c_int]),
     "dgs_profile_read": (c_int, [ctypes.POINTER(c_dbl), p_i64, ctypes.POINTER(c_dbl), p_i64,
                                  ctypes.POINTER(c_dbl), p_i64]),
@@ -110,7 +123,7 @@ for _name, (_res, _args) in _SIGS.items():
 
 EXPORTED = sorted(_SIGS)
 
-ABI_VERSION = 6  # include/dgs_amd.h DGS_ABI_VERSION, the argument lists in _SIGS
+ABI_VERSION = 7  # include/dgs_amd.h DGS_ABI_VERSION, the argument lists in _SIGS
 if lib.dgs_abi_version() != ABI_VERSION:
     raise ImportError(f"dgs: {LIB_PATH} has ABI revision {lib.dgs_abi_version()}, this binding "
                       f"expects {ABI_VERSION}: rebuild the library")

@@ -9,6 +9,7 @@ import torch
 
 from ._lib import c_i64, c_vp, check, i64_array, lib, stream_ptr, vp_array
 from ._util import as_i64, check_cpu, check_cuda, device_view, ptr, row_bytes
+from .state import StateCache  # noqa: F401  (ADDITIVE)
 
 
 def _host_i64(t, name):

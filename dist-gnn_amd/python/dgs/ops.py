@@ -10,6 +10,7 @@ import torch
 from . import _lib
 from ._lib import c_i64, check, i64_array, lib, stream_ptr, vp_array
 from ._util import as_i64, check_cuda, ptr, row_bytes
+from .state import evict_rows, neighbour_table  # noqa: F401  (ADDITIVE)
 
 __all__ = [
     "_CAPI_get_unique_id", "_CAPI_set_nccl", "_CAPI_compute_frontier_heat",
@@ -19,6 +20,7 @@ __all__ = [
     "_CAPI_cuda_index_select", "_Test_Randn", "_Test_NCCLTensorAllGather",
     "_Test_GetLocalRank", "_Test_GetWorldSize", "_Test_ExtractEdgeData", "_Test_ExtractIndptr",
     "_CAPI_set_random_seed", "_CAPI_set_host_comm", "draw_launch_seeds", "_Test_BiasKeyBounds",
+    "evict_rows", "neighbour_table",
 ]
 
 # host storage registered by _CAPI_tensor_pin_memory: data_ptr -> (the tensor, the registered

@@ -94,7 +94,7 @@ int dgs_host_memory_state(int64_t *n_registrations, int64_t *mirror_bytes, int64
 /* ADDITIVE: the ABI revision of this header (DGS_ABI_VERSION).  Round 5 inserted num_rows /
  * label_rows arguments into dgs_index_select, dgs_index_select_device and dgs_loader_gather;
  * a binding checks this at load time instead of passing shifted arguments. */
-#define DGS_ABI_VERSION 6
+#define DGS_ABI_VERSION 7
 int dgs_abi_version(void);
 
 /* ------------------------------------------------------------------------------------
@@ -326,6 +326,75 @@ int dgs_loader_gather(dgs_sampler *s, dgs_feature_server *fs, void *producer, vo
  * v & (2^w - 1); w = 0 is the whole-graph-in-HBM identity), no per-node table read. */
 int dgs_feature_server_layout(const dgs_feature_server *s, int *wshift);
 int dgs_feature_server_destroy(dgs_feature_server *s);
+
+/* ------------------------------------------------------------------------------------
+ * ADDITIVE: state cache -- rows of K and V held in 4 bits and read by id, the attention over
+ * them, and eviction of rows by accumulated attention weight.  Serving only: no gradients.
+ *
+ * A cache has `pages` pages of page_size slots (a power of two); a slot holds one row of every
+ * head.  Graph nodes use page_size 1 (page = node id, a table row = a seed's sampled
+ * neighbours), sequences use larger pages.
+ *   codes  uint8    [pages, heads, page_size, head_dim / 2]   two channels a byte, the even one low
+ *   scales bfloat16 [pages, heads, page_size, head_dim / group, 2]   scale s, base b
+ * value = s * code + b.  head_dim: a multiple of 8 up to 256; group: a multiple of 8 that divides
+ * it.  The four buffers are contiguous, 16-byte aligned device memory.  A flat slot is
+ * page * page_size + offset.  A page, slot or length outside the cache or its table is left out (or
+ * clamped) by the kernel, and the next gather or state entry point (or dgs_check_async_errors)
+ * raises.  No function here synchronises or allocates; all can be captured into a graph.
+ * ---------------------------------------------------------------------------------- */
+#define DGS_STATE_F32 0
+#define DGS_STATE_BF16 1
+#define DGS_STATE_F16 2
+typedef struct dgs_state_cache {
+  void *k_codes, *k_scales, *v_codes, *v_scales;
+  int64_t pages;
+  int32_t page_size, heads, head_dim, group;
+} dgs_state_cache;
+/* Quantises n tokens' rows (k, v [n, heads, head_dim] of `dtype`, strides in elements for tokens
+ * and heads, channels contiguous, rows 16-byte aligned) into flat slots (int64; negative: skip).
+ * Per group: s = bf16((max - min) / 15), b = bf16(min), code = clamp(rint((x - b) / s), 0, 15) of
+ * the exact quotient; s = 0 gives code 0; a group with a NaN or an infinity reads back as NaN.
+ * Two tokens for one slot in a call: which of them a channel group keeps is not defined. */
+int dgs_state_write(const dgs_state_cache *c, const void *k, const void *v, int dtype, int64_t n,
+                    int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head,
+                    const int64_t *slots, void *stream);
+/* The same for one token per sequence, into slot lens[i] of table row i ([n, width] page ids and
+ * [n] lengths, int32 or int64 by their *_bytes).  slots_out[i] (int64) = the flat slot. */
+int dgs_state_append(const dgs_state_cache *c, const void *k, const void *v, int dtype, int64_t n,
+                     int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head,
+                     const void *table, int table_bytes, int64_t width, const void *lens,
+                     int lens_bytes, int64_t *slots_out, void *stream);
+/* k_out, v_out [n, heads, head_dim] of `dtype` = the rows' values, rounded once; a negative slot
+ * gives zeros. */
+int dgs_state_read(const dgs_state_cache *c, const int64_t *slots, int64_t n, int dtype,
+                   void *k_out, void *v_out, void *stream);
+/* out[i, a] = sum_j softmax_j(scale * q[i, a] . K[j, h]) V[j, h], j over the first lens[i] slots of
+ * table row i, h = a / (q_heads / heads); lens[i] = 0 gives zeros.  q [rows, q_heads, head_dim]
+ * with strides, out contiguous, both of `dtype`.  weights (float [rows, heads, weights_cols],
+ * weights_cols >= width * page_size, or NULL): weights[i, h, j] = decay * weights[i, h, j] + the
+ * sum of head h's query heads' probabilities, for j < lens[i]; decay 0 does not read them. */
+int dgs_state_attend_workspace(const dgs_state_cache *c, int64_t rows, int q_heads, int64_t width,
+                               int with_weights, int dtype, int64_t *bytes);
+int dgs_state_attend(const dgs_state_cache *c, const void *q, int dtype, int64_t rows,
+                     int q_heads, int64_t q_row, int64_t q_head, const void *table,
+                     int table_bytes, int64_t width, const void *lens, int lens_bytes,
+                     double scale, float *weights, int64_t weights_cols, double decay, void *out,
+                     void *workspace, int64_t workspace_bytes, void *stream);
+/* Per (row, head) of a paged cache with n = lens[row] > budget slots, keeps the `budget` slots that
+ * come first by (protected, weight descending, slot ascending); protected: position < sinks or
+ * position >= highest + 1 - recent (sinks + recent <= budget); a NaN weight counts as the lowest.
+ * The i-th dropped slot below budget receives the row of the i-th kept slot at or past it, in every
+ * store ([pages, heads, page_size, row_bytes] device memory, at most 8; in place).  weights (float)
+ * and positions (int32 or NULL: position = slot) are [rows, heads, cols], cols >= width * page_size;
+ * the *_out arrays (others than the inputs) receive them for the slots that stay, 0 and -1 behind;
+ * lens_out (of lens' type) = min(n, budget).  Table rows must not share pages that move. */
+int dgs_evict_workspace(int64_t rows, int heads, int64_t cols, int64_t budget, int64_t *bytes);
+int dgs_evict_rows(void *const *stores, const int64_t *row_bytes, int nstores, int64_t pages,
+                   int heads, int64_t page_size, const float *weights, const int32_t *positions,
+                   float *weights_out, int32_t *positions_out, int64_t rows, int64_t cols,
+                   const void *table, int table_bytes, int64_t width, const void *lens,
+                   int lens_bytes, void *lens_out, int64_t budget, int64_t sinks, int64_t recent,
+                   void *workspace, int64_t workspace_bytes, void *stream);
 
 /* ------------------------------------------------------------------------------------
  * Instrumentation (bench.py).  `mask` selects what is timed: DGS_PROFILE_GATHER = feature-

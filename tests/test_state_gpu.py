@@ -1,0 +1,598 @@
+"""The state cache on the GPU against plain 64-bit forms (tests/state_ref.py).
+
+Tolerances.  Codes, scales, moves, lengths and copied values have to be equal.  attend: with
+u = 2^-24, a logit is a sum of D products of 32-bit values (each value one rounding of s * c + b, a
+query scaled with one rounding, and one more where the query is split into two 16-bit terms), so it
+is off by at most (D + 4) u S, S the largest scale * sum |q k|; half of that again covers sums of
+codes taken before their base.  A probability is off by twice that, plus the hardware exp2 (1 unit
+in 2^-23, an argument of |x| <= 2 S log2 e rounded: 3 S u) and, in the matrix form, the rounding of
+p times a scale to two bfloat16 terms (2^-17); sums of n terms in 32 bits in a tree of chunks add
+less than 64 u.  The output is a mean of values of size V under such weights, plus its own
+rounding, eps / 2."""
+import math
+import os
+
+import numpy as np
+import pytest
+import torch
+
+import dgs
+import state_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def prob_error(dim, size):
+    return 3 * (dim + 4) * U * size + 6 * size * U + 2.0 ** -17 + 80 * U
+
+
+def states(shape, gen, dtype):
+    x = torch.randn(shape, generator=gen) * (torch.rand(shape[-1], generator=gen) + 0.5)
+    return (x + torch.randn(shape[-1], generator=gen) * 0.5).to(dtype).cuda()
+
+
+def full_cache(pages, page, heads, dim, group, seed=0):
+    """A cache whose every slot holds a row, written by the plain form."""
+    gen = torch.Generator().manual_seed(seed)
+    bufs = []
+    for _ in range(2):
+        c, s = ref.quantise(torch.randn(pages, heads, page, dim, generator=gen) +
+                            torch.randn(dim, generator=gen), group)
+        bufs += [ref.pack(c).cuda(), s.cuda()]
+    return dgs.classes.StateCache.wrap(*bufs)
+
+
+def buffers(c):
+    return [c.k_codes, c.k_scales, c.v_codes, c.v_scales]
+
+
+def same_bits(a, b):
+    v = {1: torch.uint8, 2: torch.int16, 4: torch.int32}[a.element_size()]
+    return torch.equal(a.cpu().view(v), b.cpu().view(v))
+
+
+# ------------------------------------------------------------------------------ rows
+SHAPES = [(128, 64, 16, 8), (128, 128, 1, 1), (128, 32, 32, 2), (64, 64, 8, 3), (80, 40, 2, 5),
+          (96, 96, 4, 2), (8, 8, 1, 1), (256, 64, 64, 2), (40, 8, 1, 4), (24, 24, 128, 1)]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("dim, group, page, heads", SHAPES)
+@pytest.mark.parametrize("tokens", [1, 77])
+def test_write_and_read(dim, group, page, heads, tokens, dtype):
+    gen = torch.Generator().manual_seed(dim + tokens)
+    pages = -(-(tokens + 5) // page)
+    cache = dgs.classes.StateCache(pages, page, heads, dim, group)
+    before = [b.fill_(7) for b in buffers(cache)]
+    before = [b.clone() for b in before]
+    qkv = states((tokens, 3 * heads, dim), gen, TYPES[dtype])
+    k, v = qkv[:, heads:2 * heads], qkv[:, 2 * heads:]  # views of a fused projection
+    slots = torch.randperm(pages * page, generator=gen)[:tokens]
+    slots[tokens // 2] = -1 if tokens > 1 else slots[0]
+    cache.write(k, v, slots.cuda())
+    live = slots >= 0
+    for x, codes, scales, c0, s0 in ((k, cache.k_codes, cache.k_scales, before[0], before[1]),
+                                     (v, cache.v_codes, cache.v_scales, before[2], before[3])):
+        qc, qs = ref.quantise(x, group)
+        c0, s0 = c0.cpu(), s0.cpu()
+        at = slots[live] // page, slots[live] % page
+        c0[at[0], :, at[1]], s0[at[0], :, at[1]] = ref.pack(qc[live]), qs[live]
+        assert same_bits(codes, c0) and same_bits(scales, s0)  # others left as they were
+    for t in TYPES.values():
+        got = cache.read(slots.int().cuda(), t)
+        for x, g in zip((k, v), got):
+            qc, qs = ref.quantise(x, group)
+            want = ref.values(ref.pack(qc), qs)
+            want[~live] = 0
+            # s * c has 12 bits; one rounding to 32 bits, one more to a 16-bit type
+            assert torch.equal(g.cpu(), want.float().to(t))
+
+
+def test_quantiser_borders():
+    """Groups where the code hangs on a rounding: ties, tiny, constant and wide ranges, signs."""
+    gen = torch.Generator().manual_seed(3)
+    n, dim, group = 4096, 64, 8
+    x = torch.randn(n, 1, dim, generator=gen)
+    g = x.view(n, dim // 8, 8)
+    g[:512, :, 0], g[:512, :, 7] = 0, 15  # scale 1, base 0: halves are ties
+    g[:512, :, 1:7] = torch.randint(0, 30, (512, dim // 8, 6), generator=gen) / 2
+    g[512:700] = torch.nextafter(g[:188], torch.tensor(8.0))
+    g[700:900] *= 1e-38
+    g[900:1000] *= 1e-41  # below the normal range
+    g[1000:1100] = g[1000:1100, :, :1]
+    g[1100:1200] *= 1e37
+    g[1200:1300] += 1000
+    g[1300:1400] = 0
+    g[1400:1500] = -0.0
+    for i, bad in enumerate((math.nan, math.inf, -math.inf)):
+        g[1500 + 50 * i:1550 + 50 * i, ::2, i] = bad
+    g[1700:1750, :, 0], g[1700:1750, :, 1] = 3e38, -3e38
+    cache = dgs.classes.StateCache(n, 1, 1, dim, group)
+    cache.write(x.cuda(), x.flip(0).cuda(), torch.arange(n).cuda())
+    codes, scales = ref.quantise(x, group)
+    assert torch.equal(cache.k_codes.cpu()[:, 0, 0], ref.pack(codes)[:, 0])
+    nan = scales.isnan()[:, 0]
+    assert torch.equal(cache.k_scales.cpu()[:, 0, 0].isnan(), nan)
+    got = cache.k_scales.cpu()[:, 0, 0]
+    assert torch.equal(torch.where(nan, 0, got), torch.where(nan, 0, scales[:, 0]))
+    k, v = cache.read(torch.arange(n).cuda())
+    want = ref.values(ref.pack(codes), scales).float()
+    assert torch.equal(k.cpu().isnan(), want.isnan())
+    assert torch.equal(k.cpu().nan_to_num(), want.nan_to_num())
+    assert torch.equal(v.cpu().nan_to_num(), want.flip(0).nan_to_num())
+
+
+@pytest.mark.parametrize("ids", [torch.int32, torch.int64])
+def test_append(ids):
+    gen = torch.Generator().manual_seed(5)
+    n, page, heads, dim = 13, 4, 3, 64
+    lens = torch.randint(0, 20, (n,), generator=gen)
+    lens[0], lens[1] = 0, 19  # the first slot, the last slot of the table
+    table = torch.randperm(n * 5, generator=gen).view(n, 5)
+    cache = dgs.classes.StateCache(n * 5, page, heads, dim)
+    other = dgs.classes.StateCache(n * 5, page, heads, dim)
+    k, v = (states((n, heads, dim), gen, torch.bfloat16) for _ in range(2))
+    slots = cache.append(k, v, table.to(ids).cuda(), lens.to(ids).cuda())
+    want = table[torch.arange(n), lens // page] * page + lens % page
+    assert torch.equal(slots.cpu(), want)
+    other.write(k, v, want.cuda())
+    assert all(same_bits(a, b) for a, b in zip(buffers(cache), buffers(other)))
+
+
+def test_empty_calls():
+    cache = dgs.classes.StateCache(2, 4, 2, 64)
+    z = torch.zeros(0, 2, 64, device="cuda")
+    i = torch.zeros(0, dtype=torch.int64, device="cuda")
+    cache.write(z, z, i)
+    assert cache.append(z, z, i.view(0, 1), i).shape == (0,)
+    assert cache.read(i)[0].shape == (0, 2, 64)
+    assert cache.attend(z, i.view(0, 1), i).shape == (0, 2, 64)
+    q = torch.randn(3, 4, 64, device="cuda")
+    out = cache.attend(q, torch.zeros(3, 0, dtype=torch.int32, device="cuda"),
+                       torch.zeros(3, dtype=torch.int32, device="cuda"))
+    assert torch.equal(out, torch.zeros_like(q))
+    w = torch.zeros(0, 2, 8, device="cuda")
+    got = dgs.ops.evict_rows([cache.k_codes], w, None, i.view(0, 2), i, 4)
+    assert got[0].shape == (0, 2, 8) and got[2].shape == (0,)
+
+
+# ------------------------------------------------------------------------------ attention
+def check_attend(cache, q, table, lens, scale=None, weights=None, decay=1.0):
+    dim = cache.head_dim
+    sc = dim ** -0.5 if scale is None else scale
+    want, prob, size, vmax = ref.attend(q, cache, table, lens, abs(sc))
+    if sc < 0:
+        want, prob, size, vmax = ref.attend(-q, cache, table, lens, -sc)
+    before = None if weights is None else weights.clone()
+    got = cache.attend(q, table, lens, scale=scale, weights=weights, decay=decay)
+    assert got.dtype == q.dtype and got.shape == q.shape
+    err = (got.cpu().double() - want).abs()
+    rel = prob_error(dim, size)
+    tol = 2 * rel * vmax + torch.finfo(q.dtype).eps / 2 * (want.abs() + 2 * rel * vmax) + 1e-30
+    if q.dtype == torch.float16:
+        tol = tol + 2.0 ** -25  # half a step below the normal range
+    assert bool((err <= tol).all()), (float(err.max()), float(tol.max()))
+    if weights is not None:
+        g = q.shape[1] // cache.heads
+        inside = torch.arange(prob.shape[2]) < lens.cpu().long()[:, None, None]
+        old = before.cpu().double()[..., :prob.shape[2]]
+        exp = torch.where(inside, prob + (decay * old if decay else 0.0), old)
+        werr = (weights.cpu().double()[..., :prob.shape[2]] - exp).abs()
+        wtol = 2 * rel * prob + 4 * U * exp.abs() + g * U * prob + 1e-30
+        assert bool((werr <= wtol)[inside.expand_as(werr)].all()), float(werr.max())
+        keep = ~torch.zeros_like(before, dtype=torch.bool)
+        keep[..., :prob.shape[2]] = ~inside.cuda()
+        assert same_bits(weights[keep], before[keep])  # behind the lengths nothing changes
+    return got
+
+
+ATTEND = [  # q_heads, heads, dim, group, page
+    (8, 2, 128, 64, 16), (32, 8, 128, 64, 16), (4, 4, 32, 32, 1), (12, 12, 80, 40, 8),
+    (7, 1, 128, 128, 64), (16, 1, 128, 32, 2), (6, 2, 64, 32, 4), (4, 1, 256, 64, 32),
+    (20, 1, 64, 64, 128), (5, 5, 96, 96, 16), (2, 2, 8, 8, 1), (33, 1, 128, 64, 32),
+    (9, 3, 24, 8, 4), (70, 1, 32, 32, 8), (8, 8, 128, 64, 1), (4, 2, 192, 64, 16)]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("q_heads, heads, dim, group, page", ATTEND)
+@pytest.mark.parametrize("keep", [False, True])
+def test_attend(q_heads, heads, dim, group, page, dtype, keep):
+    gen = torch.Generator().manual_seed(q_heads * dim + page)
+    lens = torch.tensor([0, 1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 130, 257, 300])
+    rows, width = len(lens), -(-300 // page)
+    cache = full_cache(rows * width + 1, page, heads, dim, group, seed=dim)
+    table = (torch.randperm(rows * width, generator=gen) + 1).view(rows, width)
+    # what lies behind a row's length must not matter: NaN in its slots, ids of no page
+    for i, n in enumerate(lens.tolist()):
+        for p in range(n // page, width):
+            first = n - p * page if p == n // page else 0
+            cache.k_scales[table[i, p], :, max(first, 0):] = math.nan
+            cache.v_scales[table[i, p], :, max(first, 0):] = math.nan
+            if first == 0:
+                table[i, p] = -12345 if p % 2 else 2 ** 31 - 1
+    q = states((rows, q_heads, dim), gen, TYPES[dtype])
+    w = torch.rand(rows, heads, width * page + 3, generator=gen).cuda() if keep else None
+    check_attend(cache, q, table.int().cuda(), lens.cuda(), weights=w,
+                 decay=[1.0, 0.5, 0.0][dim % 3])
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("q_heads, heads, dim, group, page", [
+    (8, 2, 128, 64, 16), (16, 1, 64, 64, 1), (3, 3, 80, 40, 8), (40, 1, 128, 128, 64)])
+def test_attend_long(q_heads, heads, dim, group, page, dtype):
+    """Rows long enough to be split, beside short ones; each page used by several rows."""
+    gen = torch.Generator().manual_seed(dim)
+    lens = torch.tensor([20011, 1, 0, 4097, 12288, 777])
+    pages = 30000 // page
+    cache = full_cache(pages, page, heads, dim, group, seed=1)
+    table = torch.randint(0, pages, (len(lens), -(-20480 // page)), generator=gen)
+    q = states((len(lens), q_heads, dim), gen, TYPES[dtype])
+    w = torch.zeros(len(lens), heads, table.shape[1] * page, device="cuda")
+    check_attend(cache, q, table.cuda(), lens.int().cuda(), weights=w)
+    check_attend(cache, q, table.int().cuda(), lens.cuda(), scale=0.3)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attend_many_short_rows(dtype):
+    """Sampled neighbours: many rows of at most 15 slots, pages of one slot."""
+    gen = torch.Generator().manual_seed(2)
+    rows, nodes = 3001, 5000
+    cache = full_cache(nodes, 1, 4, 32, 32)
+    table = torch.randint(0, nodes, (rows, 15), generator=gen)
+    lens = torch.randint(0, 16, (rows,), generator=gen)
+    q = states((rows, 4, 32), gen, TYPES[dtype])
+    w = torch.full((rows, 4, 15), 0.25, device="cuda")
+    check_attend(cache, q, table.cuda(), lens.cuda(), weights=w)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_attend_large_logits(dtype):
+    """Logits far apart: one slot takes everything, also when a later chunk holds it."""
+    gen = torch.Generator().manual_seed(4)
+    cache = full_cache(64, 64, 2, 128, 64)
+    q = (torch.randn(3, 8, 128, generator=gen) * 4).to(TYPES[dtype]).cuda()
+    table = torch.randperm(64, generator=gen)[None].repeat(3, 1).cuda()
+    lens = torch.tensor([4096, 4001, 5]).cuda()
+    for scale in (1.0, -1.0):
+        check_attend(cache, q, table, lens, scale=scale)
+
+
+def test_attend_nan_and_infinity_stay_in_their_rows():
+    cache = full_cache(8, 16, 2, 128, 64)
+    q = torch.randn(4, 8, 128, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    table = torch.arange(8).view(4, 2).cuda()
+    lens = torch.tensor([32, 20, 32, 17]).cuda()
+    clean = cache.attend(q, table, lens)
+    cache.k_scales[3, 0, 3] = math.nan  # row 1, slot 19, head 0
+    cache.v_scales[3, 1, 4] = math.nan  # behind row 1's length
+    q2 = q.clone()
+    q2[2, 5] = math.inf
+    q2[3, 0, 7] = math.nan
+    got = cache.attend(q2, table, lens)
+    bad = torch.zeros(4, 8, dtype=torch.bool)
+    bad[1, :4] = bad[2, 5] = bad[3, 0] = True
+    assert torch.equal(got.isnan().all(-1).cpu(), bad)
+    assert torch.equal(got.isnan().any(-1).cpu(), bad)
+    assert torch.equal(got[~bad], clean[~bad])
+
+
+def test_attend_views_and_repeats():
+    """Strided queries and weights of another step; the same call twice gives the same bits."""
+    gen = torch.Generator().manual_seed(9)
+    cache = full_cache(40, 16, 2, 128, 64)
+    qkv = states((5, 12, 128), gen, torch.bfloat16)
+    table = torch.randperm(40, generator=gen).view(5, 8).cuda()
+    lens = torch.tensor([128, 7, 0, 100, 33]).cuda()
+    q = qkv[:, 2:10]
+    a = check_attend(cache, q, table, lens)
+    assert torch.equal(a, cache.attend(q.contiguous(), table, lens))
+    odd = torch.empty(5 * 8 * 128 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(5, 8, 128)
+    odd.copy_(q)  # rows that are not 16-byte aligned
+    assert torch.equal(a, cache.attend(odd, table, lens))
+    assert torch.equal(a, cache.attend(q.transpose(0, 1).contiguous().transpose(0, 1), table, lens))
+    every = table.repeat_interleave(2, 1)[:, ::2]
+    assert torch.equal(a, cache.attend(q, every, lens.int()))
+
+
+def test_offsets_past_32_bits():
+    """Rows past 2^31 and 2^32 bytes of a buffer."""
+    pages, page, heads, dim = 300000, 64, 4, 128
+    bufs = []
+    for _ in range(2):
+        bufs += [torch.empty(pages, heads, page, dim // 2, dtype=torch.uint8, device="cuda"),
+                 torch.empty(pages, heads, page, 2, 2, dtype=torch.bfloat16, device="cuda")]
+    assert bufs[0].numel() > 2 ** 32
+    cache = dgs.classes.StateCache.wrap(*bufs)
+    gen = torch.Generator().manual_seed(0)
+    use = torch.tensor([3, 131071, 131073, 262145, 299999])
+    slots = (use[:, None] * page + torch.arange(page)).flatten()
+    k, v = (states((slots.numel(), heads, dim), gen, torch.bfloat16) for _ in range(2))
+    cache.write(k, v, slots.cuda())
+    got = cache.read(slots.cuda())
+    small = dgs.classes.StateCache(5, page, heads, dim)
+    small.write(k, v, torch.arange(5 * page).cuda())
+    want = small.read(torch.arange(5 * page).cuda())
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    q = states((1, 16, dim), gen, torch.bfloat16)
+    n = torch.tensor([5 * page - 3]).cuda()
+    assert torch.equal(cache.attend(q, use[None].cuda(), n),
+                       small.attend(q, torch.arange(5)[None].cuda(), n))
+    # eviction moves rows out there too
+    w = torch.rand(1, heads, 5 * page, generator=gen).cuda()
+    a = cache.evict(w, None, use[None].cuda(), n, 100)
+    b = small.evict(w, None, torch.arange(5)[None].cuda(), n, 100)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    assert torch.equal(cache.read(slots[:100].cuda())[1],
+                       small.read(torch.arange(100).cuda())[1])
+
+
+# ------------------------------------------------------------------------------ eviction
+@pytest.mark.parametrize("rows, heads, page, width, budget, sinks, recent", [
+    (7, 2, 16, 12, 64, 2, 8), (3, 1, 1, 77, 50, 0, 10), (5, 3, 8, 40, 1, 0, 0),
+    (4, 2, 64, 40, 700, 4, 300), (2, 4, 32, 200, 6300, 0, 1), (3, 2, 4, 20, 80, 3, 77),
+    (2, 1, 16, 8, 500, 1, 1), (3, 2, 2, 1500, 1024, 0, 0), (2, 2, 3, 30, 40, 1, 2)])
+@pytest.mark.parametrize("ids", [torch.int32, torch.int64])
+@pytest.mark.parametrize("given", [False, True])
+def test_evict(rows, heads, page, width, budget, sinks, recent, ids, given):
+    rng = np.random.default_rng(rows * width + budget)
+    cap = width * page
+    lens = rng.integers(0, cap + 1, rows)
+    lens[0] = cap
+    if rows > 2:
+        lens[1], lens[2] = 0, min(budget + 1, cap)
+    w = np.exp(rng.standard_normal((rows, heads, cap + 5)) * 2).astype(np.float32)
+    w = np.where(rng.random(w.shape) < 0.5, np.round(w), w)  # many ties
+    w[rng.random(w.shape) < 0.05] = 0.0
+    w[rng.random(w.shape) < 0.02] = -0.0
+    w[rng.random(w.shape) < 0.02] = np.nan
+    w[rng.random(w.shape) < 0.01] = np.inf
+    w[rng.random(w.shape) < 0.01] = -np.inf
+    w = w.astype(np.float32)
+    pos = None
+    if given:
+        pos = np.stack([rng.permutation(3 * cap + 15)[:cap + 5] for _ in range(rows * heads)])
+        pos = pos.reshape(rows, heads, cap + 5).astype(np.int32)
+    table = rng.permutation(rows * width + 3)[:rows * width].reshape(rows, width)
+    pages = rows * width + 3
+    gen = torch.Generator().manual_seed(1)
+    stores = [torch.randn(pages, heads, page, 40, generator=gen).bfloat16().cuda(),
+              torch.randint(0, 255, (pages, heads, page, 7), generator=gen).byte().cuda(),
+              torch.randn(pages, heads, page, generator=gen).cuda(),
+              torch.randn(pages, heads, page, 3, 5, generator=gen).cuda()]
+    want_w, want_p, want_n, moves = ref.evict(w, pos, lens, budget, sinks, recent)
+    expect = [s.cpu().clone() for s in stores]
+    if moves:
+        i, h, s, d = (torch.tensor(x) for x in zip(*moves))
+        t = torch.tensor(table)
+        for e in expect:
+            e[t[i, d // page], h, d % page] = e[t[i, s // page], h, s % page].clone()
+    tab = torch.tensor(table)
+    for r, n in enumerate(lens):
+        tab[r, -(-int(n) // page):] = -1
+    for again in range(2):  # a second call on the same inputs gives the same
+        got_w, got_p, got_n = dgs.ops.evict_rows(
+            stores, torch.tensor(w).cuda(), None if pos is None else torch.tensor(pos).cuda(),
+            tab.to(ids).cuda(), torch.tensor(lens).to(ids).cuda(), budget, sinks=sinks,
+            recent=recent)
+        assert got_n.dtype == ids and np.array_equal(got_n.cpu().numpy(), want_n)
+        assert np.array_equal(got_p.cpu().numpy(), want_p)
+        assert np.array_equal(got_w.cpu().numpy(), want_w, equal_nan=True)
+        for a, b in zip(stores, expect):
+            assert same_bits(a, b)
+
+
+@pytest.mark.parametrize("value", [0.0, math.nan, math.inf, 1.0])
+def test_evict_all_equal(value):
+    """Only ties: the first slots stay, nothing moves."""
+    st = torch.arange(64.0, device="cuda").view(4, 1, 16, 1)
+    w = torch.full((1, 1, 64), value, device="cuda")
+    before = st.clone()
+    _, p, n = dgs.ops.evict_rows([st], w, None, torch.arange(4).view(1, 4).cuda(),
+                                 torch.tensor([61]).cuda(), 20)
+    assert torch.equal(st, before) and n.item() == 20
+    assert p[0, 0, :20].tolist() == list(range(20)) and bool((p[0, 0, 20:] == -1).all())
+
+
+def test_evict_long():
+    """One long row: every digit of the selection and every chunk of the numbering."""
+    rng = np.random.default_rng(0)
+    cap, budget = 131072, 4096
+    w = rng.random((1, 2, cap), dtype=np.float32)
+    st = torch.arange(2 * cap, dtype=torch.int32, device="cuda").view(cap // 64, 2, 64, 1)
+    before = st.cpu().clone()
+    lens = np.array([cap - 5])
+    want_w, want_p, _, moves = ref.evict(w, None, lens, budget, 4, 1000)
+    t = torch.arange(cap // 64).view(1, -1).cuda()
+    got_w, got_p, _ = dgs.ops.evict_rows([st], torch.tensor(w).cuda(), None, t,
+                                         torch.tensor(lens).cuda(), budget, 4, 1000)
+    assert np.array_equal(got_p.cpu().numpy(), want_p)
+    assert np.array_equal(got_w.cpu().numpy(), want_w)
+    for _, h, s, d in moves:
+        before[d // 64, h, d % 64] = before[s // 64, h, s % 64]
+    assert torch.equal(st.cpu(), before)
+
+
+# ------------------------------------------------------------------------------ errors, streams
+def raises_next(match):
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match=match):
+        dgs.ops._check_async_errors()
+    dgs.ops._check_async_errors()
+
+
+def test_ids_outside_are_left_out_and_reported():
+    """The kernels compare every page, slot and length with its bound before they use it."""
+    gen = torch.Generator().manual_seed(0)
+    cache = full_cache(8, 16, 2, 128, 64)
+    before = [b.clone() for b in buffers(cache)]
+    k = states((2, 2, 128), gen, torch.bfloat16)
+    cache.write(k, k, torch.tensor([8 * 16, -1]).cuda())
+    raises_next("page or slot 128, outside")
+    one = torch.tensor([[3], [8]]).cuda()
+    assert cache.append(k, k, one, torch.tensor([16, 0]).cuda()).tolist() == [-1, -1]
+    raises_next("state cache call met")
+    assert all(same_bits(a, b) for a, b in zip(buffers(cache), before))
+    assert bool((cache.read(torch.tensor([128]).cuda())[0] == 0).all())
+    raises_next("page or slot 128, outside")
+    q = states((2, 8, 128), gen, torch.bfloat16)
+    ok = cache.attend(q, torch.tensor([[1, 2], [3, 4]]).cuda(), torch.tensor([16, 32]).cuda())
+    got = cache.attend(q, torch.tensor([[1, 9], [3, 4]]).cuda(), torch.tensor([32, 32]).cuda())
+    raises_next("page or slot 9, outside")
+    assert torch.equal(got[1], ok[1])
+    torch.testing.assert_close(got[0], ok[0], rtol=2 ** -7, atol=2 ** -8)
+    got = cache.attend(q, torch.tensor([[1, 2], [3, 4]]).cuda(), torch.tensor([16, 33]).cuda())
+    raises_next("length 33, outside")
+    assert torch.equal(got, ok)
+    w = torch.rand(1, 2, 32, generator=gen).cuda()
+    _, _, n = cache.evict(w, None, torch.tensor([[1, 2]]).cuda(), torch.tensor([40]).cuda(), 8)
+    raises_next("length 40, outside")
+    assert n.item() == 8
+    w = torch.arange(32.0).expand(1, 2, 32).contiguous().cuda()
+    now = [b.clone() for b in buffers(cache)]
+    cache.evict(w, None, torch.tensor([[-3, 99]]).cuda(), torch.tensor([32]).cuda(), 8)
+    raises_next("page or slot")
+    assert all(same_bits(a, b) for a, b in zip(buffers(cache), now))
+
+
+def test_streams_run_independently():
+    gen = torch.Generator().manual_seed(0)
+    cache = full_cache(256, 16, 2, 128, 64)
+    table = torch.randperm(256, generator=gen).view(2, 128).cuda()
+    lens = torch.tensor([2048, 1999]).cuda()
+    qs = [states((2, 8, 128), gen, torch.bfloat16) for _ in range(4)]
+    ws = [torch.zeros(2, 2, 2048, device="cuda") for _ in range(4)]
+    want = [cache.attend(q, table, lens) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    got = [None] * 4
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = cache.attend(qs[i], table, lens, weights=ws[i], decay=0.0)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_graphs_replay_as_eager():
+    """A captured decoding step (append, attend, evict) and a second graph on the same cache,
+    replayed between eager calls with new inputs in place."""
+    gen = torch.Generator().manual_seed(0)
+    page, heads, dim, budget = 16, 2, 128, 40
+    cache = full_cache(8, page, heads, dim, 64)
+    table = torch.randperm(8, generator=gen).view(2, 4).cuda()
+    lens = torch.tensor([40, 23]).cuda()
+    k, v = (states((2, heads, dim), gen, torch.bfloat16) for _ in range(2))
+    q = states((2, 8, dim), gen, torch.bfloat16)
+    w0 = torch.rand(2, heads, 64, generator=gen).cuda()
+    w = w0.clone()
+    bufs0 = [b.clone() for b in buffers(cache)]
+
+    def step():
+        cache.append(k, v, table, lens)
+        n = lens + 1
+        w.copy_(w0)
+        out = cache.attend(q, table, n, weights=w)
+        return (out,) + tuple(cache.evict(w, None, table, n, budget, sinks=1, recent=4))
+
+    def look():
+        return cache.attend(q, table, lens)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(), look()
+    torch.cuda.current_stream().wait_stream(side)
+    g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g1):
+        r1 = step()
+    with torch.cuda.graph(g2):
+        r2 = look()
+    for turn in range(4):
+        for t in (k, v, q):
+            t.copy_(states(t.shape, gen, torch.bfloat16))
+        for a, b in zip(buffers(cache), bufs0):
+            a.copy_(b)
+        want2 = look().clone()
+        want = [t.clone() for t in step()]
+        after = [b.clone() for b in buffers(cache)]
+        for a, b in zip(buffers(cache), bufs0):
+            a.copy_(b)
+        g2.replay()
+        got2 = r2.clone()
+        g1.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got2, want2), turn
+        assert all(torch.equal(a, b) for a, b in zip(r1, want)), turn
+        assert all(same_bits(a, b) for a, b in zip(buffers(cache), after)), turn
+
+
+# ------------------------------------------------------------------------------ together
+def test_sampled_neighbours_attend():
+    """Sample a block, hold every node's states in the cache (page = node id), attend to the
+    sampled neighbours."""
+    from DistGNN.dataloading.synthetic import rmat_csc_numpy
+    indptr, indices = rmat_csc_numpy(10, 8, seed=3)
+    n = indptr.size - 1
+    sampler = dgs.classes.P2PCacheSampler(torch.from_numpy(indptr), torch.from_numpy(indices),
+                                          torch.Tensor(), torch.arange(n), 0)
+    dgs.ops._CAPI_set_random_seed(5)
+    seeds = torch.randperm(n, generator=torch.Generator().manual_seed(0))[:200].cuda()
+    blocks = sampler._CAPI_sample_node_classifiction(seeds, [15, 5], False)
+    gen = torch.Generator().manual_seed(0)
+    heads, dim = 4, 32
+    cache = dgs.classes.StateCache(n, 1, heads, dim)
+    k, v = (states((n, heads, dim), gen, torch.float32) for _ in range(2))
+    cache.write(k, v, torch.arange(n).cuda())
+    for block, fan_out in zip(blocks, (5, 15)):
+        table, lens = dgs.ops.neighbour_table(block, fan_out)
+        row, col = block[2].cpu().numpy(), block[3].cpu().numpy()
+        front = block[1].cpu().numpy()
+        for i in range(0, block[0].numel(), 17):
+            assert sorted(table[i, :lens[i]].tolist()) == sorted(front[col[row == i]].tolist())
+        q = states((block[0].numel(), heads, dim), gen, torch.float32)
+        check_attend(cache, q, table, lens,
+                     weights=torch.zeros(lens.numel(), heads, fan_out, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_decoding_with_a_full_cache(dtype):
+    """Append, attend with weights, evict, over many steps; every step against the plain forms on
+    the state that the step before left."""
+    gen = torch.Generator().manual_seed(0)
+    seqs, heads, q_heads, dim, page, budget = 3, 2, 6, 64, 8, 30
+    cache = dgs.classes.StateCache(seqs * 5, page, heads, dim, 32)
+    table = torch.randperm(seqs * 5, generator=gen).view(seqs, 5).int().cuda()
+    cap = 5 * page
+    lens = torch.tensor([0, 25, 30], dtype=torch.int32).cuda()
+    start = torch.randn(cap, heads, dim, generator=gen).to(TYPES[dtype]).cuda()
+    for i, n in enumerate(lens.tolist()):
+        j = torch.arange(n)
+        cache.write(start[:n], start[:n].flip(0), table[i, j // page].long() * page + j.cuda() % page)
+    weights = torch.zeros(seqs, heads, cap, device="cuda")
+    pos = torch.arange(cap, dtype=torch.int32).repeat(seqs, heads, 1).cuda()
+    token = lens.clone()
+    for _ in range(12):
+        k, v = (states((seqs, heads, dim), gen, TYPES[dtype]) for _ in range(2))
+        slots = cache.append(k, v, table, lens)
+        got = cache.read(slots)
+        want = ref.values(*[x if i else ref.pack(x) for i, x in enumerate(ref.quantise(k, 32))])
+        assert torch.equal(got[0].cpu(), want.float())
+        pos[torch.arange(seqs), :, lens.long()] = token[:, None]
+        lens, token = lens + 1, token + 1
+        q = states((seqs, q_heads, dim), gen, TYPES[dtype])
+        check_attend(cache, q, table, lens, weights=weights)
+        ww, wp, wn, moves = ref.evict(weights.cpu().numpy(), pos.cpu().numpy(),
+                                      lens.cpu().numpy(), budget, 2, 5)
+        expect = [b.cpu().clone() for b in buffers(cache)]
+        t = table.cpu().long()
+        for i, h, s, d in moves:
+            for e in expect:
+                e[t[i, d // page], h, d % page] = e[t[i, s // page], h, s % page]
+        weights, pos, lens = cache.evict(weights, pos, table, lens, budget, sinks=2, recent=5)
+        assert np.array_equal(weights.cpu().numpy(), ww) and np.array_equal(pos.cpu().numpy(), wp)
+        assert np.array_equal(lens.cpu().numpy(), wn)
+        assert all(same_bits(a, b) for a, b in zip(buffers(cache), expect))
+    assert lens.tolist() == [12, 30, 30]
