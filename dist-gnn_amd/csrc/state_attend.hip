@@ -196,6 +196,365 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
   }
 }
 
+// ------------------------------------------------------------------------------------------
+// Matrix form, for 16-bit queries.  One wave takes 16 query heads of a head (the unused ones are
+// zeros) through 32 slots at a time, in v_mfma_f32_16x16x32_bf16 (operands: lane l holds row or
+// column l & 15 and the eight k of quarter l >> 4; result: column l & 15, rows 4 (l >> 4) + i).
+//
+//  - A code c becomes the bfloat16 0x4300 | c = 128 + c, exactly, with one mask-or a pair.
+//  - x = K q: rows are slots, columns query heads, k channels; one product chain per channel group,
+//    r_g = sum q (128 + c).  Then x = sum_g s_g r_g + sum_g (b_g - 128 s_g) Q_g with Q_g = sum q over
+//    the group; the second sum is one more product whose slot operand is the stored (s, b) words
+//    themselves and whose other operand holds -128 Q_g and Q_g in three bfloat16 terms (24 bits).
+//  - The result leaves four slots of one query head in a lane, which is what the second product
+//    wants of its operand: p needs no exchange.  Which slot counts as which k is free; V follows.
+//  - out = V p: rows are channels (16 units of GROUP / 16 channels of one group), columns query
+//    heads, k slots.  a_g = p s_g is rounded to two bfloat16 terms (17 bits: one term's 2^-9 would
+//    show in the output), and the 128 sum a_g that the codes' offset adds is taken out with the same
+//    rounded terms, through a product with a constant operand.  sum p b_g is summed in 32 bits.
+//    The pairs of slots that a register of V holds are made with v_perm_b32: no transposition
+//    through LDS.
+//  - m only follows the maximum when a logit passes it by 8 (in base 2): p stays below 2^8, and
+//    the rescaling is a rare branch.
+// The waves of a workgroup take their 32 slots in turn and join through LDS in wave order.
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+union Op {
+  uint32_t u[4];
+  bf16x8 v;
+};
+
+__device__ __forceinline__ f32x4 mfma(const Op &a, const Op &b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, b.v, c, 0, 0, 0);
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  union {
+    __bf16 h[2];
+    uint32_t u;
+  } v;
+  v.h[0] = (__bf16)lo;
+  v.h[1] = (__bf16)hi;
+  return v.u;
+}
+__device__ __forceinline__ uint32_t code_pair(uint32_t x) {
+  return (x & 0x000f000fu) | 0x43004300u;
+}
+__device__ __forceinline__ float xor16(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                  false);
+  return __uint_as_float((threadIdx.x & 16) ? r[0] : r[1]);
+}
+__device__ __forceinline__ float xor32(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                  false);
+  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+
+template <int NG, int GROUP, int QT>
+__global__ __launch_bounds__(512, 2) void k_attend_mfma(AttendArgs a, int type, int tiles) {
+  constexpr int kD = NG * GROUP, kC = kD / 32, kU = GROUP / 16, kGC = GROUP / 32;
+  extern __shared__ float s_mem[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int n = lane & 15, q4 = lane >> 4;
+  int64_t b = blockIdx.x;
+  const int split = (int)(b % a.splits);
+  b /= a.splits;
+  const int rt = (int)(b % tiles);
+  b /= tiles;
+  const int h = (int)(b % a.c.heads);
+  const int64_t row = b / a.c.heads;
+  const int64_t len = row_length(a, row, split == 0 && h == 0 && rt == 0 && threadIdx.x == 0);
+  const int64_t first = (int64_t)split * a.chunk;
+  if (split > 0 && first >= len) return;
+  const int64_t last = a.splits == 1 ? len : (first + a.chunk < len ? first + a.chunk : len);
+  const int gn = a.g - rt * 16 < 16 ? a.g - rt * 16 : 16;
+  const int64_t qh0 = row * a.q_heads + h * a.g + rt * 16;
+
+  // q in bfloat16 terms, in the order in which code_pair() yields a word's channels: 0 4 1 5 2 6 3 7
+  Op qv[QT][kC], qm;
+  float qsum[NG];
+#pragma unroll
+  for (int g = 0; g < NG; ++g) qsum[g] = 0.f;
+#pragma unroll
+  for (int c = 0; c < kC; ++c) {
+    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (n < gn)
+      load_q(type, a.q, row * a.q_row + (h * a.g + rt * 16 + n) * a.q_head + 32 * c + 8 * q4, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) qsum[c / kGC] += x[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t hi = pack_bf16(x[i], x[4 + i]);
+      qv[0][c].u[i] = hi;
+      if constexpr (QT == 2)
+        qv[1][c].u[i] = pack_bf16(x[i] - __uint_as_float(hi << 16),
+                                  x[4 + i] - __uint_as_float(hi & 0xffff0000u));
+    }
+  }
+  // quarter 0 holds the first bfloat16 terms of (-128 Q_g, Q_g), 1 the second, 2 the third
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    qm.u[g] = 0;
+    if (g < NG) {
+      float s = qsum[g < NG ? g : 0];
+      s += xor16(s);
+      s += xor32(s);
+      const float t0 = (float)(__bf16)s, t1 = (float)(__bf16)(s - t0);
+      const float t2 = (s - t0) - t1;
+      const float t = q4 == 0 ? t0 : (q4 == 1 ? t1 : (q4 == 2 ? t2 : 0.f));
+      qm.u[g] = pack_bf16(-128.f * t, t);
+    }
+  }
+
+  f32x4 o[NG][kU], co[NG];
+  float cb[NG], m = -INFINITY, ms = 0.f, l = 0.f;
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    co[g] = f32x4{0.f, 0.f, 0.f, 0.f};
+    cb[g] = 0.f;
+#pragma unroll
+    for (int j = 0; j < kU; ++j) o[g][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  Op ones;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) ones.u[i] = 0x43004300u;  // 128, the codes' offset
+
+  const int64_t mask = (int64_t(1) << a.c.pshift) - 1, trow = row * a.width;
+  const int unit = n * (GROUP / 32);  // byte of this lane's unit of V in a group's codes
+  const uint32_t sel = GROUP == 128 ? 0x05040100u
+                       : GROUP == 64 ? ((unit & 2) ? 0x07060302u : 0x05040100u)
+                                     : (0x0c000c00u | (uint32_t)(unit & 3) |
+                                        ((uint32_t)(4 + (unit & 3)) << 16));
+  const int64_t step = (int64_t)waves * 32;
+
+  // The wave's own corner of LDS: the (s, b) words of its 32 slots, K then V.
+  uint32_t *s_w = (uint32_t *)s_mem + wave * (64 * NG);
+  uint32_t kq[2][kC], vq[NG][8], mw[NG];  // one tile: codes of K and V, this lane's words
+  uint32_t pk[2], pc[2];  // pages of this lane's slots of K (l & 15) and V (4 (l >> 4) of each half)
+  uint32_t bad = 0, bad_next = 0;
+  const uint32_t pages = (uint32_t)a.c.pages;
+
+  auto load_ids = [&](int64_t j0) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      int64_t k = j0 + 16 * i + n, c = j0 + 16 * i + 4 * q4;
+      k = k < last ? k : last - 1;
+      c = c < last ? c : last - 1;
+      const int64_t ik = a.table[trow + (k >> a.c.pshift)], ic = a.table[trow + (c >> a.c.pshift)];
+      pk[i] = (uint64_t)ik < pages ? (uint32_t)ik : 0u;
+      const bool out = (uint64_t)ic >= pages;
+      if (out && j0 + 16 * i + 4 * q4 < last)
+        report_bad_id(a.gd.err, kAsyncErrSlot, ic, pages, a.gd.tag);
+      pc[i] = out ? 0u : (uint32_t)ic;
+      bad_next = (bad_next & ~(1u << i)) | ((out ? 1u : 0u) << i);
+    }
+  };
+  auto load_k = [&](int64_t j0) {
+    int64_t rm = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      int64_t k = j0 + 16 * i + n;
+      k = k < last ? k : last - 1;
+      const int64_t r = (((int64_t)pk[i] * a.c.heads + h) << a.c.pshift) + (k & mask);
+      const uint32_t *kc = (const uint32_t *)(a.c.kc + r * (kD / 2)) + q4;
+#pragma unroll
+      for (int x = 0; x < kC; ++x) kq[i][x] = kc[4 * x];
+      if ((q4 & 1) == i) rm = r;
+    }
+    // quarters 0 and 1 fetch the words of K, 2 and 3 those of V
+    const uint32_t *wp = (q4 & 2 ? a.c.vs : a.c.ks) + rm * NG;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) mw[g] = wp[g];
+  };
+  auto load_v = [&](int64_t j0) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      int64_t c = j0 + 16 * i + 4 * q4;
+      c = c < last ? c : (last - 1) & ~int64_t(3);
+      const int64_t r = (((int64_t)pc[i] * a.c.heads + h) << a.c.pshift) + (c & mask);
+      const uint8_t *vc = a.c.vc + r * (kD / 2) + (unit & ~3);
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          vq[g][4 * i + x] = *(const uint32_t *)(vc + x * (kD / 2) + g * (GROUP / 2));
+    }
+  };
+
+  const int64_t j1 = first + wave * 32;
+  if (j1 < last) {
+    load_ids(j1);
+    load_k(j1);
+    load_v(j1);
+    bad = bad_next;
+    if (j1 + step < last) load_ids(j1 + step);
+  }
+  for (int64_t j0 = j1; j0 < last; j0 += step) {
+    const bool more = j0 + step < last;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) s_w[lane * NG + g] = mw[g];
+    __builtin_amdgcn_wave_barrier();
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      Op av;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) av.u[g] = g < NG ? s_w[(16 * i + n) * NG + (g < NG ? g : 0)] : 0u;
+      f32x4 s = mfma(av, qm, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        f32x4 r = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = g * kGC; c < (g + 1) * kGC; ++c) {
+          Op k;
+#pragma unroll
+          for (int y = 0; y < 4; ++y) k.u[y] = code_pair(kq[i][c] >> (4 * y));
+          r = mfma(k, qv[0][c], r);
+          if constexpr (QT == 2) r = mfma(k, qv[1][c], r);
+        }
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          s[y] = __builtin_fmaf(scale_of(s_w[(16 * i + 4 * q4 + y) * NG + g]), r[y], s[y]);
+      }
+#pragma unroll
+      for (int y = 0; y < 4; ++y) x[4 * i + y] = s[y] * a.scale2;
+    }
+    uint32_t vw[8 * NG];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int y = 0; y < 4 * NG; ++y)
+        vw[4 * NG * i + y] = s_w[(32 + 16 * i + 4 * q4) * NG + y];
+    __builtin_amdgcn_wave_barrier();
+    if (more) load_k(j0 + step);
+    if (j0 + 32 > last || __any(bad != 0)) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (j0 + 16 * (i >> 2) + 4 * q4 + (i & 3) >= last || ((bad >> (i >> 2)) & 1)) {
+          x[i] = -INFINITY;
+#pragma unroll
+          for (int g = 0; g < NG; ++g) vw[i * NG + g] = 0;
+        }
+    }
+    if (a.logits && n < gn) {
+      float *lp = a.logits + (qh0 + n) * a.cap + j0 + 4 * q4;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (j0 + 16 * i + 4 * q4 < last)  // cap is a multiple of 4: whole quads fit
+          *(f32x4 *)(lp + 16 * i) = f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
+    }
+    float top = x[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
+    if (__any(top > m + 8.f)) {
+      top = fmaxf(top, xor16(top));
+      top = fmaxf(top, xor32(top));
+      const float mn = fmaxf(m, top);
+      const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      ms = mn == -INFINITY ? 0.f : mn;
+      l *= f;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        cb[g] *= f;
+        co[g] *= f;
+#pragma unroll
+        for (int j = 0; j < kU; ++j) o[g][j] *= f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[i] = __builtin_amdgcn_exp2f(x[i] - ms);
+      l += x[i];
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      Op hi, lo;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t w0 = vw[2 * i * NG + g], w1 = vw[(2 * i + 1) * NG + g];
+        cb[g] = __builtin_fmaf(x[2 * i], base_of(w0), cb[g]);
+        cb[g] = __builtin_fmaf(x[2 * i + 1], base_of(w1), cb[g]);
+        const float a0 = x[2 * i] * scale_of(w0), a1 = x[2 * i + 1] * scale_of(w1);
+        hi.u[i] = pack_bf16(a0, a1);
+        lo.u[i] = pack_bf16(a0 - __uint_as_float(hi.u[i] << 16),
+                            a1 - __uint_as_float(hi.u[i] & 0xffff0000u));
+      }
+      co[g] = mfma(ones, hi, co[g]);
+      co[g] = mfma(ones, lo, co[g]);
+      uint32_t pair[GROUP == 128 ? 2 : 1][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        pair[0][i] = __builtin_amdgcn_perm(vq[g][2 * i + 1], vq[g][2 * i], sel);
+        if constexpr (GROUP == 128)
+          pair[1][i] = __builtin_amdgcn_perm(vq[g][2 * i + 1], vq[g][2 * i], 0x07060302u);
+      }
+#pragma unroll
+      for (int j = 0; j < kU; ++j) {
+        Op v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v.u[i] = code_pair(pair[j >> 2][i] >> (4 * (j & 3)));
+        o[g][j] = mfma(v, hi, o[g][j]);
+        o[g][j] = mfma(v, lo, o[g][j]);
+      }
+    }
+    if (more) {
+      load_v(j0 + step);
+      bad = bad_next;
+      if (j0 + 2 * step < last) load_ids(j0 + 2 * step);
+    }
+  }
+
+  __syncthreads();  // the corners become the joining area
+  // join the waves: [waves][16] maxima, [waves][16] sums, [waves][gn][kD] outputs
+  l += xor16(l);
+  l += xor32(l);
+  float *s_m = s_mem, *s_l = s_mem + waves * 16, *s_o = s_mem + waves * 32;
+  if (q4 == 0) s_m[wave * 16 + n] = m;
+  __syncthreads();
+  float all = -INFINITY;
+  for (int w = 0; w < waves; ++w) all = fmaxf(all, s_m[w * 16 + n]);
+  const float f = __builtin_amdgcn_exp2f(m - (all == -INFINITY ? 0.f : all));
+  if (q4 == 0) s_l[wave * 16 + n] = l * f;
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    float c = cb[g];
+    c += xor16(c);
+    c += xor32(c);
+    if (n < gn) {
+      float *dst = s_o + (wave * gn + n) * kD + g * GROUP + 4 * q4 * kU;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < kU; ++j) dst[i * kU + j] = (o[g][j][i] - co[g][i] + c) * f;
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < gn * (kD / 8); i += blockDim.x) {
+    const int hd = i / (kD / 8), ch = (i % (kD / 8)) * 8;
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, ls = 0.f;
+    for (int w = 0; w < waves; ++w) {
+      ls += s_l[w * 16 + hd];
+      const float *src = s_o + (w * gn + hd) * kD + ch;
+#pragma unroll
+      for (int y = 0; y < 8; ++y) acc[y] += src[y];
+    }
+    if (a.splits > 1) {
+      store8<kStateF32>(a.part_o, ((qh0 + hd) * a.splits + split) * kD + ch, acc);
+    } else {
+      const float inv = len == 0 ? 0.f : 1.f / ls;
+#pragma unroll
+      for (int y = 0; y < 8; ++y) acc[y] *= inv;
+      store_out(type, a.out, (qh0 + hd) * kD + ch, acc);
+    }
+    if (a.part_ml && ch == 0) {
+      float mm = -INFINITY;
+      for (int w = 0; w < waves; ++w) mm = fmaxf(mm, s_m[w * 16 + hd]);
+      a.part_ml[(qh0 + hd) * a.splits + split] = make_float2(mm, ls);
+    }
+  }
+}
+
 // Joins the splits of a row's head into the output and adds the weights.  Block (x, y): x =
 // (row, head), y = a range of slots of the weights; y = 0 also writes the output.
 template <int TYPE>
@@ -263,6 +622,8 @@ __global__ __launch_bounds__(kThreads) void k_attend_finish(AttendArgs a, int64_
 }
 
 struct AttendPlan {
+  bool matrix;
+  int waves;  // of a workgroup of the matrix form
   int64_t chunk;
   int splits;
   int64_t cap;
@@ -274,10 +635,24 @@ int64_t up256(int64_t x) { return (x + 255) & ~int64_t(255); }
 AttendPlan plan_attend(const StateView &c, const AttendCall &a) {
   AttendPlan p{};
   p.cap = a.width << c.pshift;
-  const int64_t work = a.rows * c.heads;  // (row, head) pairs
-  // Splits: enough waves to fill the card (256 CUs x 16), of at least 64 slots each.
-  int64_t chunk = ceil_div(p.cap * work, 4096);
-  chunk = chunk < 64 ? 64 : (chunk + 63) & ~int64_t(63);
+  const int ng = c.dim / c.group, g = a.q_heads / c.heads;
+  p.matrix = a.type != kStateF32 && (c.group == 32 || c.group == 64 || c.group == 128) &&
+             ng <= 4 && c.pshift >= 2 && p.cap > 16 && c.pages < (int64_t(1) << 32);
+  int64_t chunk;
+  if (p.matrix) {
+    const int64_t work = a.rows * c.heads * ((g + 15) / 16);
+    const int gn = g < 16 ? g : 16;
+    // 8 waves where the rows alone cannot fill the card, as far as LDS holds their outputs
+    p.waves = work * ceil_div(p.cap, 512) <= 256 ? 8 : 4;
+    while (p.waves > 4 && p.waves * gn * c.dim * 4 > 96 * 1024) p.waves >>= 1;
+    chunk = ceil_div(p.cap * work, 8192);
+    const int64_t low = p.waves * 64 > 512 ? p.waves * 64 : 512;
+    chunk = chunk < low ? low : (chunk + 127) & ~int64_t(127);
+  } else {
+    // enough waves to fill the card (256 CUs x 16), of at least 64 slots each
+    chunk = ceil_div(p.cap * a.rows * c.heads, 4096);
+    chunk = chunk < 64 ? 64 : (chunk + 63) & ~int64_t(63);
+  }
   p.splits = (int)(p.cap <= chunk ? 1 : ceil_div(p.cap, chunk));
   p.chunk = p.splits == 1 ? (p.cap > 0 ? p.cap : 1) : chunk;
   const int64_t qh = a.rows * a.q_heads;
@@ -314,6 +689,32 @@ void launch_vec(const AttendArgs &a, int type, hipStream_t st) {
     launch_vec_g<LPR, 1>(a, type, st);
   else
     launch_vec_g<LPR, 64 / LPR>(a, type, st);
+}
+
+template <int NG, int GROUP>
+void launch_mfma(const AttendArgs &a, const AttendPlan &p, int type, hipStream_t st) {
+  const int tiles = (a.g + 15) / 16, gn = a.g < 16 ? a.g : 16;
+  const int64_t blocks = a.rows * a.c.heads * tiles * a.splits;
+  DGS_CHECK(blocks < (int64_t(1) << 31), "attend: too many rows in one call");
+  const int join = 32 + gn * NG * GROUP, corner = 64 * NG;  // words a wave needs of LDS
+  const size_t lds = (size_t)p.waves * (join > corner ? join : corner) * 4;
+  if (type == kStateBF16)
+    k_attend_mfma<NG, GROUP, 1><<<(unsigned)blocks, p.waves * 64, lds, st>>>(a, type, tiles);
+  else
+    k_attend_mfma<NG, GROUP, 2><<<(unsigned)blocks, p.waves * 64, lds, st>>>(a, type, tiles);
+  DGS_LAUNCH_CHECK();
+}
+template <int GROUP>
+void launch_mfma_g(const AttendArgs &a, const AttendPlan &p, int type, hipStream_t st) {
+  switch (a.c.dim / GROUP) {
+    case 1: launch_mfma<1, GROUP>(a, p, type, st); break;
+    case 2: launch_mfma<2, GROUP>(a, p, type, st); break;
+    case 3:
+      if constexpr (GROUP < 128) launch_mfma<3, GROUP>(a, p, type, st);
+      break;
+    default:
+      if constexpr (GROUP < 128) launch_mfma<4, GROUP>(a, p, type, st);
+  }
 }
 
 }  // namespace
@@ -353,7 +754,14 @@ void state_attend(const StateView &c, const AttendCall &call, void *ws, int64_t 
   a.decay = call.decay;
   a.out = call.out;
   a.gd = state_guard(kAsyncErrSlot, c.pages);
-  switch (pow2_at_least(c.dim >> 3)) {
+  if (p.matrix) {
+    if (c.group == 32)
+      launch_mfma_g<32>(a, p, call.type, st);
+    else if (c.group == 64)
+      launch_mfma_g<64>(a, p, call.type, st);
+    else
+      launch_mfma_g<128>(a, p, call.type, st);
+  } else switch (pow2_at_least(c.dim >> 3)) {
     case 1: launch_vec<1>(a, call.type, st); break;
     case 2: launch_vec<2>(a, call.type, st); break;
     case 4: launch_vec<4>(a, call.type, st); break;

@@ -1,8 +1,8 @@
 // state_rows.hip -- rows of the 4-bit state cache: writing (quantise and store) and reading.
 //
 // A group of `group` channels x of a row is held as codes c in 0..15, a scale s and a base b:
-//   r = max x - min x,  s = bf16(r / 15),  b = bf16(min x),  c = clamp(rint((x - b) / s), 0, 15)
-// with the quotient taken exactly (ties to even), so that a code never depends on the order or
+//   r = max x - min x,  s = bf16(r * fl(1/15)),  b = bf16(min x),  c = clamp(rint((x - b) / s), 0, 15)
+// (r and the product in 32 bits) with the quotient taken exactly (ties to even), so that a code never depends on the order or
 // width of the arithmetic; s = 0 gives c = 0.  Scale and base are rounded to 16 bits because they
 // are read with every row: 32-bit ones would add 8 bytes to the 72 of a row of 128 channels in
 // groups of 64.  b is exact for bfloat16 inputs, and the codes are taken against the rounded s
@@ -107,7 +107,7 @@ __global__ __launch_bounds__(kThreads) void k_state_write(WriteArgs a, int lpg_s
     hi = fmaxf(hi, __shfl_xor(hi, o, 64));
     bad += __shfl_xor(bad, o, 64);
   }
-  uint32_t sb = bf16_rne((hi - lo) / 15.f), bb = bf16_rne(lo);
+  uint32_t sb = bf16_rne((hi - lo) * (1.f / 15.f)), bb = bf16_rne(lo);
   const float s = bf16_bits(sb << 16), b = bf16_bits(bb << 16);
   const bool nan = !(bad == 0.f) || !(s - s == 0.f) || !(b - b == 0.f);
   uint32_t w = 0;

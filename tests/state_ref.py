@@ -10,7 +10,8 @@ def quantise(x, group):
     """x [..., D] -> codes [..., D] (uint8) and scales [..., D / group, 2] (bfloat16)."""
     g = x.float().unflatten(-1, (-1, group)).cpu()
     lo, hi = g.amin(-1), g.amax(-1)
-    s, b = ((hi - lo) / 15).to(torch.bfloat16), lo.to(torch.bfloat16)
+    s = ((hi - lo) * torch.tensor(1 / 15, dtype=torch.float32)).to(torch.bfloat16)
+    b = lo.to(torch.bfloat16)
     bad = ~(torch.isfinite(g).all(-1) & torch.isfinite(s) & torch.isfinite(b))
     s = torch.where(bad, torch.full_like(s, math.nan), s)
     b = torch.where(bad, torch.full_like(b, math.nan), b)
@@ -32,17 +33,18 @@ def values(codes, scales):
 
 
 def attend(q, cache, table, lens, scale):
-    """-> out [rows, q_heads, D], probabilities per head [rows, heads, cap] and the largest
-    scale * sum |q k| of a row (for error bounds), all 64 bits, on the CPU."""
+    """-> out [rows, q_heads, D], probabilities per head [rows, heads, cap], and per row and query
+    head the largest |scale| * sum |q k|, the largest |scale| * sum |q| s (s the scale of the
+    channel's group) and the largest |v|; all 64 bits, on the CPU."""
     kc, ks, vc, vs = [t.cpu() for t in (cache.k_codes, cache.k_scales, cache.v_codes,
                                         cache.v_scales)]
     q, table, lens = q.cpu().double(), table.cpu().long(), lens.cpu().long()
     rows, nq, dim = q.shape
-    heads, page = kc.shape[1], kc.shape[2]
+    heads, page, group = kc.shape[1], kc.shape[2], dim // ks.shape[3]
     g = nq // heads
     out = torch.zeros(rows, nq, dim, dtype=torch.float64)
     prob = torch.zeros(rows, heads, table.shape[1] * page, dtype=torch.float64)
-    size, vmax = 0.0, 0.0
+    size, steps, vmax = (torch.zeros(rows, nq, dtype=torch.float64) for _ in range(3))
     for i in range(rows):
         n = int(lens[i])
         if n == 0:
@@ -51,14 +53,16 @@ def attend(q, cache, table, lens, scale):
         p, o = table[i, j // page], j % page
         for h in range(heads):
             k, v = values(kc[p, h, o], ks[p, h, o]), values(vc[p, h, o], vs[p, h, o])
-            qs = q[i, h * g:(h + 1) * g]
-            x = qs @ k.T * scale
-            e = torch.softmax(x, 1)
-            out[i, h * g:(h + 1) * g] = e @ v
+            mine = slice(h * g, (h + 1) * g)
+            qs = q[i, mine]
+            e = torch.softmax(qs @ k.T * scale, 1)
+            out[i, mine] = e @ v
             prob[i, h, :n] = e.sum(0)
-            size = max(size, float((qs.abs() @ k.abs().T).max()) * scale)
-            vmax = max(vmax, float(v.abs().max()))
-    return out, prob, size, vmax
+            s = ks[p, h, o, :, 0].double().repeat_interleave(group, 1)
+            size[i, mine] = (qs.abs() @ k.abs().T).amax(1) * abs(scale)
+            steps[i, mine] = (qs.abs() @ s.T).amax(1) * abs(scale)
+            vmax[i, mine] = v.abs().max()
+    return out, prob, size, steps, vmax
 
 
 def evict(weights, positions, lens, budget, sinks, recent):

@@ -1,14 +1,14 @@
 """The state cache on the GPU against plain 64-bit forms (tests/state_ref.py).
 
-Tolerances.  Codes, scales, moves, lengths and copied values have to be equal.  attend: with
-u = 2^-24, a logit is a sum of D products of 32-bit values (each value one rounding of s * c + b, a
-query scaled with one rounding, and one more where the query is split into two 16-bit terms), so it
-is off by at most (D + 4) u S, S the largest scale * sum |q k|; half of that again covers sums of
-codes taken before their base.  A probability is off by twice that, plus the hardware exp2 (1 unit
-in 2^-23, an argument of |x| <= 2 S log2 e rounded: 3 S u) and, in the matrix form, the rounding of
-p times a scale to two bfloat16 terms (2^-17); sums of n terms in 32 bits in a tree of chunks add
-less than 64 u.  The output is a mean of values of size V under such weights, plus its own
-rounding, eps / 2."""
+Tolerances.  Codes, scales, moves, lengths and copied values have to be equal.  attend, with
+u = 2^-24: a logit is a chain of at most D + 8 sums in 32 bits.  Its terms are products of q and
+values (size = scale * sum |q k|, the values with one rounding of their own), or, where codes are
+multiplied first, of q and codes below 144, times the scales (144 steps, steps = scale * sum |q| s),
+so it is off by at most E = (D + 8) u (size + 144 steps) (32-bit inputs take the first form only:
+E = (D + 8) u size).  A probability is off by exp(2 E) - 1, the hardware exp2 (2^-23, and its argument's
+rounding, 3 u (size + 1)), the rounding of p times a scale to two bfloat16 terms (2^-17, not for
+32-bit inputs) and sums in 32 bits (64 u): rel in all.  The output is a mean of values up to vmax
+under such weights, with the same error in the sum that divides it, plus its own rounding, eps / 2."""
 import math
 import os
 
@@ -25,8 +25,9 @@ U = 2.0 ** -24
 TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 
 
-def prob_error(dim, size):
-    return 3 * (dim + 4) * U * size + 6 * size * U + 2.0 ** -17 + 80 * U
+def prob_error(dim, size, steps, exact):
+    e = (dim + 8) * U * (size if exact else size + 144 * steps)
+    return torch.expm1(2 * e) + 2.0 ** -23 + 3 * U * (size + 1) + (0 if exact else 2.0 ** -17) + 64 * U
 
 
 def states(shape, gen, dtype):
@@ -162,29 +163,29 @@ def test_empty_calls():
 # ------------------------------------------------------------------------------ attention
 def check_attend(cache, q, table, lens, scale=None, weights=None, decay=1.0):
     dim = cache.head_dim
-    sc = dim ** -0.5 if scale is None else scale
-    want, prob, size, vmax = ref.attend(q, cache, table, lens, abs(sc))
-    if sc < 0:
-        want, prob, size, vmax = ref.attend(-q, cache, table, lens, -sc)
+    want, prob, size, steps, vmax = ref.attend(q, cache, table, lens,
+                                               dim ** -0.5 if scale is None else scale)
     before = None if weights is None else weights.clone()
     got = cache.attend(q, table, lens, scale=scale, weights=weights, decay=decay)
     assert got.dtype == q.dtype and got.shape == q.shape
-    err = (got.cpu().double() - want).abs()
-    rel = prob_error(dim, size)
-    tol = 2 * rel * vmax + torch.finfo(q.dtype).eps / 2 * (want.abs() + 2 * rel * vmax) + 1e-30
+    rel = prob_error(dim, size, steps, q.dtype == torch.float32)
+    off = (2 * rel * vmax)[..., None]
+    tol = off + torch.finfo(q.dtype).eps / 2 * (want.abs() + off)
     if q.dtype == torch.float16:
         tol = tol + 2.0 ** -25  # half a step below the normal range
+    err = (got.cpu().double() - want).abs()
     assert bool((err <= tol).all()), (float(err.max()), float(tol.max()))
     if weights is not None:
-        g = q.shape[1] // cache.heads
-        inside = torch.arange(prob.shape[2]) < lens.cpu().long()[:, None, None]
-        old = before.cpu().double()[..., :prob.shape[2]]
+        cap, g = prob.shape[2], q.shape[1] // cache.heads
+        inside = torch.arange(cap) < lens.cpu().long()[:, None, None]
+        old = before.cpu().double()[..., :cap]
         exp = torch.where(inside, prob + (decay * old if decay else 0.0), old)
-        werr = (weights.cpu().double()[..., :prob.shape[2]] - exp).abs()
-        wtol = 2 * rel * prob + 4 * U * exp.abs() + g * U * prob + 1e-30
+        werr = (weights.cpu().double()[..., :cap] - exp).abs()
+        wrel = 2 * rel.unflatten(1, (cache.heads, g)).amax(2)[..., None]
+        wtol = wrel * prob + (g + 4) * U * exp.abs()
         assert bool((werr <= wtol)[inside.expand_as(werr)].all()), float(werr.max())
-        keep = ~torch.zeros_like(before, dtype=torch.bool)
-        keep[..., :prob.shape[2]] = ~inside.cuda()
+        keep = torch.ones_like(before, dtype=torch.bool)
+        keep[..., :cap] = ~inside.cuda()
         assert same_bits(weights[keep], before[keep])  # behind the lengths nothing changes
     return got
 
