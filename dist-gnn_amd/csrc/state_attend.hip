@@ -227,17 +227,17 @@ union Op {
 __device__ __forceinline__ f32x4 mfma(const Op &a, const Op &b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, b.v, c, 0, 0, 0);
 }
+// Two floats rounded to nearest even (one instruction).
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  union {
-    __bf16 h[2];
-    uint32_t u;
-  } v;
-  v.h[0] = (__bf16)lo;
-  v.h[1] = (__bf16)hi;
-  return v.u;
+  uint32_t r;
+  asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(r) : "v"(lo), "v"(hi));
+  return r;
 }
-__device__ __forceinline__ uint32_t code_pair(uint32_t x) {
-  return (x & 0x000f000fu) | 0x43004300u;
+// The low nibbles of a word's halves as bfloat16 128 + c.  `magic` is 0x43004300 in a vector
+// register: one instruction takes one constant from a scalar register, so with both there the
+// mask-or would be two.
+__device__ __forceinline__ uint32_t code_pair(uint32_t x, uint32_t magic) {
+  return (x & 0x000f000fu) | magic;
 }
 __device__ __forceinline__ float xor16(float x) {
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false,
@@ -250,25 +250,34 @@ __device__ __forceinline__ float xor32(float x) {
   return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
 }
 
-template <int NG, int GROUP, int QT>
+// PAGE16: pages of at least 16 slots, so that each half of the 32 slots lies in one page and the
+// wave computes its address once, in scalar registers.
+template <int NG, int GROUP, int QT, bool PAGE16>
 __global__ __launch_bounds__(512, 2) void k_attend_mfma(AttendArgs a, int type, int tiles) {
   constexpr int kD = NG * GROUP, kC = kD / 32, kU = GROUP / 16, kGC = GROUP / 32;
   extern __shared__ float s_mem[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, q4 = lane >> 4;
-  int64_t b = blockIdx.x;
-  const int split = (int)(b % a.splits);
-  b /= a.splits;
-  const int rt = (int)(b % tiles);
-  b /= tiles;
-  const int h = (int)(b % a.c.heads);
-  const int64_t row = b / a.c.heads;
-  const int64_t len = row_length(a, row, split == 0 && h == 0 && rt == 0 && threadIdx.x == 0);
-  const int64_t first = (int64_t)split * a.chunk;
+  uint32_t b = blockIdx.x;
+  const int split = (int)(b % (uint32_t)a.splits);
+  b /= (uint32_t)a.splits;
+  const int rt = (int)(b % (uint32_t)tiles);
+  b /= (uint32_t)tiles;
+  const int h = (int)(b % (uint32_t)a.c.heads);
+  const int64_t row = b / (uint32_t)a.c.heads;
+  // slots of a row fit 32 bits (checked on the host)
+  const int len = __builtin_amdgcn_readfirstlane(
+      (int)row_length(a, row, split == 0 && h == 0 && rt == 0 && threadIdx.x == 0));
+  const int chunk = (int)a.chunk, first = split * chunk;
   if (split > 0 && first >= len) return;
-  const int64_t last = a.splits == 1 ? len : (first + a.chunk < len ? first + a.chunk : len);
+  const int last = a.splits == 1 ? len : (first + chunk < len ? first + chunk : len);
   const int gn = a.g - rt * 16 < 16 ? a.g - rt * 16 : 16;
   const int64_t qh0 = row * a.q_heads + h * a.g + rt * 16;
+  // logits grow with x: a negative scale is taken into q
+  const float sign = a.scale2 < 0.f ? -1.f : 1.f, scale2 = fabsf(a.scale2);
+  uint32_t magic = 0x43004300u;
+  asm volatile("" : "+v"(magic));
 
   // q in bfloat16 terms, in the order in which code_pair() yields a word's channels: 0 4 1 5 2 6 3 7
   Op qv[QT][kC], qm;
@@ -281,7 +290,10 @@ __global__ __launch_bounds__(512, 2) void k_attend_mfma(AttendArgs a, int type, 
     if (n < gn)
       load_q(type, a.q, row * a.q_row + (h * a.g + rt * 16 + n) * a.q_head + 32 * c + 8 * q4, x);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) qsum[c / kGC] += x[i];
+    for (int i = 0; i < 8; ++i) {
+      x[i] *= sign;
+      qsum[c / kGC] += x[i];
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t hi = pack_bf16(x[i], x[4 + i]);
@@ -319,77 +331,123 @@ __global__ __launch_bounds__(512, 2) void k_attend_mfma(AttendArgs a, int type, 
 #pragma unroll
   for (int i = 0; i < 4; ++i) ones.u[i] = 0x43004300u;  // 128, the codes' offset
 
-  const int64_t mask = (int64_t(1) << a.c.pshift) - 1, trow = row * a.width;
+  const int ps = a.c.pshift, mask = (1 << ps) - 1;
+  const int64_t trow = row * a.width;
   const int unit = n * (GROUP / 32);  // byte of this lane's unit of V in a group's codes
   const uint32_t sel = GROUP == 128 ? 0x05040100u
                        : GROUP == 64 ? ((unit & 2) ? 0x07060302u : 0x05040100u)
                                      : (0x0c000c00u | (uint32_t)(unit & 3) |
                                         ((uint32_t)(4 + (unit & 3)) << 16));
-  const int64_t step = (int64_t)waves * 32;
+  const int step = waves * 32;
+  const uint32_t pages = (uint32_t)a.c.pages;
 
   // The wave's own corner of LDS: the (s, b) words of its 32 slots, K then V.
   uint32_t *s_w = (uint32_t *)s_mem + wave * (64 * NG);
   uint32_t kq[2][kC], vq[NG][8], mw[NG];  // one tile: codes of K and V, this lane's words
-  uint32_t pk[2], pc[2];  // pages of this lane's slots of K (l & 15) and V (4 (l >> 4) of each half)
+  // pages of the next tile: of its two halves, or of this lane's slots of K (l & 15 of each half)
+  // and V (4 (l >> 4) + i); a page outside the cache counts as page 0 and its slots are masked
+  constexpr int kPk = 2, kPv = PAGE16 ? 1 : 8;
+  uint32_t pk[kPk], pv[kPv];
   uint32_t bad = 0, bad_next = 0;
-  const uint32_t pages = (uint32_t)a.c.pages;
 
-  auto load_ids = [&](int64_t j0) {
+  auto page_of = [&](int j, bool inside, uint32_t bit) {
+    const int64_t id = a.table[trow + (j >> ps)];
+    if ((uint64_t)id < pages) return (uint32_t)id;
+    if (inside) report_bad_id(a.gd.err, kAsyncErrSlot, id, pages, a.gd.tag);
+    bad_next |= bit;
+    return 0u;
+  };
+  auto load_ids = [&](int j0) {
+    bad_next = 0;
+    if constexpr (PAGE16) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      int64_t k = j0 + 16 * i + n, c = j0 + 16 * i + 4 * q4;
-      k = k < last ? k : last - 1;
-      c = c < last ? c : last - 1;
-      const int64_t ik = a.table[trow + (k >> a.c.pshift)], ic = a.table[trow + (c >> a.c.pshift)];
-      pk[i] = (uint64_t)ik < pages ? (uint32_t)ik : 0u;
-      const bool out = (uint64_t)ic >= pages;
-      if (out && j0 + 16 * i + 4 * q4 < last)
-        report_bad_id(a.gd.err, kAsyncErrSlot, ic, pages, a.gd.tag);
-      pc[i] = out ? 0u : (uint32_t)ic;
-      bad_next = (bad_next & ~(1u << i)) | ((out ? 1u : 0u) << i);
+      for (int i = 0; i < 2; ++i) {
+        const int j = j0 + 16 * i < last ? j0 + 16 * i : last - 1;
+        pk[i] = __builtin_amdgcn_readfirstlane(page_of(j, true, 0xfu << (4 * i)));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int k = j0 + 16 * i + n;
+        pk[i] = page_of(k < last ? k : last - 1, false, 0u);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int j = j0 + 16 * (i >> 2) + 4 * q4 + (i & 3);
+        pv[i] = page_of(j < last ? j : last - 1, j < last, 1u << i);
+      }
     }
   };
-  auto load_k = [&](int64_t j0) {
-    int64_t rm = 0;
+  // The codes of K and the (s, b) words: quarters 0 and 1 fetch those of K, 2 and 3 those of V.
+  auto load_k = [&](int j0) {
+    if constexpr (PAGE16) {
+      int64_t r[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      int64_t k = j0 + 16 * i + n;
-      k = k < last ? k : last - 1;
-      const int64_t r = (((int64_t)pk[i] * a.c.heads + h) << a.c.pshift) + (k & mask);
-      const uint32_t *kc = (const uint32_t *)(a.c.kc + r * (kD / 2)) + q4;
+      for (int i = 0; i < 2; ++i) {
+        const int j = j0 + 16 * i < last ? j0 + 16 * i : (last - 1) & ~15;
+        r[i] = (((int64_t)pk[i] * a.c.heads + h) << ps) + (j & mask);
+        const uint8_t *kc = a.c.kc + r[i] * (kD / 2);
 #pragma unroll
-      for (int x = 0; x < kC; ++x) kq[i][x] = kc[4 * x];
-      if ((q4 & 1) == i) rm = r;
+        for (int x = 0; x < kC; ++x)
+          kq[i][x] = *(const uint32_t *)(kc + (uint32_t)(n * (kD / 2) + 4 * q4 + 16 * x));
+      }
+      const uint32_t *wp = (q4 & 2 ? a.c.vs : a.c.ks) + ((q4 & 1 ? r[1] : r[0]) + n) * NG;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) mw[g] = wp[g];
+    } else {
+      int64_t rm = 0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        int k = j0 + 16 * i + n;
+        k = k < last ? k : last - 1;
+        const int64_t r = (((int64_t)pk[i] * a.c.heads + h) << ps) + (k & mask);
+        const uint8_t *kc = a.c.kc + r * (kD / 2) + 4 * q4;
+#pragma unroll
+        for (int x = 0; x < kC; ++x) kq[i][x] = *(const uint32_t *)(kc + 16 * x);
+        if ((q4 & 1) == i) rm = r;
+      }
+      const uint32_t *wp = (q4 & 2 ? a.c.vs : a.c.ks) + rm * NG;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) mw[g] = wp[g];
     }
-    // quarters 0 and 1 fetch the words of K, 2 and 3 those of V
-    const uint32_t *wp = (q4 & 2 ? a.c.vs : a.c.ks) + rm * NG;
-#pragma unroll
-    for (int g = 0; g < NG; ++g) mw[g] = wp[g];
   };
-  auto load_v = [&](int64_t j0) {
+  auto load_v = [&](int j0, const uint32_t *pg) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      int64_t c = j0 + 16 * i + 4 * q4;
-      c = c < last ? c : (last - 1) & ~int64_t(3);
-      const int64_t r = (((int64_t)pc[i] * a.c.heads + h) << a.c.pshift) + (c & mask);
-      const uint8_t *vc = a.c.vc + r * (kD / 2) + (unit & ~3);
+      if constexpr (PAGE16) {
+        const int j = j0 + 16 * i < last ? j0 + 16 * i : (last - 1) & ~15;
+        const int64_t r = (((int64_t)pg[i] * a.c.heads + h) << ps) + (j & mask);
+        const uint8_t *vc = a.c.vc + r * (kD / 2);
 #pragma unroll
-      for (int g = 0; g < NG; ++g)
+        for (int g = 0; g < NG; ++g)
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
-          vq[g][4 * i + x] = *(const uint32_t *)(vc + x * (kD / 2) + g * (GROUP / 2));
+          for (int x = 0; x < 4; ++x)
+            vq[g][4 * i + x] = *(const uint32_t *)(vc + (uint32_t)((4 * q4 + x) * (kD / 2) +
+                                                                   (unit & ~3) + g * (GROUP / 2)));
+      } else {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          int j = j0 + 16 * i + 4 * q4 + x;
+          j = j < last ? j : last - 1;
+          const int64_t r = (((int64_t)pv[(4 * i + x) % kPv] * a.c.heads + h) << ps) + (j & mask);
+          const uint8_t *vc = a.c.vc + r * (kD / 2) + (unit & ~3);
+#pragma unroll
+          for (int g = 0; g < NG; ++g) vq[g][4 * i + x] = *(const uint32_t *)(vc + g * (GROUP / 2));
+        }
+      }
     }
   };
 
-  const int64_t j1 = first + wave * 32;
+  const int j1 = first + wave * 32;
+  uint32_t pg[2] = {0, 0};  // PAGE16: the halves' pages of the tile whose V is still to load
   if (j1 < last) {
     load_ids(j1);
     load_k(j1);
-    load_v(j1);
+    load_v(j1, pk);
     bad = bad_next;
     if (j1 + step < last) load_ids(j1 + step);
   }
-  for (int64_t j0 = j1; j0 < last; j0 += step) {
+  for (int j0 = j1; j0 < last; j0 += step) {
     const bool more = j0 + step < last;
 #pragma unroll
     for (int g = 0; g < NG; ++g) s_w[lane * NG + g] = mw[g];
@@ -401,6 +459,10 @@ __global__ __launch_bounds__(512, 2) void k_attend_mfma(AttendArgs a, int type, 
 #pragma unroll
       for (int g = 0; g < 4; ++g) av.u[g] = g < NG ? s_w[(16 * i + n) * NG + (g < NG ? g : 0)] : 0u;
       f32x4 s = mfma(av, qm, f32x4{0.f, 0.f, 0.f, 0.f});
+      uint32_t kw[4 * NG];
+#pragma unroll
+      for (int y = 0; y < NG; ++y)
+        *(su32x4 *)(kw + 4 * y) = *(const su32x4 *)(s_w + (16 * i + 4 * q4) * NG + 4 * y);
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         f32x4 r = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -408,29 +470,35 @@ __global__ __launch_bounds__(512, 2) void k_attend_mfma(AttendArgs a, int type, 
         for (int c = g * kGC; c < (g + 1) * kGC; ++c) {
           Op k;
 #pragma unroll
-          for (int y = 0; y < 4; ++y) k.u[y] = code_pair(kq[i][c] >> (4 * y));
+          for (int y = 0; y < 4; ++y) k.u[y] = code_pair(kq[i][c] >> (4 * y), magic);
           r = mfma(k, qv[0][c], r);
           if constexpr (QT == 2) r = mfma(k, qv[1][c], r);
         }
 #pragma unroll
-        for (int y = 0; y < 4; ++y)
-          s[y] = __builtin_fmaf(scale_of(s_w[(16 * i + 4 * q4 + y) * NG + g]), r[y], s[y]);
+        for (int y = 0; y < 4; ++y) s[y] = __builtin_fmaf(scale_of(kw[y * NG + g]), r[y], s[y]);
       }
 #pragma unroll
-      for (int y = 0; y < 4; ++y) x[4 * i + y] = s[y] * a.scale2;
+      for (int y = 0; y < 4; ++y) x[4 * i + y] = s[y];
     }
     uint32_t vw[8 * NG];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int y = 0; y < 4 * NG; ++y)
-        vw[4 * NG * i + y] = s_w[(32 + 16 * i + 4 * q4) * NG + y];
+      for (int y = 0; y < NG; ++y)
+        *(su32x4 *)(vw + 4 * NG * i + 4 * y) =
+            *(const su32x4 *)(s_w + (32 + 16 * i + 4 * q4) * NG + 4 * y);
     __builtin_amdgcn_wave_barrier();
-    if (more) load_k(j0 + step);
+    if (more) {
+      if constexpr (PAGE16) {
+        pg[0] = pk[0];
+        pg[1] = pk[1];
+      }
+      load_k(j0 + step);
+    }
     if (j0 + 32 > last || __any(bad != 0)) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (j0 + 16 * (i >> 2) + 4 * q4 + (i & 3) >= last || ((bad >> (i >> 2)) & 1)) {
+        if (j0 + 16 * (i >> 2) + 4 * q4 + (i & 3) >= last || ((bad >> i) & 1)) {
           x[i] = -INFINITY;
 #pragma unroll
           for (int g = 0; g < NG; ++g) vw[i * NG + g] = 0;
@@ -439,13 +507,22 @@ __global__ __launch_bounds__(512, 2) void k_attend_mfma(AttendArgs a, int type, 
     if (a.logits && n < gn) {
       float *lp = a.logits + (qh0 + n) * a.cap + j0 + 4 * q4;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (j0 + 16 * i + 4 * q4 < last)  // cap is a multiple of 4: whole quads fit
-          *(f32x4 *)(lp + 16 * i) = f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
+      for (int i = 0; i < 2; ++i) {
+        if (PAGE16) {  // cap is a multiple of 4: whole quads fit
+          if (j0 + 16 * i + 4 * q4 < last)
+            *(f32x4 *)(lp + 16 * i) = f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]} * scale2;
+        } else {
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            if (j0 + 16 * i + 4 * q4 + y < last) lp[16 * i + y] = x[4 * i + y] * scale2;
+        }
+      }
     }
+    // m and ms in units of base 2
     float top = x[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
+    top *= scale2;
     if (__any(top > m + 8.f)) {
       top = fmaxf(top, xor16(top));
       top = fmaxf(top, xor32(top));
@@ -464,7 +541,7 @@ __global__ __launch_bounds__(512, 2) void k_attend_mfma(AttendArgs a, int type, 
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      x[i] = __builtin_amdgcn_exp2f(x[i] - ms);
+      x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], scale2, -ms));
       l += x[i];
     }
 #pragma unroll
@@ -493,13 +570,13 @@ __global__ __launch_bounds__(512, 2) void k_attend_mfma(AttendArgs a, int type, 
       for (int j = 0; j < kU; ++j) {
         Op v;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v.u[i] = code_pair(pair[j >> 2][i] >> (4 * (j & 3)));
+        for (int i = 0; i < 4; ++i) v.u[i] = code_pair(pair[j >> 2][i] >> (4 * (j & 3)), magic);
         o[g][j] = mfma(v, hi, o[g][j]);
         o[g][j] = mfma(v, lo, o[g][j]);
       }
     }
     if (more) {
-      load_v(j0 + step);
+      load_v(j0 + step, pg);
       bad = bad_next;
       if (j0 + 2 * step < last) load_ids(j0 + 2 * step);
     }
@@ -637,7 +714,8 @@ AttendPlan plan_attend(const StateView &c, const AttendCall &a) {
   p.cap = a.width << c.pshift;
   const int ng = c.dim / c.group, g = a.q_heads / c.heads;
   p.matrix = a.type != kStateF32 && (c.group == 32 || c.group == 64 || c.group == 128) &&
-             ng <= 4 && c.pshift >= 2 && p.cap > 16 && c.pages < (int64_t(1) << 32);
+             ng <= 4 && p.cap > 16 && p.cap < (int64_t(1) << 30) &&
+             c.pages < (int64_t(1) << 32);
   int64_t chunk;
   if (p.matrix) {
     const int64_t work = a.rows * c.heads * ((g + 15) / 16);
@@ -698,10 +776,18 @@ void launch_mfma(const AttendArgs &a, const AttendPlan &p, int type, hipStream_t
   DGS_CHECK(blocks < (int64_t(1) << 31), "attend: too many rows in one call");
   const int join = 32 + gn * NG * GROUP, corner = 64 * NG;  // words a wave needs of LDS
   const size_t lds = (size_t)p.waves * (join > corner ? join : corner) * 4;
-  if (type == kStateBF16)
-    k_attend_mfma<NG, GROUP, 1><<<(unsigned)blocks, p.waves * 64, lds, st>>>(a, type, tiles);
-  else
-    k_attend_mfma<NG, GROUP, 2><<<(unsigned)blocks, p.waves * 64, lds, st>>>(a, type, tiles);
+  const unsigned grid = (unsigned)blocks, threads = p.waves * 64;
+  if (a.c.pshift >= 4) {
+    if (type == kStateBF16)
+      k_attend_mfma<NG, GROUP, 1, true><<<grid, threads, lds, st>>>(a, type, tiles);
+    else
+      k_attend_mfma<NG, GROUP, 2, true><<<grid, threads, lds, st>>>(a, type, tiles);
+  } else {
+    if (type == kStateBF16)
+      k_attend_mfma<NG, GROUP, 1, false><<<grid, threads, lds, st>>>(a, type, tiles);
+    else
+      k_attend_mfma<NG, GROUP, 2, false><<<grid, threads, lds, st>>>(a, type, tiles);
+  }
   DGS_LAUNCH_CHECK();
 }
 template <int GROUP>
