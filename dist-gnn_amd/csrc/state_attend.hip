@@ -212,8 +212,12 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
 //    heads, k slots.  a_g = p s_g is rounded to two bfloat16 terms (17 bits: one term's 2^-9 would
 //    show in the output), and the 128 sum a_g that the codes' offset adds is taken out with the same
 //    rounded terms, through a product with a constant operand.  sum p b_g is summed in 32 bits.
-//    The pairs of slots that a register of V holds are made with v_perm_b32: no transposition
-//    through LDS.
+//    The pairs of slots that a register of V holds are made with v_perm_b32.
+//  - Rows come in 16 bytes a lane, two tiles ahead in registers, and pass through the wave's own
+//    corner of LDS, from which every lane takes its words: 26 narrow loads a tile straight to their
+//    lanes kept the wave waiting (60 % of its time) and the texture unit half busy.  A row's 16-byte
+//    pieces are stored in an order that depends on the row, so that the rows a read touches lie in
+//    different banks.
 //  - m only follows the maximum when a logit passes it by 8 (in base 2): p stays below 2^8, and
 //    the rescaling is a rare branch.
 // The waves of a workgroup take their 32 slots in turn and join through LDS in wave order.
@@ -250,9 +254,7 @@ __device__ __forceinline__ float xor32(float x) {
   return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
 }
 
-// PAGE16: pages of at least 16 slots, so that each half of the 32 slots lies in one page and the
-// wave computes its address once, in scalar registers.
-template <int NG, int GROUP, int QT, bool PAGE16>
+template <int NG, int GROUP, int QT>
 __global__ __launch_bounds__(512, 2) void k_attend_mfma(AttendArgs a, int type, int tiles) {
   constexpr int kD = NG * GROUP, kC = kD / 32, kU = GROUP / 16, kGC = GROUP / 32;
   extern __shared__ float s_mem[];
@@ -341,117 +343,105 @@ __global__ __launch_bounds__(512, 2) void k_attend_mfma(AttendArgs a, int type, 
   const int step = waves * 32;
   const uint32_t pages = (uint32_t)a.c.pages;
 
-  // The wave's own corner of LDS: the (s, b) words of its 32 slots, K then V.
-  uint32_t *s_w = (uint32_t *)s_mem + wave * (64 * NG);
-  uint32_t kq[2][kC], vq[NG][8], mw[NG];  // one tile: codes of K and V, this lane's words
-  // pages of the next tile: of its two halves, or of this lane's slots of K (l & 15 of each half)
-  // and V (4 (l >> 4) + i); a page outside the cache counts as page 0 and its slots are masked
-  constexpr int kPk = 2, kPv = PAGE16 ? 1 : 8;
-  uint32_t pk[kPk], pv[kPv];
-  uint32_t bad = 0, bad_next = 0;
+  // A tile is kPR x 64 pieces of 16 bytes: those of K, then those of V, row by row.  kL loads of a
+  // lane; load i of the first kL / 2 (kPR = 1: the lower half of the wave) belongs to K.  kRows rows
+  // a load; a lane meets kIds different slots.
+  constexpr int kPR = kD / 32, kL = kPR < 2 ? 1 : kPR, kRows = 64 / kPR > 32 ? 32 : 64 / kPR;
+  constexpr int kIds = 32 / kRows;
+  // the words of a row: NG of K, NG of V; kPR lanes of the row fetch them in kW loads
+  constexpr int kW = (2 * NG + kPR - 1) / kPR;
+  // Piece p of row r lies at p ^ key(r) (in its low two bits): rows that share banks differ.
+  auto key = [](int r) { return kPR == 1 ? 0 : (kPR == 2 ? (r >> 3) & 1 : (r >> 2) & 3); };
+  su32x4 *s_c = (su32x4 *)s_mem + wave * (kPR * 64 + NG * 16);  // codes of K, then of V
+  uint32_t *s_w = (uint32_t *)(s_c + kPR * 64);                 // words of K, then of V
+  const int lrow = (lane / kPR) % kRows, lpiece = lane % kPR;
+  // where this lane finds its words of K (chunk c: kp[c & 3]) and of V (group g: vp[g % kVP]); the
+  // keys of its rows 16 i + n and 16 i + 4 q4 + y do not depend on i and y
+  constexpr int kKP = kPR < 4 ? kPR : 4, kVP = GROUP == 128 ? 1 : (GROUP == 64 ? 2 : 4);
+  const char *kp[kKP], *vp[kVP];
+#pragma unroll
+  for (int c = 0; c < kKP; ++c) kp[c] = (const char *)(s_c + n * kPR + (c ^ key(n))) + 4 * q4;
+#pragma unroll
+  for (int g = 0; g < kVP; ++g) {
+    const int p = g * (GROUP / 32) + (unit >> 4);
+    vp[g] = (const char *)(s_c + 32 * kPR + 4 * q4 * kPR + (p ^ key(4 * q4))) + (unit & 12);
+  }
+  struct Rows {
+    su32x4 c[kL];
+    uint32_t w[kIds][kW];
+    uint64_t bad[kIds];  // lanes whose page lies outside the cache
+  };
+  Rows t0, t1;
+  // pages of the next tile's slots, as read (low and high words; looked at when its rows are
+  // loaded, without a branch on the table's type, which would wait for every load before it)
+  uint32_t id[kIds], id_hi[kIds];
+  const bool wide = a.table.bytes == 8;
+  const char *tab = (const char *)a.table.p + (trow << (wide ? 3 : 2));
 
-  auto page_of = [&](int j, bool inside, uint32_t bit) {
-    const int64_t id = a.table[trow + (j >> ps)];
-    if ((uint64_t)id < pages) return (uint32_t)id;
-    if (inside) report_bad_id(a.gd.err, kAsyncErrSlot, id, pages, a.gd.tag);
-    bad_next |= bit;
-    return 0u;
+  auto slot_of = [&](int j0, int i) {
+    const int j = j0 + i * kRows + lrow;
+    return j < last ? j : last - 1;
   };
   auto load_ids = [&](int j0) {
-    bad_next = 0;
-    if constexpr (PAGE16) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int j = j0 + 16 * i < last ? j0 + 16 * i : last - 1;
-        pk[i] = __builtin_amdgcn_readfirstlane(page_of(j, true, 0xfu << (4 * i)));
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int k = j0 + 16 * i + n;
-        pk[i] = page_of(k < last ? k : last - 1, false, 0u);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int j = j0 + 16 * (i >> 2) + 4 * q4 + (i & 3);
-        pv[i] = page_of(j < last ? j : last - 1, j < last, 1u << i);
-      }
+    for (int i = 0; i < kIds; ++i) {
+      const char *at = tab + ((int64_t)(slot_of(j0, i) >> ps) << (wide ? 3 : 2));
+      id[i] = *(const uint32_t *)at;
+      id_hi[i] = *(const uint32_t *)(at + (wide ? 4 : 0));
     }
   };
-  // The codes of K and the (s, b) words: quarters 0 and 1 fetch those of K, 2 and 3 those of V.
-  auto load_k = [&](int j0) {
-    if constexpr (PAGE16) {
-      int64_t r[2];
+  // Loads tile j0's rows, and before them the ids of tile j0 + step: memory returns in order, so
+  // whoever waits for an id would wait for rows issued before it.
+  auto load_rows = [&](int j0, Rows &t) {
+    uint32_t page[kIds];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int j = j0 + 16 * i < last ? j0 + 16 * i : (last - 1) & ~15;
-        r[i] = (((int64_t)pk[i] * a.c.heads + h) << ps) + (j & mask);
-        const uint8_t *kc = a.c.kc + r[i] * (kD / 2);
-#pragma unroll
-        for (int x = 0; x < kC; ++x)
-          kq[i][x] = *(const uint32_t *)(kc + (uint32_t)(n * (kD / 2) + 4 * q4 + 16 * x));
-      }
-      const uint32_t *wp = (q4 & 2 ? a.c.vs : a.c.ks) + ((q4 & 1 ? r[1] : r[0]) + n) * NG;
-#pragma unroll
-      for (int g = 0; g < NG; ++g) mw[g] = wp[g];
-    } else {
-      int64_t rm = 0;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        int k = j0 + 16 * i + n;
-        k = k < last ? k : last - 1;
-        const int64_t r = (((int64_t)pk[i] * a.c.heads + h) << ps) + (k & mask);
-        const uint8_t *kc = a.c.kc + r * (kD / 2) + 4 * q4;
-#pragma unroll
-        for (int x = 0; x < kC; ++x) kq[i][x] = *(const uint32_t *)(kc + 16 * x);
-        if ((q4 & 1) == i) rm = r;
-      }
-      const uint32_t *wp = (q4 & 2 ? a.c.vs : a.c.ks) + rm * NG;
-#pragma unroll
-      for (int g = 0; g < NG; ++g) mw[g] = wp[g];
+    for (int i = 0; i < kIds; ++i) {
+      const bool out = id[i] >= pages || (wide && id_hi[i] != 0);
+      if (out)
+        report_bad_id(a.gd.err, kAsyncErrSlot,
+                      wide ? (int64_t)((uint64_t)id_hi[i] << 32 | id[i]) : (int64_t)(int32_t)id[i],
+                      pages, a.gd.tag);
+      page[i] = out ? 0u : id[i];
+      t.bad[i] = __ballot(out);
     }
-  };
-  auto load_v = [&](int j0, const uint32_t *pg) {
+    load_ids(j0 + step);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if constexpr (PAGE16) {
-        const int j = j0 + 16 * i < last ? j0 + 16 * i : (last - 1) & ~15;
-        const int64_t r = (((int64_t)pg[i] * a.c.heads + h) << ps) + (j & mask);
-        const uint8_t *vc = a.c.vc + r * (kD / 2);
-#pragma unroll
-        for (int g = 0; g < NG; ++g)
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            vq[g][4 * i + x] = *(const uint32_t *)(vc + (uint32_t)((4 * q4 + x) * (kD / 2) +
-                                                                   (unit & ~3) + g * (GROUP / 2)));
+    for (int i = 0; i < kIds; ++i) {
+      const int64_t r = (((int64_t)page[i] * a.c.heads + h) << ps) + (slot_of(j0, i) & mask);
+      if constexpr (kPR == 1) {
+        t.c[0] = *(const su32x4 *)((lane < 32 ? a.c.kc : a.c.vc) + r * 16);
       } else {
+        t.c[i] = *(const su32x4 *)(a.c.kc + r * (kD / 2) + 16 * lpiece);
+        t.c[kIds + i] = *(const su32x4 *)(a.c.vc + r * (kD / 2) + 16 * lpiece);
+      }
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          int j = j0 + 16 * i + 4 * q4 + x;
-          j = j < last ? j : last - 1;
-          const int64_t r = (((int64_t)pv[(4 * i + x) % kPv] * a.c.heads + h) << ps) + (j & mask);
-          const uint8_t *vc = a.c.vc + r * (kD / 2) + (unit & ~3);
-#pragma unroll
-          for (int g = 0; g < NG; ++g) vq[g][4 * i + x] = *(const uint32_t *)(vc + g * (GROUP / 2));
-        }
+      for (int y = 0; y < kW; ++y) {
+        // word e of the row's 2 NG (kPR = 1: the lower lanes fetch K's, the upper V's)
+        const int e = kPR == 1 ? (lane < 32 ? y : NG + y) : lpiece + y * kPR;
+        const uint32_t *wp = e < NG ? a.c.ks : a.c.vs;
+        t.w[i][y] = e < 2 * NG ? wp[r * NG + (e < NG ? e : e - NG)] : 0u;
       }
     }
   };
-
-  const int j1 = first + wave * 32;
-  uint32_t pg[2] = {0, 0};  // PAGE16: the halves' pages of the tile whose V is still to load
-  if (j1 < last) {
-    load_ids(j1);
-    load_k(j1);
-    load_v(j1, pk);
-    bad = bad_next;
-    if (j1 + step < last) load_ids(j1 + step);
-  }
-  for (int j0 = j1; j0 < last; j0 += step) {
-    const bool more = j0 + step < last;
+  auto stage = [&](const Rows &t) {
 #pragma unroll
-    for (int g = 0; g < NG; ++g) s_w[lane * NG + g] = mw[g];
+    for (int i = 0; i < kIds; ++i) {
+      const int r = i * kRows + lrow;
+      if constexpr (kPR == 1) {
+        s_c[(lane < 32 ? 0 : 32) + r] = t.c[0];
+      } else {
+        s_c[r * kPR + (lpiece ^ key(r))] = t.c[i];
+        s_c[(32 + r) * kPR + (lpiece ^ key(r))] = t.c[kIds + i];
+      }
+#pragma unroll
+      for (int y = 0; y < kW; ++y) {
+        const int e = kPR == 1 ? (lane < 32 ? y : NG + y) : lpiece + y * kPR;
+        if (e < 2 * NG) s_w[e < NG ? r * NG + e : (32 + r) * NG + e - NG] = t.w[i][y];
+      }
+    }
     __builtin_amdgcn_wave_barrier();
+  };
+  auto compute = [&](int j0, const uint64_t *bad) {
     float x[8];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -459,58 +449,62 @@ __global__ __launch_bounds__(512, 2) void k_attend_mfma(AttendArgs a, int type, 
 #pragma unroll
       for (int g = 0; g < 4; ++g) av.u[g] = g < NG ? s_w[(16 * i + n) * NG + (g < NG ? g : 0)] : 0u;
       f32x4 s = mfma(av, qm, f32x4{0.f, 0.f, 0.f, 0.f});
-      uint32_t kw[4 * NG];
+      su32x4 kw[NG];
 #pragma unroll
       for (int y = 0; y < NG; ++y)
-        *(su32x4 *)(kw + 4 * y) = *(const su32x4 *)(s_w + (16 * i + 4 * q4) * NG + 4 * y);
+        kw[y] = *(const su32x4 *)(s_w + (16 * i + 4 * q4) * NG + 4 * y);
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         f32x4 r = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = g * kGC; c < (g + 1) * kGC; ++c) {
+          const uint32_t w = *(const uint32_t *)(kp[c % kKP] + 256 * kPR * i + 64 * (c / 4));
           Op k;
 #pragma unroll
-          for (int y = 0; y < 4; ++y) k.u[y] = code_pair(kq[i][c] >> (4 * y), magic);
+          for (int y = 0; y < 4; ++y) k.u[y] = code_pair(w >> (4 * y), magic);
           r = mfma(k, qv[0][c], r);
           if constexpr (QT == 2) r = mfma(k, qv[1][c], r);
         }
 #pragma unroll
-        for (int y = 0; y < 4; ++y) s[y] = __builtin_fmaf(scale_of(kw[y * NG + g]), r[y], s[y]);
+        for (int y = 0; y < 4; ++y)
+          s[y] = __builtin_fmaf(scale_of(kw[(y * NG + g) / 4][(y * NG + g) % 4]), r[y], s[y]);
       }
 #pragma unroll
       for (int y = 0; y < 4; ++y) x[4 * i + y] = s[y];
     }
-    uint32_t vw[8 * NG];
+    su32x4 vw[2 * NG];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int y = 0; y < NG; ++y)
-        *(su32x4 *)(vw + 4 * NG * i + 4 * y) =
-            *(const su32x4 *)(s_w + (32 + 16 * i + 4 * q4) * NG + 4 * y);
-    __builtin_amdgcn_wave_barrier();
-    if (more) {
-      if constexpr (PAGE16) {
-        pg[0] = pk[0];
-        pg[1] = pk[1];
-      }
-      load_k(j0 + step);
-    }
-    if (j0 + 32 > last || __any(bad != 0)) {
+        vw[NG * i + y] = *(const su32x4 *)(s_w + (32 + 16 * i + 4 * q4) * NG + 4 * y);
+    bool some = false;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (j0 + 16 * (i >> 2) + 4 * q4 + (i & 3) >= last || ((bad >> i) & 1)) {
+    for (int i = 0; i < kIds; ++i) some |= bad[i] != 0;
+    if (j0 + 32 > last || some) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = 16 * (i >> 2) + 4 * q4 + (i & 3);
+        bool out = j0 + r >= last;
+        if (some)
+#pragma unroll
+          for (int y = 0; y < kIds; ++y)
+            out |= r / kRows == y && ((bad[y] >> ((r % kRows) * (kPR == 1 ? 1 : kPR))) & 1);
+        if (out) {
           x[i] = -INFINITY;
 #pragma unroll
-          for (int g = 0; g < NG; ++g) vw[i * NG + g] = 0;
+          for (int g = 0; g < NG; ++g) vw[(i * NG + g) / 4][(i * NG + g) % 4] = 0;
         }
+      }
     }
     if (a.logits && n < gn) {
       float *lp = a.logits + (qh0 + n) * a.cap + j0 + 4 * q4;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        if (PAGE16) {  // cap is a multiple of 4: whole quads fit
+        if ((a.cap & 3) == 0) {  // whole quads fit
           if (j0 + 16 * i + 4 * q4 < last)
-            *(f32x4 *)(lp + 16 * i) = f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]} * scale2;
+            *(f32x4 *)(lp + 16 * i) =
+                f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]} * scale2;
         } else {
 #pragma unroll
           for (int y = 0; y < 4; ++y)
@@ -546,10 +540,16 @@ __global__ __launch_bounds__(512, 2) void k_attend_mfma(AttendArgs a, int type, 
     }
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
+      uint32_t vq[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        vq[i] = *(const uint32_t *)(vp[g % kVP] + 16 * kPR * (16 * (i >> 2) + (i & 3)) +
+                                    64 * (g / kVP));
       Op hi, lo;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t w0 = vw[2 * i * NG + g], w1 = vw[(2 * i + 1) * NG + g];
+        const uint32_t w0 = vw[(2 * i * NG + g) / 4][(2 * i * NG + g) % 4];
+        const uint32_t w1 = vw[((2 * i + 1) * NG + g) / 4][((2 * i + 1) * NG + g) % 4];
         cb[g] = __builtin_fmaf(x[2 * i], base_of(w0), cb[g]);
         cb[g] = __builtin_fmaf(x[2 * i + 1], base_of(w1), cb[g]);
         const float a0 = x[2 * i] * scale_of(w0), a1 = x[2 * i + 1] * scale_of(w1);
@@ -562,9 +562,9 @@ __global__ __launch_bounds__(512, 2) void k_attend_mfma(AttendArgs a, int type, 
       uint32_t pair[GROUP == 128 ? 2 : 1][4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        pair[0][i] = __builtin_amdgcn_perm(vq[g][2 * i + 1], vq[g][2 * i], sel);
+        pair[0][i] = __builtin_amdgcn_perm(vq[2 * i + 1], vq[2 * i], sel);
         if constexpr (GROUP == 128)
-          pair[1][i] = __builtin_amdgcn_perm(vq[g][2 * i + 1], vq[g][2 * i], 0x07060302u);
+          pair[1][i] = __builtin_amdgcn_perm(vq[2 * i + 1], vq[2 * i], 0x07060302u);
       }
 #pragma unroll
       for (int j = 0; j < kU; ++j) {
@@ -575,10 +575,29 @@ __global__ __launch_bounds__(512, 2) void k_attend_mfma(AttendArgs a, int type, 
         o[g][j] = mfma(v, lo, o[g][j]);
       }
     }
-    if (more) {
-      load_v(j0 + step, pg);
-      bad = bad_next;
-      if (j0 + 2 * step < last) load_ids(j0 + 2 * step);
+    __builtin_amdgcn_wave_barrier();
+  };
+
+  // Two tiles a turn, each staged from its own registers, which then take the tile after the next.
+  // Tiles past the end load the last slot again and are masked whole: without conditions in the
+  // loop the accumulators keep one set of registers.
+  auto turn = [&](int j0, Rows &t) {
+    stage(t);
+    uint64_t bad[kIds];
+#pragma unroll
+    for (int i = 0; i < kIds; ++i) bad[i] = t.bad[i];
+    load_rows(j0 + 2 * step, t);
+    compute(j0, bad);
+  };
+  const int j1 = first + wave * 32;
+  if (j1 < last) {
+    load_ids(j1);
+    load_rows(j1, t0);
+    load_rows(j1 + step, t1);
+#pragma unroll 1
+    for (int j0 = j1; j0 < last; j0 += 2 * step) {
+      turn(j0, t0);
+      turn(j0 + step, t1);
     }
   }
 
@@ -714,8 +733,8 @@ AttendPlan plan_attend(const StateView &c, const AttendCall &a) {
   p.cap = a.width << c.pshift;
   const int ng = c.dim / c.group, g = a.q_heads / c.heads;
   p.matrix = a.type != kStateF32 && (c.group == 32 || c.group == 64 || c.group == 128) &&
-             ng <= 4 && p.cap > 16 && p.cap < (int64_t(1) << 30) &&
-             c.pages < (int64_t(1) << 32);
+             (ng == 1 || ng == 2 || ng == 4) && p.cap > 16 && p.cap < (int64_t(1) << 30) &&
+             c.pages < (int64_t(1) << 31);
   int64_t chunk;
   if (p.matrix) {
     const int64_t work = a.rows * c.heads * ((g + 15) / 16);
@@ -723,7 +742,7 @@ AttendPlan plan_attend(const StateView &c, const AttendCall &a) {
     // 8 waves where the rows alone cannot fill the card, as far as LDS holds their outputs
     p.waves = work * ceil_div(p.cap, 512) <= 256 ? 8 : 4;
     while (p.waves > 4 && p.waves * gn * c.dim * 4 > 96 * 1024) p.waves >>= 1;
-    chunk = ceil_div(p.cap * work, 8192);
+    chunk = ceil_div(p.cap * work, 1024);
     const int64_t low = p.waves * 64 > 512 ? p.waves * 64 : 512;
     chunk = chunk < low ? low : (chunk + 127) & ~int64_t(127);
   } else {
@@ -774,20 +793,13 @@ void launch_mfma(const AttendArgs &a, const AttendPlan &p, int type, hipStream_t
   const int tiles = (a.g + 15) / 16, gn = a.g < 16 ? a.g : 16;
   const int64_t blocks = a.rows * a.c.heads * tiles * a.splits;
   DGS_CHECK(blocks < (int64_t(1) << 31), "attend: too many rows in one call");
-  const int join = 32 + gn * NG * GROUP, corner = 64 * NG;  // words a wave needs of LDS
+  const int join = 32 + gn * NG * GROUP, corner = 8 * NG * GROUP + 64 * NG;  // words a wave needs of LDS
   const size_t lds = (size_t)p.waves * (join > corner ? join : corner) * 4;
   const unsigned grid = (unsigned)blocks, threads = p.waves * 64;
-  if (a.c.pshift >= 4) {
-    if (type == kStateBF16)
-      k_attend_mfma<NG, GROUP, 1, true><<<grid, threads, lds, st>>>(a, type, tiles);
-    else
-      k_attend_mfma<NG, GROUP, 2, true><<<grid, threads, lds, st>>>(a, type, tiles);
-  } else {
-    if (type == kStateBF16)
-      k_attend_mfma<NG, GROUP, 1, false><<<grid, threads, lds, st>>>(a, type, tiles);
-    else
-      k_attend_mfma<NG, GROUP, 2, false><<<grid, threads, lds, st>>>(a, type, tiles);
-  }
+  if (type == kStateBF16)
+    k_attend_mfma<NG, GROUP, 1><<<grid, threads, lds, st>>>(a, type, tiles);
+  else
+    k_attend_mfma<NG, GROUP, 2><<<grid, threads, lds, st>>>(a, type, tiles);
   DGS_LAUNCH_CHECK();
 }
 template <int GROUP>
@@ -795,10 +807,7 @@ void launch_mfma_g(const AttendArgs &a, const AttendPlan &p, int type, hipStream
   switch (a.c.dim / GROUP) {
     case 1: launch_mfma<1, GROUP>(a, p, type, st); break;
     case 2: launch_mfma<2, GROUP>(a, p, type, st); break;
-    case 3:
-      if constexpr (GROUP < 128) launch_mfma<3, GROUP>(a, p, type, st);
-      break;
-    default:
+    case 4:
       if constexpr (GROUP < 128) launch_mfma<4, GROUP>(a, p, type, st);
   }
 }
