@@ -11,6 +11,7 @@
 //
 // A slot past the length, or on a page outside the cache (reported), has logit -inf, and its scale
 // and base are replaced by zeros before use: what lies there (NaN, infinities) is never multiplied.
+#include "dgs_lane.cuh"
 #include "dgs_state.cuh"
 
 namespace dgs {
@@ -50,10 +51,6 @@ __device__ __forceinline__ int64_t row_length(const AttendArgs &a, int64_t row, 
   return len;
 }
 
-template <int TYPE>
-__device__ __forceinline__ void store_row(void *out, int64_t elem, const float (&x)[8]) {
-  store8<TYPE>(out, elem, x);
-}
 __device__ __forceinline__ void store_out(int type, void *out, int64_t elem, const float (&x)[8]) {
   if (type == kStateF32)
     store8<kStateF32>(out, elem, x);
@@ -71,34 +68,49 @@ __device__ __forceinline__ void load_q(int type, const void *q, int64_t elem, fl
     load8<kStateF16>(q, elem, x);
 }
 
+template <int LPR>
+__device__ __forceinline__ float sum_lanes(float x) {
+  if constexpr (LPR >= 2) x += lane_xor32<1>(x);
+  if constexpr (LPR >= 4) x += lane_xor32<2>(x);
+  if constexpr (LPR >= 8) x += lane_xor32<4>(x);
+  if constexpr (LPR >= 16) x += lane_xor32<8>(x);
+  if constexpr (LPR >= 32) x += lane_xor32<16>(x);
+  return x;
+}
+
 // Vector form, for every type and size.  A work item is (row, head, GC query heads, split).  LPR
-// lanes hold a row (eight channels each), SL groups of them take every SL-th slot with a softmax
-// state of their own, joined at the end by exchanges between lanes.
+// lanes hold a row (eight channels each); SL groups of them take every SL-th slot with a softmax
+// state of their own, joined at the end by exchanges between lanes.  kU slots a group are loaded
+// while the kU before them are computed, ids another step ahead.  As in the matrix form, the
+// running maximum is only followed when a logit passes it by 8.
+// SL = 1 is for rows of at most 16 slots: no join, and with all query heads of a head in the item
+// the probabilities stay in registers and the item writes its weights itself.
 template <int LPR, int SL, int GC>
 __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type, int gchunks,
                                                          int64_t items) {
-  constexpr int kItem = LPR * SL, kU = SL == 1 ? 4 : 2;
+  constexpr int kItem = LPR * SL, kU = 4, kStep = SL * kU;
+  constexpr int kKeep = SL > 1 ? 1 : (LPR >= 16 ? 1 : 16 / LPR);
   const int lane = threadIdx.x & (kItem - 1);
-  int64_t item = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / kItem;
-  const bool here = item < items;
-  if (!here) return;  // whole items leave together: no exchange crosses an item
+  int64_t item64 = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / kItem;
+  if (item64 >= items) return;  // whole items leave together: no exchange crosses an item
+  uint32_t item = (uint32_t)item64;
   const int sub = lane % LPR, sl = lane / LPR;
-  const int split = (int)(item % a.splits);
-  item /= a.splits;
-  const int gc = (int)(item % gchunks);
-  item /= gchunks;
-  const int h = (int)(item % a.c.heads);
-  const int64_t row = item / a.c.heads;
+  const int split = (int)(item % (uint32_t)a.splits);
+  item /= (uint32_t)a.splits;
+  const int gc = (int)(item % (uint32_t)gchunks);
+  item /= (uint32_t)gchunks;
+  const int h = (int)(item % (uint32_t)a.c.heads);
+  const int64_t row = item / (uint32_t)a.c.heads;
   const int words = a.c.dim >> 3;
   const bool live = sub < words;
   const int w = live ? sub : 0, ng = a.c.dim / a.c.group, grp = 8 * w / a.c.group;
-  const int64_t len = row_length(a, row, split == 0 && h == 0 && gc == 0 && lane == 0);
-  const int64_t first = (int64_t)split * a.chunk;
+  const int len = (int)row_length(a, row, split == 0 && h == 0 && gc == 0 && lane == 0);
+  const int first = split * (int)a.chunk;
   if (split > 0 && first >= len) return;
-  const int64_t last = a.splits == 1 ? len : (first + a.chunk < len ? first + a.chunk : len);
+  const int last = a.splits == 1 ? len : (int)(first + a.chunk < len ? first + a.chunk : len);
   const int a0 = h * a.g + gc * GC, gn = a.g - gc * GC < GC ? a.g - gc * GC : GC;
 
-  float q[GC][8], o[GC][8], m[GC], l[GC];
+  float q[GC][8], o[GC][8], m[GC], l[GC], xs[kKeep][GC];
 #pragma unroll
   for (int g = 0; g < GC; ++g) {
     if (live && g < gn) {
@@ -114,59 +126,143 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
     }
     m[g] = -INFINITY;
     l[g] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kKeep; ++i) xs[i][g] = -INFINITY;
   }
-  const int64_t mask = (int64_t(1) << a.c.pshift) - 1;
-  for (int64_t j0 = first; j0 < last; j0 += SL * kU) {
-    uint32_t kq[kU], vq[kU], km[kU], vm[kU];
-    bool ok[kU];
+  const int ps = a.c.pshift, mask = (1 << ps) - 1;
+  const bool wide = a.table.bytes == 8;
+  const char *tab = (const char *)a.table.p + ((row * a.width) << (wide ? 3 : 2));
+  const uint32_t pages = (uint32_t)a.c.pages;
+  uint32_t id[kU], id_hi[kU];
+  struct Rows {
+    uint32_t kq[kU], vq[kU], km[kU], vm[kU], ok;
+  };
+  Rows t;
+  auto slot_of = [&](int j0, int u) {
+    const int j = j0 + u * SL + sl;
+    return j < last ? j : last - 1;
+  };
+  auto load_ids = [&](int j0) {
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      const int64_t j = j0 + u * SL + sl;
-      ok[u] = j < last;
-      const int64_t jj = ok[u] ? j : last - 1;
-      int64_t page = a.table[row * a.width + (jj >> a.c.pshift)];
-      if ((uint64_t)page >= (uint64_t)a.c.pages) {
-        if (ok[u] && sub == 0) report_bad_id(a.gd.err, kAsyncErrSlot, page, a.c.pages, a.gd.tag);
-        ok[u] = false;
-        page = 0;
-      }
-      const int64_t r = ((page * a.c.heads + h) << a.c.pshift) + (jj & mask);
-      kq[u] = *(const uint32_t *)(a.c.kc + r * (a.c.dim >> 1) + 4 * w);
-      vq[u] = *(const uint32_t *)(a.c.vc + r * (a.c.dim >> 1) + 4 * w);
-      km[u] = a.c.ks[r * ng + grp];
-      vm[u] = a.c.vs[r * ng + grp];
-      if (!ok[u] || !live) km[u] = vm[u] = 0;
+      const char *at = tab + ((int64_t)(slot_of(j0, u) >> ps) << (wide ? 3 : 2));
+      id[u] = *(const uint32_t *)at;
+      id_hi[u] = *(const uint32_t *)(at + (wide ? 4 : 0));
+    }
+  };
+  auto load_rows = [&](int j0) {
+    t.ok = 0;
+    uint32_t page[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const bool in = j0 + u * SL + sl < last;
+      const bool out = id[u] >= pages || (wide && id_hi[u] != 0);
+      if (out && in && sub == 0)
+        report_bad_id(a.gd.err, kAsyncErrSlot,
+                      wide ? (int64_t)((uint64_t)id_hi[u] << 32 | id[u]) : (int64_t)(int32_t)id[u],
+                      pages, a.gd.tag);
+      page[u] = out ? 0u : id[u];
+      t.ok |= (in && !out ? 1u : 0u) << u;
     }
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      float kv[8], vv[8];
-      codes8(kq[u], kv);
-      codes8(vq[u], vv);
-      const float ks = scale_of(km[u]), kb = base_of(km[u]);
-      const float vs = scale_of(vm[u]), vb = base_of(vm[u]);
+      const int64_t r = (((int64_t)page[u] * a.c.heads + h) << ps) + (slot_of(j0, u) & mask);
+      t.kq[u] = *(const uint32_t *)(a.c.kc + r * (a.c.dim >> 1) + 4 * w);
+      t.vq[u] = *(const uint32_t *)(a.c.vc + r * (a.c.dim >> 1) + 4 * w);
+      t.km[u] = a.c.ks[r * ng + grp];
+      t.vm[u] = a.c.vs[r * ng + grp];
+    }
+  };
+  auto compute = [&](const Rows &t, int j0, int keep) {
+    float x[GC][kU];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        kv[i] = __builtin_fmaf(kv[i], ks, kb);
-        vv[i] = __builtin_fmaf(vv[i], vs, vb);
-      }
+    for (int u = 0; u < kU; ++u) {
+      const bool ok = (t.ok >> u) & 1;
+      const uint32_t km = live ? t.km[u] : 0u;
+      const float ks = scale_of(km), kb = base_of(km);
+      float kv[8];
+      codes8(t.kq[u], kv);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) kv[i] = __builtin_fmaf(kv[i], ks, kb);
 #pragma unroll
       for (int g = 0; g < GC; ++g) {
-        float x = 0.f;
+        float s = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x = __builtin_fmaf(q[g][i], kv[i], x);
+        for (int i = 0; i < 8; ++i) s = __builtin_fmaf(q[g][i], kv[i], s);
+        s = sum_lanes<LPR>(s);
+        x[g][u] = ok ? s : -INFINITY;
+      }
+    }
+    if (SL == 1) {
 #pragma unroll
-        for (int s = LPR >> 1; s > 0; s >>= 1) x += __shfl_xor(x, s, 64);
-        if (!ok[u]) x = -INFINITY;
-        if (a.logits && sub == 0 && g < gn && j0 + u * SL + sl < last)
-          a.logits[(row * a.q_heads + a0 + g) * a.cap + j0 + u * SL + sl] = x;
-        const float mn = fmaxf(m[g], x);
-        const float ms = mn == -INFINITY ? 0.f : mn;
-        const float f = __builtin_amdgcn_exp2f(m[g] - ms);
-        const float p = __builtin_amdgcn_exp2f(x - ms);
-        m[g] = mn;
-        l[g] = __builtin_fmaf(l[g], f, p);
+      for (int u = 0; u < kU; ++u)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[g][i] = __builtin_fmaf(p, vv[i], o[g][i] * f);
+        for (int i = 0; i < kKeep; ++i)
+          if ((keep + u) / LPR == i && (keep + u) % LPR == sub)
+#pragma unroll
+            for (int g = 0; g < GC; ++g) xs[i][g] = x[g][u];
+    }
+    if (a.logits && sub == 0) {
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+        if (j0 + u * SL + sl < last)
+#pragma unroll
+          for (int g = 0; g < GC; ++g)
+            if (g < gn) a.logits[(row * a.q_heads + a0 + g) * a.cap + j0 + u * SL + sl] = x[g][u];
+    }
+#pragma unroll
+    for (int g = 0; g < GC; ++g) {
+      float top = fmaxf(fmaxf(x[g][0], x[g][1]), fmaxf(x[g][2], x[g][3]));
+      if (top > m[g] + 8.f) {
+        const float f = __builtin_amdgcn_exp2f(m[g] - top);
+        m[g] = top;
+        l[g] *= f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[g][i] *= f;
+      }
+      const float ms = m[g] == -INFINITY ? 0.f : m[g];
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        x[g][u] = __builtin_amdgcn_exp2f(x[g][u] - ms);
+        l[g] += x[g][u];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const uint32_t vm = live && ((t.ok >> u) & 1) ? t.vm[u] : 0u;
+      const float vs = scale_of(vm), vb = base_of(vm);
+      float vv[8];
+      codes8(t.vq[u], vv);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) vv[i] = __builtin_fmaf(vv[i], vs, vb);
+#pragma unroll
+      for (int g = 0; g < GC; ++g)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[g][i] = __builtin_fmaf(x[g][u], vv[i], o[g][i]);
+    }
+  };
+  if (first < last) {
+    load_ids(first);
+    load_rows(first);
+    load_ids(first + kStep);
+    if constexpr (SL == 1) {
+#pragma unroll
+      for (int st = 0; st < 4; ++st) {
+        if (4 * st >= last) break;
+        const Rows now = t;
+        if (4 * st + 4 < last) {
+          load_rows(4 * st + 4);
+          load_ids(4 * st + 8);
+        }
+        compute(now, 4 * st, 4 * st);
+      }
+    } else {
+#pragma unroll 1
+      for (int j0 = first; j0 < last; j0 += kStep) {
+        const Rows now = t;
+        load_rows(j0 + kStep);
+        load_ids(j0 + 2 * kStep);
+        compute(now, j0, 0);
       }
     }
   }
@@ -193,6 +289,24 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
       store_out(type, a.out, qh * a.c.dim + 8 * w, o[g]);
     }
     if (a.part_ml && sub == 0) a.part_ml[qh * a.splits + split] = make_float2(m[g], l[g]);
+  }
+  if constexpr (SL == 1) {
+    if (a.weights && !a.logits) {  // every query head of this head is here
+      float *wr = a.weights + (row * a.c.heads + h) * a.weights_cols;
+#pragma unroll
+      for (int i = 0; i < kKeep; ++i) {
+        const int j = i * LPR + sub;
+        if (j >= len) continue;
+        float sum = 0.f;
+#pragma unroll
+        for (int g = 0; g < GC; ++g)
+          if (g < gn) {
+            const float ms = m[g] == -INFINITY ? 0.f : m[g];
+            sum += __builtin_amdgcn_exp2f(xs[i][g] - ms) * (1.f / l[g]);
+          }
+        wr[j] = a.decay != 0.f ? sum + a.decay * wr[j] : sum;
+      }
+    }
   }
 }
 
@@ -651,69 +765,97 @@ __global__ __launch_bounds__(512, 2) void k_attend_mfma(AttendArgs a, int type, 
   }
 }
 
-// Joins the splits of a row's head into the output and adds the weights.  Block (x, y): x =
-// (row, head), y = a range of slots of the weights; y = 0 also writes the output.
+// The maximum and 1 / sum of a query head over its splits, on every lane of the wave.
+__device__ __forceinline__ float2 join_ml(const AttendArgs &a, int64_t qh, int splits, bool empty) {
+  const float2 *ml = a.part_ml + qh * a.splits;
+  float m = -INFINITY, l = 0.f;
+  const int lane = threadIdx.x & 63;
+  if (splits == 1) {
+    m = ml[0].x;
+    l = ml[0].y;
+  } else {
+    for (int s = lane; s < splits; s += 64) m = fmaxf(m, ml[s].x);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    const float ms = m == -INFINITY ? 0.f : m;
+    for (int s = lane; s < splits; s += 64) l += ml[s].y * __builtin_amdgcn_exp2f(ml[s].x - ms);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
+  }
+  return make_float2(m == -INFINITY ? 0.f : m, empty ? 0.f : 1.f / l);
+}
+
+// Joins the splits of the rows' query heads and adds the weights; every wave works alone.  The
+// first `outs` waves take a query head's output each (eight channels a lane, the lanes' groups
+// taking every n-th split), the others 256 slots of a (row, head)'s weights.
+constexpr int kSpan = 256;
 template <int TYPE>
-__global__ __launch_bounds__(kThreads) void k_attend_finish(AttendArgs a, int64_t span) {
-  __shared__ float2 s_ml[64];
-  const int64_t row = blockIdx.x / a.c.heads;
-  const int h = (int)(blockIdx.x % a.c.heads);
+__global__ __launch_bounds__(kThreads) void k_attend_finish(AttendArgs a, int64_t outs,
+                                                            int spans, int64_t waves) {
+  const int64_t id = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+  if (id >= waves) return;
+  const int lane = threadIdx.x & 63;
+  if (id < outs) {
+    const int64_t row = id / a.q_heads;
+    const int64_t len = row_length(a, row, false);
+    const int splits = (int)(len == 0 ? 1 : (len + a.chunk - 1) / a.chunk);  // that were written
+    const float2 ml = join_ml(a, id, splits, len == 0);
+    const int words = a.c.dim >> 3;
+    int lpr = 1;
+    while (lpr < words) lpr <<= 1;
+    const int w = lane & (lpr - 1), part = lane / lpr, parts = 64 / lpr;
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (w < words && len > 0)
+      for (int s = part; s < splits; s += parts) {
+        const float f = __builtin_amdgcn_exp2f(a.part_ml[id * a.splits + s].x - ml.x);
+        float x[8];
+        load8<kStateF32>(a.part_o, (id * a.splits + s) * a.c.dim + 8 * w, x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] = __builtin_fmaf(x[i], f, acc[i]);
+      }
+    for (int o = lpr; o < 64; o <<= 1)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] += __shfl_xor(acc[i], o, 64);
+    if (part == 0 && w < words) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] *= ml.y;
+      store8<TYPE>(a.out, id * a.c.dim + 8 * w, acc);
+    }
+    return;
+  }
+  const int64_t pair = (id - outs) / spans;
+  const int64_t row = pair / a.c.heads;
   const int64_t len = row_length(a, row, false);
-  const int64_t j0 = (int64_t)blockIdx.y * span;
-  if (blockIdx.y > 0 && j0 >= len) return;
-  const int splits = (int)(len == 0 ? 1 : (len + a.chunk - 1) / a.chunk);  // that were written
-  const int tid = threadIdx.x;
-  const int wave = tid >> 6, lane = tid & 63;
-  for (int gb = 0; gb < a.g; gb += 64) {
-    const int gn = a.g - gb < 64 ? a.g - gb : 64;
-    const int64_t q0 = row * a.q_heads + h * a.g + gb;
-    for (int g = wave; g < gn; g += kThreads / 64) {
-      const float2 *ml = a.part_ml + (q0 + g) * a.splits;
-      float m = -INFINITY;
-      bool nan = false;
-      for (int s = lane; s < splits; s += 64) m = fmaxf(m, ml[s].x);
+  const int64_t j0 = (id - outs) % spans * kSpan;
+  if (j0 >= len) return;
+  const int splits = (int)((len + a.chunk - 1) / a.chunk);
+  const int64_t q0 = pair * a.g;  // the head's first query head: row * q_heads + h * g
+  float sum[kSpan / 64] = {0.f, 0.f, 0.f, 0.f};
+  constexpr int kG = 4;
+  for (int g0 = 0; g0 < a.g; g0 += kG) {
+    float x[kG][kSpan / 64];
+    float2 ml[kG];
 #pragma unroll
-      for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-      const float ms = m == -INFINITY ? 0.f : m;
-      float l = 0.f;
-      for (int s = lane; s < splits; s += 64)
-        l += ml[s].y * __builtin_amdgcn_exp2f(ml[s].x - ms);
+    for (int g = 0; g < kG; ++g)
 #pragma unroll
-      for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
-      (void)nan;
-      const float inv = len == 0 ? 0.f : 1.f / l;
-      if (lane == 0) s_ml[g] = make_float2(ms, inv);
-      if (a.splits > 1 && blockIdx.y == 0) {
-        for (int w = lane; w < (a.c.dim >> 3); w += 64) {
-          float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, x[8];
-          for (int s = 0; s < splits && len > 0; ++s) {
-            const float f = __builtin_amdgcn_exp2f(ml[s].x - ms);
-            load8<kStateF32>(a.part_o, ((q0 + g) * a.splits + s) * a.c.dim + 8 * w, x);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) acc[i] = __builtin_fmaf(x[i], f, acc[i]);
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) acc[i] *= inv;
-          store8<TYPE>(a.out, (q0 + g) * a.c.dim + 8 * w, acc);
-        }
+      for (int i = 0; i < kSpan / 64; ++i) {
+        const int64_t j = j0 + 64 * i + lane;
+        x[g][i] = g0 + g < a.g && j < len ? a.logits[(q0 + g0 + g) * a.cap + j] : 0.f;
       }
-    }
-    __syncthreads();
-    if (a.weights) {
-      float *wr = a.weights + (row * a.c.heads + h) * a.weights_cols;
-      const int64_t jn = j0 + span < len ? j0 + span : len;
-      for (int64_t j = j0 + tid; j < jn; j += kThreads) {
-        float sum = 0.f;
-        for (int g = 0; g < gn; ++g)
-          sum += __builtin_amdgcn_exp2f(a.logits[(q0 + g) * a.cap + j] - s_ml[g].x) * s_ml[g].y;
-        if (gb > 0)
-          sum += wr[j];
-        else if (a.decay != 0.f)
-          sum += a.decay * wr[j];
-        wr[j] = sum;
-      }
-    }
-    __syncthreads();
+#pragma unroll
+    for (int g = 0; g < kG; ++g)
+      ml[g] = g0 + g < a.g ? join_ml(a, q0 + g0 + g, splits, false) : make_float2(0.f, 0.f);
+#pragma unroll
+    for (int g = 0; g < kG; ++g)
+#pragma unroll
+      for (int i = 0; i < kSpan / 64; ++i)
+        if (g0 + g < a.g) sum[i] += __builtin_amdgcn_exp2f(x[g][i] - ml[g].x) * ml[g].y;
+  }
+  float *wr = a.weights + pair * a.weights_cols;
+#pragma unroll
+  for (int i = 0; i < kSpan / 64; ++i) {
+    const int64_t j = j0 + 64 * i + lane;
+    if (j < len) wr[j] = a.decay != 0.f ? sum[i] + a.decay * wr[j] : sum[i];
   }
 }
 
@@ -728,13 +870,16 @@ struct AttendPlan {
 
 int64_t up256(int64_t x) { return (x + 255) & ~int64_t(255); }
 
+// Query heads of a work item of the vector form, and items a head needs.
+int vec_gc(int g) { return g >= 4 ? 4 : (g >= 2 ? 2 : 1); }
+int vec_gchunks(int g) { return (g + vec_gc(g) - 1) / vec_gc(g); }
+
 AttendPlan plan_attend(const StateView &c, const AttendCall &a) {
   AttendPlan p{};
   p.cap = a.width << c.pshift;
   const int ng = c.dim / c.group, g = a.q_heads / c.heads;
   p.matrix = a.type != kStateF32 && (c.group == 32 || c.group == 64 || c.group == 128) &&
-             (ng == 1 || ng == 2 || ng == 4) && p.cap > 16 && p.cap < (int64_t(1) << 30) &&
-             c.pages < (int64_t(1) << 31);
+             (ng == 1 || ng == 2 || ng == 4) && p.cap > 16;
   int64_t chunk;
   if (p.matrix) {
     const int64_t work = a.rows * c.heads * ((g + 15) / 16);
@@ -746,16 +891,17 @@ AttendPlan plan_attend(const StateView &c, const AttendCall &a) {
     const int64_t low = p.waves * 64 > 512 ? p.waves * 64 : 512;
     chunk = chunk < low ? low : (chunk + 127) & ~int64_t(127);
   } else {
-    // enough waves to fill the card (256 CUs x 16), of at least 64 slots each
-    chunk = ceil_div(p.cap * a.rows * c.heads, 4096);
+    chunk = ceil_div(p.cap * a.rows * c.heads * vec_gchunks(g), 16384);
     chunk = chunk < 64 ? 64 : (chunk + 63) & ~int64_t(63);
   }
   p.splits = (int)(p.cap <= chunk ? 1 : ceil_div(p.cap, chunk));
   p.chunk = p.splits == 1 ? (p.cap > 0 ? p.cap : 1) : chunk;
   const int64_t qh = a.rows * a.q_heads;
   if (p.splits > 1) p.o_bytes = up256(qh * p.splits * c.dim * 4);
-  if (p.splits > 1 || a.weights) p.ml_bytes = up256(qh * p.splits * 8);
-  if (a.weights) p.logit_bytes = up256(qh * p.cap * 4);
+  // short rows of the vector form write their weights themselves
+  const bool later = a.weights && !(!p.matrix && p.cap <= 16 && vec_gchunks(g) == 1);
+  if (p.splits > 1 || later) p.ml_bytes = up256(qh * p.splits * 8);
+  if (later) p.logit_bytes = up256(qh * p.cap * 4);
   return p;
 }
 
@@ -767,11 +913,11 @@ int pow2_at_least(int x) {
 
 template <int LPR, int SL>
 void launch_vec_g(const AttendArgs &a, int type, hipStream_t st) {
-  const int gc = a.g >= 4 ? 4 : (a.g >= 2 ? 2 : 1);
-  const int gchunks = (a.g + gc - 1) / gc;
+  const int gc = vec_gc(a.g), gchunks = vec_gchunks(a.g);
   const int64_t items = a.rows * a.c.heads * gchunks * a.splits;
   const int64_t blocks = ceil_div(items * LPR * SL, kThreads);
-  DGS_CHECK(blocks < (int64_t(1) << 31), "attend: too many rows in one call");
+  DGS_CHECK(blocks < (int64_t(1) << 31) && items < (int64_t(1) << 31),
+            "attend: too many rows in one call");
   if (gc == 4)
     k_attend_vec<LPR, SL, 4><<<(unsigned)blocks, kThreads, 0, st>>>(a, type, gchunks, items);
   else if (gc == 2)
@@ -825,6 +971,8 @@ void state_attend(const StateView &c, const AttendCall &call, void *ws, int64_t 
   const AttendPlan p = plan_attend(c, call);
   const int64_t need = p.o_bytes + p.ml_bytes + p.logit_bytes;
   DGS_CHECK(ws_bytes >= need && (need == 0 || ws), "attend: workspace too small");
+  DGS_CHECK(p.cap < (int64_t(1) << 30) && c.pages < (int64_t(1) << 31),
+            "attend: rows of 2^30 slots or caches of 2^31 pages");
   AttendArgs a{};
   a.c = c;
   a.q = call.q;
@@ -865,20 +1013,19 @@ void state_attend(const StateView &c, const AttendCall &call, void *ws, int64_t 
     default: launch_vec<32>(a, call.type, st); break;
   }
   if (!a.part_ml) return;
-  const int64_t pairs = call.rows * c.heads;
-  DGS_CHECK(pairs < (int64_t(1) << 31), "attend: too many rows in one call");
-  // slots of one finishing block: all of a short row, else 1024
-  const int64_t span = 1024;
-  int64_t ny = call.weights ? ceil_div(p.cap, span) : 1;
-  if (ny < 1) ny = 1;
-  DGS_CHECK(ny < 65536, "attend: rows longer than 67 million slots");
-  const dim3 grid((unsigned)pairs, (unsigned)ny);
+  const int64_t outs = p.splits > 1 ? call.rows * call.q_heads : 0;
+  const int spans = p.logit_bytes ? (int)ceil_div(p.cap, kSpan) : 0;
+  const int64_t waves = outs + call.rows * c.heads * spans;
+  const int64_t blocks = ceil_div(waves, kThreads / 64);
+  if (blocks == 0) return;
+  DGS_CHECK(blocks < (int64_t(1) << 31), "attend: too many rows in one call");
+  const unsigned grid = (unsigned)blocks;
   if (call.type == kStateF32)
-    k_attend_finish<kStateF32><<<grid, kThreads, 0, st>>>(a, span);
+    k_attend_finish<kStateF32><<<grid, kThreads, 0, st>>>(a, outs, spans, waves);
   else if (call.type == kStateBF16)
-    k_attend_finish<kStateBF16><<<grid, kThreads, 0, st>>>(a, span);
+    k_attend_finish<kStateBF16><<<grid, kThreads, 0, st>>>(a, outs, spans, waves);
   else
-    k_attend_finish<kStateF16><<<grid, kThreads, 0, st>>>(a, span);
+    k_attend_finish<kStateF16><<<grid, kThreads, 0, st>>>(a, outs, spans, waves);
   DGS_LAUNCH_CHECK();
 }
 
