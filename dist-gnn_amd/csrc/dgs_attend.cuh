@@ -19,7 +19,7 @@ struct AttendArgs {
   int64_t chunk;  // slots per split
   int splits;
   float *part_o;   // [rows, q_heads, splits, dim], unnormalised (splits > 1)
-  float2 *part_ml;  // [rows, q_heads, splits] (splits > 1 or weights)
+  float2 *part_ml;  // [rows, q_heads, splits] (splits > 1, or weights are added by the finishing kernel)
   float *logits;   // [rows, q_heads, cap] (weights)
   int64_t cap;     // width << pshift
   float *weights;
@@ -203,58 +203,6 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
   uint32_t magic = 0x43004300u;
   asm volatile("" : "+v"(magic));
 
-  // q in bfloat16 terms, in the order in which code_pair() yields a word's channels: 0 4 1 5 2 6 3 7
-  Op qv[QT][kC], qm;
-  float qsum[NG];
-#pragma unroll
-  for (int g = 0; g < NG; ++g) qsum[g] = 0.f;
-#pragma unroll
-  for (int c = 0; c < kC; ++c) {
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (n < gn)
-      load_q(type, a.q, row * a.q_row + (h * a.g + rt * 16 + n) * a.q_head + 32 * c + 8 * q4, x);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[i] *= sign;
-      qsum[c / kGC] += x[i];
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t hi = pack_bf16(x[i], x[4 + i]);
-      qv[0][c].u[i] = hi;
-      if constexpr (QT == 2)
-        qv[1][c].u[i] = pack_bf16(x[i] - __uint_as_float(hi << 16),
-                                  x[4 + i] - __uint_as_float(hi & 0xffff0000u));
-    }
-  }
-  // quarter 0 holds the first bfloat16 terms of (-128 Q_g, Q_g), 1 the second, 2 the third
-#pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    qm.u[g] = 0;
-    if (g < NG) {
-      float s = qsum[g < NG ? g : 0];
-      s += xor16(s);
-      s += xor32(s);
-      const float t0 = (float)(__bf16)s, t1 = (float)(__bf16)(s - t0);
-      const float t2 = (s - t0) - t1;
-      const float t = q4 == 0 ? t0 : (q4 == 1 ? t1 : (q4 == 2 ? t2 : 0.f));
-      qm.u[g] = pack_bf16(-128.f * t, t);
-    }
-  }
-
-  f32x4 o[NG][kU], co[NG];
-  float cb[NG], m = -INFINITY, ms = 0.f, l = 0.f;  // m, ms: in base 2, of head n % GR
-#pragma unroll
-  for (int g = 0; g < NG; ++g) {
-    co[g] = f32x4{0.f, 0.f, 0.f, 0.f};
-    cb[g] = 0.f;
-#pragma unroll
-    for (int j = 0; j < kU; ++j) o[g][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  Op ones;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) ones.u[i] = 0x43004300u;  // 128, the codes' offset
-
   const int ps = a.c.pshift, mask = (1 << ps) - 1;
   const int64_t trow = row * a.width;
   const int unit = n * (GROUP / 32);  // byte of this lane's unit of V in a group's codes
@@ -376,6 +324,66 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
     }
     __builtin_amdgcn_wave_barrier();
   };
+  // the first tiles, then the query: its loads and arithmetic run while the rows are on their way
+  const int j1 = first + wave * 32;
+  if (j1 < last) {
+    load_ids(j1);
+    load_rows(j1, t0);
+    load_rows(j1 + step, t1);
+  }
+
+  // q in bfloat16 terms, in the order in which code_pair() yields a word's channels: 0 4 1 5 2 6 3 7
+  Op qv[QT][kC], qm;
+  float qsum[NG];
+#pragma unroll
+  for (int g = 0; g < NG; ++g) qsum[g] = 0.f;
+#pragma unroll
+  for (int c = 0; c < kC; ++c) {
+    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (n < gn)
+      load_q(type, a.q, row * a.q_row + (h * a.g + rt * 16 + n) * a.q_head + 32 * c + 8 * q4, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[i] *= sign;
+      qsum[c / kGC] += x[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t hi = pack_bf16(x[i], x[4 + i]);
+      qv[0][c].u[i] = hi;
+      if constexpr (QT == 2)
+        qv[1][c].u[i] = pack_bf16(x[i] - __uint_as_float(hi << 16),
+                                  x[4 + i] - __uint_as_float(hi & 0xffff0000u));
+    }
+  }
+  // quarter 0 holds the first bfloat16 terms of (-128 Q_g, Q_g), 1 the second, 2 the third
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    qm.u[g] = 0;
+    if (g < NG) {
+      float s = qsum[g < NG ? g : 0];
+      s += xor16(s);
+      s += xor32(s);
+      const float t0 = (float)(__bf16)s, t1 = (float)(__bf16)(s - t0);
+      const float t2 = (s - t0) - t1;
+      const float t = q4 == 0 ? t0 : (q4 == 1 ? t1 : (q4 == 2 ? t2 : 0.f));
+      qm.u[g] = pack_bf16(-128.f * t, t);
+    }
+  }
+
+  f32x4 o[NG][kU], co[NG];
+  float cb[NG], m = -INFINITY, ms = 0.f, l = 0.f;  // m, ms: in base 2, of head n % GR
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    co[g] = f32x4{0.f, 0.f, 0.f, 0.f};
+    cb[g] = 0.f;
+#pragma unroll
+    for (int j = 0; j < kU; ++j) o[g][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  Op ones;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) ones.u[i] = 0x43004300u;  // 128, the codes' offset
+
   // word g of this lane's slot v
   auto word_at = [&](const uint32_t *w, int v, int g) {
     return w[(GR == 16 ? 16 * (v >> 2) + (v & 3) : v) * NG + g];
@@ -528,11 +536,7 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
     load_rows(j0 + 2 * step, t);
     compute(j0, bad);
   };
-  const int j1 = first + wave * 32;
   if (j1 < last) {
-    load_ids(j1);
-    load_rows(j1, t0);
-    load_rows(j1 + step, t1);
 #pragma unroll 1
     for (int j0 = j1; j0 < last; j0 += 2 * step) {
       turn(j0, t0);
@@ -590,6 +594,30 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
       for (int w = 0; w < waves; ++w) mm = fmaxf(mm, s_m[w * 16 + hd]);
       a.part_ml[(qh0 + hd) * a.splits + split] = make_float2(mm, ls);
     }
+  }
+  if (!a.logits || a.part_ml) return;
+  // The row and all its query heads are this workgroup's: it adds the weights from the logits
+  // that it has just written (visible to it after the barriers above).
+  float mh[GR], ih[GR];
+#pragma unroll
+  for (int g = 0; g < GR; ++g) {
+    float mm = -INFINITY, ls = 0.f;
+    if (g < gn)
+      for (int w = 0; w < waves; ++w) {
+        mm = fmaxf(mm, s_m[w * 16 + g]);
+        ls += s_l[w * 16 + g];
+      }
+    mh[g] = g < gn ? (mm == -INFINITY ? 0.f : mm) : INFINITY;  // no head: exp2(-inf) * 0
+    ih[g] = g < gn ? 1.f / ls : 0.f;
+  }
+  const float *lg = a.logits + qh0 * a.cap;
+  float *wr = a.weights + (row * a.c.heads + h) * a.weights_cols;
+  for (int j = threadIdx.x; j < len; j += blockDim.x) {
+    float sum = 0.f;
+#pragma unroll
+    for (int g = 0; g < GR; ++g)
+      sum += __builtin_amdgcn_exp2f(lg[(g < gn ? g : 0) * a.cap + j] - mh[g]) * ih[g];
+    wr[j] = a.decay != 0.f ? sum + a.decay * wr[j] : sum;
   }
 }
 

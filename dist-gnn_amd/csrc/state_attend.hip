@@ -326,33 +326,32 @@ __global__ __launch_bounds__(kThreads) void k_attend_finish(AttendArgs a, int64_
   if (j0 >= len) return;
   const int splits = (int)((len + a.chunk - 1) / a.chunk);
   const int64_t q0 = pair * a.g;  // the head's first query head: row * q_heads + h * g
-  float sum[kSpan / 64] = {0.f, 0.f, 0.f, 0.f};
-  constexpr int kG = 4;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  // lane t takes slots j0 + t, + 64, + 128, + 192; a slot past the end reads the last one
+  int64_t j[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) j[i] = j0 + 64 * i + lane < len ? j0 + 64 * i + lane : len - 1;
+  constexpr int kG = 4;  // heads whose loads are in flight together
   for (int g0 = 0; g0 < a.g; g0 += kG) {
-    float x[kG][kSpan / 64];
-    float2 ml[kG];
+    float x[kG][4];
 #pragma unroll
-    for (int g = 0; g < kG; ++g)
+    for (int g = 0; g < kG; ++g) {
+      const float *lg = a.logits + (q0 + (g0 + g < a.g ? g0 + g : g0)) * a.cap;
 #pragma unroll
-      for (int i = 0; i < kSpan / 64; ++i) {
-        const int64_t j = j0 + 64 * i + lane;
-        x[g][i] = g0 + g < a.g && j < len ? a.logits[(q0 + g0 + g) * a.cap + j] : 0.f;
-      }
+      for (int i = 0; i < 4; ++i) x[g][i] = lg[j[i]];
+    }
 #pragma unroll
-    for (int g = 0; g < kG; ++g)
-      ml[g] = g0 + g < a.g ? join_ml(a, q0 + g0 + g, splits, false) : make_float2(0.f, 0.f);
+    for (int g = 0; g < kG; ++g) {
+      if (g0 + g >= a.g) break;
+      const float2 ml = join_ml(a, q0 + g0 + g, splits, false);
 #pragma unroll
-    for (int g = 0; g < kG; ++g)
-#pragma unroll
-      for (int i = 0; i < kSpan / 64; ++i)
-        if (g0 + g < a.g) sum[i] += __builtin_amdgcn_exp2f(x[g][i] - ml[g].x) * ml[g].y;
+      for (int i = 0; i < 4; ++i) sum[i] += __builtin_amdgcn_exp2f(x[g][i] - ml.x) * ml.y;
+    }
   }
   float *wr = a.weights + pair * a.weights_cols;
 #pragma unroll
-  for (int i = 0; i < kSpan / 64; ++i) {
-    const int64_t j = j0 + 64 * i + lane;
-    if (j < len) wr[j] = a.decay != 0.f ? sum[i] + a.decay * wr[j] : sum[i];
-  }
+  for (int i = 0; i < 4; ++i)
+    if (j0 + 64 * i + lane < len) wr[j[i]] = a.decay != 0.f ? sum[i] + a.decay * wr[j[i]] : sum[i];
 }
 
 struct AttendPlan {
@@ -361,6 +360,7 @@ struct AttendPlan {
   int64_t chunk;
   int splits;
   int64_t cap;
+  bool finish;  // the finishing kernel runs
   int64_t o_bytes, ml_bytes, logit_bytes;
 };
 
@@ -384,8 +384,11 @@ AttendPlan plan_attend(const StateView &c, const AttendCall &a) {
     p.waves = work * ceil_div(p.cap, 512) <= 256 && c.dim < 256 ? 8 : 4;
     while (p.waves > 1 && p.waves * attend_matrix_lds(c.dim, c.group, g) * 4 > 64 * 1024)
       p.waves >>= 1;
-    chunk = ceil_div(p.cap * work, 1024);
-    const int64_t low = p.waves * 64 > 512 ? p.waves * 64 : 512;
+    // One round of workgroups (two a CU): starting one takes as long as some tiles, three loads
+    // that wait for each other.  64 rows of up to 8192 slots: 93 us in 512 workgroups, 104 in
+    // 1024, 117 in 2048; 8 rows of 131072: 216, 227, 230 us.
+    chunk = ceil_div(p.cap * work, 512);
+    const int64_t low = p.waves == 8 ? 1024 : 512;
     chunk = chunk < low ? low : (chunk + 127) & ~int64_t(127);
   } else {
     chunk = ceil_div(p.cap * a.rows * c.heads * vec_gchunks(g), 16384);
@@ -395,10 +398,14 @@ AttendPlan plan_attend(const StateView &c, const AttendCall &a) {
   p.chunk = p.splits == 1 ? (p.cap > 0 ? p.cap : 1) : chunk;
   const int64_t qh = a.rows * a.q_heads;
   if (p.splits > 1) p.o_bytes = up256(qh * p.splits * c.dim * 4);
-  // short rows of the vector form write their weights themselves
-  const bool later = a.weights && !(!p.matrix && p.cap <= 16 && vec_gchunks(g) == 1);
-  if (p.splits > 1 || later) p.ml_bytes = up256(qh * p.splits * 8);
-  if (later) p.logit_bytes = up256(qh * p.cap * 4);
+  // An item or workgroup that has a row and all its query heads to itself adds its weights itself:
+  // in the vector form from registers, in the matrix form from the logits it wrote (a long row
+  // would be a tail: 8192 slots 38 us, the finishing kernel 17).
+  const bool own_m = p.matrix && p.splits == 1 && g <= 16 && p.cap <= 1024;
+  const bool own_v = !p.matrix && p.cap <= 16 && vec_gchunks(g) == 1;
+  p.finish = p.splits > 1 || (a.weights && !own_m && !own_v);
+  if (p.finish) p.ml_bytes = up256(qh * p.splits * 8);
+  if (a.weights && !own_v) p.logit_bytes = up256(qh * p.cap * 4);
   return p;
 }
 
@@ -481,7 +488,7 @@ void state_attend(const StateView &c, const AttendCall &call, void *ws, int64_t 
     case 16: launch_vec<16>(a, call.type, st); break;
     default: launch_vec<32>(a, call.type, st); break;
   }
-  if (!a.part_ml) return;
+  if (!p.finish) return;
   const int64_t outs = p.splits > 1 ? call.rows * call.q_heads : 0;
   const int spans = p.logit_bytes ? (int)ceil_div(p.cap, kSpan) : 0;
   const int64_t waves = outs + call.rows * c.heads * spans;
