@@ -8,9 +8,11 @@
 // overlap, every move is independent, and only the rows that must move do (one a head when a full
 // cache took one token).  Weights and positions go to new arrays; the rows move in place.
 //
-// The plan, one workgroup per (row, head): the budget-th best key by counting digits (keys are 32
-// bits, larger is better, kept in LDS), then the slots in order, every wave a run of them: ties,
-// holes and movers are numbered by counting lanes, so that three barriers join the waves.
+// The plan, one workgroup per (row, head): weights and positions are read once, four slots a load,
+// and stay in registers as keys (32 bits, larger is better; rows past 32768 slots read them again
+// each time); the budget-th best key by counting digits; then ties, holes and movers are numbered in
+// slot order by counting lanes, the waves' counts joined by a scan.  What lies below the budget is
+// copied as it passes and the holes are overwritten afterwards.
 // The moves are a kernel of their own, over all stores; where there can only be a few (a cache
 // that takes single tokens) the plan's workgroup does them.
 #include "dgs_block.cuh"
@@ -21,7 +23,7 @@ namespace {
 
 constexpr int kMoveThreads = 256;
 constexpr int kDigits = 2048;  // 11 bits: the sign, the exponent and two bits of the mantissa first
-constexpr int kMaxKeys = 32768;  // keys that fit LDS (128 KB of 160)
+constexpr int kVecs = 8;  // loads of four slots a thread keeps
 constexpr int kFewMoves = 32;
 
 struct EvictArgs {
@@ -87,71 +89,169 @@ __device__ __forceinline__ void move_store(const EvictStore &st, const int64_t (
     move_rows<uint8_t, kU>(st, s, d, sub, lg);
 }
 
-// FUSED: this workgroup moves the rows too.
-template <int THREADS, bool IN_LDS, bool FUSED>
-__global__ __launch_bounds__(THREADS) void k_evict_plan(EvictArgs a) {
-  constexpr int kWaves = THREADS / 64, kOwn = kDigits / THREADS;
-  extern __shared__ uint32_t s_key[];
-  __shared__ uint32_t s_hist[kDigits];
-  __shared__ uint32_t s_scan[kWaves], s_cnt[3][kWaves];
-  __shared__ int32_t s_max[kWaves];
-  __shared__ uint32_t s_digit, s_left;
+// What both plans share: the row's sizes, the slots that no eviction touches, its outputs.
+struct PlanRow {
+  int64_t pair, row;
+  int h, n, cols, budget, keep;
+  const float *w;
+  const int32_t *pos;
+  float *wo;
+  int32_t *po;
+};
+template <int THREADS>
+__device__ __forceinline__ PlanRow plan_row(const EvictArgs &a) {
   const EvictCall &e = a.e;
-  const int64_t pair = blockIdx.x;
-  const int64_t row = pair / e.heads;
-  const int h = (int)(pair % e.heads);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int n = evict_length(a, row, tid == 0 && h == 0), cols = (int)e.cols;
-  const float *w = e.weights + pair * e.cols;
-  const int32_t *pos = e.positions ? e.positions + pair * e.cols : nullptr;
-  float *wo = e.weights_out + pair * e.cols;
-  int32_t *po = e.positions_out + pair * e.cols;
-  const int budget = (int)(e.budget < cols ? e.budget : cols);
-  const int keep = n < budget ? n : budget;
-  if (tid == 0) {
-    if (h == 0) {
+  PlanRow r;
+  r.pair = blockIdx.x;
+  r.row = r.pair / e.heads;
+  r.h = (int)(r.pair % e.heads);
+  r.n = evict_length(a, r.row, threadIdx.x == 0 && r.h == 0);
+  r.cols = (int)e.cols;
+  r.w = e.weights + r.pair * e.cols;
+  r.pos = e.positions ? e.positions + r.pair * e.cols : nullptr;
+  r.wo = e.weights_out + r.pair * e.cols;
+  r.po = e.positions_out + r.pair * e.cols;
+  r.budget = (int)(e.budget < r.cols ? e.budget : r.cols);
+  r.keep = r.n < r.budget ? r.n : r.budget;
+  if (threadIdx.x == 0) {
+    if (r.h == 0) {
       if (e.lens.bytes == 8)
-        ((int64_t *)e.lens_out)[row] = keep;
+        ((int64_t *)e.lens_out)[r.row] = r.keep;
       else
-        ((int32_t *)e.lens_out)[row] = keep;
+        ((int32_t *)e.lens_out)[r.row] = r.keep;
     }
-    if (n <= budget) a.moves[pair] = 0;
+    if (r.n <= r.budget) a.moves[r.pair] = 0;
   }
-  for (int j = keep + tid; j < cols; j += THREADS) {
-    wo[j] = 0.f;
-    po[j] = -1;
+  for (int j = r.keep + (int)threadIdx.x; j < r.cols; j += THREADS) {
+    r.wo[j] = 0.f;
+    r.po[j] = -1;
   }
-  if (n <= budget) {
-    for (int j = tid; j < n; j += THREADS) {
-      wo[j] = w[j];
-      po[j] = pos ? pos[j] : j;
-    }
-    return;
-  }
-  // the highest position + 1
-  int32_t top = -1;
-  if (pos) {
-#pragma unroll 4
-    for (int j = tid; j < n; j += THREADS) top = pos[j] > top ? pos[j] : top;
+  return r;
+}
+// The largest x of the workgroup (barrier inside).
+template <int THREADS>
+__device__ __forceinline__ int32_t block_max(int32_t x, int32_t *lds) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      const int32_t x = __shfl_xor(top, o, 64);
-      top = x > top ? x : top;
-    }
-    if (lane == 0) s_max[wave] = top;
-    __syncthreads();
-    for (int i = 0; i < kWaves; ++i) top = s_max[i] > top ? s_max[i] : top;
-  } else {
-    top = n - 1;
+  for (int o = 32; o > 0; o >>= 1) {
+    const int32_t y = __shfl_xor(x, o, 64);
+    x = y > x ? y : x;
   }
-  const int64_t newest = (int64_t)top + 1 - e.recent;
-  auto fetch = [&](int j) {
-    const int32_t p = pos ? pos[j] : j;
-    return key_of(w[j], p < e.sinks || p >= newest);
-  };
-  auto key_at = [&](int j) { return IN_LDS ? s_key[j] : fetch(j); };
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < THREADS / 64; ++i) x = lds[i] > x ? lds[i] : x;
+  return x;
+}
+// The digit that holds the `left`-th largest key of the histogram; left becomes its rank there.
+template <int THREADS>
+__device__ __forceinline__ uint32_t pick_digit(const uint32_t *hist, uint32_t &left, uint32_t *scan,
+                                               uint32_t *found) {
+  constexpr int kOwn = kDigits / THREADS;
+  // thread t owns kOwn digits counted from the largest: an ascending scan of them
+  uint32_t mine[kOwn], sum = 0, total;
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) {
+    mine[i] = hist[kDigits - 1 - ((int)threadIdx.x * kOwn + i)];
+    sum += mine[i];
+  }
+  uint32_t before = block_exclusive_scan<THREADS>(sum, &total, scan);
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) {
+    if (before < left && left <= before + mine[i]) {
+      found[0] = kDigits - 1 - ((int)threadIdx.x * kOwn + i);
+      found[1] = left - before;
+    }
+    before += mine[i];
+  }
+  __syncthreads();
+  left = found[1];
+  return found[0];
+}
+// Weights and positions of the slots that take a mover's row, and with FUSED the rows.
+template <int THREADS, bool FUSED>
+__device__ __forceinline__ void plan_end(const EvictArgs &a, const PlanRow &r, uint32_t all) {
+  const int32_t *holes = a.holes + r.pair * a.room, *movers = a.movers + r.pair * a.room;
+  if (threadIdx.x == 0) a.moves[r.pair] = (int32_t)all;
+  __syncthreads();  // the lists and the copies are written (a workgroup sees its stores past a barrier)
+#pragma unroll 4
+  for (uint32_t i = threadIdx.x; i < all; i += THREADS) {
+    const int32_t d = holes[i], s = movers[i];
+    r.wo[d] = r.w[s];
+    r.po[d] = r.pos ? r.pos[s] : s;
+  }
+  if constexpr (FUSED) {
+    const int lane = threadIdx.x & 63;
+    for (uint32_t i = threadIdx.x >> 6; i < all; i += THREADS / 64) {
+      const int64_t d[1] = {store_slot(a, r.row, r.h, holes[i])};
+      const int64_t s[1] = {store_slot(a, r.row, r.h, movers[i])};
+      if (d[0] >= 0 && s[0] >= 0)
+        for (int st = 0; st < a.e.nstores; ++st) move_store<1>(a.e.stores[st], s, d, lane, 6);
+    }
+  }
+}
+
+// Rows of at most THREADS * 32 slots: slot (v THREADS + t) 4 + i is thread t's.  ALIGNED: every row
+// of weights and positions starts at 16 bytes.
+template <int THREADS, bool FUSED, bool ALIGNED>
+__global__ __launch_bounds__(THREADS) void k_evict_plan(EvictArgs a) {
+  constexpr int kWaves = THREADS / 64, kRuns = kVecs * kWaves;  // a run: a wave's 256 slots of a v
+  static_assert(kRuns <= 128, "one wave scans the runs, two a lane");
+  __shared__ uint32_t s_hist[kDigits];
+  __shared__ uint32_t s_scan[kWaves], s_found[2], s_run[kRuns];
+  __shared__ int32_t s_max[kWaves];
+  const PlanRow r = plan_row<THREADS>(a);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const bool all_stay = r.n <= r.budget;
+  uint32_t key[kVecs][4];
+  int32_t p[kVecs][4], top = -1;
+#pragma unroll
+  for (int v = 0; v < kVecs; ++v) {
+    const int j = (v * THREADS + tid) * 4;
+    if (v * THREADS * 4 >= r.n) break;
+    if (ALIGNED && j + 4 <= r.cols) {
+      *(su32x4 *)key[v] = *(const su32x4 *)(r.w + j);
+      if (r.pos) *(su32x4 *)p[v] = *(const su32x4 *)(r.pos + j);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int x = j + i < r.n ? j + i : r.n - 1;
+        key[v][i] = __float_as_uint(r.w[x]);
+        if (r.pos) p[v][i] = r.pos[x];
+      }
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < kVecs; ++v) {
+    const int j = (v * THREADS + tid) * 4;
+    if (v * THREADS * 4 >= r.n) break;
+    if (!r.pos)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[v][i] = j + i;
+    if (ALIGNED && j + 4 <= r.keep) {
+      *(su32x4 *)(r.wo + j) = *(const su32x4 *)key[v];
+      *(su32x4 *)(r.po + j) = *(const su32x4 *)p[v];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (j + i < r.keep) {
+          r.wo[j + i] = __uint_as_float(key[v][i]);
+          r.po[j + i] = p[v][i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (j + i < r.n && p[v][i] > top) top = p[v][i];
+  }
+  if (all_stay) return;
+  top = block_max<THREADS>(top, s_max);
+  const int64_t newest = (int64_t)top + 1 - a.e.recent;
+#pragma unroll
+  for (int v = 0; v < kVecs; ++v)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      key[v][i] = key_of(__uint_as_float(key[v][i]), p[v][i] < a.e.sinks || p[v][i] >= newest);
   // the keep-th largest key: digits of 11, 11 and 10 bits from the top
-  uint32_t prefix = 0, left = (uint32_t)keep;
+  uint32_t prefix = 0, left = (uint32_t)r.keep;
   int shift = 32;
 #pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
@@ -160,40 +260,151 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan(EvictArgs a) {
     shift -= bits;
     for (int i = tid; i < kDigits; i += THREADS) s_hist[i] = 0;
     __syncthreads();
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) {
+      if (v * THREADS * 4 >= r.n) break;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t k = key[v][i];
+        if ((v * THREADS + tid) * 4 + i < r.n && (k & done) == prefix)
+          atomicAdd(&s_hist[(k >> shift) & ((1u << bits) - 1)], 1u);
+      }
+    }
+    __syncthreads();
+    prefix |= pick_digit<THREADS>(s_hist, left, s_scan, s_found) << shift;
+  }
+  // Exclusive sums of the runs' counts in slot order (run = v, wave), in place.
+  auto scan_runs = [&]() {
+    __syncthreads();
+    if (wave == 0) {
+      const uint32_t x = 2 * lane < kRuns ? s_run[2 * lane] : 0u;
+      const uint32_t y = 2 * lane + 1 < kRuns ? s_run[2 * lane + 1] : 0u;
+      const uint32_t before = wave_inclusive_scan(x + y) - x - y;
+      if (2 * lane < kRuns) s_run[2 * lane] = before;
+      if (2 * lane + 1 < kRuns) s_run[2 * lane + 1] = before + x;
+      if (lane == 63) s_found[0] = before + x + y;
+    }
+    __syncthreads();
+  };
+  const uint64_t below = lane == 0 ? 0ull : ~0ull >> (64 - lane);
+  // of the slots whose key equals the threshold the first `left` in slot order stay
+  uint32_t tie = 0, kept = 0;  // bit 4 v + i
+#pragma unroll
+  for (int v = 0; v < kVecs; ++v) {
+    uint32_t cnt = 0;
+    if (v * THREADS * 4 < r.n) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool in = (v * THREADS + tid) * 4 + i < r.n;
+        if (in && key[v][i] == prefix) tie |= 1u << (4 * v + i);
+        if (in && key[v][i] > prefix) kept |= 1u << (4 * v + i);
+        cnt += __popcll(__ballot((tie >> (4 * v + i)) & 1));
+      }
+    }
+    if (lane == 0) s_run[v * kWaves + wave] = cnt;
+  }
+  scan_runs();
+#pragma unroll
+  for (int v = 0; v < kVecs; ++v) {
+    if (v * THREADS * 4 >= r.n) break;
+    uint32_t rank = s_run[v * kWaves + wave];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) rank += __popcll(__ballot((tie >> (4 * v + i)) & 1) & below);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if ((tie >> (4 * v + i)) & 1) {
+        if (rank < left) kept |= 1u << (4 * v + i);
+        ++rank;
+      }
+  }
+  __syncthreads();  // s_run is written again
+  // holes (dropped below the budget) in the low half, movers (kept at or past it) in the high one:
+  // at most 32768 of each
+  uint32_t hole = 0, mover = 0;
+#pragma unroll
+  for (int v = 0; v < kVecs; ++v) {
+    uint32_t cnt = 0;
+    if (v * THREADS * 4 < r.n) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = (v * THREADS + tid) * 4 + i;
+        const bool k = (kept >> (4 * v + i)) & 1;
+        if (j < r.budget && !k) hole |= 1u << (4 * v + i);
+        if (j >= r.budget && k) mover |= 1u << (4 * v + i);
+        cnt += __popcll(__ballot((hole >> (4 * v + i)) & 1)) +
+               (__popcll(__ballot((mover >> (4 * v + i)) & 1)) << 16);
+      }
+    }
+    if (lane == 0) s_run[v * kWaves + wave] = cnt;
+  }
+  scan_runs();
+  const uint32_t all = s_found[0] & 0xffffu;
+  int32_t *holes = a.holes + r.pair * a.room, *movers = a.movers + r.pair * a.room;
+#pragma unroll
+  for (int v = 0; v < kVecs; ++v) {
+    if (v * THREADS * 4 >= r.n) break;
+    uint32_t rank = s_run[v * kWaves + wave];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      rank += __popcll(__ballot((hole >> (4 * v + i)) & 1) & below) +
+              (__popcll(__ballot((mover >> (4 * v + i)) & 1) & below) << 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int j = (v * THREADS + tid) * 4 + i;
+      if ((hole >> (4 * v + i)) & 1) holes[rank++ & 0xffffu] = j;
+      if ((mover >> (4 * v + i)) & 1) {
+        movers[rank >> 16] = j;
+        rank += 0x10000u;
+      }
+    }
+  }
+  plan_end<THREADS, FUSED>(a, r, all);
+}
+
+// Longer rows: every step reads weights and positions again.  In slot order a wave takes a run of
+// n / kWaves slots.
+template <int THREADS, bool FUSED>
+__global__ __launch_bounds__(THREADS) void k_evict_plan_long(EvictArgs a) {
+  constexpr int kWaves = THREADS / 64;
+  __shared__ uint32_t s_hist[kDigits];
+  __shared__ uint32_t s_scan[kWaves], s_found[2], s_cnt[3][kWaves];
+  __shared__ int32_t s_max[kWaves];
+  const PlanRow r = plan_row<THREADS>(a);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = r.n;
+  int32_t top = -1;
+#pragma unroll 4
+  for (int j = tid; j < n; j += THREADS) {
+    const int32_t p = r.pos ? r.pos[j] : j;
+    if (j < r.keep) {
+      r.wo[j] = r.w[j];
+      r.po[j] = p;
+    }
+    top = p > top ? p : top;
+  }
+  if (n <= r.budget) return;
+  top = block_max<THREADS>(top, s_max);
+  const int64_t newest = (int64_t)top + 1 - a.e.recent;
+  auto key_at = [&](int j) {
+    const int32_t p = r.pos ? r.pos[j] : j;
+    return key_of(r.w[j], p < a.e.sinks || p >= newest);
+  };
+  uint32_t prefix = 0, left = (uint32_t)r.keep;
+  int shift = 32;
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int bits = pass < 2 ? 11 : 10;
+    const uint32_t done = pass == 0 ? 0u : ~0u << shift;
+    shift -= bits;
+    for (int i = tid; i < kDigits; i += THREADS) s_hist[i] = 0;
+    __syncthreads();
 #pragma unroll 4
     for (int j = tid; j < n; j += THREADS) {
-      uint32_t k;
-      if (pass == 0) {
-        k = fetch(j);
-        if (IN_LDS) s_key[j] = k;
-      } else {
-        k = key_at(j);
-      }
+      const uint32_t k = key_at(j);
       if ((k & done) == prefix) atomicAdd(&s_hist[(k >> shift) & ((1u << bits) - 1)], 1u);
     }
     __syncthreads();
-    // thread t owns kOwn digits counted from the largest: an ascending scan of them
-    uint32_t mine[kOwn], sum = 0, total;
-#pragma unroll
-    for (int i = 0; i < kOwn; ++i) {
-      mine[i] = s_hist[kDigits - 1 - (tid * kOwn + i)];
-      sum += mine[i];
-    }
-    uint32_t before = block_exclusive_scan<THREADS>(sum, &total, s_scan);
-#pragma unroll
-    for (int i = 0; i < kOwn; ++i) {
-      if (before < left && left <= before + mine[i]) {
-        s_digit = kDigits - 1 - (tid * kOwn + i);
-        s_left = left - before;
-      }
-      before += mine[i];
-    }
-    __syncthreads();
-    prefix |= s_digit << shift;
-    left = s_left;
-    __syncthreads();
+    prefix |= pick_digit<THREADS>(s_hist, left, s_scan, s_found) << shift;
   }
-  // In slot order, wave by wave: of the slots whose key equals the threshold the first `left` stay.
   const int seg = ((n + kWaves - 1) / kWaves + 63) & ~63;
   const int j0 = wave * seg, j1 = j0 + seg < n ? j0 + seg : n;
   const uint64_t below = lane == 0 ? 0ull : ~0ull >> (64 - lane);
@@ -208,27 +419,23 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan(EvictArgs a) {
   if (lane == 0) s_cnt[0][wave] = cnt;
   __syncthreads();
   const uint32_t tie0 = before_wave(s_cnt[0]);
-  int32_t *holes = a.holes + pair * a.room, *movers = a.movers + pair * a.room;
+  int32_t *holes = a.holes + r.pair * a.room, *movers = a.movers + r.pair * a.room;
   uint32_t nh = 0, nm = 0;
   for (int turn = 0; turn < 2; ++turn) {  // count, then write
     uint32_t ties = tie0;
     for (int b = j0; b < j1; b += 64) {
       const int j = b + lane;
       const bool in = j < j1;
-      const uint32_t k = in ? key_at(j) : 0u;
+      const uint32_t k = key_at(in ? j : j1 - 1);
       const bool tie = in && k == prefix;
       const uint64_t tb = __ballot(tie);
       const bool kept = in && (k > prefix || (tie && ties + __popcll(tb & below) < left));
       ties += __popcll(tb);
-      const uint64_t hb = __ballot(in && !kept && j < budget);
-      const uint64_t mb = __ballot(kept && j >= budget);
+      const uint64_t hb = __ballot(in && !kept && j < r.budget);
+      const uint64_t mb = __ballot(kept && j >= r.budget);
       if (turn == 1) {
         if ((hb >> lane) & 1) holes[nh + __popcll(hb & below)] = j;
         if ((mb >> lane) & 1) movers[nm + __popcll(mb & below)] = j;
-        if (kept && j < budget) {
-          wo[j] = w[j];
-          po[j] = pos ? pos[j] : j;
-        }
       }
       nh += __popcll(hb);
       nm += __popcll(mb);
@@ -245,21 +452,7 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan(EvictArgs a) {
   }
   uint32_t all = 0;
   for (int i = 0; i < kWaves; ++i) all += s_cnt[1][i];
-  if (tid == 0) a.moves[pair] = (int32_t)all;
-  __syncthreads();  // the lists are written (a workgroup's stores are visible to it past a barrier)
-  for (uint32_t i = tid; i < all; i += THREADS) {
-    const int32_t d = holes[i], s = movers[i];
-    wo[d] = w[s];
-    po[d] = pos ? pos[s] : s;
-  }
-  if constexpr (FUSED) {
-    for (int st = 0; st < e.nstores; ++st)
-      for (uint32_t i = wave; i < all; i += kWaves) {
-        int64_t d[1] = {store_slot(a, row, h, holes[i])};
-        int64_t s[1] = {store_slot(a, row, h, movers[i])};
-        if (d[0] >= 0 && s[0] >= 0) move_store<1>(e.stores[st], s, d, lane, 6);
-      }
-  }
+  plan_end<THREADS, FUSED>(a, r, all);
 }
 
 // Block (x, y, z): (row, head), a share of its moves, a store.  1 << lg lanes move a row (as many
@@ -296,27 +489,27 @@ int64_t evict_room(const EvictCall &e) {
 }
 int64_t up256(int64_t x) { return (x + 255) & ~int64_t(255); }
 
-template <int THREADS, bool IN_LDS, bool FUSED>
+template <int THREADS, bool FUSED>
 void launch_plan(const EvictArgs &a, hipStream_t st) {
-  const int64_t pairs = a.e.rows * a.e.heads;
-  const size_t lds = IN_LDS ? (size_t)a.e.cols * 4 : 0;
-  if (lds > 48 * 1024) {
-    static const hipError_t once = hipFuncSetAttribute(
-        (const void *)k_evict_plan<THREADS, IN_LDS, FUSED>,
-        hipFuncAttributeMaxDynamicSharedMemorySize, kMaxKeys * 4);
-    DGS_HIP(once);
-  }
-  k_evict_plan<THREADS, IN_LDS, FUSED><<<(unsigned)pairs, THREADS, lds, st>>>(a);
-  DGS_LAUNCH_CHECK();
+  const unsigned pairs = (unsigned)(a.e.rows * a.e.heads);
+  const uintptr_t at = (uintptr_t)a.e.weights | (uintptr_t)a.e.positions |
+                       (uintptr_t)a.e.weights_out | (uintptr_t)a.e.positions_out;
+  if (a.e.cols % 4 == 0 && at % 16 == 0)
+    k_evict_plan<THREADS, FUSED, true><<<pairs, THREADS, 0, st>>>(a);
+  else
+    k_evict_plan<THREADS, FUSED, false><<<pairs, THREADS, 0, st>>>(a);
 }
 template <bool FUSED>
 void plan(const EvictArgs &a, hipStream_t st) {
-  if (a.e.cols <= 8192)
-    launch_plan<256, true, FUSED>(a, st);
-  else if (a.e.cols <= kMaxKeys)
-    launch_plan<1024, true, FUSED>(a, st);
+  if (a.e.cols <= 2048)
+    launch_plan<256, FUSED>(a, st);
+  else if (a.e.cols <= 512 * 4 * kVecs)
+    launch_plan<512, FUSED>(a, st);
+  else if (a.e.cols <= 1024 * 4 * kVecs)
+    launch_plan<1024, FUSED>(a, st);
   else
-    launch_plan<1024, false, FUSED>(a, st);
+    k_evict_plan_long<1024, FUSED><<<(unsigned)(a.e.rows * a.e.heads), 1024, 0, st>>>(a);
+  DGS_LAUNCH_CHECK();
 }
 
 }  // namespace
