@@ -23,7 +23,6 @@ namespace {
 
 constexpr int kMoveThreads = 256;
 constexpr int kDigits = 2048;  // 11 bits: the sign, the exponent and two bits of the mantissa first
-constexpr int kVecs = 8;  // loads of four slots a thread keeps
 constexpr int kFewMoves = 32;
 
 struct EvictArgs {
@@ -169,8 +168,9 @@ __device__ __forceinline__ uint32_t pick_digit(const uint32_t *hist, uint32_t &l
 }
 // Weights and positions of the slots that take a mover's row, and with FUSED the rows.
 template <int THREADS, bool FUSED>
-__device__ __forceinline__ void plan_end(const EvictArgs &a, const PlanRow &r, uint32_t all) {
-  const int32_t *holes = a.holes + r.pair * a.room, *movers = a.movers + r.pair * a.room;
+__device__ __forceinline__ void plan_end(const EvictArgs &a, const PlanRow &r,
+                                         const int32_t *holes, const int32_t *movers,
+                                         uint32_t all) {
   if (threadIdx.x == 0) a.moves[r.pair] = (int32_t)all;
   __syncthreads();  // the lists and the copies are written (a workgroup sees its stores past a barrier)
 #pragma unroll 4
@@ -190,36 +190,47 @@ __device__ __forceinline__ void plan_end(const EvictArgs &a, const PlanRow &r, u
   }
 }
 
-// Rows of at most THREADS * 32 slots: slot (v THREADS + t) 4 + i is thread t's.  ALIGNED: every row
-// of weights and positions starts at 16 bytes.
-template <int THREADS, bool FUSED, bool ALIGNED>
+// Rows of at most THREADS * kVecs * 4 slots: slot (v THREADS + t) 4 + i is thread t's.  ALIGNED:
+// every row of weights and positions starts at 16 bytes.  Where one slot too many is held, as
+// after every token of a full cache, the digits are not counted: the lowest key goes (of equal ones
+// the last), one exchange over the workgroup.
+template <int THREADS, int kVecs, bool FUSED, bool ALIGNED>
 __global__ __launch_bounds__(THREADS) void k_evict_plan(EvictArgs a) {
   constexpr int kWaves = THREADS / 64, kRuns = kVecs * kWaves;  // a run: a wave's 256 slots of a v
   static_assert(kRuns <= 128, "one wave scans the runs, two a lane");
-  __shared__ uint32_t s_hist[kDigits];
+  __shared__ uint32_t s_hist[3][kDigits];
   __shared__ uint32_t s_scan[kWaves], s_found[2], s_run[kRuns];
   __shared__ int32_t s_max[kWaves];
-  const PlanRow r = plan_row<THREADS>(a);
+  __shared__ uint64_t s_low[kWaves];
+  __shared__ int32_t s_list[2 * kFewMoves];  // FUSED: holes, movers
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const bool all_stay = r.n <= r.budget;
   uint32_t key[kVecs][4];
   int32_t p[kVecs][4], top = -1;
+  {
+    // whole rows of the arrays, while the length is on its way
+    const float *w = a.e.weights + blockIdx.x * a.e.cols;
+    const int32_t *pos = a.e.positions ? a.e.positions + blockIdx.x * a.e.cols : nullptr;
+    const int cols = (int)a.e.cols;
 #pragma unroll
-  for (int v = 0; v < kVecs; ++v) {
-    const int j = (v * THREADS + tid) * 4;
-    if (v * THREADS * 4 >= r.n) break;
-    if (ALIGNED && j + 4 <= r.cols) {
-      *(su32x4 *)key[v] = *(const su32x4 *)(r.w + j);
-      if (r.pos) *(su32x4 *)p[v] = *(const su32x4 *)(r.pos + j);
-    } else {
+    for (int v = 0; v < kVecs; ++v) {
+      const int j = (v * THREADS + tid) * 4;
+      if (v * THREADS * 4 >= cols) break;
+      if (ALIGNED) {
+        const int x = j < cols ? j : 0;
+        *(su32x4 *)key[v] = *(const su32x4 *)(w + x);
+        if (pos) *(su32x4 *)p[v] = *(const su32x4 *)(pos + x);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int x = j + i < r.n ? j + i : r.n - 1;
-        key[v][i] = __float_as_uint(r.w[x]);
-        if (r.pos) p[v][i] = r.pos[x];
+        for (int i = 0; i < 4; ++i) {
+          const int x = j + i < cols ? j + i : 0;
+          key[v][i] = __float_as_uint(w[x]);
+          if (pos) p[v][i] = pos[x];
+        }
       }
     }
   }
+  for (int i = tid; i < 3 * kDigits; i += THREADS) (&s_hist[0][0])[i] = 0;
+  const PlanRow r = plan_row<THREADS>(a);
 #pragma unroll
   for (int v = 0; v < kVecs; ++v) {
     const int j = (v * THREADS + tid) * 4;
@@ -242,7 +253,7 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan(EvictArgs a) {
     for (int i = 0; i < 4; ++i)
       if (j + i < r.n && p[v][i] > top) top = p[v][i];
   }
-  if (all_stay) return;
+  if (r.n <= r.budget) return;
   top = block_max<THREADS>(top, s_max);
   const int64_t newest = (int64_t)top + 1 - a.e.recent;
 #pragma unroll
@@ -250,6 +261,35 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan(EvictArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       key[v][i] = key_of(__uint_as_float(key[v][i]), p[v][i] < a.e.sinks || p[v][i] >= newest);
+  int32_t *holes = FUSED ? s_list : a.holes + r.pair * a.room;
+  int32_t *movers = FUSED ? s_list + kFewMoves : a.movers + r.pair * a.room;
+  if (r.n == r.budget + 1) {
+    uint64_t low = ~0ull;  // key, then the complement of the slot
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = (v * THREADS + tid) * 4 + i;
+        const uint64_t x = (uint64_t)key[v][i] << 32 | ~(uint32_t)j;
+        if (j < r.n && x < low) low = x;
+      }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      const uint64_t x = __shfl_xor((unsigned long long)low, o, 64);
+      low = x < low ? x : low;
+    }
+    if (lane == 0) s_low[wave] = low;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) low = s_low[i] < low ? s_low[i] : low;
+    const int drop = (int)~(uint32_t)low;
+    if (tid == 0) {
+      holes[0] = drop;
+      movers[0] = r.budget;
+    }
+    plan_end<THREADS, FUSED>(a, r, holes, movers, drop < r.budget ? 1u : 0u);
+    return;
+  }
   // the keep-th largest key: digits of 11, 11 and 10 bits from the top
   uint32_t prefix = 0, left = (uint32_t)r.keep;
   int shift = 32;
@@ -258,8 +298,6 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan(EvictArgs a) {
     const int bits = pass < 2 ? 11 : 10;
     const uint32_t done = pass == 0 ? 0u : ~0u << shift;  // bits settled so far
     shift -= bits;
-    for (int i = tid; i < kDigits; i += THREADS) s_hist[i] = 0;
-    __syncthreads();
 #pragma unroll
     for (int v = 0; v < kVecs; ++v) {
       if (v * THREADS * 4 >= r.n) break;
@@ -267,11 +305,11 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan(EvictArgs a) {
       for (int i = 0; i < 4; ++i) {
         const uint32_t k = key[v][i];
         if ((v * THREADS + tid) * 4 + i < r.n && (k & done) == prefix)
-          atomicAdd(&s_hist[(k >> shift) & ((1u << bits) - 1)], 1u);
+          atomicAdd(&s_hist[pass][(k >> shift) & ((1u << bits) - 1)], 1u);
       }
     }
     __syncthreads();
-    prefix |= pick_digit<THREADS>(s_hist, left, s_scan, s_found) << shift;
+    prefix |= pick_digit<THREADS>(s_hist[pass], left, s_scan, s_found) << shift;
   }
   // Exclusive sums of the runs' counts in slot order (run = v, wave), in place.
   auto scan_runs = [&]() {
@@ -339,7 +377,6 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan(EvictArgs a) {
   }
   scan_runs();
   const uint32_t all = s_found[0] & 0xffffu;
-  int32_t *holes = a.holes + r.pair * a.room, *movers = a.movers + r.pair * a.room;
 #pragma unroll
   for (int v = 0; v < kVecs; ++v) {
     if (v * THREADS * 4 >= r.n) break;
@@ -358,7 +395,7 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan(EvictArgs a) {
       }
     }
   }
-  plan_end<THREADS, FUSED>(a, r, all);
+  plan_end<THREADS, FUSED>(a, r, holes, movers, all);
 }
 
 // Longer rows: every step reads weights and positions again.  In slot order a wave takes a run of
@@ -452,7 +489,7 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan_long(EvictArgs a) {
   }
   uint32_t all = 0;
   for (int i = 0; i < kWaves; ++i) all += s_cnt[1][i];
-  plan_end<THREADS, FUSED>(a, r, all);
+  plan_end<THREADS, FUSED>(a, r, holes, movers, all);
 }
 
 // Block (x, y, z): (row, head), a share of its moves, a store.  1 << lg lanes move a row (as many
@@ -489,24 +526,26 @@ int64_t evict_room(const EvictCall &e) {
 }
 int64_t up256(int64_t x) { return (x + 255) & ~int64_t(255); }
 
-template <int THREADS, bool FUSED>
+template <int THREADS, int kVecs, bool FUSED>
 void launch_plan(const EvictArgs &a, hipStream_t st) {
   const unsigned pairs = (unsigned)(a.e.rows * a.e.heads);
   const uintptr_t at = (uintptr_t)a.e.weights | (uintptr_t)a.e.positions |
                        (uintptr_t)a.e.weights_out | (uintptr_t)a.e.positions_out;
   if (a.e.cols % 4 == 0 && at % 16 == 0)
-    k_evict_plan<THREADS, FUSED, true><<<pairs, THREADS, 0, st>>>(a);
+    k_evict_plan<THREADS, kVecs, FUSED, true><<<pairs, THREADS, 0, st>>>(a);
   else
-    k_evict_plan<THREADS, FUSED, false><<<pairs, THREADS, 0, st>>>(a);
+    k_evict_plan<THREADS, kVecs, FUSED, false><<<pairs, THREADS, 0, st>>>(a);
 }
 template <bool FUSED>
 void plan(const EvictArgs &a, hipStream_t st) {
-  if (a.e.cols <= 2048)
-    launch_plan<256, FUSED>(a, st);
-  else if (a.e.cols <= 512 * 4 * kVecs)
-    launch_plan<512, FUSED>(a, st);
-  else if (a.e.cols <= 1024 * 4 * kVecs)
-    launch_plan<1024, FUSED>(a, st);
+  if (a.e.cols <= 1024)
+    launch_plan<256, 1, FUSED>(a, st);
+  else if (a.e.cols <= 8192)
+    launch_plan<512, 4, FUSED>(a, st);
+  else if (a.e.cols <= 16384)
+    launch_plan<1024, 4, FUSED>(a, st);
+  else if (a.e.cols <= 32768)
+    launch_plan<1024, 8, FUSED>(a, st);
   else
     k_evict_plan_long<1024, FUSED><<<(unsigned)(a.e.rows * a.e.heads), 1024, 0, st>>>(a);
   DGS_LAUNCH_CHECK();
