@@ -119,7 +119,7 @@ __device__ __forceinline__ PlanRow plan_row(const EvictArgs &a) {
       else
         ((int32_t *)e.lens_out)[r.row] = r.keep;
     }
-    if (r.n <= r.budget) a.moves[r.pair] = 0;
+    if (a.moves && r.n <= r.budget) a.moves[r.pair] = 0;
   }
   for (int j = r.keep + (int)threadIdx.x; j < r.cols; j += THREADS) {
     r.wo[j] = 0.f;
@@ -171,7 +171,7 @@ template <int THREADS, bool FUSED>
 __device__ __forceinline__ void plan_end(const EvictArgs &a, const PlanRow &r,
                                          const int32_t *holes, const int32_t *movers,
                                          uint32_t all) {
-  if (threadIdx.x == 0) a.moves[r.pair] = (int32_t)all;
+  if (!FUSED && threadIdx.x == 0) a.moves[r.pair] = (int32_t)all;
   __syncthreads();  // the lists and the copies are written (a workgroup sees its stores past a barrier)
 #pragma unroll 4
   for (uint32_t i = threadIdx.x; i < all; i += THREADS) {
@@ -400,7 +400,7 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan(EvictArgs a) {
 
 // Longer rows: every step reads weights and positions again.  In slot order a wave takes a run of
 // n / kWaves slots.
-template <int THREADS, bool FUSED>
+template <int THREADS>
 __global__ __launch_bounds__(THREADS) void k_evict_plan_long(EvictArgs a) {
   constexpr int kWaves = THREADS / 64;
   __shared__ uint32_t s_hist[kDigits];
@@ -489,7 +489,7 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan_long(EvictArgs a) {
   }
   uint32_t all = 0;
   for (int i = 0; i < kWaves; ++i) all += s_cnt[1][i];
-  plan_end<THREADS, FUSED>(a, r, holes, movers, all);
+  plan_end<THREADS, false>(a, r, holes, movers, all);
 }
 
 // Block (x, y, z): (row, head), a share of its moves, a store.  1 << lg lanes move a row (as many
@@ -546,37 +546,42 @@ void plan(const EvictArgs &a, hipStream_t st) {
     launch_plan<1024, 4, FUSED>(a, st);
   else if (a.e.cols <= 32768)
     launch_plan<1024, 8, FUSED>(a, st);
-  else
-    k_evict_plan_long<1024, FUSED><<<(unsigned)(a.e.rows * a.e.heads), 1024, 0, st>>>(a);
+  else if constexpr (!FUSED)
+    k_evict_plan_long<1024><<<(unsigned)(a.e.rows * a.e.heads), 1024, 0, st>>>(a);
   DGS_LAUNCH_CHECK();
 }
+
+// Few moves: the lists stay in LDS (rows of more than 32768 slots need them all the same).
+bool few_moves(const EvictCall &e) { return evict_room(e) <= kFewMoves && e.cols <= 32768; }
 
 }  // namespace
 
 int64_t evict_workspace(const EvictCall &e) {
   const int64_t pairs = e.rows * e.heads;
+  if (few_moves(e)) return 0;
   return up256(pairs * 4) + 2 * up256(pairs * evict_room(e) * 4);
 }
 
 void evict_rows(const EvictCall &e, void *ws, int64_t ws_bytes, hipStream_t st) {
   const int64_t pairs = e.rows * e.heads;
   if (pairs <= 0) return;
-  DGS_CHECK(ws && ws_bytes >= evict_workspace(e), "evict: workspace too small");
+  const int64_t need = evict_workspace(e);
+  DGS_CHECK(ws_bytes >= need && (need == 0 || ws), "evict: workspace too small");
   DGS_CHECK(pairs < (int64_t(1) << 31) && e.cols < (int64_t(1) << 30) &&
                 e.page < (int64_t(1) << 31),
             "evict: too many rows or columns");
   EvictArgs a{};
   a.e = e;
   a.room = evict_room(e);
+  a.gd = state_guard(kAsyncErrSlot, e.pages);
+  if (few_moves(e)) {
+    plan<true>(a, st);
+    return;
+  }
   char *w = static_cast<char *>(ws);
   a.moves = (int32_t *)w;
   a.holes = (int32_t *)(w + up256(pairs * 4));
   a.movers = (int32_t *)(w + up256(pairs * 4) + up256(pairs * a.room * 4));
-  a.gd = state_guard(kAsyncErrSlot, e.pages);
-  if (a.room <= kFewMoves) {
-    plan<true>(a, st);
-    return;
-  }
   plan<false>(a, st);
   if (e.nstores == 0) return;
   // enough blocks to fill the card, at least 8 rows for each of a block's groups

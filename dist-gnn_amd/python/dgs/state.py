@@ -29,13 +29,12 @@ class _CCache(ctypes.Structure):
 
 
 _HERE = contextlib.nullcontext()
+_current = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def _on(device):
-    """Makes `device` the current one for the call (the library launches on the current one)."""
-    if device.index == torch.cuda.current_device():
-        return _HERE
-    return torch.cuda.device(device)
+def _on(index):
+    """Makes device `index` the current one for the call (the library launches on the current one)."""
+    return _HERE if _current() == index else torch.cuda.device(index)
 
 
 def _require(cond, msg):
@@ -49,16 +48,18 @@ def _ids(t, name):
 
 
 def _no_grad(*tensors):
-    if torch.is_grad_enabled():
-        for t in tensors:
-            _require(not t.requires_grad,
-                     "the state cache has no backward: detach the tensor or use torch.no_grad()")
+    for t in tensors:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("the state cache has no backward: detach the tensor or use "
+                               "torch.no_grad()")
 
 
-def _same_device(device, **tensors):
-    for name, t in tensors.items():
-        _require(t.is_cuda, f"{name} must be a CUDA tensor")
-        _require(t.device == device, f"{name} must be on {device}, the cache's device")
+def _same_device(index, *tensors):
+    """Every tensor lies on CUDA device `index` (the cache's, or the weights')."""
+    for t in tensors:
+        if t.get_device() != index or not t.is_cuda:
+            raise RuntimeError(f"every tensor of a call must be a CUDA tensor on device {index}, "
+                               f"not on {t.device}")
 
 
 def _rows16(t):
@@ -117,8 +118,8 @@ class StateCache:
                         ("v_scales", v_scales)):
             _require(t.is_contiguous() and t.data_ptr() % 16 == 0,
                      f"{name} must be contiguous and 16-byte aligned")
-        _same_device(k_codes.device, k_codes=k_codes, k_scales=k_scales, v_codes=v_codes,
-                     v_scales=v_scales)
+        _require(k_codes.is_cuda, "the state cache lives on a CUDA device")
+        _same_device(k_codes.get_device(), k_scales, v_codes, v_scales)
         self._adopt(k_codes, k_scales, v_codes, v_scales)
         return self
 
@@ -139,12 +140,13 @@ class StateCache:
         self.head_dim = 2 * k_codes.shape[3]
         self.group = self.head_dim // k_scales.shape[3]
         self.device = k_codes.device
+        self._index = k_codes.get_device()
         self._c = _CCache(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
                           v_scales.data_ptr(), self.num_pages, self.page_size, self.heads,
                           self.head_dim, self.group)
         self._ref = ctypes.addressof(self._c)
         self._room = {}
-        with _on(self.device):
+        with _on(self._index):
             check(lib.dgs_check_async_errors())  # makes the report words (never inside a capture)
 
     def _rows(self, k, v):
@@ -154,7 +156,7 @@ class StateCache:
             _require(t.dtype in _DTYPES, f"{name} must be float32, bfloat16 or float16")
         _require(k.shape == v.shape and k.dtype == v.dtype, "k and v must be alike")
         _no_grad(k, v)
-        _same_device(self.device, k=k, v=v)
+        _same_device(self._index, k, v)
         return _rows16(k), _rows16(v)
 
     def write(self, k, v, slots):
@@ -164,12 +166,12 @@ class StateCache:
         _require(slots.dim() == 1 and slots.numel() == k.shape[0], "slots must be [tokens]")
         slots = _ids(slots, "slots")
         k, v = self._rows(k, v)
-        _same_device(self.device, slots=slots)
-        with _on(self.device):
+        _same_device(self._index, slots)
+        with _on(self._index):
             s = slots if slots.dtype == torch.int64 else slots.long()
             check(lib.dgs_state_write(self._ref, k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype],
                                       k.shape[0], k.stride(0), k.stride(1), v.stride(0),
-                                      v.stride(1), s.data_ptr(), stream_ptr(self.device)))
+                                      v.stride(1), s.data_ptr(), stream_ptr(self._index)))
 
     def append(self, k, v, table, lens):
         """One new row per sequence: k[i], v[i] go to slot lens[i] of table row i (page ids
@@ -180,14 +182,14 @@ class StateCache:
         _require(lens.dim() == 1 and lens.numel() == n, "lens must be [tokens]")
         table, lens = _ids(table, "table"), _ids(lens, "lens")
         k, v = self._rows(k, v)
-        _same_device(self.device, table=table, lens=lens)
-        with _on(self.device):
+        _same_device(self._index, table, lens)
+        with _on(self._index):
             slots = torch.empty(n, dtype=torch.int64, device=self.device)
             check(lib.dgs_state_append(self._ref, k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype],
                                        n, k.stride(0), k.stride(1), v.stride(0), v.stride(1),
                                        table.data_ptr(), table.element_size(), table.shape[1],
                                        lens.data_ptr(), lens.element_size(), slots.data_ptr(),
-                                       stream_ptr(self.device)))
+                                       stream_ptr(self._index)))
         return slots
 
     def read(self, slots, dtype=torch.float32):
@@ -195,14 +197,14 @@ class StateCache:
         _require(slots.dim() == 1, "slots must have one dimension")
         _require(dtype in _DTYPES, "rows are read as float32, bfloat16 or float16")
         slots = _ids(slots, "slots")
-        _same_device(self.device, slots=slots)
-        with _on(self.device):
+        _same_device(self._index, slots)
+        with _on(self._index):
             s = slots if slots.dtype == torch.int64 else slots.long()
             k = torch.empty((s.numel(), self.heads, self.head_dim), dtype=dtype,
                             device=self.device)
             v = torch.empty_like(k)
             check(lib.dgs_state_read(self._ref, s.data_ptr(), s.numel(), _DTYPES[dtype],
-                                     k.data_ptr(), v.data_ptr(), stream_ptr(self.device)))
+                                     k.data_ptr(), v.data_ptr(), stream_ptr(self._index)))
         return k, v
 
     def attend(self, q, table, lens, scale=None, weights=None, decay=1.0):
@@ -231,12 +233,12 @@ class StateCache:
                      f"weights must be float32 [rows, {self.heads}, >= pages * page_size]")
             _require(weights.is_contiguous(), "weights must be contiguous (updated in place)")
             _no_grad(weights)
-            _same_device(self.device, weights=weights)
-        _same_device(self.device, q=q, table=table, lens=lens)
+            _same_device(self._index, weights)
+        _same_device(self._index, q, table, lens)
         scale = 1.0 / math.sqrt(self.head_dim) if scale is None else float(scale)
         q = _rows16(q)
         dt = _DTYPES[q.dtype]
-        with _on(self.device):
+        with _on(self._index):
             out = torch.empty((rows, q_heads, self.head_dim), dtype=q.dtype, device=self.device)
             if rows == 0:
                 return out
@@ -256,13 +258,16 @@ class StateCache:
                 table.data_ptr(), table.element_size(), width, lens.data_ptr(),
                 lens.element_size(), scale, None if weights is None else weights.data_ptr(),
                 0 if weights is None else weights.shape[2], float(decay), out.data_ptr(),
-                None if ws is None else ws.data_ptr(), room, stream_ptr(self.device)))
+                None if ws is None else ws.data_ptr(), room, stream_ptr(self._index)))
         return out
 
     def evict(self, weights, positions, table, lens, budget, sinks=0, recent=0):
         """evict_rows over this cache's buffers."""
         return evict_rows([self.k_codes, self.k_scales, self.v_codes, self.v_scales], weights,
                           positions, table, lens, budget, sinks=sinks, recent=recent)
+
+
+_evict_room = {}  # workspace bytes by (rows, heads, cols, budget)
 
 
 def evict_rows(stores, weights, positions, table, lens, budget, sinks=0, recent=0):
@@ -295,22 +300,21 @@ def evict_rows(stores, weights, positions, table, lens, budget, sinks=0, recent=
              "sinks + recent must lie between 0 and budget")
     stores = list(stores)
     _require(0 < len(stores) <= 8, "evict_rows takes one to eight stores")
-    lead = tuple(stores[0].shape[:3])
+    lead = stores[0].shape[:3]
     _require(len(lead) == 3 and lead[0] > 0 and lead[1] == heads and lead[2] > 0,
              f"a store must be [pages, {heads}, page_size, ...]")
     for s in stores:
-        _require(tuple(s.shape[:3]) == lead, "the stores must have the same pages")
+        _require(s.shape[:3] == lead, "the stores must have the same pages")
         _require(s.is_contiguous() and s.numel() > 0, "a store must be contiguous and not empty")
     _require(cols >= table.shape[1] * lead[2],
              "weights need a column for every slot of the table")
     _no_grad(weights, *stores)
-    device = weights.device
-    for s in stores:
-        _same_device(device, store=s)
-    _same_device(device, weights=weights, table=table, lens=lens)
+    _require(weights.is_cuda, "weights must be a CUDA tensor")
+    index, device = weights.get_device(), weights.device
+    _same_device(index, table, lens, *stores)
     if positions is not None:
-        _same_device(device, positions=positions)
-    with _on(device):
+        _same_device(index, positions)
+    with _on(index):
         w = weights.contiguous()
         p = None if positions is None else positions.contiguous()
         new_w = torch.empty((rows, heads, cols), dtype=torch.float32, device=device)
@@ -318,9 +322,15 @@ def evict_rows(stores, weights, positions, table, lens, budget, sinks=0, recent=
         new_lens = torch.empty_like(lens)
         if rows == 0:
             return new_w, new_p, new_lens
-        room = c_i64()
-        check(lib.dgs_evict_workspace(rows, heads, cols, budget, ctypes.byref(room)))
-        ws = torch.empty(room.value, dtype=torch.uint8, device=device)
+        key = (rows, heads, cols, budget)
+        room = _evict_room.get(key)
+        if room is None:
+            n = c_i64()
+            check(lib.dgs_evict_workspace(rows, heads, cols, budget, ctypes.byref(n)))
+            if len(_evict_room) >= 1024:
+                _evict_room.clear()
+            room = _evict_room[key] = n.value
+        ws = torch.empty(room, dtype=torch.uint8, device=device) if room else None
         ptrs = (c_vp * len(stores))(*[s.data_ptr() for s in stores])
         slots = lead[0] * heads * lead[2]
         nbytes = (c_i64 * len(stores))(*[s.numel() // slots * s.element_size() for s in stores])
@@ -328,8 +338,8 @@ def evict_rows(stores, weights, positions, table, lens, budget, sinks=0, recent=
             ptrs, nbytes, len(stores), lead[0], heads, lead[2], w.data_ptr(),
             None if p is None else p.data_ptr(), new_w.data_ptr(), new_p.data_ptr(), rows, cols,
             table.data_ptr(), table.element_size(), table.shape[1], lens.data_ptr(),
-            lens.element_size(), new_lens.data_ptr(), budget, sinks, recent, ws.data_ptr(),
-            room.value, stream_ptr(device)))
+            lens.element_size(), new_lens.data_ptr(), budget, sinks, recent,
+            None if ws is None else ws.data_ptr(), room, stream_ptr(index)))
     return new_w, new_p, new_lens
 
 

@@ -14,7 +14,7 @@ def _fake(**kw):
     """A cache object without memory, for the binding's checks."""
     c = StateCache.__new__(StateCache)
     c.num_pages, c.page_size, c.heads, c.head_dim, c.group = 4, 8, 2, 64, 32
-    c.device = torch.device("cuda", 0)
+    c.device, c._index = torch.device("cuda", 0), 0
     for k, v in kw.items():
         setattr(c, k, v)
     return c
