@@ -223,6 +223,23 @@ __device__ __forceinline__ uint4 philox4x32_10(uint4 c, const PhiloxKeys &K) {
   return c;
 }
 
+// x / d for 32-bit x via multiply-high (Granlund-Montgomery).
+struct FastDivU32 {
+  uint32_t d, m, s;
+  static FastDivU32 make(uint32_t d) {
+    FastDivU32 f;
+    f.d = d;
+    uint32_t s = 0;
+    while ((uint64_t(1) << s) < d) ++s;
+    f.s = s;
+    f.m = (uint32_t)(((uint64_t(1) << 32) * ((uint64_t(1) << s) - d)) / d + 1);
+    return f;
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t x) const {
+    return (uint32_t)(((uint64_t)__umulhi(x, m) + x) >> s);
+  }
+};
+
 // Issue priority of the latency-bound per-hop kernels (prep, row sampling, compaction,
 // relabel) over co-resident waves of the throughput-bound hub kernels of other batches in
 // flight (s_setprio; 0 = the hardware default).

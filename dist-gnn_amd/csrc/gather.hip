@@ -63,23 +63,6 @@ struct VecT<1> {
   using T = uint8_t;
 };
 
-// x / d for 32-bit x via multiply-high (Granlund-Montgomery).
-struct FastDivU32 {
-  uint32_t d, m, s;
-  static FastDivU32 make(uint32_t d) {
-    FastDivU32 f;
-    f.d = d;
-    uint32_t s = 0;
-    while ((uint64_t(1) << s) < d) ++s;
-    f.s = s;
-    f.m = (uint32_t)(((uint64_t(1) << 32) * ((uint64_t(1) << s) - d)) / d + 1);
-    return f;
-  }
-  __device__ __forceinline__ uint32_t div(uint32_t x) const {
-    return (uint32_t)(((uint64_t)__umulhi(x, m) + x) >> s);
-  }
-};
-
 // Row sources.  row_ptr(r) = address of output row r's source row.  Each is split in two
 // stages (id load, then address) so the kernel can batch the loads of its U chunks.
 template <typename IdT>

@@ -8,6 +8,9 @@
 // groups of 64.  b is exact for bfloat16 inputs, and the codes are taken against the rounded s
 // and b, so their rounding costs at most 15 s / 512 + |b| / 512 at the ends of the range.  A group
 // that holds a NaN or an infinity, or whose s or b is not finite, reads back as NaN (s = b = NaN).
+#include <algorithm>
+
+#include "dgs_lane.cuh"
 #include "dgs_state.cuh"
 
 namespace dgs {
@@ -24,22 +27,60 @@ __device__ __forceinline__ uint32_t bf16_rne(float x) {
   return v.u;
 }
 
-// One code.  The quotient in 32 bits is off by at most 2.5 of its units in the last place (one
-// rounding in x - b, one in the reciprocal, one in the product), 2.5e-6 below 16; within 1e-5 of
-// a rounding border, and for scales too small for a normal reciprocal, it is taken in 64 bits,
-// where x - b and s are exact and the quotient's distance from a border survives its rounding.
-__device__ __forceinline__ uint32_t code_of(float x, float b, float s, float inv, bool tiny) {
-  const float t = (x - b) * inv;
-  float r = rintf(t);
-  if (tiny || fabsf(fabsf(t - r) - 0.5f) < 1e-5f)
-    r = s == 0.f ? 0.f : (float)rint(fmin(fmax(((double)x - (double)b) / (double)s, -1.0), 16.0));
-  return (uint32_t)fminf(fmaxf(r, 0.f), 15.f);
+// The eight codes of a word.  The quotient in 32 bits is off by at most 2.5 of its units in the
+// last place (one rounding in x - b, one in the reciprocal, one in the product), 2.5e-6 below 16.
+// Within 1e-5 of a rounding border h (a multiple of a half) the sign of (x - b) - h s decides, which
+// 32 bits give exactly: h s has 13 bits, the difference to the rounded x - b is exact because the two
+// nearly cancel, and what x - b lost in rounding is added (an error-free difference).  Scales too
+// small for a normal reciprocal take the quotient in 64 bits, where it is exact enough by far.
+constexpr float kNear = 0.5f - 1e-5f;
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float b, float s) {
+  if (!(s >= 1e-30f)) {
+    uint32_t w = 0;
+    for (int i = 0; i < 8; ++i) {
+      const double t = s == 0.f ? 0. : ((double)x[i] - (double)b) / (double)s;
+      w |= (uint32_t)fmin(fmax(rint(t), 0.), 15.) << (4 * i);
+    }
+    return w;
+  }
+  const float inv = 1.f / s;
+  uint32_t w = 0;
+  float far = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float t = (x[i] - b) * inv, r = rintf(t);
+    far = fmaxf(far, fabsf(t - r));
+    w |= (uint32_t)fminf(fmaxf(r, 0.f), 15.f) << (4 * i);
+  }
+  if (far <= kNear) return w;
+  // One channel near a border at a time: of bfloat16 inputs one in some hundreds lies on one, so
+  // that most waves have a few, but hardly a lane two.
+  uint32_t near = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float t = (x[i] - b) * inv;
+    near |= (fabsf(t - rintf(t)) > kNear ? 1u : 0u) << i;
+  }
+  while (near) {
+    const int i = __ffs(near) - 1;
+    near &= near - 1;
+    float v = x[0];
+#pragma unroll
+    for (int y = 1; y < 8; ++y) v = i == y ? x[y] : v;
+    const float d = v - b, back = v - d;
+    const float lost = (back - b) + (v - (d + back));
+    const float low = floorf(d * inv), h = low + 0.5f;
+    const float e = __builtin_fmaf(-h, s, d) + lost;
+    const float r = e > 0.f || (e == 0.f && ((int)low & 1)) ? low + 1.f : low;
+    w = (w & ~(15u << (4 * i))) | (uint32_t)fminf(fmaxf(r, 0.f), 15.f) << (4 * i);
+  }
+  return w;
 }
 
 struct WriteArgs {
   StateView c;
   StateRows x;
-  int64_t n;
+  int64_t n, t0;  // tokens, the launch's first
   const int64_t *slots;  // flat slots, or null: append
   IdArray table, lens;
   int64_t width;
@@ -71,90 +112,128 @@ __device__ __forceinline__ int64_t write_slot(const WriteArgs &a, int64_t t, boo
   return (page << a.c.pshift) | (len & ((int64_t(1) << a.c.pshift) - 1));
 }
 
-// LPG lanes (a power of two, at least group / 8) share a group; a lane holds eight channels.
-template <int TYPE>
-__global__ __launch_bounds__(kThreads) void k_state_write(WriteArgs a, int lpg_shift) {
-  const int lpg = 1 << lpg_shift, words = a.c.group >> 3, ng = a.c.dim / a.c.group;
-  const int64_t units = a.n * 2 * a.c.heads * ng;
-  const int64_t u =
-      ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> lpg_shift;
-  if (u >= units) return;  // whole groups of lanes leave together
-  const int sub = threadIdx.x & (lpg - 1);
-  const int g = (int)(u % ng);
-  const int64_t r = u / ng;
-  const int h = (int)(r % a.c.heads);
-  const int kv = (int)((r / a.c.heads) & 1);
-  const int64_t t = r / (2 * a.c.heads);
-  const int64_t slot = write_slot(a, t, sub == 0);
-  if (a.slots_out && sub == 0 && g == 0 && h == 0 && kv == 0) a.slots_out[t] = slot;
-  if (slot < 0) return;
+// lpg lanes (a power of two, at least group / 8) share a group; a lane holds eight channels.  Block
+// row y: 0 = K, 1 = V.  A group of lanes takes kWU units (group `g` of head h of token t: unit (t heads
+// + h) ng + g) at a time, for their loads to overlap.  Bound by HBM: 65536 tokens of 8 heads x 128
+// bfloat16 channels to scattered slots (343 MB) in MEASURED_WRITE.
+constexpr int kWU = 4;
+template <int TYPE, int LPG>
+__global__ __launch_bounds__(kThreads) void k_state_write(WriteArgs a, uint32_t units,
+                                                          FastDivU32 per_token, FastDivU32 per_head) {
+  const int words = a.c.group >> 3, ng = (int)per_head.d;
+  const int sub = threadIdx.x % LPG;
   const bool live = sub < words;
-  const int ch = g * a.c.group + (live ? sub : 0) * 8;
-  float x[8];
-  if (kv == 0)
-    load8<TYPE>(a.x.k, t * a.x.kt + h * a.x.kh + ch, x);
-  else
-    load8<TYPE>(a.x.v, t * a.x.vt + h * a.x.vh + ch, x);
-  float lo = x[0], hi = x[0], bad = 0.f;
+  const int kv = blockIdx.y;
+  const uint32_t u0 = blockIdx.x * (kThreads / LPG * kWU) + threadIdx.x / LPG;
+  const void *src = kv ? a.x.v : a.x.k;
+  const int64_t st = kv ? a.x.vt : a.x.kt, sh = kv ? a.x.vh : a.x.kh;
+  float x[kWU][8];
+  int64_t slot[kWU];
+  int h[kWU], g[kWU];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-    bad += x[i] - x[i];  // NaN when x is NaN or infinite
+  for (int i = 0; i < kWU; ++i) {
+    const uint32_t u = u0 + i * (kThreads / LPG);
+    const bool in = u < units;
+    const uint32_t t = in ? per_token.div(u) : 0, r = in ? u - t * per_token.d : 0;
+    h[i] = (int)per_head.div(r);
+    g[i] = (int)(r - h[i] * per_head.d);
+    slot[i] = in ? write_slot(a, a.t0 + t, sub == 0) : -1;
+    if (in && a.slots_out && sub == 0 && r == 0 && kv == 0) a.slots_out[a.t0 + t] = slot[i];
+    load8<TYPE>(src, (a.t0 + t) * st + h[i] * sh + g[i] * a.c.group + (live ? sub : 0) * 8, x[i]);
   }
-  for (int o = lpg >> 1; o > 0; o >>= 1) {
-    lo = fminf(lo, __shfl_xor(lo, o, 64));
-    hi = fmaxf(hi, __shfl_xor(hi, o, 64));
-    bad += __shfl_xor(bad, o, 64);
-  }
-  uint32_t sb = bf16_rne((hi - lo) * (1.f / 15.f)), bb = bf16_rne(lo);
-  const float s = bf16_bits(sb << 16), b = bf16_bits(bb << 16);
-  const bool nan = !(bad == 0.f) || !(s - s == 0.f) || !(b - b == 0.f);
-  uint32_t w = 0;
-  if (!nan) {
-    const bool tiny = !(s >= 1e-30f);
-    const float inv = tiny ? 0.f : 1.f / s;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w |= code_of(x[i], b, s, inv, tiny) << (4 * i);
-  } else {
-    sb = bb = 0x7fc0u;
+  for (int i = 0; i < kWU; ++i) {
+    // NaN passes through minimum and maximum, an infinity shows in the range
+    float lo = x[i][0], hi = x[i][0];
+#pragma unroll
+    for (int y = 1; y < 8; ++y) {
+      lo = __builtin_elementwise_minimum(lo, x[i][y]);
+      hi = __builtin_elementwise_maximum(hi, x[i][y]);
+    }
+#pragma unroll
+    for (int o = 1; o < LPG; o <<= 1) {
+      lo = __builtin_elementwise_minimum(lo, lane_xor32v(lo, o));
+      hi = __builtin_elementwise_maximum(hi, lane_xor32v(hi, o));
+    }
+    if (slot[i] < 0) continue;
+    const float range = hi - lo;
+    uint32_t sb = bf16_rne(range * (1.f / 15.f)), bb = bf16_rne(lo);
+    const float s = bf16_bits(sb << 16), b = bf16_bits(bb << 16);
+    uint32_t w = 0;
+    if (range - range == 0.f && b - b == 0.f)
+      w = codes_of(x[i], b, s);
+    else
+      sb = bb = 0x7fc0u;
+    const int64_t row = (((slot[i] >> a.c.pshift) * a.c.heads + h[i]) << a.c.pshift) +
+                        (slot[i] & ((int64_t(1) << a.c.pshift) - 1));
+    if (live)
+      *(uint32_t *)((kv ? a.c.vc : a.c.kc) + row * (a.c.dim >> 1) + ((g[i] * a.c.group) >> 1) +
+                    4 * sub) = w;
+    if (sub == 0) (kv ? a.c.vs : a.c.ks)[row * ng + g[i]] = sb | (bb << 16);
   }
-  const int64_t page = slot >> a.c.pshift;
-  const int64_t row = ((page * a.c.heads + h) << a.c.pshift) +
-                      (slot & ((int64_t(1) << a.c.pshift) - 1));
-  if (live)
-    *(uint32_t *)((kv ? a.c.vc : a.c.kc) + row * (a.c.dim >> 1) + (ch >> 1)) = w;
-  if (sub == 0) (kv ? a.c.vs : a.c.ks)[row * ng + g] = sb | (bb << 16);
 }
 
+// A lane writes 16 bytes of output (four or eight channels): piece i of K (block row 0) or V (1) is
+// the i-th 16 bytes of the output.  kRU pieces a lane are in flight.  Bound by HBM: MEASURED_READ.
+constexpr int kRU = 4;
 template <int TYPE>
 __global__ __launch_bounds__(kThreads) void k_state_read(StateView c, const int64_t *slots,
-                                                         int64_t n, void *k_out, void *v_out,
+                                                         uint32_t pieces, FastDivU32 per_row,
+                                                         FastDivU32 heads, void *out_k, void *out_v,
                                                          GatherGuard gd) {
-  const int words = c.dim >> 3;
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (i >= n * 2 * c.heads * words) return;
-  const int w = (int)(i % words);
-  const int64_t r = i / words;
-  const int h = (int)(r % c.heads);
-  const int64_t t = (r / c.heads) >> 1;
-  const int kv = (int)((r / c.heads) & 1);
-  const int64_t slot = slots[t];
+  constexpr int kCh = TYPE == kStateF32 ? 4 : 8;
+  const int kv = blockIdx.y, ng = c.dim / c.group;
+  const uint8_t *codes = kv ? c.vc : c.kc;
+  const uint32_t *words = kv ? c.vs : c.ks;
   const uint64_t total = (uint64_t)c.pages << c.pshift;
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (slot >= 0 && (uint64_t)slot < total) {
-    const int64_t row = (((slot >> c.pshift) * c.heads + h) << c.pshift) +
-                        (slot & ((int64_t(1) << c.pshift) - 1));
-    const uint32_t q = *(const uint32_t *)((kv ? c.vc : c.kc) + row * (c.dim >> 1) + 4 * w);
-    const uint32_t m = (kv ? c.vs : c.ks)[row * (c.dim / c.group) + (8 * w) / c.group];
-    const float s = scale_of(m), b = base_of(m);
-    codes8(q, x);
+  const uint32_t i0 = blockIdx.x * (kThreads * kRU) + threadIdx.x;
+  uint32_t q[kRU], m[kRU];
+  int64_t slot[kRU];
+  uint32_t h[kRU], ch[kRU];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = x[j] * s + b;
-  } else if (slot >= 0 && w == 0 && h == 0 && kv == 0) {
-    report_bad_id(gd.err, kAsyncErrSlot, slot, total, gd.tag);
+  for (int u = 0; u < kRU; ++u) {
+    uint32_t i = i0 + u * kThreads;
+    i = i < pieces ? i : pieces - 1;
+    const uint32_t r = per_row.div(i), t = heads.div(r);
+    ch[u] = (i - r * per_row.d) * kCh;
+    h[u] = r - t * heads.d;
+    slot[u] = slots[t];
   }
-  store8<TYPE>(kv ? v_out : k_out, (t * c.heads + h) * c.dim + 8 * w, x);
+#pragma unroll
+  for (int u = 0; u < kRU; ++u) {
+    const bool in = slot[u] >= 0 && (uint64_t)slot[u] < total;
+    if (!in && slot[u] >= 0 && ch[u] == 0 && h[u] == 0 && kv == 0)
+      report_bad_id(gd.err, kAsyncErrSlot, slot[u], total, gd.tag);
+    const int64_t s = in ? slot[u] : 0;
+    const int64_t row = (((s >> c.pshift) * c.heads + h[u]) << c.pshift) +
+                        (s & ((int64_t(1) << c.pshift) - 1));
+    const uint8_t *at = codes + row * (c.dim >> 1) + (ch[u] >> 1);
+    if constexpr (TYPE == kStateF32)
+      q[u] = *(const uint16_t *)at;
+    else
+      q[u] = *(const uint32_t *)at;
+    m[u] = words[row * ng + ch[u] / (uint32_t)c.group];
+    if (!in) q[u] = m[u] = 0;
+  }
+#pragma unroll
+  for (int u = 0; u < kRU; ++u) {
+    const uint32_t i = i0 + u * kThreads;
+    if (i >= pieces) break;
+    float x[8];
+    codes8(q[u], x);
+    const float s = scale_of(m[u]), b = base_of(m[u]);
+#pragma unroll
+    for (int y = 0; y < kCh; ++y) x[y] = x[y] * s + b;
+    su32x4 *dst = (su32x4 *)(kv ? out_v : out_k) + i;
+    su32x4 v;
+    if constexpr (TYPE == kStateF32) {
+#pragma unroll
+      for (int y = 0; y < 4; ++y) v[y] = __float_as_uint(x[y]);
+    } else {
+      store8<TYPE>(&v, 0, x);
+    }
+    __builtin_nontemporal_store(v, dst);
+  }
 }
 
 int shift_of(int words) {
@@ -163,18 +242,47 @@ int shift_of(int words) {
   return s;
 }
 
-void launch_write(const WriteArgs &a, StateType type, hipStream_t st) {
-  if (a.n <= 0) return;
+template <int TYPE>
+void launch_write_t(const WriteArgs &a, int64_t n, hipStream_t st) {
   const int sh = shift_of(a.c.group >> 3);
-  const int64_t lanes = (a.n * 2 * a.c.heads * (a.c.dim / a.c.group)) << sh;
-  const int64_t blocks = ceil_div(lanes, kThreads);
-  DGS_CHECK(blocks < (int64_t(1) << 31), "state write: too many rows in one call");
-  if (type == kStateF32)
-    k_state_write<kStateF32><<<(unsigned)blocks, kThreads, 0, st>>>(a, sh);
-  else if (type == kStateBF16)
-    k_state_write<kStateBF16><<<(unsigned)blocks, kThreads, 0, st>>>(a, sh);
-  else
-    k_state_write<kStateF16><<<(unsigned)blocks, kThreads, 0, st>>>(a, sh);
+  const uint32_t ng = a.c.dim / a.c.group, per_token = a.c.heads * ng;
+  const uint32_t units = (uint32_t)(n * per_token);
+  const FastDivU32 ft = FastDivU32::make(per_token), fh = FastDivU32::make(ng);
+  const dim3 grid((unsigned)ceil_div((int64_t)units << sh, kThreads * kWU), 2);
+  switch (sh) {
+    case 0: k_state_write<TYPE, 1><<<grid, kThreads, 0, st>>>(a, units, ft, fh); break;
+    case 1: k_state_write<TYPE, 2><<<grid, kThreads, 0, st>>>(a, units, ft, fh); break;
+    case 2: k_state_write<TYPE, 4><<<grid, kThreads, 0, st>>>(a, units, ft, fh); break;
+    case 3: k_state_write<TYPE, 8><<<grid, kThreads, 0, st>>>(a, units, ft, fh); break;
+    case 4: k_state_write<TYPE, 16><<<grid, kThreads, 0, st>>>(a, units, ft, fh); break;
+    default: k_state_write<TYPE, 32><<<grid, kThreads, 0, st>>>(a, units, ft, fh); break;
+  }
+  DGS_LAUNCH_CHECK();
+}
+// Units and pieces of a launch are counted in 32 bits: more tokens take several launches.
+int64_t tokens_a_launch(const StateView &c) {
+  return std::max<int64_t>(1, (int64_t(1) << 30) / ((int64_t)c.heads * c.dim));
+}
+void launch_write(WriteArgs a, StateType type, hipStream_t st) {
+  const int64_t step = tokens_a_launch(a.c);
+  for (a.t0 = 0; a.t0 < a.n; a.t0 += step) {
+    const int64_t n = std::min(step, a.n - a.t0);
+    if (type == kStateF32)
+      launch_write_t<kStateF32>(a, n, st);
+    else if (type == kStateBF16)
+      launch_write_t<kStateBF16>(a, n, st);
+    else
+      launch_write_t<kStateF16>(a, n, st);
+  }
+}
+template <int TYPE>
+void launch_read(const StateView &c, const int64_t *slots, int64_t n, void *k_out, void *v_out,
+                 const GatherGuard &gd, hipStream_t st) {
+  constexpr int kCh = TYPE == kStateF32 ? 4 : 8;
+  const uint32_t pieces = (uint32_t)(n * c.heads * (c.dim / kCh));
+  const dim3 grid((unsigned)ceil_div(pieces, kThreads * kRU), 2);
+  const FastDivU32 fr = FastDivU32::make(c.dim / kCh), fh = FastDivU32::make(c.heads);
+  k_state_read<TYPE><<<grid, kThreads, 0, st>>>(c, slots, pieces, fr, fh, k_out, v_out, gd);
   DGS_LAUNCH_CHECK();
 }
 
@@ -210,16 +318,18 @@ void state_read(const StateView &c, const int64_t *slots, int64_t n, StateType t
                 void *v_out, hipStream_t st) {
   if (n <= 0) return;
   const GatherGuard gd = state_guard(kAsyncErrSlot, c.pages);
-  const int64_t blocks = ceil_div(n * 2 * c.heads * (c.dim >> 3), kThreads);
-  DGS_CHECK(blocks < (int64_t(1) << 31), "state read: too many rows in one call");
-  if (type == kStateF32)
-    k_state_read<kStateF32><<<(unsigned)blocks, kThreads, 0, st>>>(c, slots, n, k_out, v_out, gd);
-  else if (type == kStateBF16)
-    k_state_read<kStateBF16>
-        <<<(unsigned)blocks, kThreads, 0, st>>>(c, slots, n, k_out, v_out, gd);
-  else
-    k_state_read<kStateF16><<<(unsigned)blocks, kThreads, 0, st>>>(c, slots, n, k_out, v_out, gd);
-  DGS_LAUNCH_CHECK();
+  const int64_t step = tokens_a_launch(c);
+  const int64_t row = (int64_t)c.heads * c.dim * (type == kStateF32 ? 4 : 2);
+  for (int64_t t = 0; t < n; t += step) {
+    const int64_t m = std::min(step, n - t);
+    void *k = (char *)k_out + t * row, *v = (char *)v_out + t * row;
+    if (type == kStateF32)
+      launch_read<kStateF32>(c, slots + t, m, k, v, gd, st);
+    else if (type == kStateBF16)
+      launch_read<kStateBF16>(c, slots + t, m, k, v, gd, st);
+    else
+      launch_read<kStateF16>(c, slots + t, m, k, v, gd, st);
+  }
 }
 
 }  // namespace dgs
