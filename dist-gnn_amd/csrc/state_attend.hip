@@ -29,14 +29,26 @@ __device__ __forceinline__ float sum_lanes(float x) {
   return x;
 }
 
+// x of lane u of this lane's four.
+__device__ __forceinline__ uint32_t of_quad(uint32_t x, int u) {
+  switch (u) {
+    case 0: return (uint32_t)dpp_keep<0x00>((int32_t)x, (int32_t)x);
+    case 1: return (uint32_t)dpp_keep<0x55>((int32_t)x, (int32_t)x);
+    case 2: return (uint32_t)dpp_keep<0xAA>((int32_t)x, (int32_t)x);
+    default: return (uint32_t)dpp_keep<0xFF>((int32_t)x, (int32_t)x);
+  }
+}
+
 // Vector form, for every type and size.  A work item is (row, head, GC query heads, split).  LPR
-// lanes hold a row (eight channels each); SL groups of them take every SL-th slot with a softmax
-// state of their own, joined at the end by exchanges between lanes.  kU slots a group are loaded
-// while the kU before them are computed, ids another step ahead.  As in the matrix form, the
-// running maximum is only followed when a logit passes it by 8.
+// lanes hold a row (eight channels each); SL groups of them take four slots in a row at a time, with
+// a softmax state of their own, joined at the end by exchanges between lanes.  Rows are loaded one
+// step ahead of the arithmetic, ids another one.  What belongs to a slot and not to a channel - its
+// page and address, and with QG (groups of a multiple of 32 channels) its scale and base - is fetched
+// by one lane of every four and passed on by lane moves: 11 loads a step instead of 24.  As in the
+// matrix form, the running maximum is only followed when a logit passes it by 8.
 // SL = 1 is for rows of at most 16 slots: no join, and with all query heads of a head in the item
 // the probabilities stay in registers and the item writes its weights itself.
-template <int LPR, int SL, int GC>
+template <int LPR, int SL, int GC, bool QG>
 __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type, int gchunks,
                                                          int64_t items) {
   constexpr int kItem = LPR * SL, kU = 4, kStep = SL * kU;
@@ -45,7 +57,7 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
   int64_t item64 = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / kItem;
   if (item64 >= items) return;  // whole items leave together: no exchange crosses an item
   uint32_t item = (uint32_t)item64;
-  const int sub = lane % LPR, sl = lane / LPR;
+  const int sub = lane % LPR, sl = lane / LPR, mine = sub & 3;  // mine: the slot of four I look up
   const int split = (int)(item % (uint32_t)a.splits);
   item /= (uint32_t)a.splits;
   const int gc = (int)(item % (uint32_t)gchunks);
@@ -83,45 +95,53 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
   const int ps = a.c.pshift, mask = (1 << ps) - 1;
   const bool wide = a.table.bytes == 8;
   const char *tab = (const char *)a.table.p + ((row * a.width) << (wide ? 3 : 2));
-  const uint32_t pages = (uint32_t)a.c.pages;
-  uint32_t id[kU], id_hi[kU];
+  const uint32_t pages = (uint32_t)a.c.pages, half = (uint32_t)a.c.dim >> 1;
+  uint32_t id = 0, id_hi = 0;  // of my slot of the next step
   struct Rows {
-    uint32_t kq[kU], vq[kU], km[kU], vm[kU], ok;
+    uint32_t kq[kU], vq[kU], km[QG ? 1 : kU], vm[QG ? 1 : kU], ok;
   };
   Rows t;
-  auto slot_of = [&](int j0, int u) {
-    const int j = j0 + u * SL + sl;
+  auto slot_of = [&](int j0) {
+    const int j = j0 + sl * kU + mine;
     return j < last ? j : last - 1;
   };
   auto load_ids = [&](int j0) {
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const char *at = tab + ((int64_t)(slot_of(j0, u) >> ps) << (wide ? 3 : 2));
-      id[u] = *(const uint32_t *)at;
-      id_hi[u] = *(const uint32_t *)(at + (wide ? 4 : 0));
-    }
+    const char *at = tab + ((int64_t)(slot_of(j0) >> ps) << (wide ? 3 : 2));
+    id = *(const uint32_t *)at;
+    if (wide) id_hi = *(const uint32_t *)(at + 4);
   };
+  // Loads a step's rows, and before them the next step's ids: memory returns in order, so whoever
+  // waits for an id would wait for rows issued before it.
   auto load_rows = [&](int j0) {
-    t.ok = 0;
-    uint32_t page[kU];
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const bool in = j0 + u * SL + sl < last;
-      const bool out = id[u] >= pages || (wide && id_hi[u] != 0);
-      if (out && in && sub == 0)
-        report_bad_id(a.gd.err, kAsyncErrSlot,
-                      wide ? (int64_t)((uint64_t)id_hi[u] << 32 | id[u]) : (int64_t)(int32_t)id[u],
-                      pages, a.gd.tag);
-      page[u] = out ? 0u : id[u];
-      t.ok |= (in && !out ? 1u : 0u) << u;
+    const bool in = j0 + sl * kU + mine < last;
+    const bool out = id >= pages || id_hi != 0;
+    if (out && in && sub < 4)
+      report_bad_id(a.gd.err, kAsyncErrSlot,
+                    wide ? (int64_t)((uint64_t)id_hi << 32 | id) : (int64_t)(int32_t)id, pages,
+                    a.gd.tag);
+    const uint32_t page = out ? 0u : id;
+    const int64_t r = (((int64_t)page * a.c.heads + h) << ps) + (slot_of(j0) & mask);
+    const uint64_t at = (uint64_t)r * half;
+    const uint32_t good = in && !out ? 1u : 0u;
+    load_ids(j0 + kStep);
+    if constexpr (QG) {
+      t.km[0] = a.c.ks[r * ng + grp];
+      t.vm[0] = a.c.vs[r * ng + grp];
     }
+    t.ok = 0;
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      const int64_t r = (((int64_t)page[u] * a.c.heads + h) << ps) + (slot_of(j0, u) & mask);
-      t.kq[u] = *(const uint32_t *)(a.c.kc + r * (a.c.dim >> 1) + 4 * w);
-      t.vq[u] = *(const uint32_t *)(a.c.vc + r * (a.c.dim >> 1) + 4 * w);
-      t.km[u] = a.c.ks[r * ng + grp];
-      t.vm[u] = a.c.vs[r * ng + grp];
+      const uint64_t to =
+          ((uint64_t)of_quad((uint32_t)(at >> 32), u) << 32 | of_quad((uint32_t)at, u)) + 4 * w;
+      t.kq[u] = *(const uint32_t *)(a.c.kc + to);
+      t.vq[u] = *(const uint32_t *)(a.c.vc + to);
+      t.ok |= of_quad(good, u) << u;
+      if constexpr (!QG) {
+        const uint64_t rw = ((uint64_t)of_quad((uint32_t)((uint64_t)r >> 32), u) << 32 |
+                             of_quad((uint32_t)r, u)) * ng + grp;
+        t.km[u] = a.c.ks[rw];
+        t.vm[u] = a.c.vs[rw];
+      }
     }
   };
   auto compute = [&](const Rows &t, int j0, int keep) {
@@ -129,7 +149,8 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       const bool ok = (t.ok >> u) & 1;
-      const uint32_t km = live ? t.km[u] : 0u;
+      const uint32_t kw = QG ? of_quad(t.km[0], u) : t.km[QG ? 0 : u];
+      const uint32_t km = live ? kw : 0u;
       const float ks = scale_of(km), kb = base_of(km);
       float kv[8];
       codes8(t.kq[u], kv);
@@ -156,10 +177,10 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
     if (a.logits && sub == 0) {
 #pragma unroll
       for (int u = 0; u < kU; ++u)
-        if (j0 + u * SL + sl < last)
+        if (j0 + sl * kU + u < last)
 #pragma unroll
           for (int g = 0; g < GC; ++g)
-            if (g < gn) a.logits[(row * a.q_heads + a0 + g) * a.cap + j0 + u * SL + sl] = x[g][u];
+            if (g < gn) a.logits[(row * a.q_heads + a0 + g) * a.cap + j0 + sl * kU + u] = x[g][u];
     }
 #pragma unroll
     for (int g = 0; g < GC; ++g) {
@@ -180,7 +201,8 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
     }
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      const uint32_t vm = live && ((t.ok >> u) & 1) ? t.vm[u] : 0u;
+      const uint32_t vw = QG ? of_quad(t.vm[0], u) : t.vm[QG ? 0 : u];
+      const uint32_t vm = live && ((t.ok >> u) & 1) ? vw : 0u;
       const float vs = scale_of(vm), vb = base_of(vm);
       float vv[8];
       codes8(t.vq[u], vv);
@@ -195,16 +217,12 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
   if (first < last) {
     load_ids(first);
     load_rows(first);
-    load_ids(first + kStep);
     if constexpr (SL == 1) {
 #pragma unroll
       for (int st = 0; st < 4; ++st) {
         if (4 * st >= last) break;
         const Rows now = t;
-        if (4 * st + 4 < last) {
-          load_rows(4 * st + 4);
-          load_ids(4 * st + 8);
-        }
+        if (4 * st + 4 < last) load_rows(4 * st + 4);
         compute(now, 4 * st, 4 * st);
       }
     } else {
@@ -212,7 +230,6 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
       for (int j0 = first; j0 < last; j0 += kStep) {
         const Rows now = t;
         load_rows(j0 + kStep);
-        load_ids(j0 + 2 * kStep);
         compute(now, j0, 0);
       }
     }
@@ -415,27 +432,35 @@ int pow2_at_least(int x) {
   return p;
 }
 
-template <int LPR, int SL>
+template <int LPR, int SL, bool QG>
 void launch_vec_g(const AttendArgs &a, int type, hipStream_t st) {
   const int gc = vec_gc(a.g), gchunks = vec_gchunks(a.g);
   const int64_t items = a.rows * a.c.heads * gchunks * a.splits;
   const int64_t blocks = ceil_div(items * LPR * SL, kThreads);
   DGS_CHECK(blocks < (int64_t(1) << 31) && items < (int64_t(1) << 31),
             "attend: too many rows in one call");
+  const unsigned grid = (unsigned)blocks;
   if (gc == 4)
-    k_attend_vec<LPR, SL, 4><<<(unsigned)blocks, kThreads, 0, st>>>(a, type, gchunks, items);
+    k_attend_vec<LPR, SL, 4, QG><<<grid, kThreads, 0, st>>>(a, type, gchunks, items);
   else if (gc == 2)
-    k_attend_vec<LPR, SL, 2><<<(unsigned)blocks, kThreads, 0, st>>>(a, type, gchunks, items);
+    k_attend_vec<LPR, SL, 2, QG><<<grid, kThreads, 0, st>>>(a, type, gchunks, items);
   else
-    k_attend_vec<LPR, SL, 1><<<(unsigned)blocks, kThreads, 0, st>>>(a, type, gchunks, items);
+    k_attend_vec<LPR, SL, 1, QG><<<grid, kThreads, 0, st>>>(a, type, gchunks, items);
   DGS_LAUNCH_CHECK();
+}
+template <int LPR, int SL>
+void launch_vec_s(const AttendArgs &a, int type, hipStream_t st) {
+  if (a.c.group % 32 == 0)
+    launch_vec_g<LPR, SL, true>(a, type, st);
+  else
+    launch_vec_g<LPR, SL, false>(a, type, st);
 }
 template <int LPR>
 void launch_vec(const AttendArgs &a, int type, hipStream_t st) {
   if (a.cap <= 16)
-    launch_vec_g<LPR, 1>(a, type, st);
+    launch_vec_s<LPR, 1>(a, type, st);
   else
-    launch_vec_g<LPR, 64 / LPR>(a, type, st);
+    launch_vec_s<LPR, 64 / LPR>(a, type, st);
 }
 
 }  // namespace
@@ -481,8 +506,8 @@ void state_attend(const StateView &c, const AttendCall &call, void *ws, int64_t 
     (c.group == 32 ? attend_matrix_32 : c.group == 64 ? attend_matrix_64 : attend_matrix_128)(
         a, p.waves, call.type, st);
   } else switch (pow2_at_least(c.dim >> 3)) {
-    case 1: launch_vec<1>(a, call.type, st); break;
-    case 2: launch_vec<2>(a, call.type, st); break;
+    case 1:
+    case 2:
     case 4: launch_vec<4>(a, call.type, st); break;
     case 8: launch_vec<8>(a, call.type, st); break;
     case 16: launch_vec<16>(a, call.type, st); break;
