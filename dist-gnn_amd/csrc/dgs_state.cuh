@@ -14,14 +14,18 @@ __device__ __forceinline__ float bf16_bits(uint32_t hi) { return __uint_as_float
 __device__ __forceinline__ float scale_of(uint32_t m) { return __uint_as_float(m << 16); }
 __device__ __forceinline__ float base_of(uint32_t m) { return __uint_as_float(m & 0xffff0000u); }
 
-// The eight codes of a word as floats, in channel order.
+// The eight codes of a word as floats, in channel order.  (Byte i of a word as a float is one
+// instruction; written in C it becomes a field extraction and a conversion.)
 __device__ __forceinline__ void codes8(uint32_t w, float (&c)[8]) {
   const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    c[2 * i] = (float)((lo >> (8 * i)) & 0xffu);
-    c[2 * i + 1] = (float)((hi >> (8 * i)) & 0xffu);
-  }
+  asm("v_cvt_f32_ubyte0_e32 %0, %1" : "=v"(c[0]) : "v"(lo));
+  asm("v_cvt_f32_ubyte0_e32 %0, %1" : "=v"(c[1]) : "v"(hi));
+  asm("v_cvt_f32_ubyte1_e32 %0, %1" : "=v"(c[2]) : "v"(lo));
+  asm("v_cvt_f32_ubyte1_e32 %0, %1" : "=v"(c[3]) : "v"(hi));
+  asm("v_cvt_f32_ubyte2_e32 %0, %1" : "=v"(c[4]) : "v"(lo));
+  asm("v_cvt_f32_ubyte2_e32 %0, %1" : "=v"(c[5]) : "v"(hi));
+  asm("v_cvt_f32_ubyte3_e32 %0, %1" : "=v"(c[6]) : "v"(lo));
+  asm("v_cvt_f32_ubyte3_e32 %0, %1" : "=v"(c[7]) : "v"(hi));
 }
 
 // Eight consecutive values of a row (16-byte aligned) <-> floats.

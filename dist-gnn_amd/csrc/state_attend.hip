@@ -49,21 +49,18 @@ __device__ __forceinline__ uint32_t of_quad(uint32_t x, int u) {
 // SL = 1 is for rows of at most 16 slots: no join, and with all query heads of a head in the item
 // the probabilities stay in registers and the item writes its weights itself.
 template <int LPR, int SL, int GC, bool QG>
-__global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type, int gchunks,
-                                                         int64_t items) {
+__global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
+                                                         FastDivU32 splits, FastDivU32 gchunks,
+                                                         FastDivU32 heads, uint32_t items) {
   constexpr int kItem = LPR * SL, kU = 4, kStep = SL * kU;
   constexpr int kKeep = SL > 1 ? 1 : (LPR >= 16 ? 1 : 16 / LPR);
   const int lane = threadIdx.x & (kItem - 1);
-  int64_t item64 = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / kItem;
-  if (item64 >= items) return;  // whole items leave together: no exchange crosses an item
-  uint32_t item = (uint32_t)item64;
+  const uint32_t item = (blockIdx.x * (uint32_t)kThreads + threadIdx.x) / kItem;
+  if (item >= items) return;  // whole items leave together: no exchange crosses an item
   const int sub = lane % LPR, sl = lane / LPR, mine = sub & 3;  // mine: the slot of four I look up
-  const int split = (int)(item % (uint32_t)a.splits);
-  item /= (uint32_t)a.splits;
-  const int gc = (int)(item % (uint32_t)gchunks);
-  item /= (uint32_t)gchunks;
-  const int h = (int)(item % (uint32_t)a.c.heads);
-  const int64_t row = item / (uint32_t)a.c.heads;
+  const uint32_t is = splits.div(item), ig = gchunks.div(is), row = heads.div(ig);
+  const int split = (int)(item - is * splits.d), gc = (int)(is - ig * gchunks.d);
+  const int h = (int)(ig - row * heads.d);
   const int words = a.c.dim >> 3;
   const bool live = sub < words;
   const int w = live ? sub : 0, ng = a.c.dim / a.c.group, grp = 8 * w / a.c.group;
@@ -77,7 +74,7 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
 #pragma unroll
   for (int g = 0; g < GC; ++g) {
     if (live && g < gn) {
-      load_q(type, a.q, row * a.q_row + (a0 + g) * a.q_head + 8 * w, q[g]);
+      load_q(type, a.q, (int64_t)row * a.q_row + (a0 + g) * a.q_head + 8 * w, q[g]);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) q[g][i] = 0.f;
@@ -94,11 +91,13 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
   }
   const int ps = a.c.pshift, mask = (1 << ps) - 1;
   const bool wide = a.table.bytes == 8;
-  const char *tab = (const char *)a.table.p + ((row * a.width) << (wide ? 3 : 2));
+  const char *tab = (const char *)a.table.p + (((int64_t)row * a.width) << (wide ? 3 : 2));
   const uint32_t pages = (uint32_t)a.c.pages, half = (uint32_t)a.c.dim >> 1;
   uint32_t id = 0, id_hi = 0;  // of my slot of the next step
   struct Rows {
-    uint32_t kq[kU], vq[kU], km[QG ? 1 : kU], vm[QG ? 1 : kU], ok;
+    uint32_t kq[kU], vq[kU], km[QG ? 1 : kU], vm[QG ? 1 : kU];
+    int n;         // slots of the step before the end
+    uint32_t bad;  // bit u: slot u's page lies outside the cache
   };
   Rows t;
   auto slot_of = [&](int j0) {
@@ -113,29 +112,31 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
   // Loads a step's rows, and before them the next step's ids: memory returns in order, so whoever
   // waits for an id would wait for rows issued before it.
   auto load_rows = [&](int j0) {
-    const bool in = j0 + sl * kU + mine < last;
     const bool out = id >= pages || id_hi != 0;
-    if (out && in && sub < 4)
-      report_bad_id(a.gd.err, kAsyncErrSlot,
-                    wide ? (int64_t)((uint64_t)id_hi << 32 | id) : (int64_t)(int32_t)id, pages,
-                    a.gd.tag);
+    t.n = last - j0 - sl * kU;
+    t.bad = 0;
+    if (__any(out)) {
+      if (out && mine < t.n && sub < 4)
+        report_bad_id(a.gd.err, kAsyncErrSlot,
+                      wide ? (int64_t)((uint64_t)id_hi << 32 | id) : (int64_t)(int32_t)id, pages,
+                      a.gd.tag);
+#pragma unroll
+      for (int u = 0; u < kU; ++u) t.bad |= of_quad(out ? 1u : 0u, u) << u;
+    }
     const uint32_t page = out ? 0u : id;
     const int64_t r = (((int64_t)page * a.c.heads + h) << ps) + (slot_of(j0) & mask);
     const uint64_t at = (uint64_t)r * half;
-    const uint32_t good = in && !out ? 1u : 0u;
     load_ids(j0 + kStep);
     if constexpr (QG) {
       t.km[0] = a.c.ks[r * ng + grp];
       t.vm[0] = a.c.vs[r * ng + grp];
     }
-    t.ok = 0;
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       const uint64_t to =
           ((uint64_t)of_quad((uint32_t)(at >> 32), u) << 32 | of_quad((uint32_t)at, u)) + 4 * w;
       t.kq[u] = *(const uint32_t *)(a.c.kc + to);
       t.vq[u] = *(const uint32_t *)(a.c.vc + to);
-      t.ok |= of_quad(good, u) << u;
       if constexpr (!QG) {
         const uint64_t rw = ((uint64_t)of_quad((uint32_t)((uint64_t)r >> 32), u) << 32 |
                              of_quad((uint32_t)r, u)) * ng + grp;
@@ -148,7 +149,7 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
     float x[GC][kU];
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      const bool ok = (t.ok >> u) & 1;
+      const bool ok = u < t.n && !((t.bad >> u) & 1);
       const uint32_t kw = QG ? of_quad(t.km[0], u) : t.km[QG ? 0 : u];
       const uint32_t km = live ? kw : 0u;
       const float ks = scale_of(km), kb = base_of(km);
@@ -180,7 +181,7 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
         if (j0 + sl * kU + u < last)
 #pragma unroll
           for (int g = 0; g < GC; ++g)
-            if (g < gn) a.logits[(row * a.q_heads + a0 + g) * a.cap + j0 + sl * kU + u] = x[g][u];
+            if (g < gn) a.logits[((int64_t)row * a.q_heads + a0 + g) * a.cap + j0 + sl * kU + u] = x[g][u];
     }
 #pragma unroll
     for (int g = 0; g < GC; ++g) {
@@ -202,7 +203,7 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       const uint32_t vw = QG ? of_quad(t.vm[0], u) : t.vm[QG ? 0 : u];
-      const uint32_t vm = live && ((t.ok >> u) & 1) ? vw : 0u;
+      const uint32_t vm = live && u < t.n && !((t.bad >> u) & 1) ? vw : 0u;
       const float vs = scale_of(vm), vb = base_of(vm);
       float vv[8];
       codes8(t.vq[u], vv);
@@ -247,7 +248,7 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
       for (int i = 0; i < 8; ++i) o[g][i] = o[g][i] * f + __shfl_xor(o[g][i], s, 64) * fo;
     }
     if (g >= gn || sl != 0) continue;
-    const int64_t qh = row * a.q_heads + a0 + g;
+    const int64_t qh = (int64_t)row * a.q_heads + a0 + g;
     if (a.splits > 1) {
       if (live) store8<kStateF32>(a.part_o, (qh * a.splits + split) * a.c.dim + 8 * w, o[g]);
     } else if (live) {
@@ -260,7 +261,7 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
   }
   if constexpr (SL == 1) {
     if (a.weights && !a.logits) {  // every query head of this head is here
-      float *wr = a.weights + (row * a.c.heads + h) * a.weights_cols;
+      float *wr = a.weights + ((int64_t)row * a.c.heads + h) * a.weights_cols;
 #pragma unroll
       for (int i = 0; i < kKeep; ++i) {
         const int j = i * LPR + sub;
@@ -437,15 +438,18 @@ void launch_vec_g(const AttendArgs &a, int type, hipStream_t st) {
   const int gc = vec_gc(a.g), gchunks = vec_gchunks(a.g);
   const int64_t items = a.rows * a.c.heads * gchunks * a.splits;
   const int64_t blocks = ceil_div(items * LPR * SL, kThreads);
-  DGS_CHECK(blocks < (int64_t(1) << 31) && items < (int64_t(1) << 31),
+  DGS_CHECK(items * LPR * SL < (int64_t(1) << 32) - kThreads,
             "attend: too many rows in one call");
   const unsigned grid = (unsigned)blocks;
+  const FastDivU32 fs = FastDivU32::make(a.splits), fg = FastDivU32::make(gchunks),
+                   fh = FastDivU32::make(a.c.heads);
+  const uint32_t n = (uint32_t)items;
   if (gc == 4)
-    k_attend_vec<LPR, SL, 4, QG><<<grid, kThreads, 0, st>>>(a, type, gchunks, items);
+    k_attend_vec<LPR, SL, 4, QG><<<grid, kThreads, 0, st>>>(a, type, fs, fg, fh, n);
   else if (gc == 2)
-    k_attend_vec<LPR, SL, 2, QG><<<grid, kThreads, 0, st>>>(a, type, gchunks, items);
+    k_attend_vec<LPR, SL, 2, QG><<<grid, kThreads, 0, st>>>(a, type, fs, fg, fh, n);
   else
-    k_attend_vec<LPR, SL, 1, QG><<<grid, kThreads, 0, st>>>(a, type, gchunks, items);
+    k_attend_vec<LPR, SL, 1, QG><<<grid, kThreads, 0, st>>>(a, type, fs, fg, fh, n);
   DGS_LAUNCH_CHECK();
 }
 template <int LPR, int SL>
