@@ -16,10 +16,15 @@ struct AttendArgs {
   IdArray table, lens;
   int64_t width;
   float scale2;  // scale * log2 e
-  int64_t chunk;  // slots per split
-  int splits;
-  float *part_o;   // [rows, q_heads, splits, dim], unnormalised (splits > 1)
-  float2 *part_ml;  // [rows, q_heads, splits] (splits > 1, or weights are added by the finishing kernel)
+  // How the work is cut.  Vector form: into `splits` chunks of slots a row.  Matrix form: a workgroup
+  // a (row, head, 16 query heads) "pair", or, with `stream` waves, their tiles of 32 slots in a line
+  // cut evenly over the waves.  What is cut leaves parts: a (maximum, sum) and an unnormalised output
+  // each.  Parts of a query head: vector form (row q_heads + head) splits + split; matrix form
+  // (pair + wave) * min(g, 16) + query head, so that a pair's parts follow each other.
+  int64_t chunk;
+  int splits, stream;
+  float *part_o;    // [parts, dim]
+  float2 *part_ml;  // [parts]
   float *logits;   // [rows, q_heads, cap] (weights)
   int64_t cap;     // width << pshift
   float *weights;
@@ -29,16 +34,17 @@ struct AttendArgs {
   GatherGuard gd;
 };
 
-// The matrix form for channel groups of 32, 64 or 128 and head_dim / group of 1, 2 or 4 (state_m*.hip):
-// workgroups of `waves` waves.
+// The matrix form for channel groups of 32, 64 or 128 and head_dim / group of 1, 2 or 4
+// (state_m*.hip): workgroups of `waves` waves.
 void attend_matrix_32(const AttendArgs &a, int waves, int type, hipStream_t st);
 void attend_matrix_64(const AttendArgs &a, int waves, int type, hipStream_t st);
 void attend_matrix_128(const AttendArgs &a, int waves, int type, hipStream_t st);
 // Words of LDS that a wave of it needs.
-inline int attend_matrix_lds(int dim, int group, int g) {
-  const int join = 32 + (g < 16 ? g : 16) * dim, corner = 8 * dim + 64 * (dim / group);
+inline int attend_matrix_lds(int dim, int group, int g, bool stream) {
+  const int join = stream ? 0 : 32 + (g < 16 ? g : 16) * dim, corner = 8 * dim + 64 * (dim / group);
   return join > corner ? join : corner;
 }
+constexpr int kStreamRows = 1024;  // rows whose lengths a wave of the stream form adds up
 
 namespace {
 
@@ -68,6 +74,38 @@ __device__ __forceinline__ void load_q(int type, const void *q, int64_t elem, fl
     load8<kStateF16>(q, elem, x);
 }
 
+// The stream form's line of units: rows in order, a row's pairs in order, and of a pair kPairCost
+// units for taking it up, then its tiles.  (Three loads that wait for each other, the query, the
+// write of its part: as long as some tiles.  64 rows of 1 to 8192 slots with weights: 112 us
+// without, 91 us at 2 units, 77 at 4, 76 at 6 and 8.)
+constexpr int kPairCost = 6;
+__device__ __forceinline__ int row_units(const AttendArgs &a, int64_t row) {
+  const int tiles = (int)((row_length(a, row, false) + 31) >> 5);
+  return tiles ? tiles + kPairCost : 0;
+}
+// Lane l adds up rows [l n / 64 ..): the line up to its rows, and what its rows hold.
+__device__ __forceinline__ void stream_sums(const AttendArgs &a, int lane, int per, int &before,
+                                            int &own, int &total) {
+  own = 0;
+  for (int i = 0; i < per; ++i) {
+    const int64_t r = (int64_t)lane * per + i;
+    if (r < a.rows) own += row_units(a, r);
+  }
+  int x = own;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(x, o, 64);
+    if (lane >= o) x += y;
+  }
+  before = x - own;
+  total = __shfl(x, 63, 64);
+}
+// Units a wave takes.
+__device__ __forceinline__ int stream_share(const AttendArgs &a, int64_t units) {
+  const int64_t q = (units + a.stream - 1) / a.stream;
+  return (int)(q < 4 + kPairCost ? 4 + kPairCost : (q + 1) & ~int64_t(1));
+}
+
 // Matrix form, for 16-bit queries.  One wave takes up to 16 query heads of a head (the columns left
 // over are zeros) through 32 slots at a time, in v_mfma_f32_16x16x32_bf16 (operands: lane l holds
 // row or column l & 15 and the eight k of quarter l >> 4; result: column l & 15, rows 4 (l >> 4) + i).
@@ -95,7 +133,10 @@ __device__ __forceinline__ void load_q(int type, const void *q, int64_t elem, fl
 //    order that depends on the row, so that the rows a read touches lie in different banks.
 //  - P16: pages of at least 16 slots; a load's rows lie in one page, whose address stays in scalar
 //    registers.
-// The waves of a workgroup take their 32 slots in turn and join through LDS in wave order.
+// STREAM = false: a workgroup a pair (row, head, 16 query heads), for rows that are short or many; its
+// waves take 32 slots in turn and join through LDS in wave order.  STREAM: every wave takes an equal
+// run of the tiles of all pairs, however long the rows are, and leaves its parts of a pair; the
+// finishing kernel joins them.
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 union Op {
@@ -175,7 +216,7 @@ __device__ __forceinline__ void collect(const uint32_t (&w)[GR / 4], Op &op) {
   }
 }
 
-template <int NG, int GROUP, int QT, int GR, bool P16>
+template <int NG, int GROUP, int QT, int GR, bool P16, bool STREAM>
 __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 1 : 2)
     void k_attend_matrix(AttendArgs a, int type, int tiles) {
   constexpr int kD = NG * GROUP, kC = kD / 32, kU = GROUP / 16, kGC = GROUP / 32, kV = GR / 2;
@@ -183,34 +224,69 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
   const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, q4 = lane >> 4;
-  uint32_t b = blockIdx.x;
-  const int split = (int)(b % (uint32_t)a.splits);
-  b /= (uint32_t)a.splits;
-  const int rt = (int)(b % (uint32_t)tiles);
-  b /= (uint32_t)tiles;
-  const int h = (int)(b % (uint32_t)a.c.heads);
-  const int64_t row = b / (uint32_t)a.c.heads;
+  const int pairs = a.c.heads * tiles;  // of a row
+  const int gs = a.g < 16 ? a.g : 16;
+  int64_t row;
+  int pair;  // of the row
+  // STREAM: this wave's units [at, end) of the line; `unit0`, `tile` = the first of its pair
+  int64_t at = 0, end = 0;
+  int unit0 = 0, tile = 0, units = 0;
+  const int w_id = (int)blockIdx.x * waves + wave;
+  if constexpr (STREAM) {
+    const int per = (int)((a.rows + 63) >> 6);
+    int before, own, total;
+    stream_sums(a, lane, per, before, own, total);
+    const int share = stream_share(a, (int64_t)total * pairs);
+    at = (int64_t)w_id * share;
+    end = at + share < (int64_t)total * pairs ? at + share : (int64_t)total * pairs;
+    if (at >= end) return;
+    // the lane, then the row, that holds unit `at`
+    const int64_t t = at / pairs;  // rows' boundaries are multiples of `pairs` in the line
+    const uint64_t has = __ballot(before <= t && t < (int64_t)before + own);
+    const int who = __ffsll((unsigned long long)has) - 1;
+    int front = __shfl(before, who, 64);
+    int64_t r = (int64_t)who * per;
+    while (true) {
+      units = row_units(a, r);
+      if (t < front + units) break;
+      front += units;
+      ++r;
+    }
+    row = __builtin_amdgcn_readfirstlane((int)r);
+    units = __builtin_amdgcn_readfirstlane(units);
+    const int64_t in_row = at - (int64_t)front * pairs;
+    pair = __builtin_amdgcn_readfirstlane((int)(in_row / units));
+    unit0 = __builtin_amdgcn_readfirstlane((int)(in_row % units));
+    tile = unit0 < kPairCost ? 0 : unit0 - kPairCost;
+  } else {
+    row = blockIdx.x / (uint32_t)pairs;
+    pair = (int)(blockIdx.x % (uint32_t)pairs);
+  }
   // slots of a row fit 32 bits (checked on the host)
-  const int len = __builtin_amdgcn_readfirstlane(
-      (int)row_length(a, row, split == 0 && h == 0 && rt == 0 && threadIdx.x == 0));
-  const int chunk = (int)a.chunk, first = split * chunk;
-  if (split > 0 && first >= len) return;
-  const int last = a.splits == 1 ? len : (first + chunk < len ? first + chunk : len);
-  const int gn = a.g - rt * 16 < 16 ? a.g - rt * 16 : 16;  // query heads, at most GR
-  const int64_t qh0 = row * a.q_heads + h * a.g + rt * 16;
+  int len = __builtin_amdgcn_readfirstlane(
+      (int)row_length(a, row, pair == 0 && (STREAM ? tile == 0 && lane == 0 : threadIdx.x == 0)));
+  int h = pair / tiles, rt = pair - h * tiles;
+  int gn = a.g - rt * 16 < 16 ? a.g - rt * 16 : 16;  // query heads, at most GR
+  int64_t qh0 = row * a.q_heads + h * a.g + rt * 16;
+  // the slots [first, last) this wave takes, every step-th tile of 32
+  const int step = STREAM ? 32 : waves * 32;
+  int j1 = STREAM ? tile * 32 : wave * 32;
+  int last = len;
+  if constexpr (STREAM) {
+    const int64_t stop = (unit0 + (end - at) - kPairCost) * 32;  // none of its tiles: not positive
+    if (stop < last) last = stop < 0 ? 0 : (int)stop;
+  }
   // logits grow with x: a negative scale is taken into q
   const float sign = a.scale2 < 0.f ? -1.f : 1.f, scale2 = fabsf(a.scale2);
   uint32_t magic = 0x43004300u;
   asm volatile("" : "+v"(magic));
 
   const int ps = a.c.pshift, mask = (1 << ps) - 1;
-  const int64_t trow = row * a.width;
   const int unit = n * (GROUP / 32);  // byte of this lane's unit of V in a group's codes
   const uint32_t sel = GROUP == 128 ? 0x05040100u
                        : GROUP == 64 ? ((unit & 2) ? 0x07060302u : 0x05040100u)
                                      : (0x0c000c00u | (uint32_t)(unit & 3) |
                                         ((uint32_t)(4 + (unit & 3)) << 16));
-  const int step = waves * 32;
   const uint32_t pages = (uint32_t)a.c.pages;
 
   // A tile is kPR x 64 pieces of 16 bytes: those of K, then those of V, row by row.  kL loads of a
@@ -251,7 +327,7 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
   // loaded, without a branch on the table's type, which would wait for every load before it)
   uint32_t id[kIds], id_hi[kIds];
   const bool wide = a.table.bytes == 8;
-  const char *tab = (const char *)a.table.p + (trow << (wide ? 3 : 2));
+  const char *tab;  // the row's
 
   // P16: the first slot of load i's rows, the same for all lanes; else this lane's
   auto slot_of = [&](int j0, int i) {
@@ -324,62 +400,9 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
     }
     __builtin_amdgcn_wave_barrier();
   };
-  // the first tiles, then the query: its loads and arithmetic run while the rows are on their way
-  const int j1 = first + wave * 32;
-  if (j1 < last) {
-    load_ids(j1);
-    load_rows(j1, t0);
-    load_rows(j1 + step, t1);
-  }
-
-  // q in bfloat16 terms, in the order in which code_pair() yields a word's channels: 0 4 1 5 2 6 3 7
   Op qv[QT][kC], qm;
-  float qsum[NG];
-#pragma unroll
-  for (int g = 0; g < NG; ++g) qsum[g] = 0.f;
-#pragma unroll
-  for (int c = 0; c < kC; ++c) {
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (n < gn)
-      load_q(type, a.q, row * a.q_row + (h * a.g + rt * 16 + n) * a.q_head + 32 * c + 8 * q4, x);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[i] *= sign;
-      qsum[c / kGC] += x[i];
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t hi = pack_bf16(x[i], x[4 + i]);
-      qv[0][c].u[i] = hi;
-      if constexpr (QT == 2)
-        qv[1][c].u[i] = pack_bf16(x[i] - __uint_as_float(hi << 16),
-                                  x[4 + i] - __uint_as_float(hi & 0xffff0000u));
-    }
-  }
-  // quarter 0 holds the first bfloat16 terms of (-128 Q_g, Q_g), 1 the second, 2 the third
-#pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    qm.u[g] = 0;
-    if (g < NG) {
-      float s = qsum[g < NG ? g : 0];
-      s += xor16(s);
-      s += xor32(s);
-      const float t0 = (float)(__bf16)s, t1 = (float)(__bf16)(s - t0);
-      const float t2 = (s - t0) - t1;
-      const float t = q4 == 0 ? t0 : (q4 == 1 ? t1 : (q4 == 2 ? t2 : 0.f));
-      qm.u[g] = pack_bf16(-128.f * t, t);
-    }
-  }
-
   f32x4 o[NG][kU], co[NG];
-  float cb[NG], m = -INFINITY, ms = 0.f, l = 0.f;  // m, ms: in base 2, of head n % GR
-#pragma unroll
-  for (int g = 0; g < NG; ++g) {
-    co[g] = f32x4{0.f, 0.f, 0.f, 0.f};
-    cb[g] = 0.f;
-#pragma unroll
-    for (int j = 0; j < kU; ++j) o[g][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  float cb[NG], m, ms, l;  // m, ms: in base 2, of head n % GR
   Op ones;
 #pragma unroll
   for (int i = 0; i < 4; ++i) ones.u[i] = 0x43004300u;  // 128, the codes' offset
@@ -536,22 +559,128 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
     load_rows(j0 + 2 * step, t);
     compute(j0, bad);
   };
-  if (j1 < last) {
-#pragma unroll 1
-    for (int j0 = j1; j0 < last; j0 += 2 * step) {
-      turn(j0, t0);
-      turn(j0 + step, t1);
-    }
-  }
-
-  __syncthreads();  // the corners become the joining area:
-  // [waves][16] maxima, [waves][16] sums, [waves][gn][kD] outputs
   auto over_columns = [&](float x) {
     if constexpr (GR < 16) x += lane_xor32<8>(x);
     if constexpr (GR < 8) x += lane_xor32<4>(x);
     x += xor16(x);
     return x + xor32(x);
   };
+#pragma unroll 1
+  while (true) {
+    // the first tiles, then the query: its loads and arithmetic run while the rows are on their way
+    tab = (const char *)a.table.p + ((row * a.width) << (wide ? 3 : 2));
+    if (j1 < last) {
+      load_ids(j1);
+      load_rows(j1, t0);
+      load_rows(j1 + step, t1);
+    }
+
+    // q in bfloat16 terms, in the order in which code_pair() yields a word's channels: 0 4 1 5 2 6 3 7
+    float qsum[NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) qsum[g] = 0.f;
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (n < gn)
+        load_q(type, a.q, row * a.q_row + (h * a.g + rt * 16 + n) * a.q_head + 32 * c + 8 * q4, x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] *= sign;
+        qsum[c / kGC] += x[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t hi = pack_bf16(x[i], x[4 + i]);
+        qv[0][c].u[i] = hi;
+        if constexpr (QT == 2)
+          qv[1][c].u[i] = pack_bf16(x[i] - __uint_as_float(hi << 16),
+                                    x[4 + i] - __uint_as_float(hi & 0xffff0000u));
+      }
+    }
+    // quarter 0 holds the first bfloat16 terms of (-128 Q_g, Q_g), 1 the second, 2 the third
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      qm.u[g] = 0;
+      if (g < NG) {
+        float s = qsum[g < NG ? g : 0];
+        s += xor16(s);
+        s += xor32(s);
+        const float t0 = (float)(__bf16)s, t1 = (float)(__bf16)(s - t0);
+        const float t2 = (s - t0) - t1;
+        const float t = q4 == 0 ? t0 : (q4 == 1 ? t1 : (q4 == 2 ? t2 : 0.f));
+        qm.u[g] = pack_bf16(-128.f * t, t);
+      }
+    }
+
+    m = -INFINITY;
+    ms = l = 0.f;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      co[g] = f32x4{0.f, 0.f, 0.f, 0.f};
+      cb[g] = 0.f;
+#pragma unroll
+      for (int j = 0; j < kU; ++j) o[g][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    if (j1 < last) {
+#pragma unroll 1
+      for (int j0 = j1; j0 < last; j0 += 2 * step) {
+        turn(j0, t0);
+        turn(j0 + step, t1);
+      }
+    }
+    if constexpr (!STREAM) {
+      break;
+    } else {
+      if (j1 < last) {
+        // this wave's part of the pair; a pair that it holds whole is finished here
+        const bool whole = tile == 0 && last == len;
+        l = over_columns(l);
+        const int64_t part = (row * pairs + pair + w_id) * gs + n;
+        const float inv = whole ? 1.f / l : 1.f;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const float c = over_columns(cb[g]);
+          if (n < gn) {
+            const int ch = g * GROUP + 4 * q4 * kU;
+#pragma unroll
+            for (int e = 0; e < 4 * kU; e += 8) {
+              float x[8];
+#pragma unroll
+              for (int y = 0; y < 8; ++y)
+                x[y] = (o[g][(e + y) % kU][(e + y) / kU] - co[g][(e + y) / kU] + c) * inv;
+              if (whole)
+                store_out(type, a.out, (qh0 + n) * kD + ch + e, x);
+              else
+                store8<kStateF32>(a.part_o, part * kD + ch + e, x);
+            }
+          }
+        }
+        if (q4 == 0 && n < gn) a.part_ml[part] = make_float2(m, l);
+      }
+      at += units - unit0;
+      if (at >= end) return;
+      unit0 = tile = 0;
+      if (++pair == pairs) {
+        pair = 0;
+        do {
+          ++row;
+          units = __builtin_amdgcn_readfirstlane(row_units(a, row));
+        } while (units == 0);  // `at` lies before the end of the line: there is one
+      }
+      len = __builtin_amdgcn_readfirstlane((int)row_length(a, row, pair == 0 && lane == 0));
+      h = pair / tiles;
+      rt = pair - h * tiles;
+      gn = a.g - rt * 16 < 16 ? a.g - rt * 16 : 16;
+      qh0 = row * a.q_heads + h * a.g + rt * 16;
+      j1 = 0;
+      if (end - at <= kPairCost) return;  // the next wave has its tiles
+      last = (int64_t)len < (end - at - kPairCost) * 32 ? len : (int)((end - at - kPairCost) * 32);
+    }
+  }
+
+  __syncthreads();  // the corners become the joining area:
+  // [waves][16] maxima, [waves][16] sums, [waves][gn][kD] outputs
   l = over_columns(l);
   float *s_m = s_mem, *s_l = s_mem + waves * 16, *s_o = s_mem + waves * 32;
   if (q4 == 0) s_m[wave * 16 + n] = m;
@@ -581,18 +710,14 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
 #pragma unroll
       for (int y = 0; y < 8; ++y) acc[y] += src[y];
     }
-    if (a.splits > 1) {
-      store8<kStateF32>(a.part_o, ((qh0 + hd) * a.splits + split) * kD + ch, acc);
-    } else {
-      const float inv = len == 0 ? 0.f : 1.f / ls;
+    const float inv = len == 0 ? 0.f : 1.f / ls;
 #pragma unroll
-      for (int y = 0; y < 8; ++y) acc[y] *= inv;
-      store_out(type, a.out, (qh0 + hd) * kD + ch, acc);
-    }
+    for (int y = 0; y < 8; ++y) acc[y] *= inv;
+    store_out(type, a.out, (qh0 + hd) * kD + ch, acc);
     if (a.part_ml && ch == 0) {
       float mm = -INFINITY;
       for (int w = 0; w < waves; ++w) mm = fmaxf(mm, s_m[w * 16 + hd]);
-      a.part_ml[(qh0 + hd) * a.splits + split] = make_float2(mm, ls);
+      a.part_ml[(row * pairs + pair) * gs + hd] = make_float2(mm, ls);
     }
   }
   if (!a.logits || a.part_ml) return;
@@ -621,31 +746,38 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
   }
 }
 
-template <int NG, int GROUP, int QT, int GR>
+template <int NG, int GROUP, int QT, int GR, bool STREAM>
 void launch_matrix_gr(const AttendArgs &a, int waves, int type, hipStream_t st) {
   const int tiles = (a.g + 15) / 16;
-  const int64_t blocks = a.rows * a.c.heads * tiles * a.splits;
+  const int64_t blocks = STREAM ? ceil_div(a.stream, waves) : a.rows * a.c.heads * tiles;
   DGS_CHECK(blocks < (int64_t(1) << 31), "attend: too many rows in one call");
-  const size_t lds = (size_t)waves * attend_matrix_lds(NG * GROUP, GROUP, a.g) * 4;
+  const size_t lds = (size_t)waves * attend_matrix_lds(NG * GROUP, GROUP, a.g, STREAM) * 4;
   const unsigned grid = (unsigned)blocks, threads = waves * 64;
   if constexpr (NG * GROUP >= 128) {
     if (a.c.pshift >= 4) {
-      k_attend_matrix<NG, GROUP, QT, GR, true><<<grid, threads, lds, st>>>(a, type, tiles);
+      k_attend_matrix<NG, GROUP, QT, GR, true, STREAM><<<grid, threads, lds, st>>>(a, type, tiles);
       DGS_LAUNCH_CHECK();
       return;
     }
   }
-  k_attend_matrix<NG, GROUP, QT, GR, false><<<grid, threads, lds, st>>>(a, type, tiles);
+  k_attend_matrix<NG, GROUP, QT, GR, false, STREAM><<<grid, threads, lds, st>>>(a, type, tiles);
   DGS_LAUNCH_CHECK();
+}
+template <int NG, int GROUP, int QT, int GR>
+void launch_matrix_st(const AttendArgs &a, int waves, int type, hipStream_t st) {
+  if (a.stream)
+    launch_matrix_gr<NG, GROUP, QT, GR, true>(a, waves, type, st);
+  else
+    launch_matrix_gr<NG, GROUP, QT, GR, false>(a, waves, type, st);
 }
 template <int NG, int GROUP, int QT>
 void launch_matrix_qt(const AttendArgs &a, int waves, int type, hipStream_t st) {
   if (a.g <= 4)
-    launch_matrix_gr<NG, GROUP, QT, 4>(a, waves, type, st);
+    launch_matrix_st<NG, GROUP, QT, 4>(a, waves, type, st);
   else if (a.g <= 8)
-    launch_matrix_gr<NG, GROUP, QT, 8>(a, waves, type, st);
+    launch_matrix_st<NG, GROUP, QT, 8>(a, waves, type, st);
   else
-    launch_matrix_gr<NG, GROUP, QT, 16>(a, waves, type, st);
+    launch_matrix_st<NG, GROUP, QT, 16>(a, waves, type, st);
 }
 template <int NG, int GROUP>
 void launch_matrix(const AttendArgs &a, int waves, int type, hipStream_t st) {

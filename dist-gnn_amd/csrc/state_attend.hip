@@ -279,29 +279,60 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
   }
 }
 
-// The maximum and 1 / sum of a query head over its splits, on every lane of the wave.
-__device__ __forceinline__ float2 join_ml(const AttendArgs &a, int64_t qh, int splits, bool empty) {
-  const float2 *ml = a.part_ml + qh * a.splits;
+// The parts of a query head: n of them, the first at `part`, `stride` apart.
+struct Parts {
+  int64_t part;
+  int stride, n;
+};
+__device__ __forceinline__ Parts parts_of(const AttendArgs &a, int64_t row, int head, int64_t len) {
+  if (a.splits)
+    return Parts{(row * a.q_heads + head) * a.splits, 1,
+                 len == 0 ? 1 : (int)((len + a.chunk - 1) / a.chunk)};
+  const int tiles = (a.g + 15) / 16, pairs = a.c.heads * tiles, gs = a.g < 16 ? a.g : 16;
+  const int h = head / a.g, n = head - h * a.g, pair = h * tiles + n / 16;
+  int64_t part = row * pairs + pair;
+  int parts = 1;
+  if (a.stream) {
+    const int lane = threadIdx.x & 63, per = (int)((a.rows + 63) >> 6);
+    int before, own, total;
+    stream_sums(a, lane, per, before, own, total);
+    const int who = (int)(row / per);
+    int64_t front = __shfl(before, who, 64);
+    for (int64_t r = (int64_t)who * per; r < row; ++r) front += row_units(a, r);
+    const int q = stream_share(a, (int64_t)total * pairs), u = row_units(a, row);
+    const int64_t start = front * pairs + (int64_t)pair * u;
+    const int64_t w0 = (start + kPairCost) / q;  // the wave of its first tile
+    parts = u == 0 ? 1 : (int)((start + u - 1) / q - w0) + 1;
+    part += w0;
+  }
+  return Parts{part * gs + n % 16, gs, parts};
+}
+// The maximum and 1 / sum of a query head over its parts, on every lane of the wave.
+__device__ __forceinline__ float2 join_ml(const AttendArgs &a, const Parts &p) {
+  const float2 *ml = a.part_ml + p.part;
   float m = -INFINITY, l = 0.f;
   const int lane = threadIdx.x & 63;
-  if (splits == 1) {
+  if (p.n == 1) {
     m = ml[0].x;
     l = ml[0].y;
   } else {
-    for (int s = lane; s < splits; s += 64) m = fmaxf(m, ml[s].x);
+    for (int s = lane; s < p.n; s += 64) m = fmaxf(m, ml[(int64_t)s * p.stride].x);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
     const float ms = m == -INFINITY ? 0.f : m;
-    for (int s = lane; s < splits; s += 64) l += ml[s].y * __builtin_amdgcn_exp2f(ml[s].x - ms);
+    for (int s = lane; s < p.n; s += 64) {
+      const float2 x = ml[(int64_t)s * p.stride];
+      l += x.y * __builtin_amdgcn_exp2f(x.x - ms);
+    }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
   }
-  return make_float2(m == -INFINITY ? 0.f : m, empty ? 0.f : 1.f / l);
+  return make_float2(m == -INFINITY ? 0.f : m, 1.f / l);
 }
 
-// Joins the splits of the rows' query heads and adds the weights; every wave works alone.  The
+// Joins the parts of the rows' query heads and adds the weights; every wave works alone.  The
 // first `outs` waves take a query head's output each (eight channels a lane, the lanes' groups
-// taking every n-th split), the others 256 slots of a (row, head)'s weights.
+// taking every n-th part), the others 256 slots of a (row, head)'s weights.
 constexpr int kSpan = 256;
 template <int TYPE>
 __global__ __launch_bounds__(kThreads) void k_attend_finish(AttendArgs a, int64_t outs,
@@ -312,29 +343,31 @@ __global__ __launch_bounds__(kThreads) void k_attend_finish(AttendArgs a, int64_
   if (id < outs) {
     const int64_t row = id / a.q_heads;
     const int64_t len = row_length(a, row, false);
-    const int splits = (int)(len == 0 ? 1 : (len + a.chunk - 1) / a.chunk);  // that were written
-    const float2 ml = join_ml(a, id, splits, len == 0);
+    const Parts p = parts_of(a, row, (int)(id % a.q_heads), len);
+    if (a.stream && p.n == 1 && len > 0) return;  // written by the wave that had it whole
     const int words = a.c.dim >> 3;
     int lpr = 1;
     while (lpr < words) lpr <<= 1;
     const int w = lane & (lpr - 1), part = lane / lpr, parts = 64 / lpr;
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (w < words && len > 0)
-      for (int s = part; s < splits; s += parts) {
-        const float f = __builtin_amdgcn_exp2f(a.part_ml[id * a.splits + s].x - ml.x);
-        float x[8];
-        load8<kStateF32>(a.part_o, (id * a.splits + s) * a.c.dim + 8 * w, x);
+    if (len > 0) {
+      const float2 ml = join_ml(a, p);
+      if (w < words)
+        for (int s = part; s < p.n; s += parts) {
+          const int64_t at = p.part + (int64_t)s * p.stride;
+          const float f = __builtin_amdgcn_exp2f(a.part_ml[at].x - ml.x);
+          float x[8];
+          load8<kStateF32>(a.part_o, at * a.c.dim + 8 * w, x);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] = __builtin_fmaf(x[i], f, acc[i]);
-      }
-    for (int o = lpr; o < 64; o <<= 1)
+          for (int i = 0; i < 8; ++i) acc[i] = __builtin_fmaf(x[i], f, acc[i]);
+        }
+      for (int o = lpr; o < 64; o <<= 1)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i] += __shfl_xor(acc[i], o, 64);
-    if (part == 0 && w < words) {
+        for (int i = 0; i < 8; ++i) acc[i] += __shfl_xor(acc[i], o, 64);
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc[i] *= ml.y;
-      store8<TYPE>(a.out, id * a.c.dim + 8 * w, acc);
     }
+    if (part == 0 && w < words) store8<TYPE>(a.out, id * a.c.dim + 8 * w, acc);
     return;
   }
   const int64_t pair = (id - outs) / spans;
@@ -342,14 +375,15 @@ __global__ __launch_bounds__(kThreads) void k_attend_finish(AttendArgs a, int64_
   const int64_t len = row_length(a, row, false);
   const int64_t j0 = (id - outs) % spans * kSpan;
   if (j0 >= len) return;
-  const int splits = (int)((len + a.chunk - 1) / a.chunk);
-  const int64_t q0 = pair * a.g;  // the head's first query head: row * q_heads + h * g
+  const int head0 = (int)(pair % a.c.heads) * a.g;  // the head's first query head
+  const int64_t q0 = row * a.q_heads + head0;
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
   // lane t takes slots j0 + t, + 64, + 128, + 192; a slot past the end reads the last one
   int64_t j[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) j[i] = j0 + 64 * i + lane < len ? j0 + 64 * i + lane : len - 1;
   constexpr int kG = 4;  // heads whose loads are in flight together
+  Parts p = parts_of(a, row, head0, len);
   for (int g0 = 0; g0 < a.g; g0 += kG) {
     float x[kG][4];
 #pragma unroll
@@ -358,10 +392,13 @@ __global__ __launch_bounds__(kThreads) void k_attend_finish(AttendArgs a, int64_
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[g][i] = lg[j[i]];
     }
+    // 16 query heads share their parts' places (kG divides 16)
+    if (a.splits || (g0 > 0 && g0 % 16 == 0)) p = parts_of(a, row, head0 + g0, len);
 #pragma unroll
     for (int g = 0; g < kG; ++g) {
       if (g0 + g >= a.g) break;
-      const float2 ml = join_ml(a, q0 + g0 + g, splits, false);
+      const Parts pg{p.part + (a.splits ? (int64_t)g * a.splits : (g0 % 16 + g)), p.stride, p.n};
+      const float2 ml = join_ml(a, pg);
 #pragma unroll
       for (int i = 0; i < 4; ++i) sum[i] += __builtin_amdgcn_exp2f(x[g][i] - ml.x) * ml.y;
     }
@@ -374,9 +411,10 @@ __global__ __launch_bounds__(kThreads) void k_attend_finish(AttendArgs a, int64_
 
 struct AttendPlan {
   bool matrix;
-  int waves;  // of a workgroup of the matrix form
+  int waves;   // of a workgroup of the matrix form
+  int stream;  // its stream form's waves, or 0
   int64_t chunk;
-  int splits;
+  int splits;  // vector form
   int64_t cap;
   bool finish;  // the finishing kernel runs
   int64_t o_bytes, ml_bytes, logit_bytes;
@@ -394,36 +432,40 @@ AttendPlan plan_attend(const StateView &c, const AttendCall &a) {
   const int ng = c.dim / c.group, g = a.q_heads / c.heads;
   p.matrix = a.type != kStateF32 && (c.group == 32 || c.group == 64 || c.group == 128) &&
              (ng == 1 || ng == 2 || ng == 4) && p.cap > 16;
-  int64_t chunk;
+  const int64_t qh = a.rows * a.q_heads;
   if (p.matrix) {
-    const int64_t work = a.rows * c.heads * ((g + 15) / 16);
-    // 8 waves where the rows alone cannot fill the card, as far as 64 KB of LDS go (256 channels
-    // take the registers of two waves)
-    p.waves = work * ceil_div(p.cap, 512) <= 256 && c.dim < 256 ? 8 : 4;
-    while (p.waves > 1 && p.waves * attend_matrix_lds(c.dim, c.group, g) * 4 > 64 * 1024)
+    const int64_t pairs = a.rows * c.heads * ((g + 15) / 16);
+    // Rows that can be longer than 1024 slots, and few enough to add up, are cut evenly over the
+    // waves that fit the card at once (256 CUs x 4 SIMDs x 2).
+    p.stream = p.cap > 1024 && a.rows <= kStreamRows &&
+                       a.rows * ceil_div(p.cap, 32) < (int64_t(1) << 31)
+                   ? 2048
+                   : 0;
+    // else 8 waves a pair where the rows alone cannot fill the card, as far as 64 KB of LDS go
+    // (256 channels take the registers of two waves)
+    p.waves = !p.stream && pairs * ceil_div(p.cap, 512) <= 256 && c.dim < 256 ? 8 : 4;
+    while (p.waves > 1 &&
+           p.waves * attend_matrix_lds(c.dim, c.group, g, p.stream != 0) * 4 > 64 * 1024)
       p.waves >>= 1;
-    // One round of workgroups (two a CU): starting one takes as long as some tiles, three loads
-    // that wait for each other.  64 rows of up to 8192 slots: 93 us in 512 workgroups, 104 in
-    // 1024, 117 in 2048; 8 rows of 131072: 216, 227, 230 us.
-    chunk = ceil_div(p.cap * work, 512);
-    const int64_t low = p.waves == 8 ? 1024 : 512;
-    chunk = chunk < low ? low : (chunk + 127) & ~int64_t(127);
-  } else {
-    chunk = ceil_div(p.cap * a.rows * c.heads * vec_gchunks(g), 16384);
-    chunk = chunk < 64 ? 64 : (chunk + 63) & ~int64_t(63);
+    const int64_t parts = (pairs + p.stream) * (g < 16 ? g : 16);
+    // a workgroup that has a row and all its query heads adds its weights itself, from the logits
+    // that it wrote (a long row would be a tail: 8192 slots 38 us, the finishing kernel 17)
+    p.finish = p.stream || (a.weights && (g > 16 || p.cap > 1024));
+    if (p.stream) p.o_bytes = up256(parts * c.dim * 4);
+    if (p.finish) p.ml_bytes = up256(parts * 8);
+    if (a.weights) p.logit_bytes = up256(qh * p.cap * 4);
+    return p;
   }
+  int64_t chunk = ceil_div(p.cap * a.rows * c.heads * vec_gchunks(g), 16384);
+  chunk = chunk < 64 ? 64 : (chunk + 63) & ~int64_t(63);
   p.splits = (int)(p.cap <= chunk ? 1 : ceil_div(p.cap, chunk));
   p.chunk = p.splits == 1 ? (p.cap > 0 ? p.cap : 1) : chunk;
-  const int64_t qh = a.rows * a.q_heads;
+  // items of short rows with all query heads of a head add their weights from registers
+  const bool own = p.cap <= 16 && vec_gchunks(g) == 1;
+  p.finish = p.splits > 1 || (a.weights && !own);
   if (p.splits > 1) p.o_bytes = up256(qh * p.splits * c.dim * 4);
-  // An item or workgroup that has a row and all its query heads to itself adds its weights itself:
-  // in the vector form from registers, in the matrix form from the logits it wrote (a long row
-  // would be a tail: 8192 slots 38 us, the finishing kernel 17).
-  const bool own_m = p.matrix && p.splits == 1 && g <= 16 && p.cap <= 1024;
-  const bool own_v = !p.matrix && p.cap <= 16 && vec_gchunks(g) == 1;
-  p.finish = p.splits > 1 || (a.weights && !own_m && !own_v);
   if (p.finish) p.ml_bytes = up256(qh * p.splits * 8);
-  if (a.weights && !own_v) p.logit_bytes = up256(qh * p.cap * 4);
+  if (a.weights && !own) p.logit_bytes = up256(qh * p.cap * 4);
   return p;
 }
 
@@ -496,6 +538,7 @@ void state_attend(const StateView &c, const AttendCall &call, void *ws, int64_t 
   a.scale2 = call.scale * kLog2e;
   a.chunk = p.chunk;
   a.splits = p.splits;
+  a.stream = p.stream;
   char *w = static_cast<char *>(ws);
   if (p.o_bytes) a.part_o = (float *)w;
   if (p.ml_bytes) a.part_ml = (float2 *)(w + p.o_bytes);
@@ -518,7 +561,7 @@ void state_attend(const StateView &c, const AttendCall &call, void *ws, int64_t 
     default: launch_vec<32>(a, call.type, st); break;
   }
   if (!p.finish) return;
-  const int64_t outs = p.splits > 1 ? call.rows * call.q_heads : 0;
+  const int64_t outs = p.splits > 1 || p.stream ? call.rows * call.q_heads : 0;
   const int spans = p.logit_bytes ? (int)ceil_div(p.cap, kSpan) : 0;
   const int64_t waves = outs + call.rows * c.heads * spans;
   const int64_t blocks = ceil_div(waves, kThreads / 64);
