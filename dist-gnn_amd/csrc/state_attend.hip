@@ -307,33 +307,65 @@ __device__ __forceinline__ Parts parts_of(const AttendArgs &a, int64_t row, int 
   }
   return Parts{part * gs + n % 16, gs, parts};
 }
-// The maximum and 1 / sum of a query head over its parts, on every lane of the wave.
-__device__ __forceinline__ float2 join_ml(const AttendArgs &a, const Parts &p) {
-  const float2 *ml = a.part_ml + p.part;
-  float m = -INFINITY, l = 0.f;
+// The maximum and 1 / sum of kG query heads over their parts (head g's `step` g behind), on every
+// lane of the wave; heads at or past g_end repeat the first.
+template <int kG>
+__device__ __forceinline__ void join_ml(const AttendArgs &a, const Parts &p, int64_t step,
+                                        int g_end, float2 (&out)[kG]) {
   const int lane = threadIdx.x & 63;
-  if (p.n == 1) {
-    m = ml[0].x;
-    l = ml[0].y;
-  } else {
-    for (int s = lane; s < p.n; s += 64) m = fmaxf(m, ml[(int64_t)s * p.stride].x);
+  float m[kG], l[kG];
+  const float2 *ml[kG];
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    const float ms = m == -INFINITY ? 0.f : m;
-    for (int s = lane; s < p.n; s += 64) {
-      const float2 x = ml[(int64_t)s * p.stride];
-      l += x.y * __builtin_amdgcn_exp2f(x.x - ms);
+  for (int g = 0; g < kG; ++g) {
+    ml[g] = a.part_ml + p.part + (g < g_end ? g * step : 0);
+    m[g] = -INFINITY;
+    l[g] = 0.f;
+  }
+  if (p.n <= 64) {  // one part a lane
+    float2 x[kG];
+#pragma unroll
+    for (int g = 0; g < kG; ++g)
+      x[g] = lane < p.n ? ml[g][(int64_t)lane * p.stride] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+    for (int g = 0; g < kG; ++g) {
+      m[g] = x[g].x;
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) m[g] = fmaxf(m[g], __shfl_xor(m[g], o, 64));
     }
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
+    for (int g = 0; g < kG; ++g) {
+      m[g] = m[g] == -INFINITY ? 0.f : m[g];
+      l[g] = lane < p.n ? x[g].y * __builtin_amdgcn_exp2f(x[g].x - m[g]) : 0.f;
+    }
+  } else {
+    for (int s = lane; s < p.n; s += 64)
+#pragma unroll
+      for (int g = 0; g < kG; ++g) m[g] = fmaxf(m[g], ml[g][(int64_t)s * p.stride].x);
+#pragma unroll
+    for (int g = 0; g < kG; ++g) {
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) m[g] = fmaxf(m[g], __shfl_xor(m[g], o, 64));
+      m[g] = m[g] == -INFINITY ? 0.f : m[g];
+    }
+    for (int s = lane; s < p.n; s += 64)
+#pragma unroll
+      for (int g = 0; g < kG; ++g) {
+        const float2 x = ml[g][(int64_t)s * p.stride];
+        l[g] += x.y * __builtin_amdgcn_exp2f(x.x - m[g]);
+      }
   }
-  return make_float2(m == -INFINITY ? 0.f : m, 1.f / l);
+#pragma unroll
+  for (int g = 0; g < kG; ++g) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) l[g] += __shfl_xor(l[g], o, 64);
+    out[g] = make_float2(m[g], 1.f / l[g]);
+  }
 }
 
 // Joins the parts of the rows' query heads and adds the weights; every wave works alone.  The
 // first `outs` waves take a query head's output each (eight channels a lane, the lanes' groups
-// taking every n-th part), the others 256 slots of a (row, head)'s weights.
-constexpr int kSpan = 256;
+// taking every n-th part), the others 1024 slots of a (row, head)'s weights.
+constexpr int kSpan = 1024;
 template <int TYPE>
 __global__ __launch_bounds__(kThreads) void k_attend_finish(AttendArgs a, int64_t outs,
                                                             int spans, int64_t waves) {
@@ -351,7 +383,9 @@ __global__ __launch_bounds__(kThreads) void k_attend_finish(AttendArgs a, int64_
     const int w = lane & (lpr - 1), part = lane / lpr, parts = 64 / lpr;
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (len > 0) {
-      const float2 ml = join_ml(a, p);
+      float2 joined[1];
+      join_ml<1>(a, p, 0, 1, joined);
+      const float2 ml = joined[0];
       if (w < words)
         for (int s = part; s < p.n; s += parts) {
           const int64_t at = p.part + (int64_t)s * p.stride;
@@ -377,36 +411,49 @@ __global__ __launch_bounds__(kThreads) void k_attend_finish(AttendArgs a, int64_
   if (j0 >= len) return;
   const int head0 = (int)(pair % a.c.heads) * a.g;  // the head's first query head
   const int64_t q0 = row * a.q_heads + head0;
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  // lane t takes slots j0 + t, + 64, + 128, + 192; a slot past the end reads the last one
-  int64_t j[4];
+  constexpr int kG = 4, kI = 4, kRuns = kSpan / (64 * kI);  // heads and slots in flight together
+  // lane t takes slots j0 + t, + 64, ...; a slot past the end reads the last one
+  float sum[kRuns][kI];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) j[i] = j0 + 64 * i + lane < len ? j0 + 64 * i + lane : len - 1;
-  constexpr int kG = 4;  // heads whose loads are in flight together
+  for (int r = 0; r < kRuns; ++r)
+#pragma unroll
+    for (int i = 0; i < kI; ++i) sum[r][i] = 0.f;
   Parts p = parts_of(a, row, head0, len);
   for (int g0 = 0; g0 < a.g; g0 += kG) {
-    float x[kG][4];
-#pragma unroll
-    for (int g = 0; g < kG; ++g) {
-      const float *lg = a.logits + (q0 + (g0 + g < a.g ? g0 + g : g0)) * a.cap;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[g][i] = lg[j[i]];
-    }
     // 16 query heads share their parts' places (kG divides 16)
     if (a.splits || (g0 > 0 && g0 % 16 == 0)) p = parts_of(a, row, head0 + g0, len);
+    const Parts pg{p.part + (a.splits ? 0 : g0 % 16), p.stride, p.n};
+    float2 ml[kG];
+    join_ml<kG>(a, pg, a.splits ? a.splits : 1, a.g - g0, ml);
 #pragma unroll
-    for (int g = 0; g < kG; ++g) {
-      if (g0 + g >= a.g) break;
-      const Parts pg{p.part + (a.splits ? (int64_t)g * a.splits : (g0 % 16 + g)), p.stride, p.n};
-      const float2 ml = join_ml(a, pg);
+    for (int r = 0; r < kRuns; ++r) {
+      if (j0 + r * kI * 64 >= len) break;
+      float x[kG][kI];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum[i] += __builtin_amdgcn_exp2f(x[g][i] - ml.x) * ml.y;
+      for (int g = 0; g < kG; ++g) {
+        const float *lg = a.logits + (q0 + (g0 + g < a.g ? g0 + g : g0)) * a.cap;
+#pragma unroll
+        for (int i = 0; i < kI; ++i) {
+          const int64_t j = j0 + (r * kI + i) * 64 + lane;
+          x[g][i] = lg[j < len ? j : len - 1];
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < kG; ++g)
+        if (g0 + g < a.g)
+#pragma unroll
+          for (int i = 0; i < kI; ++i)
+            sum[r][i] += __builtin_amdgcn_exp2f(x[g][i] - ml[g].x) * ml[g].y;
     }
   }
   float *wr = a.weights + pair * a.weights_cols;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (j0 + 64 * i + lane < len) wr[j[i]] = a.decay != 0.f ? sum[i] + a.decay * wr[j[i]] : sum[i];
+  for (int r = 0; r < kRuns; ++r)
+#pragma unroll
+    for (int i = 0; i < kI; ++i) {
+      const int64_t j = j0 + (r * kI + i) * 64 + lane;
+      if (j < len) wr[j] = a.decay != 0.f ? sum[r][i] + a.decay * wr[j] : sum[r][i];
+    }
 }
 
 struct AttendPlan {
@@ -441,9 +488,15 @@ AttendPlan plan_attend(const StateView &c, const AttendCall &a) {
                        a.rows * ceil_div(p.cap, 32) < (int64_t(1) << 31)
                    ? 2048
                    : 0;
-    // else 8 waves a pair where the rows alone cannot fill the card, as far as 64 KB of LDS go
-    // (256 channels take the registers of two waves)
-    p.waves = !p.stream && pairs * ceil_div(p.cap, 512) <= 256 && c.dim < 256 ? 8 : 4;
+    // Else the waves of a pair: one where the pairs fill the card (it holds 2048 waves), up to 8 where
+    // they cannot, as far as 64 KB of LDS go (256 channels take the registers of two waves).  3713
+    // rows of 8 heads, 9 to 13 slots in pages of 128: 485 us with 4 waves, 234 with 2, 128 with one;
+    // 1500 rows of 100 to 1000 slots: 286, 214, 187 us.
+    p.waves = p.stream || (pairs > 256 && pairs <= 512) ? 4
+              : pairs > 1024                            ? 1
+              : pairs > 512                             ? 2
+              : pairs * ceil_div(p.cap, 512) <= 256 && c.dim < 256 ? 8
+                                                                   : 4;
     while (p.waves > 1 &&
            p.waves * attend_matrix_lds(c.dim, c.group, g, p.stream != 0) * 4 > 64 * 1024)
       p.waves >>= 1;
