@@ -10,8 +10,8 @@
 //
 // The plan, one workgroup per (row, head): weights and positions are read once, four slots a load,
 // and stay in registers as keys (32 bits, larger is better; rows past 32768 slots read them again
-// each time); the budget-th best key by counting digits; then ties, holes and movers are numbered in
-// slot order by counting lanes, the waves' counts joined by a scan.  What lies below the budget is
+// each time); the budget-th best key by counting digits; then ties, holes and movers are numbered
+// in slot order by counting lanes, the waves' counts joined by a scan.  What lies below the budget is
 // copied as it passes and the holes are overwritten afterwards.
 // The moves are a kernel of their own, over all stores; where there can only be a few (a cache
 // that takes single tokens) the plan's workgroup does them.
@@ -141,7 +141,8 @@ __device__ __forceinline__ int32_t block_max(int32_t x, int32_t *lds) {
   for (int i = 0; i < THREADS / 64; ++i) x = lds[i] > x ? lds[i] : x;
   return x;
 }
-// The digit that holds the `left`-th largest key of the histogram; left becomes its rank there.
+// The digit that holds the `left`-th largest key of the histogram; left becomes its rank there,
+// found[2] the keys there.
 template <int THREADS>
 __device__ __forceinline__ uint32_t pick_digit(const uint32_t *hist, uint32_t &left, uint32_t *scan,
                                                uint32_t *found) {
@@ -159,6 +160,7 @@ __device__ __forceinline__ uint32_t pick_digit(const uint32_t *hist, uint32_t &l
     if (before < left && left <= before + mine[i]) {
       found[0] = kDigits - 1 - ((int)threadIdx.x * kOwn + i);
       found[1] = left - before;
+      found[2] = mine[i];
     }
     before += mine[i];
   }
@@ -172,7 +174,7 @@ __device__ __forceinline__ void plan_end(const EvictArgs &a, const PlanRow &r,
                                          const int32_t *holes, const int32_t *movers,
                                          uint32_t all) {
   if (!FUSED && threadIdx.x == 0) a.moves[r.pair] = (int32_t)all;
-  __syncthreads();  // the lists and the copies are written (a workgroup sees its stores past a barrier)
+  __syncthreads();  // the lists and the copies are written: a workgroup sees its stores past a barrier
 #pragma unroll 4
   for (uint32_t i = threadIdx.x; i < all; i += THREADS) {
     const int32_t d = holes[i], s = movers[i];
@@ -199,7 +201,7 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan(EvictArgs a) {
   constexpr int kWaves = THREADS / 64, kRuns = kVecs * kWaves;  // a run: a wave's 256 slots of a v
   static_assert(kRuns <= 128, "one wave scans the runs, two a lane");
   __shared__ uint32_t s_hist[3][kDigits];
-  __shared__ uint32_t s_scan[kWaves], s_found[2], s_run[kRuns];
+  __shared__ uint32_t s_scan[kWaves], s_found[3], s_run[kRuns];
   __shared__ int32_t s_max[kWaves];
   __shared__ uint64_t s_low[kWaves];
   __shared__ int32_t s_list[2 * kFewMoves];  // FUSED: holes, movers
@@ -325,37 +327,50 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan(EvictArgs a) {
     __syncthreads();
   };
   const uint64_t below = lane == 0 ? 0ull : ~0ull >> (64 - lane);
-  // of the slots whose key equals the threshold the first `left` in slot order stay
-  uint32_t tie = 0, kept = 0;  // bit 4 v + i
-#pragma unroll
-  for (int v = 0; v < kVecs; ++v) {
-    uint32_t cnt = 0;
-    if (v * THREADS * 4 < r.n) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool in = (v * THREADS + tid) * 4 + i < r.n;
-        if (in && key[v][i] == prefix) tie |= 1u << (4 * v + i);
-        if (in && key[v][i] > prefix) kept |= 1u << (4 * v + i);
-        cnt += __popcll(__ballot((tie >> (4 * v + i)) & 1));
-      }
-    }
-    if (lane == 0) s_run[v * kWaves + wave] = cnt;
-  }
-  scan_runs();
+  uint32_t kept = 0;  // bit 4 v + i
+  const bool all_ties = s_found[2] == left;
 #pragma unroll
   for (int v = 0; v < kVecs; ++v) {
     if (v * THREADS * 4 >= r.n) break;
-    uint32_t rank = s_run[v * kWaves + wave];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) rank += __popcll(__ballot((tie >> (4 * v + i)) & 1) & below);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if ((tie >> (4 * v + i)) & 1) {
-        if (rank < left) kept |= 1u << (4 * v + i);
-        ++rank;
-      }
+    for (int i = 0; i < 4; ++i) {
+      const bool in = (v * THREADS + tid) * 4 + i < r.n;
+      if (in && (key[v][i] > prefix || (all_ties && key[v][i] == prefix)))
+        kept |= 1u << (4 * v + i);
+    }
   }
-  __syncthreads();  // s_run is written again
+  if (!all_ties) {
+    // of the slots whose key equals the threshold the first `left` in slot order stay
+    uint32_t tie = 0;
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) {
+      uint32_t cnt = 0;
+      if (v * THREADS * 4 < r.n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool in = (v * THREADS + tid) * 4 + i < r.n;
+          if (in && key[v][i] == prefix) tie |= 1u << (4 * v + i);
+          cnt += __popcll(__ballot((tie >> (4 * v + i)) & 1));
+        }
+      }
+      if (lane == 0) s_run[v * kWaves + wave] = cnt;
+    }
+    scan_runs();
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) {
+      if (v * THREADS * 4 >= r.n) break;
+      uint32_t rank = s_run[v * kWaves + wave];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) rank += __popcll(__ballot((tie >> (4 * v + i)) & 1) & below);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if ((tie >> (4 * v + i)) & 1) {
+          if (rank < left) kept |= 1u << (4 * v + i);
+          ++rank;
+        }
+    }
+    __syncthreads();  // s_run is written again
+  }
   // holes (dropped below the budget) in the low half, movers (kept at or past it) in the high one:
   // at most 32768 of each
   uint32_t hole = 0, mover = 0;
@@ -404,7 +419,7 @@ template <int THREADS>
 __global__ __launch_bounds__(THREADS) void k_evict_plan_long(EvictArgs a) {
   constexpr int kWaves = THREADS / 64;
   __shared__ uint32_t s_hist[kDigits];
-  __shared__ uint32_t s_scan[kWaves], s_found[2], s_cnt[3][kWaves];
+  __shared__ uint32_t s_scan[kWaves], s_found[3], s_cnt[3][kWaves];
   __shared__ int32_t s_max[kWaves];
   const PlanRow r = plan_row<THREADS>(a);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = r.n;
@@ -589,7 +604,8 @@ void evict_rows(const EvictCall &e, void *ws, int64_t ws_bytes, hipStream_t st) 
   const int64_t fill = ceil_div(4096, pairs);
   if (ny > fill) ny = fill;
   if (ny > 1024) ny = 1024;
-  k_evict_move<<<dim3((unsigned)pairs, (unsigned)ny, (unsigned)e.nstores), kMoveThreads, 0, st>>>(a);
+  const dim3 grid((unsigned)pairs, (unsigned)ny, (unsigned)e.nstores);
+  k_evict_move<<<grid, kMoveThreads, 0, st>>>(a);
   DGS_LAUNCH_CHECK();
 }
 

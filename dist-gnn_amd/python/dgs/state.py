@@ -33,7 +33,7 @@ _current = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_devi
 
 
 def _on(index):
-    """Makes device `index` the current one for the call (the library launches on the current one)."""
+    """Makes device `index` the current one for the call: the library launches on that."""
     return _HERE if _current() == index else torch.cuda.device(index)
 
 
@@ -43,7 +43,8 @@ def _require(cond, msg):
 
 
 def _ids(t, name):
-    _require(t.dtype in (torch.int32, torch.int64), f"{name}: ID can only be int32 or int64")
+    if t.dtype is not torch.int32 and t.dtype is not torch.int64:
+        raise RuntimeError(f"{name}: ID can only be int32 or int64")
     return t if t.is_contiguous() else t.contiguous()
 
 
@@ -151,10 +152,12 @@ class StateCache:
 
     def _rows(self, k, v):
         for name, t in (("k", k), ("v", v)):
-            _require(t.dim() == 3 and tuple(t.shape[1:]) == (self.heads, self.head_dim),
-                     f"{name} must be [tokens, {self.heads}, {self.head_dim}]")
-            _require(t.dtype in _DTYPES, f"{name} must be float32, bfloat16 or float16")
-        _require(k.shape == v.shape and k.dtype == v.dtype, "k and v must be alike")
+            if not (t.dim() == 3 and tuple(t.shape[1:]) == (self.heads, self.head_dim)):
+                raise RuntimeError(f"{name} must be [tokens, {self.heads}, {self.head_dim}]")
+            if not (t.dtype in _DTYPES):
+                raise RuntimeError(f"{name} must be float32, bfloat16 or float16")
+        if not (k.shape == v.shape and k.dtype == v.dtype):
+            raise RuntimeError("k and v must be alike")
         _no_grad(k, v)
         _same_device(self._index, k, v)
         return _rows16(k), _rows16(v)
@@ -163,7 +166,8 @@ class StateCache:
         """Rows k[t], v[t] ([tokens, heads, head_dim]) go to flat slot slots[t]; a negative slot
         is skipped.  With a slot twice in a call it is not defined which row a channel group
         keeps."""
-        _require(slots.dim() == 1 and slots.numel() == k.shape[0], "slots must be [tokens]")
+        if slots.dim() != 1 or slots.numel() != k.shape[0]:
+            raise RuntimeError("slots must be [tokens]")
         slots = _ids(slots, "slots")
         k, v = self._rows(k, v)
         _same_device(self._index, slots)
@@ -177,9 +181,12 @@ class StateCache:
         """One new row per sequence: k[i], v[i] go to slot lens[i] of table row i (page ids
         [sequences, pages]; lens is not changed).  Returns the flat slots (int64)."""
         n = k.shape[0]
-        _require(table.dim() == 2 and table.shape[0] == n, "table must be [tokens, pages]")
-        _require(n == 0 or table.shape[1] > 0, "the table has no columns")
-        _require(lens.dim() == 1 and lens.numel() == n, "lens must be [tokens]")
+        if table.dim() != 2 or table.shape[0] != n:
+            raise RuntimeError("table must be [tokens, pages]")
+        if n > 0 and table.shape[1] == 0:
+            raise RuntimeError("the table has no columns")
+        if lens.dim() != 1 or lens.numel() != n:
+            raise RuntimeError("lens must be [tokens]")
         table, lens = _ids(table, "table"), _ids(lens, "lens")
         k, v = self._rows(k, v)
         _same_device(self._index, table, lens)
@@ -194,8 +201,10 @@ class StateCache:
 
     def read(self, slots, dtype=torch.float32):
         """The rows' values as (k, v), each [n, heads, head_dim]; a negative slot gives zeros."""
-        _require(slots.dim() == 1, "slots must have one dimension")
-        _require(dtype in _DTYPES, "rows are read as float32, bfloat16 or float16")
+        if slots.dim() != 1:
+            raise RuntimeError("slots must have one dimension")
+        if dtype not in _DTYPES:
+            raise RuntimeError("rows are read as float32, bfloat16 or float16")
         slots = _ids(slots, "slots")
         _same_device(self._index, slots)
         with _on(self._index):
@@ -215,23 +224,28 @@ class StateCache:
         weights[i, h, j] = decay * weights[i, h, j] + the probabilities of head h's query heads,
         for j < lens[i].  Several query tokens of one sequence are several rows with the same
         table row, each with the length that it may see."""
-        _require(q.dim() == 3 and q.shape[2] == self.head_dim,
-                 f"q must be [rows, q_heads, {self.head_dim}]")
+        if q.dim() != 3 or q.shape[2] != self.head_dim:
+            raise RuntimeError(f"q must be [rows, q_heads, {self.head_dim}]")
         rows, q_heads = q.shape[0], q.shape[1]
-        _require(q.dtype in _DTYPES, "q must be float32, bfloat16 or float16")
-        _require(q_heads > 0 and q_heads % self.heads == 0,
-                 f"q_heads must be a multiple of {self.heads}")
-        _require(table.dim() == 2 and table.shape[0] == rows, "table must be [rows, pages]")
-        _require(lens.dim() == 1 and lens.numel() == rows, "lens must be [rows]")
+        if q.dtype not in _DTYPES:
+            raise RuntimeError("q must be float32, bfloat16 or float16")
+        if q_heads == 0 or q_heads % self.heads:
+            raise RuntimeError(f"q_heads must be a multiple of {self.heads}")
+        if table.dim() != 2 or table.shape[0] != rows:
+            raise RuntimeError("table must be [rows, pages]")
+        if lens.dim() != 1 or lens.numel() != rows:
+            raise RuntimeError("lens must be [rows]")
         table, lens = _ids(table, "table"), _ids(lens, "lens")
         width = table.shape[1]
         _no_grad(q)
         if weights is not None:
-            _require(weights.dtype == torch.float32 and weights.dim() == 3 and
-                     tuple(weights.shape[:2]) == (rows, self.heads) and
-                     weights.shape[2] >= width * self.page_size,
-                     f"weights must be float32 [rows, {self.heads}, >= pages * page_size]")
-            _require(weights.is_contiguous(), "weights must be contiguous (updated in place)")
+            if (weights.dtype != torch.float32 or weights.dim() != 3 or
+                    weights.shape[:2] != (rows, self.heads) or
+                    weights.shape[2] < width * self.page_size):
+                raise RuntimeError(f"weights must be float32 [rows, {self.heads}, >= pages * "
+                                   "page_size]")
+            if not weights.is_contiguous():
+                raise RuntimeError("weights must be contiguous (updated in place)")
             _no_grad(weights)
             _same_device(self._index, weights)
         _same_device(self._index, q, table, lens)
@@ -284,32 +298,40 @@ def evict_rows(stores, weights, positions, table, lens, budget, sinks=0, recent=
     weights: float32 [rows, heads, cols], positions: int32 of that shape or None (position = slot),
     cols >= table.shape[1] * page_size.  Returns new (weights, positions, lens): the kept slots'
     weights and positions in their new order, 0 and -1 behind them, min(n, budget)."""
-    _require(weights.dim() == 3 and weights.dtype == torch.float32,
-             "weights must be float32 [rows, heads, slots]")
+    if weights.dim() != 3 or weights.dtype != torch.float32:
+        raise RuntimeError("weights must be float32 [rows, heads, slots]")
     rows, heads, cols = weights.shape
-    _require(heads > 0, "weights must be float32 [rows, heads, slots]")
-    _require(positions is None or (positions.dtype == torch.int32 and
-                                   positions.shape == weights.shape),
-             "positions must be int32 of the weights' shape")
-    _require(table.dim() == 2 and table.shape[0] == rows, "table must be [rows, pages]")
-    _require(lens.dim() == 1 and lens.numel() == rows, "lens must be [rows]")
+    if heads == 0:
+        raise RuntimeError("weights must have heads")
+    if positions is not None and (positions.dtype != torch.int32 or
+                                  positions.shape != weights.shape):
+        raise RuntimeError("positions must be int32 of the weights' shape")
+    if table.dim() != 2 or table.shape[0] != rows:
+        raise RuntimeError("table must be [rows, pages]")
+    if lens.dim() != 1 or lens.numel() != rows:
+        raise RuntimeError("lens must be [rows]")
     table, lens = _ids(table, "table"), _ids(lens, "lens")
     budget, sinks, recent = int(budget), int(sinks), int(recent)
-    _require(budget > 0, "budget must be positive")
-    _require(sinks >= 0 and recent >= 0 and sinks + recent <= budget,
-             "sinks + recent must lie between 0 and budget")
+    if budget <= 0:
+        raise RuntimeError("budget must be positive")
+    if sinks < 0 or recent < 0 or sinks + recent > budget:
+        raise RuntimeError("sinks + recent must lie between 0 and budget")
     stores = list(stores)
-    _require(0 < len(stores) <= 8, "evict_rows takes one to eight stores")
+    if not 0 < len(stores) <= 8:
+        raise RuntimeError("evict_rows takes one to eight stores")
     lead = stores[0].shape[:3]
-    _require(len(lead) == 3 and lead[0] > 0 and lead[1] == heads and lead[2] > 0,
-             f"a store must be [pages, {heads}, page_size, ...]")
+    if len(lead) != 3 or lead[0] == 0 or lead[1] != heads or lead[2] == 0:
+        raise RuntimeError(f"a store must be [pages, {heads}, page_size, ...]")
     for s in stores:
-        _require(s.shape[:3] == lead, "the stores must have the same pages")
-        _require(s.is_contiguous() and s.numel() > 0, "a store must be contiguous and not empty")
-    _require(cols >= table.shape[1] * lead[2],
-             "weights need a column for every slot of the table")
+        if s.shape[:3] != lead:
+            raise RuntimeError("the stores must have the same pages")
+        if not s.is_contiguous() or s.numel() == 0:
+            raise RuntimeError("a store must be contiguous and not empty")
+    if cols < table.shape[1] * lead[2]:
+        raise RuntimeError("weights need a column for every slot of the table")
     _no_grad(weights, *stores)
-    _require(weights.is_cuda, "weights must be a CUDA tensor")
+    if not weights.is_cuda:
+        raise RuntimeError("weights must be a CUDA tensor")
     index, device = weights.get_device(), weights.device
     _same_device(index, table, lens, *stores)
     if positions is not None:
