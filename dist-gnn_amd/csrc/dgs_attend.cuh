@@ -276,8 +276,9 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
     const int64_t stop = (unit0 + (end - at) - kPairCost) * 32;  // none of its tiles: not positive
     if (stop < last) last = stop < 0 ? 0 : (int)stop;
   }
-  // logits grow with x: a negative scale is taken into q
-  const float sign = a.scale2 < 0.f ? -1.f : 1.f, scale2 = fabsf(a.scale2);
+  // logits grow with x: a negative scale is taken into q, and so is 0 (masked slots are -inf)
+  const float sign = a.scale2 < 0.f ? -1.f : (a.scale2 == 0.f ? 0.f : 1.f);
+  const float scale2 = a.scale2 == 0.f ? 1.f : fabsf(a.scale2);
   uint32_t magic = 0x43004300u;
   asm volatile("" : "+v"(magic));
 

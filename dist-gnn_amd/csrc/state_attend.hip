@@ -485,7 +485,7 @@ AttendPlan plan_attend(const StateView &c, const AttendCall &a) {
     // Rows that can be longer than 1024 slots, and few enough to add up, are cut evenly over the
     // waves that fit the card at once (256 CUs x 4 SIMDs x 2).
     p.stream = p.cap > 1024 && a.rows <= kStreamRows &&
-                       a.rows * ceil_div(p.cap, 32) < (int64_t(1) << 31)
+                       a.rows * ceil_div(p.cap, 32) < (int64_t(1) << 30)
                    ? 2048
                    : 0;
     // Else the waves of a pair: one where the pairs fill the card (it holds 2048 waves), up to 8 where

@@ -134,9 +134,14 @@ class StateCache:
         _require(group > 0 and group % 8 == 0 and head_dim % group == 0,
                  "group must be a multiple of 8 that divides head_dim")
 
+    # read-only: the library holds their addresses
+    k_codes = property(lambda self: self._buffers[0])
+    k_scales = property(lambda self: self._buffers[1])
+    v_codes = property(lambda self: self._buffers[2])
+    v_scales = property(lambda self: self._buffers[3])
+
     def _adopt(self, k_codes, k_scales, v_codes, v_scales):
-        self.k_codes, self.k_scales = k_codes, k_scales
-        self.v_codes, self.v_scales = v_codes, v_scales
+        self._buffers = (k_codes, k_scales, v_codes, v_scales)
         self.num_pages, self.heads, self.page_size = k_codes.shape[:3]
         self.head_dim = 2 * k_codes.shape[3]
         self.group = self.head_dim // k_scales.shape[3]
@@ -277,8 +282,8 @@ class StateCache:
 
     def evict(self, weights, positions, table, lens, budget, sinks=0, recent=0):
         """evict_rows over this cache's buffers."""
-        return evict_rows([self.k_codes, self.k_scales, self.v_codes, self.v_scales], weights,
-                          positions, table, lens, budget, sinks=sinks, recent=recent)
+        return evict_rows(self._buffers, weights, positions, table, lens, budget, sinks=sinks,
+                          recent=recent)
 
 
 _evict_room = {}  # workspace bytes by (rows, heads, cols, budget)
@@ -367,15 +372,17 @@ def evict_rows(stores, weights, positions, table, lens, budget, sinks=0, recent=
 
 def neighbour_table(block, fan_out):
     """The table and lengths that StateCache.attend takes (pages of one slot, page = node id) for a
-    block of the sampler (seeds, frontier, coo_row, coo_col): table row i = the at most `fan_out`
-    sampled neighbours of the block's i-th target node, -1 behind them.  No synchronisation."""
+    block of the sampler (seeds, frontier, coo_row, coo_col): table row i = the sampled neighbours
+    of the block's i-th target node, the first `fan_out` if there are more, -1 behind them.  No
+    synchronisation."""
     seeds, frontier, row, col = block
     _require(fan_out > 0, "fan_out must be positive")
     row, col = row.long(), col.long()
     lens = torch.zeros(seeds.numel(), dtype=torch.int64, device=row.device)
     lens.scatter_add_(0, row, torch.ones_like(row))
-    # a block's edges are grouped by target, in target order
+    # a block's edges are grouped by target, in target order; what passes fan_out goes to a column
+    # that is cut off
     at = torch.arange(row.numel(), device=row.device) - (lens.cumsum(0) - lens)[row]
-    table = torch.full((seeds.numel(), fan_out), -1, dtype=torch.int64, device=row.device)
-    table[row, at] = frontier.long()[col]
-    return table, lens
+    table = torch.full((seeds.numel(), fan_out + 1), -1, dtype=torch.int64, device=row.device)
+    table[row, at.clamp(max=fan_out)] = frontier.long()[col]
+    return table[:, :fan_out].contiguous(), lens.clamp(max=fan_out)

@@ -190,5 +190,12 @@ def test_neighbour_table():
     table, lens = dgs.ops.neighbour_table((seeds, frontier, row, col), 4)
     assert lens.tolist() == [2, 0, 3]
     assert table.tolist() == [[20, 3, -1, -1], [-1] * 4, [21, 21, 7, -1]]
+    short, lens = dgs.ops.neighbour_table((seeds, frontier, row.int(), col.int()), 2)
+    assert lens.tolist() == [2, 0, 2] and short.tolist() == [[20, 3], [-1, -1], [21, 21]]
     with pytest.raises(RuntimeError, match="fan_out"):
         dgs.ops.neighbour_table((seeds, frontier, row, col), 0)
+
+
+def test_buffers_cannot_be_replaced():
+    with pytest.raises(AttributeError):
+        _fake().k_codes = torch.zeros(1)

@@ -236,6 +236,38 @@ def test_attend_long(q_heads, heads, dim, group, page, dtype):
     check_attend(cache, q, table.int().cuda(), lens.cuda(), scale=0.3)
 
 
+@pytest.mark.parametrize("rows, high, heads, g, page", [
+    (600, 3000, 1, 2, 16), (1024, 1500, 1, 1, 4), (1025, 1500, 1, 2, 16), (1100, 500, 1, 20, 8),
+    (700, 600, 1, 4, 32), (300, 900, 2, 3, 2), (1, 5000, 1, 1, 64), (2, 1100, 2, 17, 1024)])
+@pytest.mark.parametrize("keep", [False, True])
+def test_attend_ragged_rows(rows, high, heads, g, page, keep):
+    """Many rows of very different lengths, most of them short or empty, some long: every way of
+    cutting the work."""
+    gen = torch.Generator().manual_seed(rows)
+    lens = (torch.rand(rows, generator=gen) ** 12 * high).long()
+    lens[rows // 2], lens[-1] = high, (0 if rows > 2 else high - 1)
+    lens[rows // 3:rows // 3 + 70] = 0 if rows > 300 else lens[rows // 3]
+    pages = 4000 // page + 1
+    cache = full_cache(pages, page, heads, 64, 64, seed=3)
+    table = torch.randint(0, pages, (rows, -(-high // page)), generator=gen)
+    q = states((rows, heads * g, 64), gen, torch.bfloat16)
+    w = torch.rand(rows, heads, table.shape[1] * page, generator=gen).cuda() if keep else None
+    check_attend(cache, q, table.int().cuda(), lens.cuda(), weights=w)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("page", [1, 16])
+def test_attend_scale_zero(dtype, page):
+    """All logits equal: the mean of the values."""
+    gen = torch.Generator().manual_seed(0)
+    cache = full_cache(4096 // page, page, 2, 64, 64)
+    q = states((3, 4, 64), gen, TYPES[dtype])
+    table = torch.randint(0, 4096 // page, (3, 2048 // page), generator=gen).cuda()
+    check_attend(cache, q, table, torch.tensor([2001, 5, 0]).cuda(), scale=0.0)
+    check_attend(cache, q, table[:, :64 // page].contiguous(), torch.tensor([61, 5, 0]).cuda(),
+                 scale=0.0)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_attend_many_short_rows(dtype):
     """Sampled neighbours: many rows of at most 15 slots, pages of one slot."""
