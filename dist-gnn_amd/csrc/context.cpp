@@ -265,7 +265,11 @@ void host_pin(void *p, int64_t bytes) {
     }
     // pin_memory.cc:7-12 registers the tensor's own range (cudaHostRegisterDefault); mapped
     // here, so kernels read it through the device pointer
-    DGS_HIP(hipHostRegister(p, nb, hipHostRegisterMapped));
+    const hipError_t reg = hipHostRegister(p, nb, hipHostRegisterMapped);
+    if (reg != hipSuccess) {
+      (void)hipGetLastError();  // reported here, not by the next launch too
+      throw Error(std::string("hipHostRegister failed: ") + hipGetErrorString(reg));
+    }
     void *d = nullptr;
     const hipError_t e = hipHostGetDevicePointer(&d, p, 0);
     if (e != hipSuccess) {

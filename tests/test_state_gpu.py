@@ -629,3 +629,18 @@ def test_decoding_with_a_full_cache(dtype):
         assert np.array_equal(lens.cpu().numpy(), wn)
         assert all(same_bits(a, b) for a, b in zip(buffers(cache), expect))
     assert lens.tolist() == [12, 30, 30]
+
+
+def test_a_refused_registration_is_not_reported_again():
+    """Where the driver does not map memory that exists already, the call that asked for it raises,
+    and the launches after it do not."""
+    host = torch.zeros(4096, dtype=torch.uint8)
+    try:
+        dgs.ops._CAPI_tensor_pin_memory(host)
+    except RuntimeError as e:
+        assert "hipHostRegister" in str(e)
+    else:
+        dgs.ops._CAPI_tensor_unpin_memory(host)
+    cache = full_cache(2, 4, 1, 64, 64)
+    got = cache.read(torch.arange(8).cuda())
+    assert got[0].shape == (8, 1, 64) and torch.isfinite(got[0]).all()
