@@ -16,13 +16,15 @@ struct AttendArgs {
   IdArray table, lens;
   int64_t width;
   float scale2;  // scale * log2 e
-  // How the work is cut.  Vector form: into `splits` chunks of slots a row.  Matrix form: a workgroup
-  // a (row, head, 16 query heads) "pair", or, with `stream` waves, their tiles of 32 slots in a line
-  // cut evenly over the waves.  What is cut leaves parts: a (maximum, sum) and an unnormalised output
-  // each.  Parts of a query head: vector form (row q_heads + head) splits + split; matrix form
-  // (pair + wave) * min(g, 16) + query head, so that a pair's parts follow each other.
+  // How the work is cut.  A "pair" is a row and up to `together` query heads of one head (matrix form
+  // 16, vector form 4).  With `stream` waves, the pairs' tiles of 2^shift slots lie in a line that is
+  // cut evenly over the waves; else the matrix form takes a workgroup a pair and the vector form
+  // `splits` chunks of slots a row.  What is cut leaves parts: a (maximum, sum) and an unnormalised
+  // output each.  Parts of a query head: with splits (row q_heads + head) splits + split, else
+  // (pair + wave) * min(g, together) + query head, so that a pair's parts follow each other.
   int64_t chunk;
-  int splits, stream;
+  int splits, stream, together;
+  int shift, cost, least;  // of the line: see row_units, stream_share
   float *part_o;    // [parts, dim]
   float2 *part_ml;  // [parts]
   float *logits;   // [rows, q_heads, cap] (weights)
@@ -74,22 +76,19 @@ __device__ __forceinline__ void load_q(int type, const void *q, int64_t elem, fl
     load8<kStateF16>(q, elem, x);
 }
 
-// The stream form's line of units: rows in order, a row's pairs in order, and of a pair kPairCost
-// units for taking it up, then its tiles.  (Three loads that wait for each other, the query, the
-// write of its part: as long as some tiles.  64 rows of 1 to 8192 slots with weights: 112 us
-// without, 91 us at 2 units, 77 at 4, 76 at 6 and 8.)
-constexpr int kPairCost = 6;
-__device__ __forceinline__ int row_units(const AttendArgs &a, int64_t row) {
-  const int tiles = (int)((row_length(a, row, false) + 31) >> 5);
-  return tiles ? tiles + kPairCost : 0;
+// The stream form's line of units: rows in order, a row's pairs in order, and of a pair `cost` units
+// for taking it up, then its tiles of 2^shift slots.
+__device__ __forceinline__ int row_units(const AttendArgs &a, int64_t row, int shift, int cost) {
+  const int tiles = (int)((row_length(a, row, false) + (1 << shift) - 1) >> shift);
+  return tiles ? tiles + cost : 0;
 }
 // Lane l adds up rows [l n / 64 ..): the line up to its rows, and what its rows hold.
-__device__ __forceinline__ void stream_sums(const AttendArgs &a, int lane, int per, int &before,
-                                            int &own, int &total) {
+__device__ __forceinline__ void stream_sums(const AttendArgs &a, int shift, int cost, int lane,
+                                            int per, int &before, int &own, int &total) {
   own = 0;
   for (int i = 0; i < per; ++i) {
     const int64_t r = (int64_t)lane * per + i;
-    if (r < a.rows) own += row_units(a, r);
+    if (r < a.rows) own += row_units(a, r, shift, cost);
   }
   int x = own;
 #pragma unroll
@@ -98,13 +97,72 @@ __device__ __forceinline__ void stream_sums(const AttendArgs &a, int lane, int p
     if (lane >= o) x += y;
   }
   before = x - own;
-  total = __shfl(x, 63, 64);
+  total = __builtin_amdgcn_readlane(x, 63);
 }
-// Units a wave takes.
-__device__ __forceinline__ int stream_share(const AttendArgs &a, int64_t units) {
+// Units a wave takes: at least a pair's cost and `least` tiles.
+__device__ __forceinline__ int stream_share(const AttendArgs &a, int cost, int least, int64_t units) {
   const int64_t q = (units + a.stream - 1) / a.stream;
-  return (int)(q < 4 + kPairCost ? 4 + kPairCost : (q + 1) & ~int64_t(1));
+  return (int)(q < least + cost ? least + cost : q);
 }
+// A wave's units [at, end) of the line, and where it is in them: a pair of a row, of which it takes
+// the tiles from `tile` on and the slots before last().  All in scalar registers.
+struct Run {
+  int64_t at, end, row;
+  int pairs, units, pair, unit0, tile;
+
+  __device__ __forceinline__ bool start(const AttendArgs &a, int shift, int cost, int least,
+                                        int pairs_of_row, int wave, int lane) {
+    pairs = pairs_of_row;
+    const int per = (int)((a.rows + 63) >> 6);
+    int before, own, total;
+    stream_sums(a, shift, cost, lane, per, before, own, total);
+    const int share = stream_share(a, cost, least, (int64_t)total * pairs);
+    at = (int64_t)wave * share;
+    end = at + share < (int64_t)total * pairs ? at + share : (int64_t)total * pairs;
+    if (at >= end) return false;
+    // the lane, then the row, that holds unit `at`
+    const int64_t t = at / pairs;  // rows' boundaries are multiples of `pairs` in the line
+    const uint64_t has = __ballot(before <= t && t < (int64_t)before + own);
+    const int who = __ffsll((unsigned long long)has) - 1;
+    int front = __shfl(before, who, 64);
+    int64_t r = (int64_t)who * per;
+    while (true) {
+      units = row_units(a, r, shift, cost);
+      if (t < front + units) break;
+      front += units;
+      ++r;
+    }
+    row = __builtin_amdgcn_readfirstlane((int)r);
+    units = __builtin_amdgcn_readfirstlane(units);
+    const int64_t in_row = at - (int64_t)front * pairs;
+    pair = __builtin_amdgcn_readfirstlane((int)(in_row / units));
+    unit0 = __builtin_amdgcn_readfirstlane((int)(in_row % units));
+    tile = unit0 < cost ? 0 : unit0 - cost;
+    return true;
+  }
+  // The end of this wave's slots of its pair (none of them: not past the first).
+  __device__ __forceinline__ int last(int shift, int cost, int len) const {
+    const int64_t stop = (unit0 + (end - at) - cost) * ((int64_t)1 << shift);
+    return stop < 0 ? 0 : (stop < len ? (int)stop : len);
+  }
+  __device__ __forceinline__ bool next(const AttendArgs &a, int shift, int cost) {
+    at += units - unit0;
+    if (at >= end) return false;
+    unit0 = tile = 0;
+    if (++pair == pairs) {
+      pair = 0;
+      do {
+        ++row;
+        units = __builtin_amdgcn_readfirstlane(row_units(a, row, shift, cost));
+      } while (units == 0);  // `at` lies before the end of the line: there is one
+    }
+    return end - at > cost;  // else the next wave has its tiles
+  }
+};
+// Matrix form: tiles of 32 slots, and 6 units for a pair (three loads that wait for each other, the
+// query, the write of its part: as long as some tiles.  64 rows of 1 to 8192 slots with weights:
+// 112 us without, 91 us at 2 units, 77 at 4, 76 at 6 and 8).
+constexpr int kMatrixShift = 5, kMatrixCost = 6, kMatrixLeast = 4;
 
 // Matrix form, for 16-bit queries.  One wave takes up to 16 query heads of a head (the columns left
 // over are zeros) through 32 slots at a time, in v_mfma_f32_16x16x32_bf16 (operands: lane l holds
@@ -226,56 +284,24 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
   const int n = lane & 15, q4 = lane >> 4;
   const int pairs = a.c.heads * tiles;  // of a row
   const int gs = a.g < 16 ? a.g : 16;
-  int64_t row;
-  int pair;  // of the row
-  // STREAM: this wave's units [at, end) of the line; `unit0`, `tile` = the first of its pair
-  int64_t at = 0, end = 0;
-  int unit0 = 0, tile = 0, units = 0;
-  const int w_id = (int)blockIdx.x * waves + wave;
+  Run run;
   if constexpr (STREAM) {
-    const int per = (int)((a.rows + 63) >> 6);
-    int before, own, total;
-    stream_sums(a, lane, per, before, own, total);
-    const int share = stream_share(a, (int64_t)total * pairs);
-    at = (int64_t)w_id * share;
-    end = at + share < (int64_t)total * pairs ? at + share : (int64_t)total * pairs;
-    if (at >= end) return;
-    // the lane, then the row, that holds unit `at`
-    const int64_t t = at / pairs;  // rows' boundaries are multiples of `pairs` in the line
-    const uint64_t has = __ballot(before <= t && t < (int64_t)before + own);
-    const int who = __ffsll((unsigned long long)has) - 1;
-    int front = __shfl(before, who, 64);
-    int64_t r = (int64_t)who * per;
-    while (true) {
-      units = row_units(a, r);
-      if (t < front + units) break;
-      front += units;
-      ++r;
-    }
-    row = __builtin_amdgcn_readfirstlane((int)r);
-    units = __builtin_amdgcn_readfirstlane(units);
-    const int64_t in_row = at - (int64_t)front * pairs;
-    pair = __builtin_amdgcn_readfirstlane((int)(in_row / units));
-    unit0 = __builtin_amdgcn_readfirstlane((int)(in_row % units));
-    tile = unit0 < kPairCost ? 0 : unit0 - kPairCost;
+    if (!run.start(a, kMatrixShift, kMatrixCost, kMatrixLeast, pairs,
+                   (int)blockIdx.x * waves + wave, lane)) return;
   } else {
-    row = blockIdx.x / (uint32_t)pairs;
-    pair = (int)(blockIdx.x % (uint32_t)pairs);
+    run.row = blockIdx.x / (uint32_t)pairs;
+    run.pair = (int)(blockIdx.x % (uint32_t)pairs);
   }
   // slots of a row fit 32 bits (checked on the host)
   int len = __builtin_amdgcn_readfirstlane(
-      (int)row_length(a, row, pair == 0 && (STREAM ? tile == 0 && lane == 0 : threadIdx.x == 0)));
-  int h = pair / tiles, rt = pair - h * tiles;
+      (int)row_length(a, run.row, !STREAM && run.pair == 0 && threadIdx.x == 0));
+  int h = run.pair / tiles, rt = run.pair - h * tiles;
   int gn = a.g - rt * 16 < 16 ? a.g - rt * 16 : 16;  // query heads, at most GR
-  int64_t qh0 = row * a.q_heads + h * a.g + rt * 16;
+  int64_t qh0 = run.row * a.q_heads + h * a.g + rt * 16;
   // the slots [first, last) this wave takes, every step-th tile of 32
   const int step = STREAM ? 32 : waves * 32;
-  int j1 = STREAM ? tile * 32 : wave * 32;
-  int last = len;
-  if constexpr (STREAM) {
-    const int64_t stop = (unit0 + (end - at) - kPairCost) * 32;  // none of its tiles: not positive
-    if (stop < last) last = stop < 0 ? 0 : (int)stop;
-  }
+  int j1 = STREAM ? run.tile * 32 : wave * 32;
+  int last = STREAM ? run.last(kMatrixShift, kMatrixCost, len) : len;
   // logits grow with x: a negative scale is taken into q, and so is 0 (masked slots are -inf)
   const float sign = a.scale2 < 0.f ? -1.f : (a.scale2 == 0.f ? 0.f : 1.f);
   const float scale2 = a.scale2 == 0.f ? 1.f : fabsf(a.scale2);
@@ -569,7 +595,7 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
 #pragma unroll 1
   while (true) {
     // the first tiles, then the query: its loads and arithmetic run while the rows are on their way
-    tab = (const char *)a.table.p + ((row * a.width) << (wide ? 3 : 2));
+    tab = (const char *)a.table.p + ((run.row * a.width) << (wide ? 3 : 2));
     if (j1 < last) {
       load_ids(j1);
       load_rows(j1, t0);
@@ -584,7 +610,7 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
     for (int c = 0; c < kC; ++c) {
       float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       if (n < gn)
-        load_q(type, a.q, row * a.q_row + (h * a.g + rt * 16 + n) * a.q_head + 32 * c + 8 * q4, x);
+        load_q(type, a.q, run.row * a.q_row + (h * a.g + rt * 16 + n) * a.q_head + 32 * c + 8 * q4, x);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         x[i] *= sign;
@@ -635,9 +661,9 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
     } else {
       if (j1 < last) {
         // this wave's part of the pair; a pair that it holds whole is finished here
-        const bool whole = tile == 0 && last == len;
+        const bool whole = run.tile == 0 && last == len;
         l = over_columns(l);
-        const int64_t part = (row * pairs + pair + w_id) * gs + n;
+        const int64_t part = (run.row * pairs + run.pair + blockIdx.x * waves + wave) * gs + n;
         const float inv = whole ? 1.f / l : 1.f;
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
@@ -659,24 +685,14 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
         }
         if (q4 == 0 && n < gn) a.part_ml[part] = make_float2(m, l);
       }
-      at += units - unit0;
-      if (at >= end) return;
-      unit0 = tile = 0;
-      if (++pair == pairs) {
-        pair = 0;
-        do {
-          ++row;
-          units = __builtin_amdgcn_readfirstlane(row_units(a, row));
-        } while (units == 0);  // `at` lies before the end of the line: there is one
-      }
-      len = __builtin_amdgcn_readfirstlane((int)row_length(a, row, pair == 0 && lane == 0));
-      h = pair / tiles;
-      rt = pair - h * tiles;
+      if (!run.next(a, kMatrixShift, kMatrixCost)) return;
+      len = __builtin_amdgcn_readfirstlane((int)row_length(a, run.row, false));
+      h = run.pair / tiles;
+      rt = run.pair - h * tiles;
       gn = a.g - rt * 16 < 16 ? a.g - rt * 16 : 16;
-      qh0 = row * a.q_heads + h * a.g + rt * 16;
+      qh0 = run.row * a.q_heads + h * a.g + rt * 16;
       j1 = 0;
-      if (end - at <= kPairCost) return;  // the next wave has its tiles
-      last = (int64_t)len < (end - at - kPairCost) * 32 ? len : (int)((end - at - kPairCost) * 32);
+      last = run.last(kMatrixShift, kMatrixCost, len);
     }
   }
 
@@ -718,7 +734,7 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
     if (a.part_ml && ch == 0) {
       float mm = -INFINITY;
       for (int w = 0; w < waves; ++w) mm = fmaxf(mm, s_m[w * 16 + hd]);
-      a.part_ml[(row * pairs + pair) * gs + hd] = make_float2(mm, ls);
+      a.part_ml[(run.row * pairs + run.pair) * gs + hd] = make_float2(mm, ls);
     }
   }
   if (!a.logits || a.part_ml) return;
@@ -737,7 +753,7 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
     ih[g] = g < gn ? 1.f / ls : 0.f;
   }
   const float *lg = a.logits + qh0 * a.cap;
-  float *wr = a.weights + (row * a.c.heads + h) * a.weights_cols;
+  float *wr = a.weights + (run.row * a.c.heads + h) * a.weights_cols;
   for (int j = threadIdx.x; j < len; j += blockDim.x) {
     float sum = 0.f;
 #pragma unroll

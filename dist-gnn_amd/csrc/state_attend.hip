@@ -19,6 +19,22 @@ namespace {
 constexpr int kThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+
+// A word's codes as 16-bit floats: channel c is number c / 4 of pair c % 4.  A code in the low bits
+// of such a float is code * 2^-24 below its normal range, four bits up it is code * 2^-20: no
+// conversion, and exact.  The multiply-adds that take 16-bit factors widen them by themselves.
+struct Codes {
+  half2v p[4];
+};
+__device__ __forceinline__ Codes codes_of(uint32_t w) {
+  const uint32_t y = w >> 8;
+  return Codes{{__builtin_bit_cast(half2v, w & 0x000f000fu), __builtin_bit_cast(half2v, w & 0x00f000f0u),
+                __builtin_bit_cast(half2v, y & 0x000f000fu), __builtin_bit_cast(half2v, y & 0x00f000f0u)}};
+}
+// Channel c's unit, as the caller's factors: 2^-24 on even channels, 2^-20 on odd ones.
+constexpr float kTiny = 0x1p-24f, kUnTiny[2] = {0x1p24f, 0x1p20f};
+
 template <int LPR>
 __device__ __forceinline__ float sum_lanes(float x) {
   if constexpr (LPR >= 2) x += lane_xor32<1>(x);
@@ -39,59 +55,62 @@ __device__ __forceinline__ uint32_t of_quad(uint32_t x, int u) {
   }
 }
 
-// Vector form, for every type and size.  A work item is (row, head, GC query heads, split).  LPR
-// lanes hold a row (eight channels each); SL groups of them take four slots in a row at a time, with
-// a softmax state of their own, joined at the end by exchanges between lanes.  Rows are loaded one
-// step ahead of the arithmetic, ids another one.  What belongs to a slot and not to a channel - its
-// page and address, and with QG (groups of a multiple of 32 channels) its scale and base - is fetched
-// by one lane of every four and passed on by lane moves: 11 loads a step instead of 24.  As in the
-// matrix form, the running maximum is only followed when a logit passes it by 8.
+// Vector form, for every type and size.  A work item is (row, head, GC query heads) and the slots it
+// takes: a run of the stream form, or one of the equal chunks.  LPR lanes hold a row (eight channels
+// each); SL groups of them take four slots in a row at a time, with a softmax state of their own,
+// joined at the end by exchanges between lanes.  Rows are loaded one step ahead of the arithmetic, ids
+// another one.  What belongs to a slot and not to a channel - its page and address, and with QG (groups
+// of a multiple of 32 channels) its scale and base - is fetched by one lane of every four and passed on
+// by lane moves: 11 loads a step instead of 24.  K is taken as values (one multiply-add a code, then
+// one a query head); of V the codes are summed with p * scale, the bases apart.  As in the matrix form,
+// the running maximum is only followed when a logit passes it by 8.
 // SL = 1 is for rows of at most 16 slots: no join, and with all query heads of a head in the item
 // the probabilities stay in registers and the item writes its weights itself.
-template <int LPR, int SL, int GC, bool QG>
+// Bound by the vector instructions: 10 million of a wave in the 22.6 us of 16 rows of 8 heads (128
+// channels, 32-bit, 1 to 8192 slots) keep the SIMDs busy for 17; the sampled neighbours' rows (40960
+// rows of 0 to 15 slots, 4 heads of 32 channels) take 32 us, 21 of them in instructions.
+template <int LPR, int SL, int GC, bool QG, bool STREAM>
 __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
                                                          FastDivU32 splits, FastDivU32 gchunks,
                                                          FastDivU32 heads, uint32_t items) {
   constexpr int kItem = LPR * SL, kU = 4, kStep = SL * kU;
   constexpr int kKeep = SL > 1 ? 1 : (LPR >= 16 ? 1 : 16 / LPR);
   const int lane = threadIdx.x & (kItem - 1);
-  const uint32_t item = (blockIdx.x * (uint32_t)kThreads + threadIdx.x) / kItem;
-  if (item >= items) return;  // whole items leave together: no exchange crosses an item
   const int sub = lane % LPR, sl = lane / LPR, mine = sub & 3;  // mine: the slot of four I look up
-  const uint32_t is = splits.div(item), ig = gchunks.div(is), row = heads.div(ig);
-  const int split = (int)(item - is * splits.d), gc = (int)(is - ig * gchunks.d);
-  const int h = (int)(ig - row * heads.d);
+  uint32_t item = (blockIdx.x * (uint32_t)kThreads + threadIdx.x) / kItem;
+  if (kItem == 64) item = __builtin_amdgcn_readfirstlane(item);
+  Run run;
+  int64_t row;
+  int h, gc, split = 0, len, first, last;
+  if constexpr (STREAM) {
+    if (!run.start(a, a.shift, a.cost, a.least, a.c.heads * (int)gchunks.d, (int)item, lane)) return;
+    row = run.row;
+    h = run.pair / (int)gchunks.d;
+    gc = run.pair - h * (int)gchunks.d;
+    len = __builtin_amdgcn_readfirstlane((int)row_length(a, row, false));
+    first = run.tile << a.shift;
+    last = run.last(a.shift, a.cost, len);
+  } else {
+    if (item >= items) return;  // whole items leave together: no exchange crosses an item
+    const uint32_t is = splits.div(item), ig = gchunks.div(is);
+    row = heads.div(ig);
+    split = (int)(item - is * splits.d);
+    gc = (int)(is - ig * gchunks.d);
+    h = (int)(ig - (uint32_t)row * heads.d);
+    len = (int)row_length(a, row, split == 0 && h == 0 && gc == 0 && lane == 0);
+    first = split * (int)a.chunk;
+    if (split > 0 && first >= len) return;
+    last = a.splits == 1 ? len : (int)(first + a.chunk < len ? first + a.chunk : len);
+  }
   const int words = a.c.dim >> 3;
   const bool live = sub < words;
   const int w = live ? sub : 0, ng = a.c.dim / a.c.group, grp = 8 * w / a.c.group;
-  const int len = (int)row_length(a, row, split == 0 && h == 0 && gc == 0 && lane == 0);
-  const int first = split * (int)a.chunk;
-  if (split > 0 && first >= len) return;
-  const int last = a.splits == 1 ? len : (int)(first + a.chunk < len ? first + a.chunk : len);
-  const int a0 = h * a.g + gc * GC, gn = a.g - gc * GC < GC ? a.g - gc * GC : GC;
+  int a0 = h * a.g + gc * GC, gn = a.g - gc * GC < GC ? a.g - gc * GC : GC;
 
-  float q[GC][8], o[GC][8], m[GC], l[GC], xs[kKeep][GC];
-#pragma unroll
-  for (int g = 0; g < GC; ++g) {
-    if (live && g < gn) {
-      load_q(type, a.q, (int64_t)row * a.q_row + (a0 + g) * a.q_head + 8 * w, q[g]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) q[g][i] = 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      q[g][i] *= a.scale2;
-      o[g][i] = 0.f;
-    }
-    m[g] = -INFINITY;
-    l[g] = 0.f;
-#pragma unroll
-    for (int i = 0; i < kKeep; ++i) xs[i][g] = -INFINITY;
-  }
+  float q[GC][8], o[GC][8], ob[GC], m[GC], l[GC], xs[kKeep][GC];
   const int ps = a.c.pshift, mask = (1 << ps) - 1;
   const bool wide = a.table.bytes == 8;
-  const char *tab = (const char *)a.table.p + (((int64_t)row * a.width) << (wide ? 3 : 2));
+  const char *tab;  // the row's
   const uint32_t pages = (uint32_t)a.c.pages, half = (uint32_t)a.c.dim >> 1;
   uint32_t id = 0, id_hi = 0;  // of my slot of the next step
   struct Rows {
@@ -152,17 +171,18 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
       const bool ok = u < t.n && !((t.bad >> u) & 1);
       const uint32_t kw = QG ? of_quad(t.km[0], u) : t.km[QG ? 0 : u];
       const uint32_t km = live ? kw : 0u;
-      const float ks = scale_of(km), kb = base_of(km);
+      // values in units of 2^-24: no scale leaves the range
+      const float ks[2] = {scale_of(km), scale_of(km) * 0x1p-4f}, kb = base_of(km) * kTiny;
+      const Codes kc = codes_of(t.kq[u]);
       float kv[8];
-      codes8(t.kq[u], kv);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) kv[i] = __builtin_fmaf(kv[i], ks, kb);
+      for (int i = 0; i < 8; ++i) kv[i] = __builtin_fmaf((float)kc.p[i & 3][i >> 2], ks[i & 1], kb);
 #pragma unroll
       for (int g = 0; g < GC; ++g) {
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) s = __builtin_fmaf(q[g][i], kv[i], s);
-        s = sum_lanes<LPR>(s);
+        s = sum_lanes<LPR>(s) * kUnTiny[0];
         x[g][u] = ok ? s : -INFINITY;
       }
     }
@@ -190,6 +210,7 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
         const float f = __builtin_amdgcn_exp2f(m[g] - top);
         m[g] = top;
         l[g] *= f;
+        ob[g] *= f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) o[g][i] *= f;
       }
@@ -205,59 +226,105 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
       const uint32_t vw = QG ? of_quad(t.vm[0], u) : t.vm[QG ? 0 : u];
       const uint32_t vm = live && u < t.n && !((t.bad >> u) & 1) ? vw : 0u;
       const float vs = scale_of(vm), vb = base_of(vm);
-      float vv[8];
-      codes8(t.vq[u], vv);
+      const Codes vc = codes_of(t.vq[u]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) vv[i] = __builtin_fmaf(vv[i], vs, vb);
+      for (int g = 0; g < GC; ++g) {
+        const float ps = x[g][u] * vs;
+        ob[g] = __builtin_fmaf(x[g][u], vb, ob[g]);
 #pragma unroll
-      for (int g = 0; g < GC; ++g)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[g][i] = __builtin_fmaf(x[g][u], vv[i], o[g][i]);
+        for (int i = 0; i < 8; ++i) o[g][i] = __builtin_fmaf((float)vc.p[i & 3][i >> 2], ps, o[g][i]);
+      }
     }
   };
-  if (first < last) {
-    load_ids(first);
-    load_rows(first);
-    if constexpr (SL == 1) {
-#pragma unroll
-      for (int st = 0; st < 4; ++st) {
-        if (4 * st >= last) break;
-        const Rows now = t;
-        if (4 * st + 4 < last) load_rows(4 * st + 4);
-        compute(now, 4 * st, 4 * st);
-      }
-    } else {
 #pragma unroll 1
-      for (int j0 = first; j0 < last; j0 += kStep) {
-        const Rows now = t;
-        load_rows(j0 + kStep);
-        compute(now, j0, 0);
+  while (true) {
+    tab = (const char *)a.table.p + ((row * a.width) << (wide ? 3 : 2));
+    if (first < last) {  // the rows are on their way while the query is read
+      load_ids(first);
+      load_rows(first);
+    }
+#pragma unroll
+    for (int g = 0; g < GC; ++g) {
+      if (live && g < gn) {
+        load_q(type, a.q, row * a.q_row + (a0 + g) * a.q_head + 8 * w, q[g]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[g][i] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        q[g][i] *= a.scale2;
+        o[g][i] = 0.f;
+      }
+      ob[g] = 0.f;
+      m[g] = -INFINITY;
+      l[g] = 0.f;
+#pragma unroll
+      for (int i = 0; i < kKeep; ++i) xs[i][g] = -INFINITY;
+    }
+    if (first < last) {
+      if constexpr (SL == 1) {
+#pragma unroll
+        for (int st = 0; st < 4; ++st) {
+          if (4 * st >= last) break;
+          const Rows now = t;
+          if (4 * st + 4 < last) load_rows(4 * st + 4);
+          compute(now, 4 * st, 4 * st);
+        }
+      } else {
+#pragma unroll 1
+        for (int j0 = first; j0 < last; j0 += kStep) {
+          const Rows now = t;
+          load_rows(j0 + kStep);
+          compute(now, j0, 0);
+        }
       }
     }
-  }
+    // a pair that a wave of the stream form holds whole is finished here
+    const bool whole = STREAM ? first == 0 && last == len : a.splits == 1;
+    if (!STREAM || first < last) {
 #pragma unroll
-  for (int g = 0; g < GC; ++g) {
+      for (int g = 0; g < GC; ++g) {
 #pragma unroll
-    for (int s = LPR; s < kItem; s <<= 1) {
-      const float mo = __shfl_xor(m[g], s, 64);
-      const float mn = fmaxf(m[g], mo), ms = mn == -INFINITY ? 0.f : mn;
-      const float f = __builtin_amdgcn_exp2f(m[g] - ms), fo = __builtin_amdgcn_exp2f(mo - ms);
-      m[g] = mn;
-      l[g] = l[g] * f + __shfl_xor(l[g], s, 64) * fo;
+        for (int i = 0; i < 8; ++i) o[g][i] = __builtin_fmaf(o[g][i], kUnTiny[i & 1], ob[g]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[g][i] = o[g][i] * f + __shfl_xor(o[g][i], s, 64) * fo;
+        for (int s = LPR; s < kItem; s <<= 1) {
+          const float mo = __shfl_xor(m[g], s, 64);
+          const float mn = fmaxf(m[g], mo), ms = mn == -INFINITY ? 0.f : mn;
+          const float f = __builtin_amdgcn_exp2f(m[g] - ms), fo = __builtin_amdgcn_exp2f(mo - ms);
+          m[g] = mn;
+          l[g] = l[g] * f + __shfl_xor(l[g], s, 64) * fo;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[g][i] = o[g][i] * f + __shfl_xor(o[g][i], s, 64) * fo;
+        }
+        if (g >= gn || sl != 0) continue;
+        const int64_t qh = row * a.q_heads + a0 + g;
+        const int64_t part = STREAM ? (row * run.pairs + run.pair + item) * (a.g < GC ? a.g : GC) + g
+                                    : qh * a.splits + split;
+        if (!whole) {
+          if (live) store8<kStateF32>(a.part_o, part * a.c.dim + 8 * w, o[g]);
+        } else if (live) {
+          const float inv = len == 0 ? 0.f : 1.f / l[g];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[g][i] *= inv;
+          store_out(type, a.out, qh * a.c.dim + 8 * w, o[g]);
+        }
+        if (a.part_ml && sub == 0) a.part_ml[part] = make_float2(m[g], l[g]);
+      }
     }
-    if (g >= gn || sl != 0) continue;
-    const int64_t qh = (int64_t)row * a.q_heads + a0 + g;
-    if (a.splits > 1) {
-      if (live) store8<kStateF32>(a.part_o, (qh * a.splits + split) * a.c.dim + 8 * w, o[g]);
-    } else if (live) {
-      const float inv = len == 0 ? 0.f : 1.f / l[g];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) o[g][i] *= inv;
-      store_out(type, a.out, qh * a.c.dim + 8 * w, o[g]);
+    if constexpr (!STREAM) {
+      break;
+    } else {
+      if (!run.next(a, a.shift, a.cost)) return;
+      row = run.row;
+      h = run.pair / (int)gchunks.d;
+      gc = run.pair - h * (int)gchunks.d;
+      a0 = h * a.g + gc * GC;
+      gn = a.g - gc * GC < GC ? a.g - gc * GC : GC;
+      len = __builtin_amdgcn_readfirstlane((int)row_length(a, row, false));
+      first = 0;
+      last = run.last(a.shift, a.cost, len);
     }
-    if (a.part_ml && sub == 0) a.part_ml[qh * a.splits + split] = make_float2(m[g], l[g]);
   }
   if constexpr (SL == 1) {
     if (a.weights && !a.logits) {  // every query head of this head is here
@@ -288,24 +355,25 @@ __device__ __forceinline__ Parts parts_of(const AttendArgs &a, int64_t row, int 
   if (a.splits)
     return Parts{(row * a.q_heads + head) * a.splits, 1,
                  len == 0 ? 1 : (int)((len + a.chunk - 1) / a.chunk)};
-  const int tiles = (a.g + 15) / 16, pairs = a.c.heads * tiles, gs = a.g < 16 ? a.g : 16;
-  const int h = head / a.g, n = head - h * a.g, pair = h * tiles + n / 16;
+  const int t = a.together, tiles = (a.g + t - 1) / t, pairs = a.c.heads * tiles;
+  const int gs = a.g < t ? a.g : t, h = head / a.g, n = head - h * a.g, pair = h * tiles + n / t;
   int64_t part = row * pairs + pair;
   int parts = 1;
   if (a.stream) {
     const int lane = threadIdx.x & 63, per = (int)((a.rows + 63) >> 6);
     int before, own, total;
-    stream_sums(a, lane, per, before, own, total);
+    stream_sums(a, a.shift, a.cost, lane, per, before, own, total);
     const int who = (int)(row / per);
     int64_t front = __shfl(before, who, 64);
-    for (int64_t r = (int64_t)who * per; r < row; ++r) front += row_units(a, r);
-    const int q = stream_share(a, (int64_t)total * pairs), u = row_units(a, row);
+    for (int64_t r = (int64_t)who * per; r < row; ++r) front += row_units(a, r, a.shift, a.cost);
+    const int q = stream_share(a, a.cost, a.least, (int64_t)total * pairs);
+    const int u = row_units(a, row, a.shift, a.cost);
     const int64_t start = front * pairs + (int64_t)pair * u;
-    const int64_t w0 = (start + kPairCost) / q;  // the wave of its first tile
+    const int64_t w0 = (start + a.cost) / q;  // the wave of its first tile
     parts = u == 0 ? 1 : (int)((start + u - 1) / q - w0) + 1;
     part += w0;
   }
-  return Parts{part * gs + n % 16, gs, parts};
+  return Parts{part * gs + n % t, gs, parts};
 }
 // The maximum and 1 / sum of kG query heads over their parts (head g's `step` g behind), on every
 // lane of the wave; heads at or past g_end repeat the first.
@@ -363,37 +431,43 @@ __device__ __forceinline__ void join_ml(const AttendArgs &a, const Parts &p, int
 }
 
 // Joins the parts of the rows' query heads and adds the weights; every wave works alone.  The
-// first `outs` waves take a query head's output each (eight channels a lane, the lanes' groups
-// taking every n-th part), the others 1024 slots of a (row, head)'s weights.
+// first `outs` waves take 8 `lpr` channels of a query head's output each (eight channels a lane, the
+// lanes' groups taking every n-th part), the others 1024 slots of a (row, head)'s weights.
 constexpr int kSpan = 1024;
 template <int TYPE>
-__global__ __launch_bounds__(kThreads) void k_attend_finish(AttendArgs a, int64_t outs,
+__global__ __launch_bounds__(kThreads) void k_attend_finish(AttendArgs a, int64_t outs, int lpr,
                                                             int spans, int64_t waves) {
   const int64_t id = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
   if (id >= waves) return;
   const int lane = threadIdx.x & 63;
   if (id < outs) {
-    const int64_t row = id / a.q_heads;
-    const int64_t len = row_length(a, row, false);
-    const Parts p = parts_of(a, row, (int)(id % a.q_heads), len);
+    const int words = a.c.dim >> 3, slices = (words + lpr - 1) / lpr;
+    const int64_t qh = id / slices, row = qh / a.q_heads;
+    const int64_t len = row_length(a, row, a.stream && id % (a.q_heads * slices) == 0 && lane == 0);
+    const Parts p = parts_of(a, row, (int)(qh % a.q_heads), len);
     if (a.stream && p.n == 1 && len > 0) return;  // written by the wave that had it whole
-    const int words = a.c.dim >> 3;
-    int lpr = 1;
-    while (lpr < words) lpr <<= 1;
-    const int w = lane & (lpr - 1), part = lane / lpr, parts = 64 / lpr;
+    const int w = (int)(id % slices) * lpr + (lane & (lpr - 1));
+    const int part = lane / lpr, parts = 64 / lpr;
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (len > 0) {
       float2 joined[1];
       join_ml<1>(a, p, 0, 1, joined);
       const float2 ml = joined[0];
       if (w < words)
-        for (int s = part; s < p.n; s += parts) {
-          const int64_t at = p.part + (int64_t)s * p.stride;
-          const float f = __builtin_amdgcn_exp2f(a.part_ml[at].x - ml.x);
-          float x[8];
-          load8<kStateF32>(a.part_o, at * a.c.dim + 8 * w, x);
+        for (int s0 = part; s0 < p.n; s0 += 4 * parts) {  // four parts in flight
+          float x[4][8], f[4];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) acc[i] = __builtin_fmaf(x[i], f, acc[i]);
+          for (int u = 0; u < 4; ++u) {
+            const int s = s0 + u * parts < p.n ? s0 + u * parts : s0;
+            const int64_t at = p.part + (int64_t)s * p.stride;
+            f[u] = __builtin_amdgcn_exp2f(a.part_ml[at].x - ml.x);
+            load8<kStateF32>(a.part_o, at * a.c.dim + 8 * w, x[u]);
+          }
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (s0 + u * parts < p.n)
+#pragma unroll
+              for (int i = 0; i < 8; ++i) acc[i] = __builtin_fmaf(x[u][i], f[u], acc[i]);
         }
       for (int o = lpr; o < 64; o <<= 1)
 #pragma unroll
@@ -401,7 +475,7 @@ __global__ __launch_bounds__(kThreads) void k_attend_finish(AttendArgs a, int64_
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc[i] *= ml.y;
     }
-    if (part == 0 && w < words) store8<TYPE>(a.out, id * a.c.dim + 8 * w, acc);
+    if (part == 0 && w < words) store8<TYPE>(a.out, qh * a.c.dim + 8 * w, acc);
     return;
   }
   const int64_t pair = (id - outs) / spans;
@@ -420,9 +494,9 @@ __global__ __launch_bounds__(kThreads) void k_attend_finish(AttendArgs a, int64_
     for (int i = 0; i < kI; ++i) sum[r][i] = 0.f;
   Parts p = parts_of(a, row, head0, len);
   for (int g0 = 0; g0 < a.g; g0 += kG) {
-    // 16 query heads share their parts' places (kG divides 16)
-    if (a.splits || (g0 > 0 && g0 % 16 == 0)) p = parts_of(a, row, head0 + g0, len);
-    const Parts pg{p.part + (a.splits ? 0 : g0 % 16), p.stride, p.n};
+    // the query heads of a pair share their parts' places (kG divides 16 and 4)
+    if (a.splits || (g0 > 0 && g0 % a.together == 0)) p = parts_of(a, row, head0 + g0, len);
+    const Parts pg{p.part + (a.splits ? 0 : g0 % a.together), p.stride, p.n};
     float2 ml[kG];
     join_ml<kG>(a, pg, a.splits ? a.splits : 1, a.g - g0, ml);
 #pragma unroll
@@ -456,12 +530,19 @@ __global__ __launch_bounds__(kThreads) void k_attend_finish(AttendArgs a, int64_
     }
 }
 
+// The vector form's line: tiles are its steps, and a pair costs two of them (16 rows of 8 heads of 128
+// channels, 1 to 8192 slots, 32-bit: 29 us; 32 to 37 us at 4 to 6 where rows are short).  4096 waves are
+// the four a SIMD that the registers of two query heads leave; 5120 and 8192 are no faster.
+constexpr int kVecWaves = 4096, kVecCost = 2, kVecLeast = 1;
+// Waves below which the joining takes narrower slices of channels.
+constexpr int kJoinWaves = 1024;
+
 struct AttendPlan {
   bool matrix;
   int waves;   // of a workgroup of the matrix form
-  int stream;  // its stream form's waves, or 0
+  int stream;  // waves of the stream form, or 0
   int64_t chunk;
-  int splits;  // vector form
+  int splits;  // vector form without
   int64_t cap;
   bool finish;  // the finishing kernel runs
   int64_t o_bytes, ml_bytes, logit_bytes;
@@ -470,7 +551,7 @@ struct AttendPlan {
 int64_t up256(int64_t x) { return (x + 255) & ~int64_t(255); }
 
 // Query heads of a work item of the vector form, and items a head needs.
-int vec_gc(int g) { return g >= 4 ? 4 : (g >= 2 ? 2 : 1); }
+int vec_gc(int g) { return g < 4 ? g : 4; }
 int vec_gchunks(int g) { return (g + vec_gc(g) - 1) / vec_gc(g); }
 
 AttendPlan plan_attend(const StateView &c, const AttendCall &a) {
@@ -509,6 +590,22 @@ AttendPlan plan_attend(const StateView &c, const AttendCall &a) {
     if (a.weights) p.logit_bytes = up256(qh * p.cap * 4);
     return p;
   }
+  // Rows that can be longer than 512 slots are cut evenly, as in the matrix form: 16 rows of 8 heads,
+  // 1 to 8192 slots, 32-bit: 29 us against 45 in equal chunks; 300 rows of 1 to 2000: 115, 152;
+  // 4 rows of 500 to 700: 20.0, 18.6; 700 rows of 5 to 300: 52, 36.
+  p.stream = p.cap > 512 && a.rows <= kStreamRows &&
+                     a.rows * ceil_div(p.cap, 8) < (int64_t(1) << 30)
+                 ? kVecWaves
+                 : 0;
+  if (p.stream) {
+    const int64_t parts =
+        (a.rows * c.heads * vec_gchunks(g) + p.stream) * (int64_t)vec_gc(g);
+    p.finish = true;
+    p.o_bytes = up256(parts * c.dim * 4);
+    p.ml_bytes = up256(parts * 8);
+    if (a.weights) p.logit_bytes = up256(qh * p.cap * 4);
+    return p;
+  }
   int64_t chunk = ceil_div(p.cap * a.rows * c.heads * vec_gchunks(g), 16384);
   chunk = chunk < 64 ? 64 : (chunk + 63) & ~int64_t(63);
   p.splits = (int)(p.cap <= chunk ? 1 : ceil_div(p.cap, chunk));
@@ -528,38 +625,42 @@ int pow2_at_least(int x) {
   return p;
 }
 
-template <int LPR, int SL, bool QG>
+template <int LPR, int SL, bool QG, bool STREAM>
 void launch_vec_g(const AttendArgs &a, int type, hipStream_t st) {
   const int gc = vec_gc(a.g), gchunks = vec_gchunks(a.g);
-  const int64_t items = a.rows * a.c.heads * gchunks * a.splits;
+  const int64_t items = STREAM ? a.stream : a.rows * a.c.heads * gchunks * a.splits;
   const int64_t blocks = ceil_div(items * LPR * SL, kThreads);
   DGS_CHECK(items * LPR * SL < (int64_t(1) << 32) - kThreads,
             "attend: too many rows in one call");
   const unsigned grid = (unsigned)blocks;
-  const FastDivU32 fs = FastDivU32::make(a.splits), fg = FastDivU32::make(gchunks),
+  const FastDivU32 fs = FastDivU32::make(STREAM ? 1 : a.splits), fg = FastDivU32::make(gchunks),
                    fh = FastDivU32::make(a.c.heads);
   const uint32_t n = (uint32_t)items;
   if (gc == 4)
-    k_attend_vec<LPR, SL, 4, QG><<<grid, kThreads, 0, st>>>(a, type, fs, fg, fh, n);
+    k_attend_vec<LPR, SL, 4, QG, STREAM><<<grid, kThreads, 0, st>>>(a, type, fs, fg, fh, n);
+  else if (gc == 3)
+    k_attend_vec<LPR, SL, 3, QG, STREAM><<<grid, kThreads, 0, st>>>(a, type, fs, fg, fh, n);
   else if (gc == 2)
-    k_attend_vec<LPR, SL, 2, QG><<<grid, kThreads, 0, st>>>(a, type, fs, fg, fh, n);
+    k_attend_vec<LPR, SL, 2, QG, STREAM><<<grid, kThreads, 0, st>>>(a, type, fs, fg, fh, n);
   else
-    k_attend_vec<LPR, SL, 1, QG><<<grid, kThreads, 0, st>>>(a, type, fs, fg, fh, n);
+    k_attend_vec<LPR, SL, 1, QG, STREAM><<<grid, kThreads, 0, st>>>(a, type, fs, fg, fh, n);
   DGS_LAUNCH_CHECK();
 }
-template <int LPR, int SL>
+template <int LPR, int SL, bool STREAM>
 void launch_vec_s(const AttendArgs &a, int type, hipStream_t st) {
   if (a.c.group % 32 == 0)
-    launch_vec_g<LPR, SL, true>(a, type, st);
+    launch_vec_g<LPR, SL, true, STREAM>(a, type, st);
   else
-    launch_vec_g<LPR, SL, false>(a, type, st);
+    launch_vec_g<LPR, SL, false, STREAM>(a, type, st);
 }
 template <int LPR>
 void launch_vec(const AttendArgs &a, int type, hipStream_t st) {
   if (a.cap <= 16)
-    launch_vec_s<LPR, 1>(a, type, st);
+    launch_vec_s<LPR, 1, false>(a, type, st);
+  else if (a.stream)
+    launch_vec_s<LPR, 64 / LPR, true>(a, type, st);
   else
-    launch_vec_s<LPR, 64 / LPR>(a, type, st);
+    launch_vec_s<LPR, 64 / LPR, false>(a, type, st);
 }
 
 }  // namespace
@@ -592,6 +693,11 @@ void state_attend(const StateView &c, const AttendCall &call, void *ws, int64_t 
   a.chunk = p.chunk;
   a.splits = p.splits;
   a.stream = p.stream;
+  a.together = p.matrix ? 16 : 4;
+  const int lanes = pow2_at_least(c.dim >> 3) < 4 ? 4 : pow2_at_least(c.dim >> 3);
+  a.shift = p.matrix ? kMatrixShift : lanes == 4 ? 6 : lanes == 8 ? 5 : lanes == 16 ? 4 : 3;
+  a.cost = p.matrix ? kMatrixCost : kVecCost;
+  a.least = p.matrix ? kMatrixLeast : kVecLeast;
   char *w = static_cast<char *>(ws);
   if (p.o_bytes) a.part_o = (float *)w;
   if (p.ml_bytes) a.part_ml = (float2 *)(w + p.o_bytes);
@@ -605,16 +711,20 @@ void state_attend(const StateView &c, const AttendCall &call, void *ws, int64_t 
   if (p.matrix) {
     (c.group == 32 ? attend_matrix_32 : c.group == 64 ? attend_matrix_64 : attend_matrix_128)(
         a, p.waves, call.type, st);
-  } else switch (pow2_at_least(c.dim >> 3)) {
-    case 1:
-    case 2:
+  } else switch (lanes) {
     case 4: launch_vec<4>(a, call.type, st); break;
     case 8: launch_vec<8>(a, call.type, st); break;
     case 16: launch_vec<16>(a, call.type, st); break;
     default: launch_vec<32>(a, call.type, st); break;
   }
   if (!p.finish) return;
-  const int64_t outs = p.splits > 1 || p.stream ? call.rows * call.q_heads : 0;
+  const int64_t qh = call.rows * call.q_heads;
+  // lanes of a part in the joining: few query heads have many parts each, which narrow slices take
+  // more at a time: 32 query heads of 256 parts 11 us, 20 with 128 channels a wave; where there are
+  // many heads it only makes waves (64 rows of 32: 67 us in all, 74 at 16384)
+  int lpr = lanes;
+  while (lpr > 4 && qh * ceil_div(c.dim >> 3, lpr) < kJoinWaves) lpr >>= 1;
+  const int64_t outs = p.splits > 1 || p.stream ? qh * ceil_div(c.dim >> 3, lpr) : 0;
   const int spans = p.logit_bytes ? (int)ceil_div(p.cap, kSpan) : 0;
   const int64_t waves = outs + call.rows * c.heads * spans;
   const int64_t blocks = ceil_div(waves, kThreads / 64);
@@ -622,11 +732,11 @@ void state_attend(const StateView &c, const AttendCall &call, void *ws, int64_t 
   DGS_CHECK(blocks < (int64_t(1) << 31), "attend: too many rows in one call");
   const unsigned grid = (unsigned)blocks;
   if (call.type == kStateF32)
-    k_attend_finish<kStateF32><<<grid, kThreads, 0, st>>>(a, outs, spans, waves);
+    k_attend_finish<kStateF32><<<grid, kThreads, 0, st>>>(a, outs, lpr, spans, waves);
   else if (call.type == kStateBF16)
-    k_attend_finish<kStateBF16><<<grid, kThreads, 0, st>>>(a, outs, spans, waves);
+    k_attend_finish<kStateBF16><<<grid, kThreads, 0, st>>>(a, outs, lpr, spans, waves);
   else
-    k_attend_finish<kStateF16><<<grid, kThreads, 0, st>>>(a, outs, spans, waves);
+    k_attend_finish<kStateF16><<<grid, kThreads, 0, st>>>(a, outs, lpr, spans, waves);
   DGS_LAUNCH_CHECK();
 }
 

@@ -644,3 +644,39 @@ def test_a_refused_registration_is_not_reported_again():
     cache = full_cache(2, 4, 1, 64, 64)
     got = cache.read(torch.arange(8).cuda())
     assert got[0].shape == (8, 1, 64) and torch.isfinite(got[0]).all()
+
+
+@pytest.mark.parametrize("dim, group, heads, g, dtype", [
+    (80, 40, 3, 1, "f16"), (96, 32, 1, 3, "bf16"), (128, 64, 2, 2, "f32"), (256, 64, 1, 1, "f32"),
+    (16, 8, 2, 5, "bf16"), (32, 32, 2, 4, "f32"), (40, 40, 1, 7, "f32")])
+@pytest.mark.parametrize("rows, high, page", [(300, 1000, 8), (1024, 700, 16), (1025, 700, 1),
+                                              (3, 6000, 64), (1, 520, 1), (40, 600, 128)])
+def test_attend_ragged_rows_of_every_size(dim, group, heads, g, dtype, rows, high, page):
+    """As test_attend_ragged_rows, for the channels, groups and types of the vector form."""
+    gen = torch.Generator().manual_seed(rows + dim)
+    lens = (torch.rand(rows, generator=gen) ** 8 * high).long()
+    lens[rows // 2], lens[-1] = high, (0 if rows > 2 else high - 1)
+    lens[rows // 3:rows // 3 + 70] = 0 if rows > 200 else lens[rows // 3]
+    pages = 2000 // page + 1
+    cache = full_cache(pages, page, heads, dim, group, seed=4)
+    table = torch.randint(0, pages, (rows, -(-high // page)), generator=gen)
+    q = states((rows, heads * g, dim), gen, TYPES[dtype])
+    w = torch.rand(rows, heads, table.shape[1] * page, generator=gen).cuda()
+    w = w if rows % 2 else None
+    check_attend(cache, q, table.int().cuda() if page > 1 else table.cuda(), lens.cuda(), weights=w)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("cap", [16, 64, 2048])
+def test_lengths_outside_are_reported_however_the_work_is_cut(cap, dtype):
+    gen = torch.Generator().manual_seed(cap)
+    cache = full_cache(cap // 16, 16, 2, 64, 64)
+    table = torch.arange(cap // 16, dtype=torch.int32).repeat(3, 1).cuda()
+    q = states((3, 4, 64), gen, TYPES[dtype])
+    want = cache.attend(q, table, torch.tensor([0, cap, 5]).cuda())
+    for bad, shown in ((-1, "length -1, outside"), (cap + 1, f"length {cap + 1}, outside")):
+        got = cache.attend(q, table, torch.tensor([bad, cap, 5]).cuda())
+        raises_next(shown)
+        assert torch.equal(got[1:], want[1:])
+        if bad < 0:
+            assert bool((got[0] == 0).all())
