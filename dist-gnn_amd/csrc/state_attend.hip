@@ -56,8 +56,8 @@ __device__ __forceinline__ uint32_t of_quad(uint32_t x, int u) {
 }
 
 // Vector form, for every type and size.  A work item is (row, head, GC query heads) and the slots it
-// takes: a run of the stream form, or one of the equal chunks.  LPR lanes hold a row (eight channels
-// each); SL groups of them take four slots in a row at a time, with a softmax state of their own,
+// takes: a run of the stream form, or one of the equal chunks.  LPR lanes hold a row (W words of eight
+// channels each); SL groups of them take four slots in a row at a time, with a softmax state of their own,
 // joined at the end by exchanges between lanes.  Rows are loaded one step ahead of the arithmetic, ids
 // another one.  What belongs to a slot and not to a channel - its page and address, and with QG (groups
 // of a multiple of 32 channels) its scale and base - is fetched by one lane of every four and passed on
@@ -69,7 +69,7 @@ __device__ __forceinline__ uint32_t of_quad(uint32_t x, int u) {
 // Bound by the vector instructions: 10 million of a wave in the 22.6 us of 16 rows of 8 heads (128
 // channels, 32-bit, 1 to 8192 slots) keep the SIMDs busy for 17; the sampled neighbours' rows (40960
 // rows of 0 to 15 slots, 4 heads of 32 channels) take 32 us, 21 of them in instructions.
-template <int LPR, int SL, int GC, bool QG, bool STREAM>
+template <int LPR, int W, int SL, int GC, bool QG, bool STREAM>
 __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
                                                          FastDivU32 splits, FastDivU32 gchunks,
                                                          FastDivU32 heads, uint32_t items) {
@@ -103,18 +103,25 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
     last = a.splits == 1 ? len : (int)(first + a.chunk < len ? first + a.chunk : len);
   }
   const int words = a.c.dim >> 3;
-  const bool live = sub < words;
-  const int w = live ? sub : 0, ng = a.c.dim / a.c.group, grp = 8 * w / a.c.group;
+  const int ng = a.c.dim / a.c.group;
+  bool live[W];
+  int w[W], grp[W];  // my words of a row, and their groups
+#pragma unroll
+  for (int k = 0; k < W; ++k) {
+    live[k] = sub + k * LPR < words;
+    w[k] = live[k] ? sub + k * LPR : 0;
+    grp[k] = 8 * w[k] / a.c.group;
+  }
   int a0 = h * a.g + gc * GC, gn = a.g - gc * GC < GC ? a.g - gc * GC : GC;
 
-  float q[GC][8], o[GC][8], ob[GC], m[GC], l[GC], xs[kKeep][GC];
+  float q[GC][W][8], o[GC][W][8], ob[GC][W], m[GC], l[GC], xs[kKeep][GC];
   const int ps = a.c.pshift, mask = (1 << ps) - 1;
   const bool wide = a.table.bytes == 8;
   const char *tab;  // the row's
   const uint32_t pages = (uint32_t)a.c.pages, half = (uint32_t)a.c.dim >> 1;
   uint32_t id = 0, id_hi = 0;  // of my slot of the next step
   struct Rows {
-    uint32_t kq[kU], vq[kU], km[QG ? 1 : kU], vm[QG ? 1 : kU];
+    uint32_t kq[kU][W], vq[kU][W], km[QG ? 1 : kU][W], vm[QG ? 1 : kU][W];
     int n;         // slots of the step before the end
     uint32_t bad;  // bit u: slot u's page lies outside the cache
   };
@@ -147,20 +154,29 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
     const uint64_t at = (uint64_t)r * half;
     load_ids(j0 + kStep);
     if constexpr (QG) {
-      t.km[0] = a.c.ks[r * ng + grp];
-      t.vm[0] = a.c.vs[r * ng + grp];
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        t.km[0][k] = a.c.ks[r * ng + grp[k]];
+        t.vm[0][k] = a.c.vs[r * ng + grp[k]];
+      }
     }
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       const uint64_t to =
-          ((uint64_t)of_quad((uint32_t)(at >> 32), u) << 32 | of_quad((uint32_t)at, u)) + 4 * w;
-      t.kq[u] = *(const uint32_t *)(a.c.kc + to);
-      t.vq[u] = *(const uint32_t *)(a.c.vc + to);
+          (uint64_t)of_quad((uint32_t)(at >> 32), u) << 32 | of_quad((uint32_t)at, u);
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        t.kq[u][k] = *(const uint32_t *)(a.c.kc + to + 4 * w[k]);
+        t.vq[u][k] = *(const uint32_t *)(a.c.vc + to + 4 * w[k]);
+      }
       if constexpr (!QG) {
         const uint64_t rw = ((uint64_t)of_quad((uint32_t)((uint64_t)r >> 32), u) << 32 |
-                             of_quad((uint32_t)r, u)) * ng + grp;
-        t.km[u] = a.c.ks[rw];
-        t.vm[u] = a.c.vs[rw];
+                             of_quad((uint32_t)r, u)) * ng;
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+          t.km[u][k] = a.c.ks[rw + grp[k]];
+          t.vm[u][k] = a.c.vs[rw + grp[k]];
+        }
       }
     }
   };
@@ -169,21 +185,28 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       const bool ok = u < t.n && !((t.bad >> u) & 1);
-      const uint32_t kw = QG ? of_quad(t.km[0], u) : t.km[QG ? 0 : u];
-      const uint32_t km = live ? kw : 0u;
-      // values in units of 2^-24: no scale leaves the range
-      const float ks[2] = {scale_of(km), scale_of(km) * 0x1p-4f}, kb = base_of(km) * kTiny;
-      const Codes kc = codes_of(t.kq[u]);
-      float kv[8];
+      float s[GC];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) kv[i] = __builtin_fmaf((float)kc.p[i & 3][i >> 2], ks[i & 1], kb);
+      for (int g = 0; g < GC; ++g) s[g] = 0.f;
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        const uint32_t kw = QG ? of_quad(t.km[0][k], u) : t.km[QG ? 0 : u][k];
+        const uint32_t km = live[k] ? kw : 0u;
+        // values in units of 2^-24: no scale leaves the range
+        const float ks[2] = {scale_of(km), scale_of(km) * 0x1p-4f}, kb = base_of(km) * kTiny;
+        const Codes kc = codes_of(t.kq[u][k]);
+        float kv[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) kv[i] = __builtin_fmaf((float)kc.p[i & 3][i >> 2], ks[i & 1], kb);
+#pragma unroll
+        for (int g = 0; g < GC; ++g)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) s[g] = __builtin_fmaf(q[g][k][i], kv[i], s[g]);
+      }
 #pragma unroll
       for (int g = 0; g < GC; ++g) {
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s = __builtin_fmaf(q[g][i], kv[i], s);
-        s = sum_lanes<LPR>(s) * kUnTiny[0];
-        x[g][u] = ok ? s : -INFINITY;
+        const float x0 = sum_lanes<LPR>(s[g]) * kUnTiny[0];
+        x[g][u] = ok ? x0 : -INFINITY;
       }
     }
     if (SL == 1) {
@@ -210,9 +233,12 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
         const float f = __builtin_amdgcn_exp2f(m[g] - top);
         m[g] = top;
         l[g] *= f;
-        ob[g] *= f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[g][i] *= f;
+        for (int k = 0; k < W; ++k) {
+          ob[g][k] *= f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[g][k][i] *= f;
+        }
       }
       const float ms = m[g] == -INFINITY ? 0.f : m[g];
 #pragma unroll
@@ -222,19 +248,22 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
       }
     }
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const uint32_t vw = QG ? of_quad(t.vm[0], u) : t.vm[QG ? 0 : u];
-      const uint32_t vm = live && u < t.n && !((t.bad >> u) & 1) ? vw : 0u;
-      const float vs = scale_of(vm), vb = base_of(vm);
-      const Codes vc = codes_of(t.vq[u]);
+    for (int u = 0; u < kU; ++u)
 #pragma unroll
-      for (int g = 0; g < GC; ++g) {
-        const float ps = x[g][u] * vs;
-        ob[g] = __builtin_fmaf(x[g][u], vb, ob[g]);
+      for (int k = 0; k < W; ++k) {
+        const uint32_t vw = QG ? of_quad(t.vm[0][k], u) : t.vm[QG ? 0 : u][k];
+        const uint32_t vm = live[k] && u < t.n && !((t.bad >> u) & 1) ? vw : 0u;
+        const float vs = scale_of(vm), vb = base_of(vm);
+        const Codes vc = codes_of(t.vq[u][k]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[g][i] = __builtin_fmaf((float)vc.p[i & 3][i >> 2], ps, o[g][i]);
+        for (int g = 0; g < GC; ++g) {
+          const float ps = x[g][u] * vs;
+          ob[g][k] = __builtin_fmaf(x[g][u], vb, ob[g][k]);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            o[g][k][i] = __builtin_fmaf((float)vc.p[i & 3][i >> 2], ps, o[g][k][i]);
+        }
       }
-    }
   };
 #pragma unroll 1
   while (true) {
@@ -245,18 +274,21 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
     }
 #pragma unroll
     for (int g = 0; g < GC; ++g) {
-      if (live && g < gn) {
-        load_q(type, a.q, row * a.q_row + (a0 + g) * a.q_head + 8 * w, q[g]);
-      } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q[g][i] = 0.f;
-      }
+      for (int k = 0; k < W; ++k) {
+        if (live[k] && g < gn) {
+          load_q(type, a.q, row * a.q_row + (a0 + g) * a.q_head + 8 * w[k], q[g][k]);
+        } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        q[g][i] *= a.scale2;
-        o[g][i] = 0.f;
+          for (int i = 0; i < 8; ++i) q[g][k][i] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          q[g][k][i] *= a.scale2;
+          o[g][k][i] = 0.f;
+        }
+        ob[g][k] = 0.f;
       }
-      ob[g] = 0.f;
       m[g] = -INFINITY;
       l[g] = 0.f;
 #pragma unroll
@@ -286,7 +318,10 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
 #pragma unroll
       for (int g = 0; g < GC; ++g) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[g][i] = __builtin_fmaf(o[g][i], kUnTiny[i & 1], ob[g]);
+        for (int k = 0; k < W; ++k)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            o[g][k][i] = __builtin_fmaf(o[g][k][i], kUnTiny[i & 1], ob[g][k]);
 #pragma unroll
         for (int s = LPR; s < kItem; s <<= 1) {
           const float mo = __shfl_xor(m[g], s, 64);
@@ -295,19 +330,26 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
           m[g] = mn;
           l[g] = l[g] * f + __shfl_xor(l[g], s, 64) * fo;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) o[g][i] = o[g][i] * f + __shfl_xor(o[g][i], s, 64) * fo;
+          for (int k = 0; k < W; ++k)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              o[g][k][i] = o[g][k][i] * f + __shfl_xor(o[g][k][i], s, 64) * fo;
         }
         if (g >= gn || sl != 0) continue;
         const int64_t qh = row * a.q_heads + a0 + g;
         const int64_t part = STREAM ? (row * run.pairs + run.pair + item) * (a.g < GC ? a.g : GC) + g
                                     : qh * a.splits + split;
-        if (!whole) {
-          if (live) store8<kStateF32>(a.part_o, part * a.c.dim + 8 * w, o[g]);
-        } else if (live) {
-          const float inv = len == 0 ? 0.f : 1.f / l[g];
+        const float inv = len == 0 ? 0.f : 1.f / l[g];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) o[g][i] *= inv;
-          store_out(type, a.out, qh * a.c.dim + 8 * w, o[g]);
+        for (int k = 0; k < W; ++k) {
+          if (!live[k]) continue;
+          if (!whole) {
+            store8<kStateF32>(a.part_o, part * a.c.dim + 8 * w[k], o[g][k]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[g][k][i] *= inv;
+            store_out(type, a.out, qh * a.c.dim + 8 * w[k], o[g][k]);
+          }
         }
         if (a.part_ml && sub == 0) a.part_ml[part] = make_float2(m[g], l[g]);
       }
@@ -625,42 +667,72 @@ int pow2_at_least(int x) {
   return p;
 }
 
-template <int LPR, int SL, bool QG, bool STREAM>
-void launch_vec_g(const AttendArgs &a, int type, hipStream_t st) {
-  const int gc = vec_gc(a.g), gchunks = vec_gchunks(a.g);
+// How a row's words lie in lanes.  Two or three words a lane make less work of a slot (its softmax and
+// addresses are shared by more channels, and 10 or 12 words fill their lanes), but steps of more slots,
+// so not where slots are few or rows short, and not with the registers of three query heads: 16 rows
+// of 8 heads, 1 to 8192 slots, of 256 channels 45 to 40 us, of 96 with two query heads a head 37 to 33;
+// 700 rows of 1 to 1000 slots, 128 channels, 109 to 97; but 37 rows of 12 heads of 80 channels, 0 to
+// 1531 slots, 28 to 31, and 5000 rows of 20 to 40 slots 96 to 200.
+struct VecShape {
+  int lanes, words;
+};
+VecShape vec_shape(const StateView &c, int g, int64_t rows, int64_t cap) {
+  const int n = c.dim >> 3;
+  if (vec_gc(g) <= 2 && cap > 256 && rows * c.heads * cap >= 1 << 20) {
+    const int lanes = n <= 12 ? 4 : (n <= 24 ? 8 : 16);
+    return VecShape{lanes, (n + lanes - 1) / lanes};
+  }
+  return VecShape{n <= 4 ? 4 : (n <= 8 ? 8 : (n <= 16 ? 16 : 32)), 1};
+}
+
+template <int LPR, int W, int SL, int GC, bool QG, bool STREAM>
+void launch_vec_k(const AttendArgs &a, int type, hipStream_t st) {
+  const int gchunks = vec_gchunks(a.g);
   const int64_t items = STREAM ? a.stream : a.rows * a.c.heads * gchunks * a.splits;
   const int64_t blocks = ceil_div(items * LPR * SL, kThreads);
   DGS_CHECK(items * LPR * SL < (int64_t(1) << 32) - kThreads,
             "attend: too many rows in one call");
-  const unsigned grid = (unsigned)blocks;
-  const FastDivU32 fs = FastDivU32::make(STREAM ? 1 : a.splits), fg = FastDivU32::make(gchunks),
-                   fh = FastDivU32::make(a.c.heads);
-  const uint32_t n = (uint32_t)items;
-  if (gc == 4)
-    k_attend_vec<LPR, SL, 4, QG, STREAM><<<grid, kThreads, 0, st>>>(a, type, fs, fg, fh, n);
-  else if (gc == 3)
-    k_attend_vec<LPR, SL, 3, QG, STREAM><<<grid, kThreads, 0, st>>>(a, type, fs, fg, fh, n);
-  else if (gc == 2)
-    k_attend_vec<LPR, SL, 2, QG, STREAM><<<grid, kThreads, 0, st>>>(a, type, fs, fg, fh, n);
-  else
-    k_attend_vec<LPR, SL, 1, QG, STREAM><<<grid, kThreads, 0, st>>>(a, type, fs, fg, fh, n);
+  k_attend_vec<LPR, W, SL, GC, QG, STREAM><<<(unsigned)blocks, kThreads, 0, st>>>(
+      a, type, FastDivU32::make(STREAM ? 1 : a.splits), FastDivU32::make(gchunks),
+      FastDivU32::make(a.c.heads), (uint32_t)items);
   DGS_LAUNCH_CHECK();
 }
-template <int LPR, int SL, bool STREAM>
-void launch_vec_s(const AttendArgs &a, int type, hipStream_t st) {
+template <int LPR, int W, int SL, int GC, bool STREAM>
+void launch_vec_q(const AttendArgs &a, int type, hipStream_t st) {
   if (a.c.group % 32 == 0)
-    launch_vec_g<LPR, SL, true, STREAM>(a, type, st);
+    launch_vec_k<LPR, W, SL, GC, true, STREAM>(a, type, st);
   else
-    launch_vec_g<LPR, SL, false, STREAM>(a, type, st);
+    launch_vec_k<LPR, W, SL, GC, false, STREAM>(a, type, st);
 }
-template <int LPR>
+template <int LPR, int W, int GC>
 void launch_vec(const AttendArgs &a, int type, hipStream_t st) {
-  if (a.cap <= 16)
-    launch_vec_s<LPR, 1, false>(a, type, st);
-  else if (a.stream)
-    launch_vec_s<LPR, 64 / LPR, true>(a, type, st);
+  if (a.stream)
+    launch_vec_q<LPR, W, 64 / LPR, GC, true>(a, type, st);
   else
-    launch_vec_s<LPR, 64 / LPR, false>(a, type, st);
+    launch_vec_q<LPR, W, 64 / LPR, GC, false>(a, type, st);
+}
+template <int LPR, int GC>
+void launch_vec_one(const AttendArgs &a, int type, hipStream_t st) {
+  if (a.cap <= 16)
+    launch_vec_q<LPR, 1, 1, GC, false>(a, type, st);
+  else
+    launch_vec<LPR, 1, GC>(a, type, st);
+}
+template <int GC>
+void launch_vec_gc(const AttendArgs &a, VecShape s, int type, hipStream_t st) {
+  if constexpr (GC <= 2) {
+    if (s.words == 2 && s.lanes == 4) return launch_vec<4, 2, GC>(a, type, st);
+    if (s.words == 2 && s.lanes == 8) return launch_vec<8, 2, GC>(a, type, st);
+    if (s.words == 2) return launch_vec<16, 2, GC>(a, type, st);
+    if (s.words == 3 && s.lanes == 4) return launch_vec<4, 3, GC>(a, type, st);
+    if (s.words == 3) return launch_vec<8, 3, GC>(a, type, st);
+  }
+  switch (s.lanes) {
+    case 4: return launch_vec_one<4, GC>(a, type, st);
+    case 8: return launch_vec_one<8, GC>(a, type, st);
+    case 16: return launch_vec_one<16, GC>(a, type, st);
+    default: return launch_vec_one<32, GC>(a, type, st);
+  }
 }
 
 }  // namespace
@@ -694,8 +766,8 @@ void state_attend(const StateView &c, const AttendCall &call, void *ws, int64_t 
   a.splits = p.splits;
   a.stream = p.stream;
   a.together = p.matrix ? 16 : 4;
-  const int lanes = pow2_at_least(c.dim >> 3) < 4 ? 4 : pow2_at_least(c.dim >> 3);
-  a.shift = p.matrix ? kMatrixShift : lanes == 4 ? 6 : lanes == 8 ? 5 : lanes == 16 ? 4 : 3;
+  const VecShape shape = vec_shape(c, a.g, call.rows, p.cap);
+  a.shift = p.matrix ? kMatrixShift : shape.lanes == 4 ? 6 : shape.lanes == 8 ? 5 : shape.lanes == 16 ? 4 : 3;
   a.cost = p.matrix ? kMatrixCost : kVecCost;
   a.least = p.matrix ? kMatrixLeast : kVecLeast;
   char *w = static_cast<char *>(ws);
@@ -711,18 +783,20 @@ void state_attend(const StateView &c, const AttendCall &call, void *ws, int64_t 
   if (p.matrix) {
     (c.group == 32 ? attend_matrix_32 : c.group == 64 ? attend_matrix_64 : attend_matrix_128)(
         a, p.waves, call.type, st);
-  } else switch (lanes) {
-    case 4: launch_vec<4>(a, call.type, st); break;
-    case 8: launch_vec<8>(a, call.type, st); break;
-    case 16: launch_vec<16>(a, call.type, st); break;
-    default: launch_vec<32>(a, call.type, st); break;
+  } else {
+    switch (vec_gc(a.g)) {
+      case 1: launch_vec_gc<1>(a, shape, call.type, st); break;
+      case 2: launch_vec_gc<2>(a, shape, call.type, st); break;
+      case 3: launch_vec_gc<3>(a, shape, call.type, st); break;
+      default: launch_vec_gc<4>(a, shape, call.type, st); break;
+    }
   }
   if (!p.finish) return;
   const int64_t qh = call.rows * call.q_heads;
   // lanes of a part in the joining: few query heads have many parts each, which narrow slices take
   // more at a time: 32 query heads of 256 parts 11 us, 20 with 128 channels a wave; where there are
   // many heads it only makes waves (64 rows of 32: 67 us in all, 74 at 16384)
-  int lpr = lanes;
+  int lpr = pow2_at_least(c.dim >> 3);
   while (lpr > 4 && qh * ceil_div(c.dim >> 3, lpr) < kJoinWaves) lpr >>= 1;
   const int64_t outs = p.splits > 1 || p.stream ? qh * ceil_div(c.dim >> 3, lpr) : 0;
   const int spans = p.logit_bytes ? (int)ceil_div(p.cap, kSpan) : 0;
