@@ -11,8 +11,8 @@
 // The plan, one workgroup per (row, head): weights and positions are read once, four slots a load,
 // and stay in registers as keys (32 bits, larger is better; rows past 32768 slots read them again
 // each time); the budget-th best key by counting digits; then ties, holes and movers are numbered
-// in slot order by counting lanes, the waves' counts joined by a scan.  What lies below the budget is
-// copied as it passes and the holes are overwritten afterwards.
+// in slot order by scans over lanes and waves.  What lies below the budget is copied as it passes and the
+// holes are overwritten afterwards.
 // The moves are a kernel of their own, over all stores; where there can only be a few (a cache
 // that takes single tokens) the plan's workgroup does them.
 #include "dgs_block.cuh"
@@ -97,7 +97,6 @@ struct PlanRow {
   float *wo;
   int32_t *po;
 };
-template <int THREADS>
 __device__ __forceinline__ PlanRow plan_row(const EvictArgs &a) {
   const EvictCall &e = a.e;
   PlanRow r;
@@ -120,10 +119,6 @@ __device__ __forceinline__ PlanRow plan_row(const EvictArgs &a) {
         ((int32_t *)e.lens_out)[r.row] = r.keep;
     }
     if (a.moves && r.n <= r.budget) a.moves[r.pair] = 0;
-  }
-  for (int j = r.keep + (int)threadIdx.x; j < r.cols; j += THREADS) {
-    r.wo[j] = 0.f;
-    r.po[j] = -1;
   }
   return r;
 }
@@ -168,7 +163,9 @@ __device__ __forceinline__ uint32_t pick_digit(const uint32_t *hist, uint32_t &l
   left = found[1];
   return found[0];
 }
-// Weights and positions of the slots that take a mover's row, and with FUSED the rows.
+// Weights and positions of the slots that take a mover's row, and with FUSED the rows.  (Taken along by
+// the kernel that moves rows they cost it 15 us and spare 2 here: 435 thousand moves of two stores of
+// 256 bytes a row.)
 template <int THREADS, bool FUSED>
 __device__ __forceinline__ void plan_end(const EvictArgs &a, const PlanRow &r,
                                          const int32_t *holes, const int32_t *movers,
@@ -232,23 +229,31 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan(EvictArgs a) {
     }
   }
   for (int i = tid; i < 3 * kDigits; i += THREADS) (&s_hist[0][0])[i] = 0;
-  const PlanRow r = plan_row<THREADS>(a);
+  const PlanRow r = plan_row(a);
 #pragma unroll
   for (int v = 0; v < kVecs; ++v) {
     const int j = (v * THREADS + tid) * 4;
-    if (v * THREADS * 4 >= r.n) break;
+    if (v * THREADS * 4 >= r.cols) break;
     if (!r.pos)
 #pragma unroll
       for (int i = 0; i < 4; ++i) p[v][i] = j + i;
-    if (ALIGNED && j + 4 <= r.keep) {
-      *(su32x4 *)(r.wo + j) = *(const su32x4 *)key[v];
-      *(su32x4 *)(r.po + j) = *(const su32x4 *)p[v];
+    su32x4 wo, po;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      wo[i] = j + i < r.keep ? key[v][i] : 0u;
+      po[i] = j + i < r.keep ? (uint32_t)p[v][i] : ~0u;
+    }
+    if (ALIGNED) {  // whole pieces of four
+      if (j < r.cols) {
+        *(su32x4 *)(r.wo + j) = wo;
+        *(su32x4 *)(r.po + j) = po;
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (j + i < r.keep) {
-          r.wo[j + i] = __uint_as_float(key[v][i]);
-          r.po[j + i] = p[v][i];
+        if (j + i < r.cols) {
+          r.wo[j + i] = __uint_as_float(wo[i]);
+          r.po[j + i] = (int32_t)po[i];
         }
     }
 #pragma unroll
@@ -326,7 +331,6 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan(EvictArgs a) {
     }
     __syncthreads();
   };
-  const uint64_t below = lane == 0 ? 0ull : ~0ull >> (64 - lane);
   uint32_t kept = 0;  // bit 4 v + i
   const bool all_ties = s_found[2] == left;
 #pragma unroll
@@ -341,27 +345,22 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan(EvictArgs a) {
   }
   if (!all_ties) {
     // of the slots whose key equals the threshold the first `left` in slot order stay
-    uint32_t tie = 0;
+    uint32_t tie = 0, at[kVecs];
 #pragma unroll
     for (int v = 0; v < kVecs; ++v) {
-      uint32_t cnt = 0;
-      if (v * THREADS * 4 < r.n) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool in = (v * THREADS + tid) * 4 + i < r.n;
-          if (in && key[v][i] == prefix) tie |= 1u << (4 * v + i);
-          cnt += __popcll(__ballot((tie >> (4 * v + i)) & 1));
-        }
+      for (int i = 0; i < 4; ++i) {
+        const bool in = (v * THREADS + tid) * 4 + i < r.n;
+        if (in && key[v][i] == prefix) tie |= 1u << (4 * v + i);
       }
-      if (lane == 0) s_run[v * kWaves + wave] = cnt;
+      const uint32_t own = __popc((tie >> (4 * v)) & 15u), sum = wave_inclusive_scan(own);
+      at[v] = sum - own;
+      if (lane == 63) s_run[v * kWaves + wave] = sum;
     }
     scan_runs();
 #pragma unroll
     for (int v = 0; v < kVecs; ++v) {
-      if (v * THREADS * 4 >= r.n) break;
-      uint32_t rank = s_run[v * kWaves + wave];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) rank += __popcll(__ballot((tie >> (4 * v + i)) & 1) & below);
+      uint32_t rank = s_run[v * kWaves + wave] + at[v];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if ((tie >> (4 * v + i)) & 1) {
@@ -373,33 +372,26 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan(EvictArgs a) {
   }
   // holes (dropped below the budget) in the low half, movers (kept at or past it) in the high one:
   // at most 32768 of each
-  uint32_t hole = 0, mover = 0;
+  uint32_t hole = 0, mover = 0, at[kVecs];
 #pragma unroll
   for (int v = 0; v < kVecs; ++v) {
-    uint32_t cnt = 0;
-    if (v * THREADS * 4 < r.n) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = (v * THREADS + tid) * 4 + i;
-        const bool k = (kept >> (4 * v + i)) & 1;
-        if (j < r.budget && !k) hole |= 1u << (4 * v + i);
-        if (j >= r.budget && k) mover |= 1u << (4 * v + i);
-        cnt += __popcll(__ballot((hole >> (4 * v + i)) & 1)) +
-               (__popcll(__ballot((mover >> (4 * v + i)) & 1)) << 16);
-      }
+    for (int i = 0; i < 4; ++i) {
+      const int j = (v * THREADS + tid) * 4 + i;
+      const bool k = (kept >> (4 * v + i)) & 1;
+      if (j < r.budget && !k) hole |= 1u << (4 * v + i);
+      if (j >= r.budget && k) mover |= 1u << (4 * v + i);
     }
-    if (lane == 0) s_run[v * kWaves + wave] = cnt;
+    const uint32_t own = __popc((hole >> (4 * v)) & 15u) | __popc((mover >> (4 * v)) & 15u) << 16;
+    const uint32_t sum = wave_inclusive_scan(own);
+    at[v] = sum - own;
+    if (lane == 63) s_run[v * kWaves + wave] = sum;
   }
   scan_runs();
   const uint32_t all = s_found[0] & 0xffffu;
 #pragma unroll
   for (int v = 0; v < kVecs; ++v) {
-    if (v * THREADS * 4 >= r.n) break;
-    uint32_t rank = s_run[v * kWaves + wave];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      rank += __popcll(__ballot((hole >> (4 * v + i)) & 1) & below) +
-              (__popcll(__ballot((mover >> (4 * v + i)) & 1) & below) << 16);
+    uint32_t rank = s_run[v * kWaves + wave] + at[v];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int j = (v * THREADS + tid) * 4 + i;
@@ -421,8 +413,12 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan_long(EvictArgs a) {
   __shared__ uint32_t s_hist[kDigits];
   __shared__ uint32_t s_scan[kWaves], s_found[3], s_cnt[3][kWaves];
   __shared__ int32_t s_max[kWaves];
-  const PlanRow r = plan_row<THREADS>(a);
+  const PlanRow r = plan_row(a);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = r.n;
+  for (int j = r.keep + tid; j < r.cols; j += THREADS) {
+    r.wo[j] = 0.f;
+    r.po[j] = -1;
+  }
   int32_t top = -1;
 #pragma unroll 4
   for (int j = tid; j < n; j += THREADS) {
