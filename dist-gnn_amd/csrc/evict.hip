@@ -23,7 +23,10 @@ namespace {
 
 constexpr int kMoveThreads = 256;
 constexpr int kDigits = 2048;  // 11 bits: the sign, the exponent and two bits of the mantissa first
-constexpr int kFewMoves = 32;
+// Moves a (row, head) can have at most for its plan's workgroup to do them.  64 rows of 8 heads of 4000
+// to 4097 slots, 256 bytes a row, room 237: 40 us, 43 with a kernel for the moves; one such row 24.6, 24.1;
+// 33 rows of 2 heads of 200 slots, room 100: 14, 18; room 500: 20 to 29 us in the plan, 18 apart.
+constexpr int kFewMoves = 256;
 
 struct EvictArgs {
   EvictCall e;
@@ -88,7 +91,31 @@ __device__ __forceinline__ void move_store(const EvictStore &st, const int64_t (
     move_rows<uint8_t, kU>(st, s, d, sub, lg);
 }
 
-// What both plans share: the row's sizes, the slots that no eviction touches, its outputs.
+// Moves first, first + stride, ... of a (row, head)'s list in one store, kU at a time.
+template <int kU>
+__device__ __forceinline__ void move_list(const EvictArgs &a, const EvictStore &st, int64_t row,
+                                          int h, const int32_t *holes, const int32_t *movers,
+                                          int moves, int first, int stride, int sub, int lg) {
+  for (int i = first; i < moves; i += kU * stride) {
+    int64_t d[kU], s[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const bool in = i + u * stride < moves;
+      const int x = in ? i + u * stride : i;
+      d[u] = store_slot(a, row, h, holes[x]);
+      s[u] = store_slot(a, row, h, movers[x]);
+      if (!in || d[u] < 0) s[u] = -1;
+    }
+    move_store<kU>(st, s, d, sub, lg);
+  }
+}
+// 1 << lg lanes for a row: one for each 16 bytes, up to a wave.
+__device__ __forceinline__ int row_lanes(const EvictStore &st, int lg) {
+  while (lg < 6 && (16 << lg) < st.row_bytes) ++lg;
+  return lg;
+}
+
+// What the plans share: the row's sizes, the slots that no eviction touches, its outputs.
 struct PlanRow {
   int64_t pair, row;
   int h, n, cols, budget, keep;
@@ -179,14 +206,81 @@ __device__ __forceinline__ void plan_end(const EvictArgs &a, const PlanRow &r,
     r.po[d] = r.pos ? r.pos[s] : s;
   }
   if constexpr (FUSED) {
-    const int lane = threadIdx.x & 63;
-    for (uint32_t i = threadIdx.x >> 6; i < all; i += THREADS / 64) {
-      const int64_t d[1] = {store_slot(a, r.row, r.h, holes[i])};
-      const int64_t s[1] = {store_slot(a, r.row, r.h, movers[i])};
-      if (d[0] >= 0 && s[0] >= 0)
-        for (int st = 0; st < a.e.nstores; ++st) move_store<1>(a.e.stores[st], s, d, lane, 6);
+    // the stores side by side, as many lanes a row as the longest has 16-byte pieces
+    int lg = 0;
+    for (int st = 0; st < a.e.nstores; ++st) lg = row_lanes(a.e.stores[st], lg);
+    const int sub = threadIdx.x & ((1 << lg) - 1), group = threadIdx.x >> lg;
+    const int groups = THREADS >> lg, per = groups > a.e.nstores ? groups / a.e.nstores : 1;
+    const int first = group % per;
+    for (int st = group / per; st < a.e.nstores; st += groups / per) {
+      const EvictStore &to = a.e.stores[st];
+      if ((int)all <= per)
+        move_list<1>(a, to, r.row, r.h, holes, movers, (int)all, first, per, sub, lg);
+      else
+        move_list<4>(a, to, r.row, r.h, holes, movers, (int)all, first, per, sub, lg);
     }
   }
+}
+
+// Rows of at most THREADS slots, one a thread: a slot stays if fewer than `keep` come before it, and
+// every thread counts them.  33 rows of 2 heads of 0 to 77 slots: 9.4 us, 13.6 with digits and one move a
+// wave at a time: a chain of loads (length, table, row), bound by nothing else.
+template <int THREADS, bool FUSED>
+__global__ __launch_bounds__(THREADS) void k_evict_plan_small(EvictArgs a) {
+  constexpr int kWaves = THREADS / 64;
+  __shared__ uint32_t s_key[THREADS], s_run[kWaves];
+  __shared__ int32_t s_max[kWaves];
+  __shared__ int32_t s_list[2 * kFewMoves];  // FUSED: holes, movers
+  const int j = threadIdx.x, lane = j & 63, wave = j >> 6;
+  const int64_t at = blockIdx.x * a.e.cols + (j < a.e.cols ? j : 0);
+  const float w = a.e.weights[at];
+  const int32_t p = a.e.positions ? a.e.positions[at] : j;
+  const PlanRow r = plan_row(a);
+  if (j < r.cols) {
+    r.wo[j] = j < r.keep ? w : 0.f;
+    r.po[j] = j < r.keep ? p : -1;
+  }
+  if (r.n <= r.budget) return;
+  const int32_t top = block_max<THREADS>(j < r.n ? p : -1, s_max);
+  const int64_t newest = (int64_t)top + 1 - a.e.recent;
+  // past the row: 0, behind every key
+  const uint32_t key = j < r.n ? key_of(w, p < a.e.sinks || p >= newest) : 0u;
+  s_key[j] = key;
+  __syncthreads();
+  // of equal keys the lower slot comes first
+  int before = 0;
+  for (int v = 0; v < kWaves; ++v) {
+    if (v * 64 >= r.n) break;
+    if (v == wave) {
+#pragma unroll 16
+      for (int i = 0; i < 64; ++i) {
+        const uint32_t k = s_key[v * 64 + i];
+        before += k > key || (k == key && i < lane);
+      }
+    } else {
+      const uint32_t least = v < wave ? key - (key != 0) : key;
+#pragma unroll 16
+      for (int i = 0; i < 64; ++i) before += s_key[v * 64 + i] > least;
+    }
+  }
+  const bool kept = j < r.n && before < r.keep;
+  const bool hole = j < r.budget && !kept, mover = j >= r.budget && kept;
+  // as many movers as holes: both numbers in a word
+  const uint32_t own = (hole ? 1u : 0u) | (mover ? 0x10000u : 0u);
+  const uint32_t sum = wave_inclusive_scan(own);
+  if (lane == 63) s_run[wave] = sum;
+  __syncthreads();
+  uint32_t rank = sum - own, all = 0;
+#pragma unroll
+  for (int v = 0; v < kWaves; ++v) {
+    if (v < wave) rank += s_run[v];
+    all += s_run[v];
+  }
+  int32_t *holes = FUSED ? s_list : a.holes + r.pair * a.room;
+  int32_t *movers = FUSED ? s_list + kFewMoves : a.movers + r.pair * a.room;
+  if (hole) holes[rank & 0xffffu] = j;
+  if (mover) movers[rank >> 16] = j;
+  plan_end<THREADS, FUSED>(a, r, holes, movers, all & 0xffffu);
 }
 
 // Rows of at most THREADS * kVecs * 4 slots: slot (v THREADS + t) 4 + i is thread t's.  ALIGNED:
@@ -503,32 +597,14 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan_long(EvictArgs a) {
   plan_end<THREADS, false>(a, r, holes, movers, all);
 }
 
-// Block (x, y, z): (row, head), a share of its moves, a store.  1 << lg lanes move a row (as many
-// as it has 16-byte pieces, up to a wave), four rows at a time.
+// Block (x, y, z): (row, head), a share of its moves, a store.
 __global__ __launch_bounds__(kMoveThreads) void k_evict_move(EvictArgs a) {
-  constexpr int kU = 4;
   const int64_t pair = blockIdx.x;
-  const int64_t row = pair / a.e.heads;
-  const int h = (int)(pair % a.e.heads);
-  const int moves = a.moves[pair];
   const EvictStore &st = a.e.stores[blockIdx.z];
-  int lg = 0;
-  while (lg < 6 && (16 << lg) < st.row_bytes) ++lg;
-  const int sub = threadIdx.x & ((1 << lg) - 1);
-  const int groups = kMoveThreads >> lg, stride = groups * gridDim.y;
-  const int32_t *holes = a.holes + pair * a.room, *movers = a.movers + pair * a.room;
-  for (int i = blockIdx.y * groups + (threadIdx.x >> lg); i < moves; i += kU * stride) {
-    int64_t d[kU], s[kU];
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const bool in = i + u * stride < moves;
-      const int x = in ? i + u * stride : i;
-      d[u] = store_slot(a, row, h, holes[x]);
-      s[u] = store_slot(a, row, h, movers[x]);
-      if (!in || d[u] < 0) s[u] = -1;
-    }
-    move_store<kU>(st, s, d, sub, lg);
-  }
+  const int lg = row_lanes(st, 0), groups = kMoveThreads >> lg;
+  move_list<4>(a, st, pair / a.e.heads, (int)(pair % a.e.heads), a.holes + pair * a.room,
+            a.movers + pair * a.room, a.moves[pair], blockIdx.y * groups + (threadIdx.x >> lg),
+            groups * gridDim.y, threadIdx.x & ((1 << lg) - 1), lg);
 }
 
 int64_t evict_room(const EvictCall &e) {
@@ -549,7 +625,12 @@ void launch_plan(const EvictArgs &a, hipStream_t st) {
 }
 template <bool FUSED>
 void plan(const EvictArgs &a, hipStream_t st) {
-  if (a.e.cols <= 1024)
+  const unsigned pairs = (unsigned)(a.e.rows * a.e.heads);
+  if (a.e.cols <= 64)
+    k_evict_plan_small<64, FUSED><<<pairs, 64, 0, st>>>(a);
+  else if (a.e.cols <= 256)
+    k_evict_plan_small<256, FUSED><<<pairs, 256, 0, st>>>(a);
+  else if (a.e.cols <= 1024)
     launch_plan<256, 1, FUSED>(a, st);
   else if (a.e.cols <= 8192)
     launch_plan<512, 4, FUSED>(a, st);
@@ -558,7 +639,7 @@ void plan(const EvictArgs &a, hipStream_t st) {
   else if (a.e.cols <= 32768)
     launch_plan<1024, 8, FUSED>(a, st);
   else if constexpr (!FUSED)
-    k_evict_plan_long<1024><<<(unsigned)(a.e.rows * a.e.heads), 1024, 0, st>>>(a);
+    k_evict_plan_long<1024><<<pairs, 1024, 0, st>>>(a);
   DGS_LAUNCH_CHECK();
 }
 

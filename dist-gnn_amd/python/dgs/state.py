@@ -169,8 +169,7 @@ class StateCache:
 
     def write(self, k, v, slots):
         """Rows k[t], v[t] ([tokens, heads, head_dim]) go to flat slot slots[t]; a negative slot
-        is skipped.  With a slot twice in a call it is not defined which row a channel group
-        keeps."""
+        is skipped.  What a slot holds that a call names twice is not defined."""
         if slots.dim() != 1 or slots.numel() != k.shape[0]:
             raise RuntimeError("slots must be [tokens]")
         slots = _ids(slots, "slots")
@@ -327,12 +326,18 @@ def evict_rows(stores, weights, positions, table, lens, budget, sinks=0, recent=
     lead = stores[0].shape[:3]
     if len(lead) != 3 or lead[0] == 0 or lead[1] != heads or lead[2] == 0:
         raise RuntimeError(f"a store must be [pages, {heads}, page_size, ...]")
+    pages, _, page = lead
+    slots, width = pages * heads * page, table.shape[1]
+    ptrs, nbytes = [], []
     for s in stores:
         if s.shape[:3] != lead:
             raise RuntimeError("the stores must have the same pages")
-        if not s.is_contiguous() or s.numel() == 0:
+        size = s.numel()
+        if size == 0 or not s.is_contiguous():
             raise RuntimeError("a store must be contiguous and not empty")
-    if cols < table.shape[1] * lead[2]:
+        ptrs.append(s.data_ptr())
+        nbytes.append(size // slots * s.element_size())
+    if cols < width * page:
         raise RuntimeError("weights need a column for every slot of the table")
     _no_grad(weights, *stores)
     if not weights.is_cuda:
@@ -342,10 +347,12 @@ def evict_rows(stores, weights, positions, table, lens, budget, sinks=0, recent=
     if positions is not None:
         _same_device(index, positions)
     with _on(index):
-        w = weights.contiguous()
-        p = None if positions is None else positions.contiguous()
-        new_w = torch.empty((rows, heads, cols), dtype=torch.float32, device=device)
-        new_p = torch.empty((rows, heads, cols), dtype=torch.int32, device=device)
+        w = weights if weights.is_contiguous() else weights.contiguous()
+        p = positions
+        if p is not None and not p.is_contiguous():
+            p = p.contiguous()
+        new_w = torch.empty_like(w)
+        new_p = torch.empty_like(w, dtype=torch.int32) if p is None else torch.empty_like(p)
         new_lens = torch.empty_like(lens)
         if rows == 0:
             return new_w, new_p, new_lens
@@ -358,13 +365,11 @@ def evict_rows(stores, weights, positions, table, lens, budget, sinks=0, recent=
                 _evict_room.clear()
             room = _evict_room[key] = n.value
         ws = torch.empty(room, dtype=torch.uint8, device=device) if room else None
-        ptrs = (c_vp * len(stores))(*[s.data_ptr() for s in stores])
-        slots = lead[0] * heads * lead[2]
-        nbytes = (c_i64 * len(stores))(*[s.numel() // slots * s.element_size() for s in stores])
+        n = len(stores)
         check(lib.dgs_evict_rows(
-            ptrs, nbytes, len(stores), lead[0], heads, lead[2], w.data_ptr(),
+            (c_vp * n)(*ptrs), (c_i64 * n)(*nbytes), n, pages, heads, page, w.data_ptr(),
             None if p is None else p.data_ptr(), new_w.data_ptr(), new_p.data_ptr(), rows, cols,
-            table.data_ptr(), table.element_size(), table.shape[1], lens.data_ptr(),
+            table.data_ptr(), table.element_size(), width, lens.data_ptr(),
             lens.element_size(), new_lens.data_ptr(), budget, sinks, recent,
             None if ws is None else ws.data_ptr(), room, stream_ptr(index)))
     return new_w, new_p, new_lens

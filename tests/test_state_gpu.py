@@ -696,3 +696,33 @@ def test_attend_many_slots_of_every_size(dim, group, g, dtype, rows, high):
     q = states((rows, 2 * g, dim), gen, TYPES[dtype])
     w = torch.rand(rows, 2, table.shape[1] * 16, generator=gen).cuda() if g == 1 else None
     check_attend(cache, q, table.int().cuda(), lens.cuda(), weights=w)
+
+
+@pytest.mark.parametrize("cols", [1, 5, 63, 64, 65, 200, 256, 257, 1000])
+@pytest.mark.parametrize("share", [0.1, 0.5, 0.95])
+def test_evict_short_rows(cols, share):
+    """Rows of few slots with many ties: every length there can be, four stores of odd rows."""
+    rng = np.random.default_rng(cols)
+    lens = np.unique(np.concatenate([np.arange(min(cols, 70) + 1), [cols // 2, cols - 1, cols]]))
+    rows, heads, budget = len(lens), 3, max(1, int(cols * share))
+    w = rng.integers(0, 5, (rows, heads, cols)).astype(np.float32) * 0.5 - 1
+    w[rng.random(w.shape) < 0.1] = np.nan
+    pos = rng.permuted(np.tile(np.arange(cols, dtype=np.int32) * 2, (rows, heads, 1)), axis=-1)
+    sinks, recent = budget // 3, budget // 2
+    table = rng.permutation(rows * cols).reshape(rows, cols)
+    stores = [torch.from_numpy(rng.integers(0, 256, (rows * cols, heads, 1, n), dtype=np.uint8)).cuda()
+              for n in (3, 16, 40, 272)]
+    expect = [s.cpu().clone() for s in stores]
+    want_w, want_p, want_n, moves = ref.evict(w, pos, lens, budget, sinks, recent)
+    t = torch.from_numpy(table)
+    for i, h, s, d in moves:
+        for e in expect:
+            e[t[i, d], h] = e[t[i, s], h]
+    got_w, got_p, got_n = dgs.ops.evict_rows(
+        stores, torch.from_numpy(w).cuda(), torch.from_numpy(pos).cuda(), t.cuda(),
+        torch.from_numpy(lens).cuda(), budget, sinks=sinks, recent=recent)
+    assert np.array_equal(got_n.cpu().numpy(), want_n)
+    assert np.array_equal(got_p.cpu().numpy(), want_p)
+    assert np.array_equal(got_w.cpu().numpy(), want_w, equal_nan=True)
+    for a, b in zip(stores, expect):
+        assert same_bits(a, b)
