@@ -156,12 +156,12 @@ class StateCache:
             check(lib.dgs_check_async_errors())  # makes the report words (never inside a capture)
 
     def _rows(self, k, v):
-        for name, t in (("k", k), ("v", v)):
-            if not (t.dim() == 3 and tuple(t.shape[1:]) == (self.heads, self.head_dim)):
-                raise RuntimeError(f"{name} must be [tokens, {self.heads}, {self.head_dim}]")
-            if not (t.dtype in _DTYPES):
-                raise RuntimeError(f"{name} must be float32, bfloat16 or float16")
-        if not (k.shape == v.shape and k.dtype == v.dtype):
+        shape = k.shape
+        if len(shape) != 3 or shape[1] != self.heads or shape[2] != self.head_dim:
+            raise RuntimeError(f"k must be [tokens, {self.heads}, {self.head_dim}]")
+        if k.dtype not in _DTYPES:
+            raise RuntimeError("k must be float32, bfloat16 or float16")
+        if v.shape != shape or v.dtype is not k.dtype:
             raise RuntimeError("k and v must be alike")
         _no_grad(k, v)
         _same_device(self._index, k, v)
@@ -195,7 +195,7 @@ class StateCache:
         k, v = self._rows(k, v)
         _same_device(self._index, table, lens)
         with _on(self._index):
-            slots = torch.empty(n, dtype=torch.int64, device=self.device)
+            slots = torch.empty_like(lens, dtype=torch.int64)
             check(lib.dgs_state_append(self._ref, k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype],
                                        n, k.stride(0), k.stride(1), v.stride(0), v.stride(1),
                                        table.data_ptr(), table.element_size(), table.shape[1],
