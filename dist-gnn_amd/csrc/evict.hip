@@ -12,7 +12,9 @@
 // and stay in registers as keys (32 bits, larger is better; rows past 32768 slots read them again
 // each time); the budget-th best key by counting digits; then ties, holes and movers are numbered
 // in slot order by scans over lanes and waves.  What lies below the budget is copied as it passes and the
-// holes are overwritten afterwards.
+// holes are overwritten afterwards.  16 rows of 8 heads of 20000 to 32768 slots to 4096: 37 us, of which
+// 13 read and write the arrays and 9 count digits; a workgroup a (row, head) leaves half of the card
+// idle there.
 // The moves are a kernel of their own, over all stores; where there can only be a few (a cache
 // that takes single tokens) the plan's workgroup does them.
 #include "dgs_block.cuh"
@@ -597,7 +599,8 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan_long(EvictArgs a) {
   plan_end<THREADS, false>(a, r, holes, movers, all);
 }
 
-// Block (x, y, z): (row, head), a share of its moves, a store.
+// Block (x, y, z): (row, head), a share of its moves, a store.  435 thousand moves of two stores of 256
+// bytes a row (446 MB): 90 us, 5.0 TB/s.
 __global__ __launch_bounds__(kMoveThreads) void k_evict_move(EvictArgs a) {
   const int64_t pair = blockIdx.x;
   const EvictStore &st = a.e.stores[blockIdx.z];

@@ -3,11 +3,11 @@
 // A group of `group` channels x of a row is held as codes c in 0..15, a scale s and a base b:
 //   r = max x - min x,  s = bf16(r * fl(1/15)),  b = bf16(min x),  c = clamp(rint((x - b) / s), 0, 15)
 // (r and the product in 32 bits) with the quotient taken exactly (ties to even), so that a code never
-// depends on the order or width of the arithmetic; s = 0 gives c = 0.  Scale and base are rounded to 16 bits because they
-// are read with every row: 32-bit ones would add 8 bytes to the 72 of a row of 128 channels in
-// groups of 64.  b is exact for bfloat16 inputs, and the codes are taken against the rounded s
-// and b, so their rounding costs at most 15 s / 512 + |b| / 512 at the ends of the range.  A group
-// that holds a NaN or an infinity, or whose s or b is not finite, reads back as NaN (s = b = NaN).
+// depends on the order or width of the arithmetic; s = 0 gives c = 0.  Scale and base are rounded to 16
+// bits because they are read with every row: 32-bit ones would add 8 bytes to the 72 of a row of 128
+// channels in groups of 64.  b is exact for bfloat16 inputs, and the codes are taken against the rounded
+// s and b, so their rounding costs at most 15 s / 512 + |b| / 512 at the ends of the range.  A group that
+// holds a NaN or an infinity, or whose s or b is not finite, reads back as NaN (s = b = NaN).
 #include <algorithm>
 
 #include "dgs_lane.cuh"
@@ -175,9 +175,9 @@ __global__ __launch_bounds__(kThreads) void k_state_write(WriteArgs a, uint32_t 
 }
 
 // A lane writes 16 bytes of output (four or eight channels): piece i of K (block row 0) or V (1) is
-// the i-th 16 bytes of the output.  kRU pieces a lane are in flight.  Bound by HBM: 65536 rows of 8 heads x 128 channels as 32-bit
-// floats (612 MB) in 112 us, 5.5 TB/s; 400000 scattered rows of 128 (467 MB) in 88 us, 115 with stores
-// that pass through the caches.
+// the i-th 16 bytes of the output.  kRU pieces a lane are in flight.  Bound by HBM: 65536 rows of 8
+// heads x 128 channels as 32-bit floats (612 MB) in 112 us, 5.5 TB/s; 400000 scattered rows of 128
+// (467 MB) in 88 us, 115 with stores that pass through the caches.
 constexpr int kRU = 4;
 template <int TYPE>
 __global__ __launch_bounds__(kThreads) void k_state_read(StateView c, const int64_t *slots,
