@@ -354,7 +354,7 @@ typedef struct dgs_state_cache {
  * and heads, channels contiguous, rows 16-byte aligned) into flat slots (int64; negative: skip).
  * Per group: s = bf16((max - min) * fl32(1/15)), b = bf16(min), code = clamp(rint((x - b) / s), 0,
  * 15) of the exact quotient; s = 0 gives code 0; a group with a NaN or an infinity reads back as NaN.
- * Two tokens for one slot in a call: which of them a channel group keeps is not defined. */
+ * What a slot holds that a call names twice is not defined. */
 int dgs_state_write(const dgs_state_cache *c, const void *k, const void *v, int dtype, int64_t n,
                     int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head,
                     const int64_t *slots, void *stream);
