@@ -234,9 +234,10 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan_small(EvictArgs a) {
   __shared__ int32_t s_max[kWaves];
   __shared__ int32_t s_list[2 * kFewMoves];  // FUSED: holes, movers
   const int j = threadIdx.x, lane = j & 63, wave = j >> 6;
-  const int64_t at = blockIdx.x * a.e.cols + (j < a.e.cols ? j : 0);
-  const float w = a.e.weights[at];
-  const int32_t p = a.e.positions ? a.e.positions[at] : j;
+  const int64_t at = blockIdx.x * a.e.cols + j;
+  const bool in = j < a.e.cols;  // a row may have no columns, and the arrays no memory
+  const float w = in ? a.e.weights[at] : 0.f;
+  const int32_t p = in && a.e.positions ? a.e.positions[at] : j;
   const PlanRow r = plan_row(a);
   if (j < r.cols) {
     r.wo[j] = j < r.keep ? w : 0.f;

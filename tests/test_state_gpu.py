@@ -726,3 +726,16 @@ def test_evict_short_rows(cols, share):
     assert np.array_equal(got_w.cpu().numpy(), want_w, equal_nan=True)
     for a, b in zip(stores, expect):
         assert same_bits(a, b)
+
+
+@pytest.mark.parametrize("given", [False, True])
+def test_evict_without_columns(given):
+    """Rows that have no slots yet: nothing is read, nothing moves."""
+    st = torch.arange(24, dtype=torch.uint8, device="cuda").view(3, 2, 4, 1)
+    w = torch.empty(5, 2, 0, device="cuda")
+    pos = torch.empty(5, 2, 0, dtype=torch.int32, device="cuda") if given else None
+    lens = torch.zeros(5, dtype=torch.int32, device="cuda")
+    table = torch.empty(5, 0, dtype=torch.int32, device="cuda")
+    gw, gp, gn = dgs.ops.evict_rows([st], w, pos, table, lens, 3)
+    assert gw.shape == gp.shape == (5, 2, 0) and gn.tolist() == [0] * 5
+    assert st.flatten().tolist() == list(range(24))
