@@ -207,7 +207,7 @@ __device__ __forceinline__ void plan_end(const EvictArgs &a, const PlanRow &r,
     r.wo[d] = r.w[s];
     r.po[d] = r.pos ? r.pos[s] : s;
   }
-  if constexpr (FUSED) {
+  if (FUSED && a.e.nstores > 0) {
     // the stores side by side, as many lanes a row as the longest has 16-byte pieces
     int lg = 0;
     for (int st = 0; st < a.e.nstores; ++st) lg = row_lanes(a.e.stores[st], lg);

@@ -739,3 +739,27 @@ def test_evict_without_columns(given):
     gw, gp, gn = dgs.ops.evict_rows([st], w, pos, table, lens, 3)
     assert gw.shape == gp.shape == (5, 2, 0) and gn.tolist() == [0] * 5
     assert st.flatten().tolist() == list(range(24))
+
+
+@pytest.mark.parametrize("cols, budget", [(50, 20), (300, 290), (2000, 300)])
+def test_evict_without_stores(cols, budget):
+    """The C entry without a store: weights and positions alone."""
+    from dgs._lib import c_i64, c_vp, check, lib, stream_ptr
+    gen = torch.Generator().manual_seed(cols)
+    rows, heads = 4, 2
+    w = torch.rand(rows, heads, cols, generator=gen)
+    pos = torch.arange(cols, dtype=torch.int32).repeat(rows, heads, 1)
+    lens = torch.tensor([0, budget, budget + 1, cols])
+    want_w, want_p, want_n, _ = ref.evict(w.numpy(), pos.numpy(), lens.numpy(), budget, 1, 2)
+    dw, dl = w.cuda(), lens.cuda()
+    ow, op, on = torch.empty_like(dw), torch.empty_like(dw, dtype=torch.int32), torch.empty_like(dl)
+    table = torch.arange(rows * cols).view(rows, cols).cuda()
+    need = c_i64()
+    check(lib.dgs_evict_workspace(rows, heads, cols, budget, need))
+    ws = torch.empty(max(need.value, 1), dtype=torch.uint8, device="cuda")
+    check(lib.dgs_evict_rows(
+        (c_vp * 1)(), (c_i64 * 1)(), 0, rows * cols, heads, 1, dw.data_ptr(), None, ow.data_ptr(),
+        op.data_ptr(), rows, cols, table.data_ptr(), 8, cols, dl.data_ptr(), 8, on.data_ptr(),
+        budget, 1, 2, ws.data_ptr() if need.value else None, need.value, stream_ptr(0)))
+    assert np.array_equal(on.cpu().numpy(), want_n)
+    assert np.array_equal(op.cpu().numpy(), want_p) and np.array_equal(ow.cpu().numpy(), want_w)
