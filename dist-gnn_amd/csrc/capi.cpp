@@ -736,6 +736,10 @@ IdArray id_array(const void *p, int bytes, const char *what) {
   DGS_CHECK(bytes == 4 || bytes == 8, std::string(what) + " must be int32 or int64");
   return IdArray{p, bytes};
 }
+// Products of a table's sizes fit 64 bits.
+void check_width(int64_t width, const char *what) {
+  DGS_CHECK(width >= 0 && width < (int64_t(1) << 30), std::string(what) + ": bad table width");
+}
 void check_rows16(const void *p, int64_t s0, int64_t s1, StateType t, const char *what) {
   const int64_t e = t == kStateF32 ? 4 : 2;
   DGS_CHECK(p, std::string(what) + " is null");
@@ -767,7 +771,8 @@ int dgs_state_append(const dgs_state_cache *c, const void *k, const void *v, int
   return guard([&] {
     const StateView view = state_view(c);
     const StateType t = state_type(dtype);
-    DGS_CHECK(n >= 0 && width >= 0, "state append: negative size");
+    DGS_CHECK(n >= 0, "state append: negative size");
+    check_width(width, "state append");
     if (n == 0) return;
     check_rows16(k, k_token, k_head, t, "k");
     check_rows16(v, v_token, v_head, t, "v");
@@ -800,7 +805,9 @@ int dgs_state_attend_workspace(const dgs_state_cache *c, int64_t rows, int q_hea
                                int with_weights, int dtype, int64_t *bytes) {
   return guard([&] {
     const StateView view = state_view(c);
-    DGS_CHECK(rows >= 0 && width >= 0, "attend: negative size");
+    DGS_CHECK(rows >= 0 && rows < (int64_t(1) << 31), "attend: bad rows");
+    check_width(width, "attend");
+    DGS_CHECK((width << view.pshift) < (int64_t(1) << 30), "attend: rows of 2^30 slots");
     DGS_CHECK(q_heads > 0 && q_heads % view.heads == 0,
               "attend: q_heads must be a multiple of the cache's heads");
     AttendCall a{};
@@ -810,6 +817,7 @@ int dgs_state_attend_workspace(const dgs_state_cache *c, int64_t rows, int q_hea
     a.type = state_type(dtype);
     static float flag;
     a.weights = with_weights ? &flag : nullptr;  // only whether there are any
+    DGS_CHECK(bytes, "attend: null bytes");
     *bytes = state_attend_workspace(view, a);
   });
 }
@@ -823,7 +831,9 @@ int dgs_state_attend(const dgs_state_cache *c, const void *q, int dtype, int64_t
     const StateView view = state_view(c);
     AttendCall a{};
     a.type = state_type(dtype);
-    DGS_CHECK(rows >= 0 && width >= 0, "attend: negative size");
+    DGS_CHECK(rows >= 0 && rows < (int64_t(1) << 31), "attend: bad rows");
+    check_width(width, "attend");
+    DGS_CHECK((width << view.pshift) < (int64_t(1) << 30), "attend: rows of 2^30 slots");
     DGS_CHECK(q_heads > 0 && q_heads % view.heads == 0,
               "attend: q_heads must be a multiple of the cache's heads");
     if (rows == 0) return;
@@ -851,12 +861,15 @@ int dgs_state_attend(const dgs_state_cache *c, const void *q, int dtype, int64_t
 
 int dgs_evict_workspace(int64_t rows, int heads, int64_t cols, int64_t budget, int64_t *bytes) {
   return guard([&] {
-    DGS_CHECK(rows >= 0 && heads > 0 && cols >= 0 && budget > 0, "evict: bad sizes");
+    DGS_CHECK(rows >= 0 && rows < (int64_t(1) << 31) && heads > 0 && cols >= 0 &&
+                  cols < (int64_t(1) << 30) && budget > 0,
+              "evict: bad sizes");
     EvictCall e{};
     e.rows = rows;
     e.heads = heads;
     e.cols = cols;
     e.budget = budget;
+    DGS_CHECK(bytes, "evict: null bytes");
     *bytes = evict_workspace(e);
   });
 }
@@ -869,12 +882,15 @@ int dgs_evict_rows(void *const *stores, const int64_t *row_bytes, int nstores, i
                    void *workspace, int64_t workspace_bytes, void *stream) {
   return guard([&] {
     EvictCall e{};
-    DGS_CHECK(rows >= 0 && heads > 0 && cols >= 0 && width >= 0 && pages > 0 && page_size > 0,
+    DGS_CHECK(rows >= 0 && heads > 0 && cols >= 0 && pages > 0 && page_size > 0 &&
+                  page_size < (int64_t(1) << 31),
               "evict: bad sizes");
+    check_width(width, "evict");
     DGS_CHECK(budget > 0, "evict: budget must be positive");
     DGS_CHECK(sinks >= 0 && recent >= 0 && sinks <= budget && recent <= budget - sinks,
               "evict: sinks + recent must lie between 0 and budget");
     DGS_CHECK(nstores >= 0 && nstores <= kEvictMaxStores, "evict: at most 8 stores");
+    DGS_CHECK(nstores == 0 || (stores && row_bytes), "evict: null stores");
     DGS_CHECK(cols >= width * page_size,
               "evict: weights need a column for every slot of the table");
     if (rows == 0) return;

@@ -183,6 +183,39 @@ def test_c_abi_refuses_bad_calls():
                                 1.0, None, None, 0, None) == 0
 
 
+@pytest.mark.parametrize("width", [1 << 30, 1 << 40, (1 << 61) + 1, (1 << 63) - 1, -1])
+def test_c_abi_refuses_tables_whose_sizes_do_not_fit(width):
+    c = _c()
+    ref = ctypes.addressof(c)
+    row = (2 * 64, 64)
+    n = c_i64(-7)
+
+    def last(rc, msg):
+        assert rc == -1 and msg in lib.dgs_last_error(), lib.dgs_last_error()
+
+    last(lib.dgs_state_append(ref, 4096, 4096, 0, 1, *row, *row, 4096, 4, width, 4096, 4, 4096, None),
+         b"width")
+    last(lib.dgs_state_attend(ref, 4096, 0, 1, 2, 128, 64, 4096, 4, width, 4096, 4, 1.0, 4096, 15,
+                              1.0, 4096, None, 0, None), b"width")
+    last(lib.dgs_state_attend_workspace(ref, 1, 2, width, 0, 0, ctypes.byref(n)), b"width")
+    last(lib.dgs_evict_rows(None, None, 0, 1, 1, 16, 4096, None, 8192, 8192, 1, 1, 4096, 4, width,
+                            4096, 4, 4096, 1, 0, 0, None, 0, None), b"width")
+    if width > 0:
+        last(lib.dgs_evict_workspace(1, 1, width, 1, ctypes.byref(n)), b"bad sizes")
+        last(lib.dgs_state_attend_workspace(ref, width * 2 if width < 1 << 60 else width, 2, 1, 0, 0,
+                                            ctypes.byref(n)), b"bad rows")
+    assert n.value == -7
+
+
+def test_c_abi_refuses_null_results():
+    c = _c()
+    assert lib.dgs_state_attend_workspace(ctypes.addressof(c), 1, 2, 1, 0, 0, None) == -1
+    assert lib.dgs_evict_workspace(1, 1, 8, 1, None) == -1
+    assert lib.dgs_evict_rows(None, None, 1, 1, 1, 1, 4096, None, 8192, 8192, 1, 1, 4096, 4, 1, 4096,
+                              4, 4096, 1, 0, 0, None, 0, None) == -1
+    assert b"null stores" in lib.dgs_last_error()
+
+
 def test_neighbour_table():
     seeds = torch.tensor([7, 3, 9])
     frontier = torch.tensor([7, 3, 9, 20, 21])
