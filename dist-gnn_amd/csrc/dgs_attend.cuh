@@ -126,14 +126,15 @@ struct Run {
     const int who = __ffsll((unsigned long long)has) - 1;
     int front = __shfl(before, who, 64);
     int64_t r = (int64_t)who * per;
-    while (true) {
+    // bounded also where a caller changes the lengths under the kernel, as is the loop of next()
+    for (int i = 1;; ++i, ++r) {
       units = row_units(a, r, shift, cost);
-      if (t < front + units) break;
+      if (t < front + units || i >= per || r + 1 >= a.rows) break;
       front += units;
-      ++r;
     }
     row = __builtin_amdgcn_readfirstlane((int)r);
     units = __builtin_amdgcn_readfirstlane(units);
+    if (units == 0) return false;
     const int64_t in_row = at - (int64_t)front * pairs;
     pair = __builtin_amdgcn_readfirstlane((int)(in_row / units));
     unit0 = __builtin_amdgcn_readfirstlane((int)(in_row % units));
@@ -152,9 +153,9 @@ struct Run {
     if (++pair == pairs) {
       pair = 0;
       do {
-        ++row;
+        if (++row >= a.rows) return false;
         units = __builtin_amdgcn_readfirstlane(row_units(a, row, shift, cost));
-      } while (units == 0);  // `at` lies before the end of the line: there is one
+      } while (units == 0);
     }
     return end - at > cost;  // else the next wave has its tiles
   }
