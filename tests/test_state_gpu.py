@@ -763,3 +763,59 @@ def test_evict_without_stores(cols, budget):
         budget, 1, 2, ws.data_ptr() if need.value else None, need.value, stream_ptr(0)))
     assert np.array_equal(on.cpu().numpy(), want_n)
     assert np.array_equal(op.cpu().numpy(), want_p) and np.array_equal(ow.cpu().numpy(), want_w)
+
+
+@pytest.mark.parametrize("dim, group, dtype, width", [
+    (128, 64, "f32", 2), (80, 40, "f16", 2), (32, 32, "f32", 1), (128, 64, "f32", 80),
+    (64, 64, "bf16", 80), (40, 8, "bf16", 80)])
+def test_nan_and_infinity_stay_in_their_rows_in_every_form(dim, group, dtype, width):
+    """As test_attend_nan_and_infinity_stay_in_their_rows; a row's parts are cut by lengths alone."""
+    pages = 4 * width
+    cache = full_cache(pages, 16, 2, dim, group)
+    q = states((4, 8, dim), torch.Generator().manual_seed(1), TYPES[dtype])
+    table = torch.arange(pages).view(4, width).cuda()
+    full = 16 * width
+    lens = torch.tensor([full, full - 5, full, full - 3]).cuda()
+    w = torch.zeros(4, 2, full, device="cuda")
+    clean = cache.attend(q, table, lens, weights=w)
+    cache.k_scales[2 * width - 1, 0, 3] = math.nan  # row 1, slot full - 13, head 0
+    cache.v_scales[2 * width - 1, 1, 12] = math.nan  # behind row 1's length
+    q2 = q.clone()
+    q2[2, 5] = math.inf
+    q2[3, 0, 7] = math.nan
+    w2 = torch.zeros_like(w)
+    got = cache.attend(q2, table, lens, weights=w2)
+    bad = torch.zeros(4, 8, dtype=torch.bool)
+    bad[1, :4] = bad[2, 5] = bad[3, 0] = True
+    assert torch.equal(got.isnan().all(-1).cpu(), bad) and torch.equal(got.isnan().any(-1).cpu(), bad)
+    assert torch.equal(got[~bad], clean[~bad])
+    heads = bad.view(4, 2, 4).any(-1)
+    inside = (torch.arange(full) < lens.cpu()[:, None])[:, None].expand(4, 2, full)
+    assert torch.equal(w2.isnan().cpu(), heads[..., None] & inside)
+    assert torch.equal(w2.cpu()[~heads], w.cpu()[~heads])
+
+
+@pytest.mark.parametrize("dim, group, dtype", [(128, 64, "f32"), (80, 40, "bf16"), (64, 64, "f16")])
+def test_attend_offsets_past_32_bits(dim, group, dtype):
+    """Rows whose bytes lie past 2^31 and 2^32, in both forms."""
+    page, heads = 64, 4
+    pages = 2 ** 32 // (heads * page * dim // 2) + 4000
+    bufs = []
+    for _ in range(2):
+        bufs += [torch.empty(pages, heads, page, dim // 2, dtype=torch.uint8, device="cuda"),
+                 torch.empty(pages, heads, page, dim // group, 2, dtype=torch.bfloat16, device="cuda")]
+    assert bufs[0].numel() > 2 ** 32
+    cache = dgs.classes.StateCache.wrap(*bufs)
+    small = full_cache(12, page, heads, dim, group, seed=6)
+    gen = torch.Generator().manual_seed(2)
+    use = torch.cat([torch.randperm(pages - 1, generator=gen)[:11], torch.tensor([pages - 1])]).cuda()
+    for b, s in zip(bufs, buffers(small)):
+        b[use] = s
+    table = torch.arange(12).view(2, 6).cuda()
+    q = states((2, 8, dim), gen, TYPES[dtype])
+    for n in (384, 301):
+        lens = torch.tensor([n, 130]).cuda()
+        w, w2 = torch.zeros(2, heads, 384, device="cuda"), torch.zeros(2, heads, 384, device="cuda")
+        want = check_attend(small, q, table, lens, weights=w)
+        got = cache.attend(q, use[table], lens, weights=w2)
+        assert torch.equal(got, want) and torch.equal(w, w2)
