@@ -819,3 +819,55 @@ def test_attend_offsets_past_32_bits(dim, group, dtype):
         want = check_attend(small, q, table, lens, weights=w)
         got = cache.attend(q, use[table], lens, weights=w2)
         assert torch.equal(got, want) and torch.equal(w, w2)
+
+
+@pytest.mark.parametrize("dim, group, dtype, cap", [
+    (128, 64, "bf16", 4096), (128, 64, "f32", 4096), (80, 40, "f16", 1024), (64, 64, "bf16", 640)])
+def test_graphs_of_cut_rows_follow_the_lengths(dim, group, dtype, cap):
+    """Two graphs of attend with weights, and an eviction with moves of its own kernel, replayed
+    between eager calls while queries and lengths change in place."""
+    gen = torch.Generator().manual_seed(cap)
+    rows, page, budget = 5, 16, cap // 3
+    cache = full_cache(rows * cap // page, page, 2, dim, group, seed=8)
+    bufs0 = [b.clone() for b in buffers(cache)]
+    table = torch.randperm(rows * cap // page, generator=gen).view(rows, cap // page).int().cuda()
+    lens = torch.full((rows,), cap, dtype=torch.int32, device="cuda")
+    q = states((rows, 6, dim), gen, TYPES[dtype])
+    w0 = torch.rand(rows, 2, cap, generator=gen).cuda()
+    wa, wb = w0.clone(), w0.clone()
+
+    def one():
+        return (cache.attend(q, table, lens, weights=wa),)
+
+    def two():
+        wb.copy_(w0)
+        out = cache.attend(q, table, lens, weights=wb, decay=0.5)
+        return (out,) + tuple(cache.evict(wb, None, table, lens, budget, sinks=2, recent=20))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        one(), two()
+    torch.cuda.current_stream().wait_stream(side)
+    g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g1):
+        r1 = one()
+    with torch.cuda.graph(g2):
+        r2 = two()
+    for turn in range(4):
+        q.copy_(states(q.shape, gen, q.dtype))
+        lens.copy_(torch.randint(0, cap + 1, (rows,), generator=gen) if turn else torch.zeros(rows))
+        want = []
+        for i, f in enumerate((one, two)):
+            for a, b in zip(buffers(cache), bufs0):
+                a.copy_(b)
+            wa.copy_(w0)
+            want.append([t.clone() for t in f()] + [wa.clone()] + [b.clone() for b in buffers(cache)])
+        torch.cuda.synchronize()
+        for f, r, g in ((one, r1, g1), (two, r2, g2)):
+            for a, b in zip(buffers(cache), bufs0):
+                a.copy_(b)
+            wa.copy_(w0)
+            g.replay()
+            got = list(r) + [wa] + buffers(cache)
+            assert all(same_bits(x, y) for x, y in zip(got, want[f is two])), (turn, f)
