@@ -27,15 +27,18 @@ __device__ __forceinline__ uint32_t bf16_rne(float x) {
   return v.u;
 }
 
-// The eight codes of a word.  The quotient in 32 bits is off by at most 2.5 of its units in the
-// last place (one rounding in x - b, one in the reciprocal, one in the product), 2.5e-6 below 16.
-// Within 1e-5 of a rounding border h (a multiple of a half) the sign of (x - b) - h s decides, which
-// 32 bits give exactly: h s has 13 bits, the difference to the rounded x - b is exact because the two
-// nearly cancel, and what x - b lost in rounding is added (an error-free difference).  Scales too
-// small for a normal reciprocal take the quotient in 64 bits, where it is exact enough by far.
-constexpr float kNear = 0.5f - 1e-5f;
+// The eight codes of a word.  The quotient in 32 bits is off by at most 4 of its units in the last place
+// (a half in x - b and in the product, one in the reciprocal), 4e-6 below 16.  Within 1e-5 of a rounding
+// border h (a multiple of a half) the sign of (x - b) - h s decides, which 32 bits give exactly: h s has
+// 13 bits, the difference to the rounded x - b is exact because the two nearly cancel, and what x - b lost
+// in rounding is added (an error-free difference).  Of bfloat16 inputs one in some hundreds lies on a
+// border, so that most waves have one or two: a branch a channel, which the wave takes for those only.
+// Scales too small or too large for a normal reciprocal take the quotient in 64 bits, where it is exact
+// enough by far.  Adding 1.5 * 2^23 rounds to an integer and leaves it in the low bits.
+constexpr float kNear = 0.5f - 1e-5f, kMagic = 12582912.f;
+constexpr uint32_t kMagicBits = 0x4b400000u + (0x4b400000u << 4) + (0x4b400000u << 8);  // a word's
 __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float b, float s) {
-  if (!(s >= 1e-30f)) {
+  if (!(s >= 1e-30f && s <= 1e30f)) {
     uint32_t w = 0;
     for (int i = 0; i < 8; ++i) {
       const double t = s == 0.f ? 0. : ((double)x[i] - (double)b) / (double)s;
@@ -43,36 +46,24 @@ __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float b, float
     }
     return w;
   }
-  const float inv = 1.f / s;
-  uint32_t w = 0;
-  float far = 0.f;
+  const float inv = __builtin_amdgcn_rcpf(s);
+  uint32_t w = 0u - kMagicBits;
+  bool near[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float t = (x[i] - b) * inv, r = rintf(t);
-    far = fmaxf(far, fabsf(t - r));
-    w |= (uint32_t)fminf(fmaxf(r, 0.f), 15.f) << (4 * i);
+    const float t = __builtin_amdgcn_fmed3f((x[i] - b) * inv, 0.f, 15.f), r = t + kMagic;
+    near[i] = fabsf(t - (r - kMagic)) > kNear;
+    w += __float_as_uint(r) << (4 * i);
   }
-  if (far <= kNear) return w;
-  // One channel near a border at a time: of bfloat16 inputs one in some hundreds lies on one, so
-  // that most waves have a few, but hardly a lane two.
-  uint32_t near = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float t = (x[i] - b) * inv;
-    near |= (fabsf(t - rintf(t)) > kNear ? 1u : 0u) << i;
-  }
-  while (near) {
-    const int i = __ffs(near) - 1;
-    near &= near - 1;
-    float v = x[0];
-#pragma unroll
-    for (int y = 1; y < 8; ++y) v = i == y ? x[y] : v;
-    const float d = v - b, back = v - d;
-    const float lost = (back - b) + (v - (d + back));
-    const float low = floorf(d * inv), h = low + 0.5f;
+    if (!__any(near[i])) continue;
+    const float d = x[i] - b, back = x[i] - d, t = __builtin_amdgcn_fmed3f(d * inv, 0.f, 15.f);
+    const float lost = (back - b) + (x[i] - (d + back));
+    const float low = floorf(t), h = low + 0.5f;
     const float e = __builtin_fmaf(-h, s, d) + lost;
-    const float r = e > 0.f || (e == 0.f && ((int)low & 1)) ? low + 1.f : low;
-    w = (w & ~(15u << (4 * i))) | (uint32_t)fminf(fmaxf(r, 0.f), 15.f) << (4 * i);
+    const uint32_t c = (uint32_t)low, up = e > 0.f || (e == 0.f && (c & 1)) ? 1u : 0u;
+    w = near[i] ? (w & ~(15u << (4 * i))) | (c + up) << (4 * i) : w;
   }
   return w;
 }
@@ -112,35 +103,47 @@ __device__ __forceinline__ int64_t write_slot(const WriteArgs &a, int64_t t, boo
   return (page << a.c.pshift) | (len & ((int64_t(1) << a.c.pshift) - 1));
 }
 
-// lpg lanes (a power of two, at least group / 8) share a group; a lane holds eight channels.  Block
+// LPG lanes (a power of two, at least group / 8) share a group; a lane holds eight channels.  Block
 // row y: 0 = K, 1 = V.  A group of lanes takes kWU units (group `g` of head h of token t: unit (t heads
-// + h) ng + g) at a time, for their loads to overlap.  Bound by HBM: 65536 tokens of 8 heads x 128
-// bfloat16 channels to scattered slots (343 MB) in 108 us, 3.2 TB/s; a large copy runs at 4.8, but here
-// a fifth of the bytes goes out in pieces of 64 and 8 bytes.
+// + h) ng + g) that follow each other, for their loads to overlap; SAME: they belong to one token, whose
+// slot is looked up once, while the rows are on their way: with a look-up a unit the kernel took 109 us
+// for 65536 tokens of 8 heads x 128 bfloat16 channels (343 MB) to scattered slots, now 93, 3.7 TB/s;
+// dense rows to consecutive slots 70, as fast as a copy.  2 and 8 units: 1 to 8 us more.
 constexpr int kWU = 4;
-template <int TYPE, int LPG>
+template <int TYPE, int LPG, bool SAME>
 __global__ __launch_bounds__(kThreads) void k_state_write(WriteArgs a, uint32_t units,
                                                           FastDivU32 per_token, FastDivU32 per_head) {
   const int words = a.c.group >> 3, ng = (int)per_head.d;
   const int sub = threadIdx.x % LPG;
   const bool live = sub < words;
   const int kv = blockIdx.y;
-  const uint32_t u0 = blockIdx.x * (kThreads / LPG * kWU) + threadIdx.x / LPG;
+  const uint32_t u0 = (blockIdx.x * (kThreads / LPG) + threadIdx.x / LPG) * kWU;
+  if (u0 >= units) return;  // whole groups of lanes
   const void *src = kv ? a.x.v : a.x.k;
   const int64_t st = kv ? a.x.vt : a.x.kt, sh = kv ? a.x.vh : a.x.kh;
   float x[kWU][8];
   int64_t slot[kWU];
   int h[kWU], g[kWU];
+  uint32_t t[kWU];
 #pragma unroll
   for (int i = 0; i < kWU; ++i) {
-    const uint32_t u = u0 + i * (kThreads / LPG);
-    const bool in = u < units;
-    const uint32_t t = in ? per_token.div(u) : 0, r = in ? u - t * per_token.d : 0;
+    const uint32_t u = u0 + i < units ? u0 + i : u0;
+    t[i] = SAME && i > 0 ? t[0] : per_token.div(u);
+    const uint32_t r = u - t[i] * per_token.d;
     h[i] = (int)per_head.div(r);
     g[i] = (int)(r - h[i] * per_head.d);
-    slot[i] = in ? write_slot(a, a.t0 + t, sub == 0) : -1;
-    if (in && a.slots_out && sub == 0 && r == 0 && kv == 0) a.slots_out[a.t0 + t] = slot[i];
-    load8<TYPE>(src, (a.t0 + t) * st + h[i] * sh + g[i] * a.c.group + (live ? sub : 0) * 8, x[i]);
+    load8<TYPE>(src, (a.t0 + t[i]) * st + h[i] * sh + g[i] * a.c.group + (live ? sub : 0) * 8, x[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kWU; ++i) {
+    if (SAME && i > 0) {
+      slot[i] = slot[0];
+      continue;
+    }
+    const bool in = u0 + i < units;
+    slot[i] = in ? write_slot(a, a.t0 + t[i], sub == 0) : -1;
+    if (in && a.slots_out && sub == 0 && h[i] == 0 && g[i] == 0 && kv == 0)
+      a.slots_out[a.t0 + t[i]] = slot[i];
   }
 #pragma unroll
   for (int i = 0; i < kWU; ++i) {
@@ -245,22 +248,28 @@ int shift_of(int words) {
   return s;
 }
 
-template <int TYPE>
-void launch_write_t(const WriteArgs &a, int64_t n, hipStream_t st) {
-  const int sh = shift_of(a.c.group >> 3);
+template <int TYPE, int LPG>
+void launch_write_l(const WriteArgs &a, int64_t n, hipStream_t st) {
   const uint32_t ng = a.c.dim / a.c.group, per_token = a.c.heads * ng;
   const uint32_t units = (uint32_t)(n * per_token);
   const FastDivU32 ft = FastDivU32::make(per_token), fh = FastDivU32::make(ng);
-  const dim3 grid((unsigned)ceil_div((int64_t)units << sh, kThreads * kWU), 2);
-  switch (sh) {
-    case 0: k_state_write<TYPE, 1><<<grid, kThreads, 0, st>>>(a, units, ft, fh); break;
-    case 1: k_state_write<TYPE, 2><<<grid, kThreads, 0, st>>>(a, units, ft, fh); break;
-    case 2: k_state_write<TYPE, 4><<<grid, kThreads, 0, st>>>(a, units, ft, fh); break;
-    case 3: k_state_write<TYPE, 8><<<grid, kThreads, 0, st>>>(a, units, ft, fh); break;
-    case 4: k_state_write<TYPE, 16><<<grid, kThreads, 0, st>>>(a, units, ft, fh); break;
-    default: k_state_write<TYPE, 32><<<grid, kThreads, 0, st>>>(a, units, ft, fh); break;
-  }
+  const dim3 grid((unsigned)ceil_div((int64_t)units * LPG, kThreads * kWU), 2);
+  if (per_token % kWU == 0)
+    k_state_write<TYPE, LPG, true><<<grid, kThreads, 0, st>>>(a, units, ft, fh);
+  else
+    k_state_write<TYPE, LPG, false><<<grid, kThreads, 0, st>>>(a, units, ft, fh);
   DGS_LAUNCH_CHECK();
+}
+template <int TYPE>
+void launch_write_t(const WriteArgs &a, int64_t n, hipStream_t st) {
+  switch (shift_of(a.c.group >> 3)) {
+    case 0: launch_write_l<TYPE, 1>(a, n, st); break;
+    case 1: launch_write_l<TYPE, 2>(a, n, st); break;
+    case 2: launch_write_l<TYPE, 4>(a, n, st); break;
+    case 3: launch_write_l<TYPE, 8>(a, n, st); break;
+    case 4: launch_write_l<TYPE, 16>(a, n, st); break;
+    default: launch_write_l<TYPE, 32>(a, n, st); break;
+  }
 }
 // Units and pieces of a launch are counted in 32 bits: more tokens take several launches.
 int64_t tokens_a_launch(const StateView &c) {
