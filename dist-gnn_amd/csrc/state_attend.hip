@@ -45,6 +45,18 @@ __device__ __forceinline__ float sum_lanes(float x) {
   return x;
 }
 
+// x of the lane o (a power of two) away.
+__device__ __forceinline__ float over(float x, int o) {
+  switch (o) {
+    case 1: return lane_xor32<1>(x);
+    case 2: return lane_xor32<2>(x);
+    case 4: return lane_xor32<4>(x);
+    case 8: return lane_xor32<8>(x);
+    case 16: return xor16(x);
+    default: return xor32(x);
+  }
+}
+
 // x of lane u of this lane's four.
 __device__ __forceinline__ uint32_t of_quad(uint32_t x, int u) {
   switch (u) {
@@ -418,58 +430,32 @@ __device__ __forceinline__ Parts parts_of(const AttendArgs &a, int64_t row, int 
   return Parts{part * gs + n % t, gs, parts};
 }
 // The maximum and 1 / sum of kG query heads over their parts (head g's `step` g behind), on every
-// lane of the wave; heads at or past g_end repeat the first.
+// lane of the wave; heads at or past g_end repeat the first.  64 / kG lanes take a head's parts.
 template <int kG>
 __device__ __forceinline__ void join_ml(const AttendArgs &a, const Parts &p, int64_t step,
                                         int g_end, float2 (&out)[kG]) {
-  const int lane = threadIdx.x & 63;
-  float m[kG], l[kG];
-  const float2 *ml[kG];
+  constexpr int kL = 64 / kG;
+  const int lane = threadIdx.x & 63, g = lane / kL, s0 = lane % kL;
+  const float2 *ml = a.part_ml + p.part + (g < g_end ? g * step : 0);
+  const float2 own = s0 < p.n ? ml[(int64_t)s0 * p.stride] : make_float2(-INFINITY, 0.f);
+  float m = own.x;
+  for (int s = s0 + kL; s < p.n; s += kL) m = fmaxf(m, ml[(int64_t)s * p.stride].x);
 #pragma unroll
-  for (int g = 0; g < kG; ++g) {
-    ml[g] = a.part_ml + p.part + (g < g_end ? g * step : 0);
-    m[g] = -INFINITY;
-    l[g] = 0.f;
-  }
-  if (p.n <= 64) {  // one part a lane
-    float2 x[kG];
-#pragma unroll
-    for (int g = 0; g < kG; ++g)
-      x[g] = lane < p.n ? ml[g][(int64_t)lane * p.stride] : make_float2(-INFINITY, 0.f);
-#pragma unroll
-    for (int g = 0; g < kG; ++g) {
-      m[g] = x[g].x;
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) m[g] = fmaxf(m[g], __shfl_xor(m[g], o, 64));
-    }
-#pragma unroll
-    for (int g = 0; g < kG; ++g) {
-      m[g] = m[g] == -INFINITY ? 0.f : m[g];
-      l[g] = lane < p.n ? x[g].y * __builtin_amdgcn_exp2f(x[g].x - m[g]) : 0.f;
-    }
-  } else {
-    for (int s = lane; s < p.n; s += 64)
-#pragma unroll
-      for (int g = 0; g < kG; ++g) m[g] = fmaxf(m[g], ml[g][(int64_t)s * p.stride].x);
-#pragma unroll
-    for (int g = 0; g < kG; ++g) {
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) m[g] = fmaxf(m[g], __shfl_xor(m[g], o, 64));
-      m[g] = m[g] == -INFINITY ? 0.f : m[g];
-    }
-    for (int s = lane; s < p.n; s += 64)
-#pragma unroll
-      for (int g = 0; g < kG; ++g) {
-        const float2 x = ml[g][(int64_t)s * p.stride];
-        l[g] += x.y * __builtin_amdgcn_exp2f(x.x - m[g]);
-      }
+  for (int o = 1; o < kL; o <<= 1) m = fmaxf(m, over(m, o));
+  m = m == -INFINITY ? 0.f : m;
+  float l = own.y * __builtin_amdgcn_exp2f(own.x - m);
+  for (int s = s0 + kL; s < p.n; s += kL) {
+    const float2 x = ml[(int64_t)s * p.stride];
+    l += x.y * __builtin_amdgcn_exp2f(x.x - m);
   }
 #pragma unroll
-  for (int g = 0; g < kG; ++g) {
+  for (int o = 1; o < kL; o <<= 1) l += over(l, o);
+  l = 1.f / l;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) l[g] += __shfl_xor(l[g], o, 64);
-    out[g] = make_float2(m[g], 1.f / l[g]);
-  }
+  for (int k = 0; k < kG; ++k)
+    out[k] = make_float2(
+        __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m), k * kL)),
+        __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(l), k * kL)));
 }
 
 // Joins the parts of the rows' query heads and adds the weights; every wave works alone.  The
@@ -513,9 +499,11 @@ __global__ __launch_bounds__(kThreads) void k_attend_finish(AttendArgs a, int64_
 #pragma unroll
               for (int i = 0; i < 8; ++i) acc[i] = __builtin_fmaf(x[u][i], f[u], acc[i]);
         }
-      for (int o = lpr; o < 64; o <<= 1)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] += __shfl_xor(acc[i], o, 64);
+      for (int o = 1; o < 64; o <<= 1)
+        if (o >= lpr)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc[i] += over(acc[i], o);
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc[i] *= ml.y;
     }
