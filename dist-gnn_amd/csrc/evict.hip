@@ -38,6 +38,18 @@ struct EvictArgs {
   GatherGuard gd;
 };
 
+// Inclusive sum over the lanes of a wave by lane moves: within rows of 16, then the rows' last lanes.
+__device__ __forceinline__ uint32_t lanes_before_and_me(uint32_t x) {
+  auto add = [&](auto moved) { x += (uint32_t)moved; };
+  add(__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, false));  // row_shr 1
+  add(__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, false));
+  add(__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, false));
+  add(__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, false));
+  add(__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false));  // lane 15 of rows 0, 2 to 1, 3
+  add(__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false));  // lane 31 to rows 2, 3
+  return x;
+}
+
 // Larger is better; a protected slot beats every weight.
 __device__ __forceinline__ uint32_t key_of(float w, bool fixed) {
   if (fixed) return 0xffffffffu;
@@ -270,7 +282,7 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan_small(EvictArgs a) {
   const bool hole = j < r.budget && !kept, mover = j >= r.budget && kept;
   // as many movers as holes: both numbers in a word
   const uint32_t own = (hole ? 1u : 0u) | (mover ? 0x10000u : 0u);
-  const uint32_t sum = wave_inclusive_scan(own);
+  const uint32_t sum = lanes_before_and_me(own);
   if (lane == 63) s_run[wave] = sum;
   __syncthreads();
   uint32_t rank = sum - own, all = 0;
@@ -421,7 +433,7 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan(EvictArgs a) {
     if (wave == 0) {
       const uint32_t x = 2 * lane < kRuns ? s_run[2 * lane] : 0u;
       const uint32_t y = 2 * lane + 1 < kRuns ? s_run[2 * lane + 1] : 0u;
-      const uint32_t before = wave_inclusive_scan(x + y) - x - y;
+      const uint32_t before = lanes_before_and_me(x + y) - x - y;
       if (2 * lane < kRuns) s_run[2 * lane] = before;
       if (2 * lane + 1 < kRuns) s_run[2 * lane + 1] = before + x;
       if (lane == 63) s_found[0] = before + x + y;
@@ -450,7 +462,7 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan(EvictArgs a) {
         const bool in = (v * THREADS + tid) * 4 + i < r.n;
         if (in && key[v][i] == prefix) tie |= 1u << (4 * v + i);
       }
-      const uint32_t own = __popc((tie >> (4 * v)) & 15u), sum = wave_inclusive_scan(own);
+      const uint32_t own = __popc((tie >> (4 * v)) & 15u), sum = lanes_before_and_me(own);
       at[v] = sum - own;
       if (lane == 63) s_run[v * kWaves + wave] = sum;
     }
@@ -480,7 +492,7 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan(EvictArgs a) {
       if (j >= r.budget && k) mover |= 1u << (4 * v + i);
     }
     const uint32_t own = __popc((hole >> (4 * v)) & 15u) | __popc((mover >> (4 * v)) & 15u) << 16;
-    const uint32_t sum = wave_inclusive_scan(own);
+    const uint32_t sum = lanes_before_and_me(own);
     at[v] = sum - own;
     if (lane == 63) s_run[v * kWaves + wave] = sum;
   }
