@@ -184,13 +184,20 @@ __device__ __forceinline__ uint32_t pick_digit(const uint32_t *hist, uint32_t &l
                                                uint32_t *found) {
   constexpr int kOwn = kDigits / THREADS;
   // thread t owns kOwn digits counted from the largest: an ascending scan of them
-  uint32_t mine[kOwn], sum = 0, total;
+  constexpr int kWaves = THREADS / 64;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t mine[kOwn], sum = 0;
 #pragma unroll
   for (int i = 0; i < kOwn; ++i) {
     mine[i] = hist[kDigits - 1 - ((int)threadIdx.x * kOwn + i)];
     sum += mine[i];
   }
-  uint32_t before = block_exclusive_scan<THREADS>(sum, &total, scan);
+  const uint32_t upto = lanes_before_and_me(sum);
+  if (lane == 63) scan[wave] = upto;
+  __syncthreads();
+  uint32_t before = upto - sum;
+#pragma unroll
+  for (int v = 0; v < kWaves; ++v) before += v < wave ? scan[v] : 0u;
 #pragma unroll
   for (int i = 0; i < kOwn; ++i) {
     if (before < left && left <= before + mine[i]) {
