@@ -169,11 +169,14 @@ constexpr int kMatrixShift = 5, kMatrixCost = 6, kMatrixLeast = 4;
 // over are zeros) through 32 slots at a time, in v_mfma_f32_16x16x32_bf16 (operands: lane l holds
 // row or column l & 15 and the eight k of quarter l >> 4; result: column l & 15, rows 4 (l >> 4) + i).
 //
-//  - A code c becomes the bfloat16 0x4300 | c = 128 + c, exactly, with one mask-or a pair.
+//  - A code c of K becomes the bfloat16 0x3f80 | c << 3 = (16 + c) / 16, exactly, with a shift and a
+//    mask-or a pair.  V's become 0x4300 | c = 128 + c, which spares one shift in four; the offset's sums,
+//    and their rounding, are 8 times as large, which K cannot have: the attention weights of 16-bit
+//    queries would be off by 4e-7 instead of 6e-8 (V's go into a 16-bit output).
 //  - x = K q: rows are slots, columns query heads, k channels; one product chain per channel group,
-//    r_g = sum q (128 + c).  Then x = sum_g s_g r_g + sum_g (b_g - 128 s_g) Q_g with Q_g = sum q over
+//    r_g = sum 16 q (16 + c) / 16.  Then x = sum_g s_g r_g + sum_g (b_g - 16 s_g) Q_g with Q_g = sum q over
 //    the group; the second sum is one more product whose slot operand is the stored (s, b) words
-//    themselves and whose other operand holds -128 Q_g and Q_g in three bfloat16 terms (24 bits).
+//    themselves and whose other operand holds -16 Q_g and Q_g in three bfloat16 terms (24 bits).
 //  - The result leaves eight slots of a query head in a lane, of which only GR = 4, 8 or 16 columns
 //    are query heads.  With fewer than 16, the other columns' lanes take over their share of the
 //    slots (lane 4 b + h of a row of 16 takes slots 2 b and 2 b + 1 of head h), with one lane move
@@ -215,11 +218,14 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(r) : "v"(lo), "v"(hi));
   return r;
 }
-// The low nibbles of a word's halves as bfloat16 128 + c.  `magic` is 0x43004300 in a vector
-// register: one instruction takes one constant from a scalar register, so with both there the
-// mask-or would be two.
-__device__ __forceinline__ uint32_t code_pair(uint32_t x, uint32_t magic) {
-  return (x & 0x000f000fu) | magic;
+// Nibbles y of a word's halves as bfloat16: of K 1 + c / 16, of V 128 + c.  `magic`, 0x3f803f80 or
+// 0x43004300, comes in a vector register: one instruction takes one constant from a scalar register, so
+// with both there the mask-or would be two.
+__device__ __forceinline__ uint32_t code_pair_k(uint32_t x, int y, uint32_t magic) {
+  return ((y == 0 ? x << 3 : x >> (4 * y - 3)) & 0x00780078u) | magic;
+}
+__device__ __forceinline__ uint32_t code_pair_v(uint32_t x, int y, uint32_t magic) {
+  return ((x >> (4 * y)) & 0x000f000fu) | magic;
 }
 __device__ __forceinline__ float xor16(float x) {
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false,
@@ -309,8 +315,8 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
   // logits grow with x: a negative scale is taken into q, and so is 0 (masked slots are -inf)
   const float sign = a.scale2 < 0.f ? -1.f : (a.scale2 == 0.f ? 0.f : 1.f);
   const float scale2 = a.scale2 == 0.f ? 1.f : fabsf(a.scale2);
-  uint32_t magic = 0x43004300u;
-  asm volatile("" : "+v"(magic));
+  uint32_t magic_k = 0x3f803f80u, magic_v = 0x43004300u;
+  asm volatile("" : "+v"(magic_k), "+v"(magic_v));
 
   const int ps = a.c.pshift, mask = (1 << ps) - 1;
   const int unit = n * (GROUP / 32);  // byte of this lane's unit of V in a group's codes
@@ -436,7 +442,7 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
   float cb[NG], m, ms, l;  // m, ms: in base 2, of head n % GR
   Op ones;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) ones.u[i] = 0x43004300u;  // 128, the codes' offset
+  for (int i = 0; i < 4; ++i) ones.u[i] = 0x43004300u;  // 128, the offset of V's codes
 
   // word g of this lane's slot v
   auto word_at = [&](const uint32_t *w, int v, int g) {
@@ -467,7 +473,7 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
           const uint32_t w = *(const uint32_t *)(kp[c % kKP] + 256 * kPR * i + 64 * (c / 4));
           Op k;
 #pragma unroll
-          for (int y = 0; y < 4; ++y) k.u[y] = code_pair(w >> (4 * y), magic);
+          for (int y = 0; y < 4; ++y) k.u[y] = code_pair_k(w, y, magic_k);
           r[i] = mfma(k, qv[0][c], r[i]);
           if constexpr (QT == 2) r[i] = mfma(k, qv[1][c], r[i]);
         }
@@ -571,7 +577,7 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
       for (int j = 0; j < kU; ++j) {
         Op v;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v.u[i] = code_pair(pair[j >> 2][i] >> (4 * (j & 3)), magic);
+        for (int i = 0; i < 4; ++i) v.u[i] = code_pair_v(pair[j >> 2][i], j & 3, magic_v);
         o[g][j] = mfma(v, hi, o[g][j]);
         o[g][j] = mfma(v, lo, o[g][j]);
       }
@@ -606,7 +612,7 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
       load_rows(j1 + step, t1);
     }
 
-    // q in bfloat16 terms, in the order in which code_pair() yields a word's channels: 0 4 1 5 2 6 3 7
+    // q in bfloat16 terms, in the order in which code_pair_k() yields a word's channels: 0 4 1 5 2 6 3 7
     float qsum[NG];
 #pragma unroll
     for (int g = 0; g < NG; ++g) qsum[g] = 0.f;
@@ -619,6 +625,7 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
       for (int i = 0; i < 8; ++i) {
         x[i] *= sign;
         qsum[c / kGC] += x[i];
+        x[i] *= 16.f;
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -629,7 +636,7 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
                                     x[4 + i] - __uint_as_float(hi & 0xffff0000u));
       }
     }
-    // quarter 0 holds the first bfloat16 terms of (-128 Q_g, Q_g), 1 the second, 2 the third
+    // quarter 0 holds the first bfloat16 terms of (-16 Q_g, Q_g), 1 the second, 2 the third
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       qm.u[g] = 0;
@@ -640,7 +647,7 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
         const float t0 = (float)(__bf16)s, t1 = (float)(__bf16)(s - t0);
         const float t2 = (s - t0) - t1;
         const float t = q4 == 0 ? t0 : (q4 == 1 ? t1 : (q4 == 2 ? t2 : 0.f));
-        qm.u[g] = pack_bf16(-128.f * t, t);
+        qm.u[g] = pack_bf16(-16.f * t, t);
       }
     }
 
