@@ -12,8 +12,8 @@
 // and stay in registers as keys (32 bits, larger is better; rows past 32768 slots read them again
 // each time); the budget-th best key by counting digits; then ties, holes and movers are numbered
 // in slot order by scans over lanes and waves.  What lies below the budget is copied as it passes and the
-// holes are overwritten afterwards.  16 rows of 8 heads of 20000 to 32768 slots to 4096: 37 us, of which
-// 13 read and write the arrays and 9 count digits; a workgroup a (row, head) leaves half of the card
+// holes are overwritten afterwards.  16 rows of 8 heads of 20000 to 32768 slots to 4096: 35 us, of which
+// 13 read and write the arrays and 8 count digits; a workgroup a (row, head) leaves half of the card
 // idle there.
 // The moves are a kernel of their own, over all stores; where there can only be a few (a cache
 // that takes single tokens) the plan's workgroup does them.
@@ -244,7 +244,7 @@ __device__ __forceinline__ void plan_end(const EvictArgs &a, const PlanRow &r,
 }
 
 // Rows of at most THREADS slots, one a thread: a slot stays if fewer than `keep` come before it, and
-// every thread counts them.  33 rows of 2 heads of 0 to 77 slots: 9.4 us, 13.6 with digits and one move a
+// every thread counts them.  33 rows of 2 heads of 0 to 77 slots: 9.1 us, 13.6 with digits and one move a
 // wave at a time: a chain of loads (length, table, row), bound by nothing else.
 template <int THREADS, bool FUSED>
 __global__ __launch_bounds__(THREADS) void k_evict_plan_small(EvictArgs a) {

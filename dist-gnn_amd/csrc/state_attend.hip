@@ -461,7 +461,7 @@ __device__ __forceinline__ void join_ml(const AttendArgs &a, const Parts &p, int
 // Joins the parts of the rows' query heads and adds the weights; every wave works alone.  The
 // first `outs` waves take 8 `lpr` channels of a query head's output each (eight channels a lane, the
 // lanes' groups taking every n-th part), the others 1024 slots of a (row, head)'s weights.  64 rows of
-// 8 heads, 32 query heads, 1 to 8192 slots (50 MB of logits and weights): 19.6 us, a third of them the
+// 8 heads, 32 query heads, 1 to 8192 slots (50 MB of logits and weights): 15.5 us, a third of them the
 // lengths, parts and maxima, loads that wait for each other; without weights 6 us.
 constexpr int kSpan = 1024;
 template <int TYPE>
