@@ -29,6 +29,7 @@ constexpr int kDigits = 2048;  // 11 bits: the sign, the exponent and two bits o
 // to 4097 slots, 256 bytes a row, room 237: 40 us, 43 with a kernel for the moves; one such row 24.6, 24.1;
 // 33 rows of 2 heads of 200 slots, room 100: 14, 18; room 500: 20 to 29 us in the plan, 18 apart.
 constexpr int kFewMoves = 256;
+static_assert(kFewMoves >= 128, "rows of 256 slots have at most 128 moves");
 
 struct EvictArgs {
   EvictCall e;
@@ -246,12 +247,12 @@ __device__ __forceinline__ void plan_end(const EvictArgs &a, const PlanRow &r,
 // Rows of at most THREADS slots, one a thread: a slot stays if fewer than `keep` come before it, and
 // every thread counts them.  33 rows of 2 heads of 0 to 77 slots: 9.1 us, 13.6 with digits and one move a
 // wave at a time: a chain of loads (length, table, row), bound by nothing else.
-template <int THREADS, bool FUSED>
+template <int THREADS>
 __global__ __launch_bounds__(THREADS) void k_evict_plan_small(EvictArgs a) {
   constexpr int kWaves = THREADS / 64;
   __shared__ uint32_t s_key[THREADS], s_run[kWaves];
   __shared__ int32_t s_max[kWaves];
-  __shared__ int32_t s_list[2 * kFewMoves];  // FUSED: holes, movers
+  __shared__ int32_t s_hole[THREADS / 2], s_mover[THREADS / 2];  // as many of one as of the other
   const int j = threadIdx.x, lane = j & 63, wave = j >> 6;
   const int64_t at = blockIdx.x * a.e.cols + j;
   const bool in = j < a.e.cols;  // a row may have no columns, and the arrays no memory
@@ -298,11 +299,9 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan_small(EvictArgs a) {
     if (v < wave) rank += s_run[v];
     all += s_run[v];
   }
-  int32_t *holes = FUSED ? s_list : a.holes + r.pair * a.room;
-  int32_t *movers = FUSED ? s_list + kFewMoves : a.movers + r.pair * a.room;
-  if (hole) holes[rank & 0xffffu] = j;
-  if (mover) movers[rank >> 16] = j;
-  plan_end<THREADS, FUSED>(a, r, holes, movers, all & 0xffffu);
+  if (hole) s_hole[rank & 0xffffu] = j;
+  if (mover) s_mover[rank >> 16] = j;
+  plan_end<THREADS, true>(a, r, s_hole, s_mover, all & 0xffffu);
 }
 
 // Rows of at most THREADS * kVecs * 4 slots: slot (v THREADS + t) 4 + i is thread t's.  ALIGNED:
@@ -649,10 +648,10 @@ void launch_plan(const EvictArgs &a, hipStream_t st) {
 template <bool FUSED>
 void plan(const EvictArgs &a, hipStream_t st) {
   const unsigned pairs = (unsigned)(a.e.rows * a.e.heads);
-  if (a.e.cols <= 64)
-    k_evict_plan_small<64, FUSED><<<pairs, 64, 0, st>>>(a);
-  else if (a.e.cols <= 256)
-    k_evict_plan_small<256, FUSED><<<pairs, 256, 0, st>>>(a);
+  if (FUSED && a.e.cols <= 64)  // at most 128 moves
+    k_evict_plan_small<64><<<pairs, 64, 0, st>>>(a);
+  else if (FUSED && a.e.cols <= 256)
+    k_evict_plan_small<256><<<pairs, 256, 0, st>>>(a);
   else if (a.e.cols <= 1024)
     launch_plan<256, 1, FUSED>(a, st);
   else if (a.e.cols <= 8192)
