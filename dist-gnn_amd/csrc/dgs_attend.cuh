@@ -78,17 +78,23 @@ __device__ __forceinline__ void load_q(int type, const void *q, int64_t elem, fl
 
 // The stream form's line of units: rows in order, a row's pairs in order, and of a pair `cost` units
 // for taking it up, then its tiles of 2^shift slots.
-__device__ __forceinline__ int row_units(const AttendArgs &a, int64_t row, int shift, int cost) {
-  const int tiles = (int)((row_length(a, row, false) + (1 << shift) - 1) >> shift);
+__device__ __forceinline__ int units_of(int len, int shift, int cost) {
+  const int tiles = (int)(((int64_t)len + (1 << shift) - 1) >> shift);
   return tiles ? tiles + cost : 0;
 }
-// Lane l adds up rows [l n / 64 ..): the line up to its rows, and what its rows hold.
+__device__ __forceinline__ int row_units(const AttendArgs &a, int64_t row, int shift, int cost) {
+  return units_of((int)row_length(a, row, false), shift, cost);
+}
+// Lane l adds up rows [l n / 64 ..): the line up to its rows, what its rows hold, the last one's length.
 __device__ __forceinline__ void stream_sums(const AttendArgs &a, int shift, int cost, int lane,
-                                            int per, int &before, int &own, int &total) {
-  own = 0;
+                                            int per, int &before, int &own, int &total, int &len) {
+  own = len = 0;
   for (int i = 0; i < per; ++i) {
     const int64_t r = (int64_t)lane * per + i;
-    if (r < a.rows) own += row_units(a, r, shift, cost);
+    if (r < a.rows) {
+      len = (int)row_length(a, r, false);
+      own += units_of(len, shift, cost);
+    }
   }
   int x = own;
 #pragma unroll
@@ -108,14 +114,14 @@ __device__ __forceinline__ int stream_share(const AttendArgs &a, int cost, int l
 // the tiles from `tile` on and the slots before last().  All in scalar registers.
 struct Run {
   int64_t at, end, row;
-  int pairs, units, pair, unit0, tile;
+  int pairs, len, units, pair, unit0, tile;
 
   __device__ __forceinline__ bool start(const AttendArgs &a, int shift, int cost, int least,
                                         int pairs_of_row, int wave, int lane) {
     pairs = pairs_of_row;
     const int per = (int)((a.rows + 63) >> 6);
-    int before, own, total;
-    stream_sums(a, shift, cost, lane, per, before, own, total);
+    int before, own, total, last_len;
+    stream_sums(a, shift, cost, lane, per, before, own, total, last_len);
     const int share = stream_share(a, cost, least, (int64_t)total * pairs);
     at = (int64_t)wave * share;
     end = at + share < (int64_t)total * pairs ? at + share : (int64_t)total * pairs;
@@ -124,16 +130,24 @@ struct Run {
     const int64_t t = at / pairs;  // rows' boundaries are multiples of `pairs` in the line
     const uint64_t has = __ballot(before <= t && t < (int64_t)before + own);
     const int who = __ffsll((unsigned long long)has) - 1;
-    int front = __shfl(before, who, 64);
-    int64_t r = (int64_t)who * per;
-    // bounded also where a caller changes the lengths under the kernel, as is the loop of next()
-    for (int i = 1;; ++i, ++r) {
-      units = row_units(a, r, shift, cost);
-      if (t < front + units || i >= per || r + 1 >= a.rows) break;
-      front += units;
+    int front = __builtin_amdgcn_readlane(before, who);
+    if (per == 1) {
+      row = who;
+      len = __builtin_amdgcn_readlane(last_len, who);
+    } else {
+      int64_t r = (int64_t)who * per;
+      // bounded also where a caller changes the lengths under the kernel, as is the loop of next()
+      for (int i = 1;; ++i, ++r) {
+        len = (int)row_length(a, r, false);
+        const int u = units_of(len, shift, cost);
+        if (t < front + u || i >= per || r + 1 >= a.rows) break;
+        front += u;
+      }
+      row = __builtin_amdgcn_readfirstlane((int)r);
+      len = __builtin_amdgcn_readfirstlane(len);
+      front = __builtin_amdgcn_readfirstlane(front);
     }
-    row = __builtin_amdgcn_readfirstlane((int)r);
-    units = __builtin_amdgcn_readfirstlane(units);
+    units = units_of(len, shift, cost);
     if (units == 0) return false;
     const int64_t in_row = at - (int64_t)front * pairs;
     pair = __builtin_amdgcn_readfirstlane((int)(in_row / units));
@@ -142,7 +156,7 @@ struct Run {
     return true;
   }
   // The end of this wave's slots of its pair (none of them: not past the first).
-  __device__ __forceinline__ int last(int shift, int cost, int len) const {
+  __device__ __forceinline__ int last(int shift, int cost) const {
     const int64_t stop = (unit0 + (end - at) - cost) * ((int64_t)1 << shift);
     return stop < 0 ? 0 : (stop < len ? (int)stop : len);
   }
@@ -154,7 +168,8 @@ struct Run {
       pair = 0;
       do {
         if (++row >= a.rows) return false;
-        units = __builtin_amdgcn_readfirstlane(row_units(a, row, shift, cost));
+        len = __builtin_amdgcn_readfirstlane((int)row_length(a, row, false));
+        units = units_of(len, shift, cost);
       } while (units == 0);
     }
     return end - at > cost;  // else the next wave has its tiles
@@ -303,15 +318,16 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
     run.pair = (int)(blockIdx.x % (uint32_t)pairs);
   }
   // slots of a row fit 32 bits (checked on the host)
-  int len = __builtin_amdgcn_readfirstlane(
-      (int)row_length(a, run.row, !STREAM && run.pair == 0 && threadIdx.x == 0));
+  int len = STREAM ? run.len
+                   : __builtin_amdgcn_readfirstlane(
+                         (int)row_length(a, run.row, run.pair == 0 && threadIdx.x == 0));
   int h = run.pair / tiles, rt = run.pair - h * tiles;
   int gn = a.g - rt * 16 < 16 ? a.g - rt * 16 : 16;  // query heads, at most GR
   int64_t qh0 = run.row * a.q_heads + h * a.g + rt * 16;
   // the slots [first, last) this wave takes, every step-th tile of 32
   const int step = STREAM ? 32 : waves * 32;
   int j1 = STREAM ? run.tile * 32 : wave * 32;
-  int last = STREAM ? run.last(kMatrixShift, kMatrixCost, len) : len;
+  int last = STREAM ? run.last(kMatrixShift, kMatrixCost) : len;
   // logits grow with x: a negative scale is taken into q, and so is 0 (masked slots are -inf)
   const float sign = a.scale2 < 0.f ? -1.f : (a.scale2 == 0.f ? 0.f : 1.f);
   const float scale2 = a.scale2 == 0.f ? 1.f : fabsf(a.scale2);
@@ -697,13 +713,13 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
         if (q4 == 0 && n < gn) a.part_ml[part] = make_float2(m, l);
       }
       if (!run.next(a, kMatrixShift, kMatrixCost)) return;
-      len = __builtin_amdgcn_readfirstlane((int)row_length(a, run.row, false));
+      len = run.len;
       h = run.pair / tiles;
       rt = run.pair - h * tiles;
       gn = a.g - rt * 16 < 16 ? a.g - rt * 16 : 16;
       qh0 = run.row * a.q_heads + h * a.g + rt * 16;
       j1 = 0;
-      last = run.last(kMatrixShift, kMatrixCost, len);
+      last = run.last(kMatrixShift, kMatrixCost);
     }
   }
 

@@ -99,9 +99,9 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
     row = run.row;
     h = run.pair / (int)gchunks.d;
     gc = run.pair - h * (int)gchunks.d;
-    len = __builtin_amdgcn_readfirstlane((int)row_length(a, row, false));
+    len = run.len;
     first = run.tile << a.shift;
-    last = run.last(a.shift, a.cost, len);
+    last = run.last(a.shift, a.cost);
   } else {
     if (item >= items) return;  // whole items leave together: no exchange crosses an item
     const uint32_t is = splits.div(item), ig = gchunks.div(is);
@@ -375,9 +375,9 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
       gc = run.pair - h * (int)gchunks.d;
       a0 = h * a.g + gc * GC;
       gn = a.g - gc * GC < GC ? a.g - gc * GC : GC;
-      len = __builtin_amdgcn_readfirstlane((int)row_length(a, row, false));
+      len = run.len;
       first = 0;
-      last = run.last(a.shift, a.cost, len);
+      last = run.last(a.shift, a.cost);
     }
   }
   if constexpr (SL == 1) {
@@ -415,8 +415,8 @@ __device__ __forceinline__ Parts parts_of(const AttendArgs &a, int64_t row, int 
   int parts = 1;
   if (a.stream) {
     const int lane = threadIdx.x & 63, per = (int)((a.rows + 63) >> 6);
-    int before, own, total;
-    stream_sums(a, a.shift, a.cost, lane, per, before, own, total);
+    int before, own, total, len_of_last;
+    stream_sums(a, a.shift, a.cost, lane, per, before, own, total, len_of_last);
     const int who = (int)(row / per);
     int64_t front = __shfl(before, who, 64);
     for (int64_t r = (int64_t)who * per; r < row; ++r) front += row_units(a, r, a.shift, a.cost);
