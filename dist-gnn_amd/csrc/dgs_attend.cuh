@@ -216,7 +216,7 @@ constexpr int kMatrixShift = 5, kMatrixCost = 6, kMatrixLeast = 4;
 // finishing kernel joins them.
 // 8 rows of 8 heads of 128 channels, 100 to 131 thousand slots, 4 query heads a head (1024 MB): 192 us,
 // 5.3 TB/s, as fast as rows come.  64 rows of 1 to 8192 slots with weights (210 MB): 50 us, 4.2 TB/s.
-// One row of 700 slots: 13 us, a chain of loads (length, pages, rows) and the waves' joining.
+// One row of 700 slots: 12 us, a chain of loads (length, pages, rows) and the waves' joining.
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 union Op {
