@@ -697,7 +697,8 @@ void evict_rows(const EvictCall &e, void *ws, int64_t ws_bytes, hipStream_t st) 
   a.holes = (int32_t *)(w + up256(pairs * 4));
   a.movers = (int32_t *)(w + up256(pairs * 4) + up256(pairs * a.room * 4));
   plan<false>(a, st);
-  if (e.nstores == 0) return;
+  // no slot can go from rows that the budget covers (long ones come this way too)
+  if (e.nstores == 0 || a.room == 0) return;
   // enough blocks to fill the card, at least 8 rows for each of a block's groups
   int64_t ny = ceil_div(a.room, 128);
   const int64_t fill = ceil_div(4096, pairs);
