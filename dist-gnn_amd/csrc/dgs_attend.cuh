@@ -59,6 +59,22 @@ __device__ __forceinline__ int64_t row_length(const AttendArgs &a, int64_t row, 
   return len;
 }
 
+// Whether every page of a row's first `len` slots lies outside the cache, where a sum of probabilities
+// is 0: only then it is inverted to 0, so that the output is zeros and the weights get nothing (logits
+// that are all -infinity give NaN, as the formula does).  The lanes of a wave look together, or each for
+// itself (kTogether = 1, rows of a few slots).
+template <int kTogether>
+__device__ __forceinline__ bool none_left(const AttendArgs &a, int64_t row, int64_t len) {
+  const int64_t n = (len + (int64_t(1) << a.c.pshift) - 1) >> a.c.pshift;
+#pragma unroll 1
+  for (int64_t p0 = 0; p0 < n; p0 += kTogether) {
+    const int64_t p = p0 + (kTogether > 1 ? threadIdx.x & 63 : 0);
+    const bool in = p < n && (uint64_t)a.table[row * a.width + p] < (uint64_t)a.c.pages;
+    if (kTogether > 1 ? __any(in) : in) return false;
+  }
+  return true;
+}
+
 __device__ __forceinline__ void store_out(int type, void *out, int64_t elem, const float (&x)[8]) {
   if (type == kStateF32)
     store8<kStateF32>(out, elem, x);
@@ -695,7 +711,8 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
         const bool whole = run.tile == 0 && last == len;
         l = over_columns(l);
         const int64_t part = (run.row * pairs + run.pair + blockIdx.x * waves + wave) * gs + n;
-        const float inv = whole ? 1.f / l : 1.f;
+        float inv = 1.f;
+        if (whole) inv = __any(l == 0.f) && none_left<64>(a, run.row, len) ? 0.f : 1.f / l;
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
           const float c = over_columns(cb[g]);
@@ -749,6 +766,12 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
     }
   }
   __syncthreads();
+  bool none = len == 0;
+  if (!none) {
+    float ls = 0.f;
+    for (int w = 0; w < waves; ++w) ls += s_l[w * 16 + n];
+    if (__any(ls == 0.f)) none = none_left<64>(a, run.row, len);
+  }
   for (int i = threadIdx.x; i < gn * (kD / 8); i += blockDim.x) {
     const int hd = i / (kD / 8), ch = (i % (kD / 8)) * 8;
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, ls = 0.f;
@@ -758,7 +781,7 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
 #pragma unroll
       for (int y = 0; y < 8; ++y) acc[y] += src[y];
     }
-    const float inv = len == 0 ? 0.f : 1.f / ls;
+    const float inv = none ? 0.f : 1.f / ls;
 #pragma unroll
     for (int y = 0; y < 8; ++y) acc[y] *= inv;
     store_out(type, a.out, (qh0 + hd) * kD + ch, acc);
@@ -781,7 +804,7 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
         ls += s_l[w * 16 + g];
       }
     mh[g] = g < gn ? (mm == -INFINITY ? 0.f : mm) : INFINITY;  // no head: exp2(-inf) * 0
-    ih[g] = g < gn ? 1.f / ls : 0.f;
+    ih[g] = g < gn && !none ? 1.f / ls : 0.f;
   }
   const float *lg = a.logits + qh0 * a.cap;
   float *wr = a.weights + (run.row * a.c.heads + h) * a.weights_cols;

@@ -223,8 +223,8 @@ class StateCache:
     def attend(self, q, table, lens, scale=None, weights=None, decay=1.0):
         """Attention of q [rows, q_heads, head_dim] (one query token a row; q_heads a multiple of
         heads, neighbouring query heads share a head) over the first lens[i] slots of table row i
-        -> [rows, q_heads, head_dim]; a row of length 0 gives zeros.  scale: 1 / sqrt(head_dim)
-        by default.  weights (float32 [rows, heads, >= pages * page_size], updated in place):
+        -> [rows, q_heads, head_dim]; a row of length 0, or with all its pages outside the cache,
+        gives zeros.  scale: 1 / sqrt(head_dim) by default.  weights (float32 [rows, heads, >= pages * page_size], updated in place):
         weights[i, h, j] = decay * weights[i, h, j] + the probabilities of head h's query heads,
         for j < lens[i].  Several query tokens of one sequence are several rows with the same
         table row, each with the length that it may see."""

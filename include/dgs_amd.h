@@ -369,8 +369,8 @@ int dgs_state_append(const dgs_state_cache *c, const void *k, const void *v, int
 int dgs_state_read(const dgs_state_cache *c, const int64_t *slots, int64_t n, int dtype,
                    void *k_out, void *v_out, void *stream);
 /* out[i, a] = sum_j softmax_j(scale * q[i, a] . K[j, h]) V[j, h], j over the first lens[i] slots of
- * table row i, h = a / (q_heads / heads); lens[i] = 0 gives zeros.  q [rows, q_heads, head_dim]
- * with strides, out contiguous, both of `dtype`.  weights (float [rows, heads, weights_cols],
+ * table row i, h = a / (q_heads / heads); lens[i] = 0 gives zeros, and so does a row all of whose
+ * pages lie outside the cache (its weights only decay).  q [rows, q_heads, head_dim] with strides, out contiguous, both of `dtype`.  weights (float [rows, heads, weights_cols],
  * weights_cols >= width * page_size, or NULL): weights[i, h, j] = decay * weights[i, h, j] + the
  * sum of head h's query heads' probabilities, for j < lens[i]; decay 0 does not read them. */
 int dgs_state_attend_workspace(const dgs_state_cache *c, int64_t rows, int q_heads, int64_t width,

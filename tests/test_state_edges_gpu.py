@@ -1,11 +1,16 @@
-"""The state cache's calls at the edges of what it documents, against plain forms."""
+"""The state cache's calls at the edges of what it documents, against plain forms.
+
+Tolerances of attend: those of test_state_gpu.py (prob_error), whose derivation counts the sums over
+the slots that are there."""
+import math
+
 import numpy as np
 import pytest
 import torch
 
 import dgs
 import state_ref as ref
-from test_state_gpu import same_bits
+from test_state_gpu import TYPES, U, full_cache, prob_error, raises_next, same_bits, states
 
 pytestmark = pytest.mark.gpu
 
@@ -36,3 +41,101 @@ def test_evict_with_room_for_every_column(cols, budget, given):
         assert np.array_equal(got_p.cpu().numpy(), want_p)
         assert np.array_equal(got_n.cpu().numpy(), want_n)
         assert same_bits(store, before)
+
+
+# ------------------------------------------------------------------------------ attention
+def plain_left_out(q, cache, table, lens):
+    """As ref.attend, with the slots on pages outside the cache left out (none left: zeros)."""
+    kc, ks, vc, vs = [t.cpu() for t in (cache.k_codes, cache.k_scales, cache.v_codes,
+                                        cache.v_scales)]
+    q, table, lens = q.cpu().double(), table.cpu().long(), lens.cpu().long()
+    rows, nq, dim = q.shape
+    pages, heads, page = kc.shape[:3]
+    group, g, scale = dim // ks.shape[3], nq // heads, dim ** -0.5
+    out = torch.zeros(rows, nq, dim, dtype=torch.float64)
+    prob = torch.zeros(rows, heads, table.shape[1] * page, dtype=torch.float64)
+    size, steps, vmax = (torch.zeros(rows, nq, dtype=torch.float64) for _ in range(3))
+    for i in range(rows):
+        j = torch.arange(int(lens[i]))
+        j = j[(table[i, j // page] >= 0) & (table[i, j // page] < pages)]
+        if j.numel() == 0:
+            continue
+        p, o = table[i, j // page], j % page
+        for h in range(heads):
+            k, v = ref.values(kc[p, h, o], ks[p, h, o]), ref.values(vc[p, h, o], vs[p, h, o])
+            mine = slice(h * g, (h + 1) * g)
+            e = torch.softmax(q[i, mine] @ k.T * scale, 1)
+            out[i, mine], prob[i, h, j] = e @ v, e.sum(0)
+            s = ks[p, h, o, :, 0].double().repeat_interleave(group, 1)
+            size[i, mine] = (q[i, mine].abs() @ k.abs().T).amax(1) * scale
+            steps[i, mine] = (q[i, mine].abs() @ s.T).amax(1) * scale
+            vmax[i, mine] = v.abs().max()
+    return out, prob, size, steps, vmax
+
+
+@pytest.mark.parametrize("page", [1, 8, 16])
+@pytest.mark.parametrize("cap", [16, 64, 2048])
+@pytest.mark.parametrize("dim, group, heads, g, dtype", [
+    (128, 64, 2, 4, "bf16"), (64, 64, 1, 1, "f32"), (80, 40, 2, 3, "f16"), (32, 32, 2, 20, "bf16"),
+    (128, 32, 1, 5, "f32"), (96, 96, 2, 2, "bf16")])
+def test_slots_outside_are_left_out(page, cap, dim, group, heads, g, dtype):
+    """Rows with none, one, some and all of their pages outside the cache: a row without a slot gives
+    zeros, and its weights receive nothing but their decay."""
+    gen = torch.Generator().manual_seed(cap + dim)
+    pages, width = 4096 // page, cap // page
+    cache = full_cache(pages, page, heads, dim, group, seed=7)
+    table = torch.randint(0, pages, (9, width), generator=gen)
+    lens = torch.tensor([cap, cap, cap, cap - 3, 0, cap, 1, cap // 2, cap])
+    bad = torch.randint(1, 2 ** 31, (9, width), generator=gen) * -1
+    bad[:, 1::2] = pages
+    table[1] = bad[1]
+    table[2, ::2] = bad[2, ::2]
+    table[3] = bad[3]
+    table[4] = bad[4]
+    table[5, -1] = bad[5, -1]
+    table[6] = bad[6]
+    table[7, :-(-cap // 2 // page)] = bad[7, :-(-cap // 2 // page)]  # only what lies in the length
+    table[8, 0] = bad[8, 0]
+    q = states((9, heads * g, dim), gen, TYPES[dtype])
+    want, prob, size, steps, vmax = plain_left_out(q, cache, table, lens)
+    rel = prob_error(dim, size, steps, dtype == "f32")
+    off = (2 * rel * vmax)[..., None]
+    tol = off + torch.finfo(q.dtype).eps / 2 * (want.abs() + off)
+    tol = tol + 2.0 ** -25 if dtype == "f16" else tol
+    w0 = torch.rand(9, heads, cap, generator=gen)
+    inside = (torch.arange(cap) < lens[:, None])[:, None]
+    for ids in (torch.int32, torch.int64):
+        for decay in (0.5, 0.0):
+            w = w0.cuda()
+            got = cache.attend(q, table.to(ids).cuda(), lens.cuda(), weights=w, decay=decay)
+            raises_next("page or slot")
+            err = (got.cpu().double() - want).abs()
+            assert bool((err <= tol).all()), (float(err.max()), float(tol.max()))
+            for none in (1, 3, 4, 6, 7):
+                assert bool((got[none] == 0).all())
+            exp = torch.where(inside, prob + decay * w0.double(), w0.double())
+            wrel = 2 * rel.unflatten(1, (heads, g)).amax(2)[..., None]
+            werr = (w.cpu().double() - exp).abs()
+            assert bool((werr <= wrel * prob + (g + 4) * U * exp.abs()).all()), float(werr.max())
+        plain = cache.attend(q, table.to(ids).cuda(), lens.cuda())
+        raises_next("page or slot")
+        assert bool(((plain.cpu().double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("cap", [16, 256, 2048])
+@pytest.mark.parametrize("g", [1, 4])
+def test_infinite_logits_are_no_empty_row(cap, g):
+    """Logits that are all -infinity have no softmax: NaN, not the zeros of a row without slots."""
+    dim = 64
+    codes = torch.full((cap, 1, 1, dim // 2), 0x11, dtype=torch.uint8, device="cuda")  # code 1
+    scales = torch.tensor([1.0, 0.0]).to(torch.bfloat16).cuda().expand(cap, 1, 1, 1, 2).contiguous()
+    cache = dgs.classes.StateCache.wrap(codes, scales, codes.clone(), scales.clone())  # all rows are 1
+    q = torch.ones(3, g, dim, device="cuda")
+    q[1, 0, 7] = -math.inf
+    table = torch.arange(cap).repeat(3, 1).cuda()
+    w = torch.zeros(3, 1, cap, device="cuda")
+    got = cache.attend(q, table, torch.tensor([cap, cap, 0]).cuda(), weights=w)
+    assert bool(got[1, 0].isnan().all()) and bool(w[1].isnan().all())
+    assert torch.equal(got[2], torch.zeros(g, dim, device="cuda")) and not w[2].any()
+    ones = torch.cat([got[0], got[1, 1:]])
+    assert bool(((ones - 1).abs() <= (cap + 8) * U).all())  # a mean of ones
