@@ -139,3 +139,26 @@ def test_infinite_logits_are_no_empty_row(cap, g):
     assert torch.equal(got[2], torch.zeros(g, dim, device="cuda")) and not w[2].any()
     ones = torch.cat([got[0], got[1, 1:]])
     assert bool(((ones - 1).abs() <= (cap + 8) * U).all())  # a mean of ones
+
+
+def test_streams_keep_their_own_weights():
+    gen = torch.Generator().manual_seed(0)
+    cache = full_cache(256, 16, 2, 128, 64)
+    table = torch.randperm(256, generator=gen).view(2, 128).cuda()
+    lens = torch.tensor([2048, 1999]).cuda()
+    for dtype in TYPES.values():
+        qs = [states((2, 8, 128), gen, dtype) for _ in range(4)]
+        want = [torch.zeros(2, 2, 2048, device="cuda") for _ in range(4)]
+        for q, w in zip(qs, want):
+            for _ in range(5):
+                cache.attend(q, table, lens, weights=w, decay=0.5)
+        torch.cuda.synchronize()
+        got = [torch.zeros(2, 2, 2048, device="cuda") for _ in range(4)]
+        streams = [torch.cuda.Stream() for _ in range(4)]
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for q, w, s in zip(qs, got, streams):
+                with torch.cuda.stream(s):
+                    cache.attend(q, table, lens, weights=w, decay=0.5)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
