@@ -51,12 +51,19 @@ __device__ __forceinline__ uint32_t lanes_before_and_me(uint32_t x) {
   return x;
 }
 
-// Larger is better; a protected slot beats every weight.
+// Larger is better; a protected slot beats every weight.  Positions that repeat can protect more slots
+// than stay: the threshold comes out as kFixed then, and the selection is made once more with
+// protected_key, which ranks them by weight and puts all others behind.
+constexpr uint32_t kFixed = 0xffffffffu;
 __device__ __forceinline__ uint32_t key_of(float w, bool fixed) {
-  if (fixed) return 0xffffffffu;
+  if (fixed) return kFixed;
   if (w != w) w = -INFINITY;
   const uint32_t u = __float_as_uint(w + 0.f);  // -0 ranks with 0
   return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+__device__ __forceinline__ uint32_t protected_key(float w, bool fixed) {
+  return fixed ? key_of(w, false) : 0u;
 }
 
 __device__ __forceinline__ int evict_length(const EvictArgs &a, int64_t row, bool report) {
@@ -250,7 +257,7 @@ __device__ __forceinline__ void plan_end(const EvictArgs &a, const PlanRow &r,
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void k_evict_plan_small(EvictArgs a) {
   constexpr int kWaves = THREADS / 64;
-  __shared__ uint32_t s_key[THREADS], s_run[kWaves];
+  __shared__ uint32_t s_key[THREADS], s_run[kWaves], s_fixed[kWaves];
   __shared__ int32_t s_max[kWaves];
   __shared__ int32_t s_hole[THREADS / 2], s_mover[THREADS / 2];  // as many of one as of the other
   const int j = threadIdx.x, lane = j & 63, wave = j >> 6;
@@ -266,10 +273,21 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan_small(EvictArgs a) {
   if (r.n <= r.budget) return;
   const int32_t top = block_max<THREADS>(j < r.n ? p : -1, s_max);
   const int64_t newest = (int64_t)top + 1 - a.e.recent;
+  const bool fixed = j < r.n && (p < a.e.sinks || p >= newest);
   // past the row: 0, behind every key
-  const uint32_t key = j < r.n ? key_of(w, p < a.e.sinks || p >= newest) : 0u;
+  uint32_t key = j < r.n ? key_of(w, fixed) : 0u;
   s_key[j] = key;
+  const uint64_t all_fixed = __ballot(fixed);
+  if (lane == 0) s_fixed[wave] = __popcll(all_fixed);
   __syncthreads();
+  uint32_t held = 0;
+#pragma unroll
+  for (int v = 0; v < kWaves; ++v) held += s_fixed[v];
+  if (held > (uint32_t)r.keep) {
+    key = protected_key(w, fixed);
+    s_key[j] = key;  // a thread's own: the others read it past the barrier
+    __syncthreads();
+  }
   // of equal keys the lower slot comes first
   int before = 0;
   for (int v = 0; v < kWaves; ++v) {
@@ -302,6 +320,94 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan_small(EvictArgs a) {
   if (hole) s_hole[rank & 0xffffu] = j;
   if (mover) s_mover[rank >> 16] = j;
   plan_end<THREADS, true>(a, r, s_hole, s_mover, all & 0xffffu);
+}
+
+// The selection where every step reads weights and positions again: the threshold by digits, then ties,
+// holes and movers in slot order, of which a wave takes a run of n / kWaves slots.  Returns the moves.
+// s_cnt: 3 kWaves words.
+template <int THREADS>
+__device__ __forceinline__ uint32_t plan_again(const EvictArgs &a, const PlanRow &r, int64_t newest,
+                                               bool only_protected, int32_t *holes, int32_t *movers,
+                                               uint32_t *s_hist, uint32_t *s_scan, uint32_t *s_found,
+                                               uint32_t *s_cnt) {
+  constexpr int kWaves = THREADS / 64;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = r.n;
+  auto key_at = [&](int j) {
+    const int32_t p = r.pos ? r.pos[j] : j;
+    const bool fixed = p < a.e.sinks || p >= newest;
+    return only_protected ? protected_key(r.w[j], fixed) : key_of(r.w[j], fixed);
+  };
+  uint32_t prefix, left;
+#pragma unroll 1
+  while (true) {
+    prefix = 0;
+    left = (uint32_t)r.keep;
+    int shift = 32;
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+      const int bits = pass < 2 ? 11 : 10;
+      const uint32_t done = pass == 0 ? 0u : ~0u << shift;
+      shift -= bits;
+      for (int i = tid; i < kDigits; i += THREADS) s_hist[i] = 0;
+      __syncthreads();
+#pragma unroll 4
+      for (int j = tid; j < n; j += THREADS) {
+        const uint32_t k = key_at(j);
+        if ((k & done) == prefix) atomicAdd(&s_hist[(k >> shift) & ((1u << bits) - 1)], 1u);
+      }
+      __syncthreads();
+      prefix |= pick_digit<THREADS>(s_hist, left, s_scan, s_found) << shift;
+    }
+    if (prefix != kFixed || s_found[2] == left) break;
+    only_protected = true;
+  }
+  const int seg = ((n + kWaves - 1) / kWaves + 63) & ~63;
+  const int j0 = wave * seg, j1 = j0 + seg < n ? j0 + seg : n;
+  const uint64_t below = lane == 0 ? 0ull : ~0ull >> (64 - lane);
+  auto before_wave = [&](const uint32_t *c) {
+    uint32_t s = 0;
+    for (int i = 0; i < wave; ++i) s += c[i];
+    return s;
+  };
+  uint32_t cnt = 0;
+  for (int b = j0; b < j1; b += 64)
+    cnt += __popcll(__ballot(b + lane < j1 && key_at(b + lane) == prefix));
+  if (lane == 0) s_cnt[wave] = cnt;
+  __syncthreads();
+  const uint32_t tie0 = before_wave(s_cnt);
+  uint32_t nh = 0, nm = 0;
+  for (int turn = 0; turn < 2; ++turn) {  // count, then write
+    uint32_t ties = tie0;
+    for (int b = j0; b < j1; b += 64) {
+      const int j = b + lane;
+      const bool in = j < j1;
+      const uint32_t k = key_at(in ? j : j1 - 1);
+      const bool tie = in && k == prefix;
+      const uint64_t tb = __ballot(tie);
+      const bool kept = in && (k > prefix || (tie && ties + __popcll(tb & below) < left));
+      ties += __popcll(tb);
+      const uint64_t hb = __ballot(in && !kept && j < r.budget);
+      const uint64_t mb = __ballot(kept && j >= r.budget);
+      if (turn == 1) {
+        if ((hb >> lane) & 1) holes[nh + __popcll(hb & below)] = j;
+        if ((mb >> lane) & 1) movers[nm + __popcll(mb & below)] = j;
+      }
+      nh += __popcll(hb);
+      nm += __popcll(mb);
+    }
+    if (turn == 0) {
+      if (lane == 0) {
+        s_cnt[kWaves + wave] = nh;
+        s_cnt[2 * kWaves + wave] = nm;
+      }
+      __syncthreads();
+      nh = before_wave(s_cnt + kWaves);
+      nm = before_wave(s_cnt + 2 * kWaves);
+    }
+  }
+  uint32_t all = 0;
+  for (int i = 0; i < kWaves; ++i) all += s_cnt[kWaves + i];
+  return all;
 }
 
 // Rows of at most THREADS * kVecs * 4 slots: slot (v THREADS + t) 4 + i is thread t's.  ALIGNED:
@@ -385,6 +491,12 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan(EvictArgs a) {
       key[v][i] = key_of(__uint_as_float(key[v][i]), p[v][i] < a.e.sinks || p[v][i] >= newest);
   int32_t *holes = FUSED ? s_list : a.holes + r.pair * a.room;
   int32_t *movers = FUSED ? s_list + kFewMoves : a.movers + r.pair * a.room;
+  // more protected slots than stay: rare, and not worth the registers
+  auto rank_protected = [&]() {
+    const uint32_t all = plan_again<THREADS>(a, r, newest, true, holes, movers, s_hist[0], s_scan, s_found,
+                                             s_hist[1]);
+    plan_end<THREADS, FUSED>(a, r, holes, movers, all);
+  };
   if (r.n == r.budget + 1) {
     uint64_t low = ~0ull;  // key, then the complement of the slot
 #pragma unroll
@@ -404,6 +516,7 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan(EvictArgs a) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) low = s_low[i] < low ? s_low[i] : low;
+    if ((uint32_t)(low >> 32) == kFixed) return rank_protected();
     const int drop = (int)~(uint32_t)low;
     if (tid == 0) {
       holes[0] = drop;
@@ -433,6 +546,7 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan(EvictArgs a) {
     __syncthreads();
     prefix |= pick_digit<THREADS>(s_hist[pass], left, s_scan, s_found) << shift;
   }
+  if (prefix == kFixed && s_found[2] != left) return rank_protected();  // pick_digit ends in a barrier
   // Exclusive sums of the runs' counts in slot order (run = v, wave), in place.
   auto scan_runs = [&]() {
     __syncthreads();
@@ -520,16 +634,15 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan(EvictArgs a) {
   plan_end<THREADS, FUSED>(a, r, holes, movers, all);
 }
 
-// Longer rows: every step reads weights and positions again.  In slot order a wave takes a run of
-// n / kWaves slots.
+// Longer rows.
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void k_evict_plan_long(EvictArgs a) {
   constexpr int kWaves = THREADS / 64;
   __shared__ uint32_t s_hist[kDigits];
-  __shared__ uint32_t s_scan[kWaves], s_found[3], s_cnt[3][kWaves];
+  __shared__ uint32_t s_scan[kWaves], s_found[3], s_cnt[3 * kWaves];
   __shared__ int32_t s_max[kWaves];
   const PlanRow r = plan_row(a);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = r.n;
+  const int tid = threadIdx.x, n = r.n;
   for (int j = r.keep + tid; j < r.cols; j += THREADS) {
     r.wo[j] = 0.f;
     r.po[j] = -1;
@@ -547,74 +660,8 @@ __global__ __launch_bounds__(THREADS) void k_evict_plan_long(EvictArgs a) {
   if (n <= r.budget) return;
   top = block_max<THREADS>(top, s_max);
   const int64_t newest = (int64_t)top + 1 - a.e.recent;
-  auto key_at = [&](int j) {
-    const int32_t p = r.pos ? r.pos[j] : j;
-    return key_of(r.w[j], p < a.e.sinks || p >= newest);
-  };
-  uint32_t prefix = 0, left = (uint32_t)r.keep;
-  int shift = 32;
-#pragma unroll 1
-  for (int pass = 0; pass < 3; ++pass) {
-    const int bits = pass < 2 ? 11 : 10;
-    const uint32_t done = pass == 0 ? 0u : ~0u << shift;
-    shift -= bits;
-    for (int i = tid; i < kDigits; i += THREADS) s_hist[i] = 0;
-    __syncthreads();
-#pragma unroll 4
-    for (int j = tid; j < n; j += THREADS) {
-      const uint32_t k = key_at(j);
-      if ((k & done) == prefix) atomicAdd(&s_hist[(k >> shift) & ((1u << bits) - 1)], 1u);
-    }
-    __syncthreads();
-    prefix |= pick_digit<THREADS>(s_hist, left, s_scan, s_found) << shift;
-  }
-  const int seg = ((n + kWaves - 1) / kWaves + 63) & ~63;
-  const int j0 = wave * seg, j1 = j0 + seg < n ? j0 + seg : n;
-  const uint64_t below = lane == 0 ? 0ull : ~0ull >> (64 - lane);
-  auto before_wave = [&](const uint32_t *c) {
-    uint32_t s = 0;
-    for (int i = 0; i < wave; ++i) s += c[i];
-    return s;
-  };
-  uint32_t cnt = 0;
-  for (int b = j0; b < j1; b += 64)
-    cnt += __popcll(__ballot(b + lane < j1 && key_at(b + lane) == prefix));
-  if (lane == 0) s_cnt[0][wave] = cnt;
-  __syncthreads();
-  const uint32_t tie0 = before_wave(s_cnt[0]);
   int32_t *holes = a.holes + r.pair * a.room, *movers = a.movers + r.pair * a.room;
-  uint32_t nh = 0, nm = 0;
-  for (int turn = 0; turn < 2; ++turn) {  // count, then write
-    uint32_t ties = tie0;
-    for (int b = j0; b < j1; b += 64) {
-      const int j = b + lane;
-      const bool in = j < j1;
-      const uint32_t k = key_at(in ? j : j1 - 1);
-      const bool tie = in && k == prefix;
-      const uint64_t tb = __ballot(tie);
-      const bool kept = in && (k > prefix || (tie && ties + __popcll(tb & below) < left));
-      ties += __popcll(tb);
-      const uint64_t hb = __ballot(in && !kept && j < r.budget);
-      const uint64_t mb = __ballot(kept && j >= r.budget);
-      if (turn == 1) {
-        if ((hb >> lane) & 1) holes[nh + __popcll(hb & below)] = j;
-        if ((mb >> lane) & 1) movers[nm + __popcll(mb & below)] = j;
-      }
-      nh += __popcll(hb);
-      nm += __popcll(mb);
-    }
-    if (turn == 0) {
-      if (lane == 0) {
-        s_cnt[1][wave] = nh;
-        s_cnt[2][wave] = nm;
-      }
-      __syncthreads();
-      nh = before_wave(s_cnt[1]);
-      nm = before_wave(s_cnt[2]);
-    }
-  }
-  uint32_t all = 0;
-  for (int i = 0; i < kWaves; ++i) all += s_cnt[1][i];
+  const uint32_t all = plan_again<THREADS>(a, r, newest, false, holes, movers, s_hist, s_scan, s_found, s_cnt);
   plan_end<THREADS, false>(a, r, holes, movers, all);
 }
 

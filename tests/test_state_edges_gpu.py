@@ -43,6 +43,43 @@ def test_evict_with_room_for_every_column(cols, budget, given):
         assert same_bits(store, before)
 
 
+@pytest.mark.parametrize("cols, budget", [
+    (50, 20), (64, 63), (200, 100), (256, 255), (300, 100), (1000, 999), (1000, 400), (4000, 3999),
+    (5003, 1000), (8000, 7900), (12000, 6000), (20001, 20000), (30000, 200), (40000, 39999),
+    (40000, 9000)])
+@pytest.mark.parametrize("kind", ["few", "same", "zeros", "negative", "half"])
+def test_evict_repeated_positions(cols, budget, kind):
+    """Positions that repeat (timestamps, zeros behind a prompt, -1 at an appended slot) protect more
+    slots than stay: of the protected ones the heaviest do."""
+    rng = np.random.default_rng(cols + budget)
+    lens = np.array([cols, budget + 1, cols - cols // 7])
+    rows, heads, sinks, recent = 3, 2, 0, min(budget, 3)
+    w = rng.integers(0, 400, (rows, heads, cols)).astype(np.float32) * 0.25 - 20  # ties too
+    w[rng.random(w.shape) < 0.05] = np.nan
+    w[rng.random(w.shape) < 0.02] = np.inf
+    w[rng.random(w.shape) < 0.02] = -np.inf
+    pos = {"few": rng.integers(0, 4, w.shape), "same": np.full(w.shape, 7),
+           "zeros": np.zeros(w.shape), "negative": np.full(w.shape, -1),
+           "half": np.where(rng.random(w.shape) < 0.5, rng.permutation(cols), 10 ** 9)}[kind]
+    pos = pos.astype(np.int32)
+    if kind in ("zeros", "negative"):
+        sinks, recent = 1, 0
+    store = torch.from_numpy(rng.integers(0, 2 ** 31, (rows * cols, heads, 1, 1), dtype=np.int32)).cuda()
+    table = rng.permutation(rows * cols).reshape(rows, cols)
+    want_w, want_p, want_n, moves = ref.evict(w, pos, lens, budget, sinks, recent)
+    expect, t = store.cpu().clone(), torch.from_numpy(table)
+    if moves:
+        i, h, s, d = (torch.tensor(x) for x in zip(*moves))
+        expect[t[i, d], h] = expect[t[i, s], h].clone()
+    got_w, got_p, got_n = dgs.ops.evict_rows(
+        [store], torch.from_numpy(w).cuda(), torch.from_numpy(pos).cuda(), t.cuda(),
+        torch.from_numpy(lens).cuda(), budget, sinks=sinks, recent=recent)
+    assert np.array_equal(got_n.cpu().numpy(), want_n)
+    assert np.array_equal(got_p.cpu().numpy(), want_p)
+    assert np.array_equal(got_w.cpu().numpy(), want_w, equal_nan=True)
+    assert same_bits(store, expect)
+
+
 # ------------------------------------------------------------------------------ attention
 def plain_left_out(q, cache, table, lens):
     """As ref.attend, with the slots on pages outside the cache left out (none left: zeros)."""
