@@ -419,6 +419,15 @@ void mirror_free(void *h, size_t bytes) {
 
 // ------------------------------------------------------------------ async errors
 namespace {
+// While it lives, this thread may allocate although a stream is being captured (a graph does not hold
+// what it allocates: the words of the first call of a process, which live as long as the process).
+struct RelaxedCapture {
+  hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+  RelaxedCapture() { DGS_HIP(hipThreadExchangeStreamCaptureMode(&mode)); }
+  ~RelaxedCapture() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
+  RelaxedCapture(const RelaxedCapture &) = delete;
+  RelaxedCapture &operator=(const RelaxedCapture &) = delete;
+};
 struct AsyncErrWords {
   int64_t *host = nullptr, *dev = nullptr;
   std::atomic<uint64_t> tag{0};
@@ -427,6 +436,7 @@ AsyncErrWords &async_err() {
   static AsyncErrWords w;
   static std::once_flag once;
   std::call_once(once, [] {
+    RelaxedCapture relaxed;
     void *h = nullptr;
     // portable: visible to every device of the process; coherent: a kernel's system-scope
     // store is seen by the host without a synchronisation

@@ -153,7 +153,7 @@ class StateCache:
         self._ref = ctypes.addressof(self._c)
         self._room = {}
         with _on(self._index):
-            check(lib.dgs_check_async_errors())  # makes the report words (never inside a capture)
+            check(lib.dgs_check_async_errors())  # makes the report words
 
     def _rows(self, k, v):
         shape = k.shape

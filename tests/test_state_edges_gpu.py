@@ -3,6 +3,9 @@
 Tolerances of attend: those of test_state_gpu.py (prob_error), whose derivation counts the sums over
 the slots that are there."""
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -78,6 +81,12 @@ def test_evict_repeated_positions(cols, budget, kind):
     assert np.array_equal(got_p.cpu().numpy(), want_p)
     assert np.array_equal(got_w.cpu().numpy(), want_w, equal_nan=True)
     assert same_bits(store, expect)
+
+
+def test_first_call_of_a_process_inside_a_capture():
+    worker = os.path.join(os.path.dirname(os.path.abspath(__file__)), "evict_capture_worker.py")
+    p = subprocess.run([sys.executable, worker], capture_output=True, text=True, timeout=100)
+    assert p.returncode == 0 and "capture worker ok" in p.stdout, p.stderr[-2000:]
 
 
 # ------------------------------------------------------------------------------ attention
