@@ -32,8 +32,9 @@ __device__ __forceinline__ Codes codes_of(uint32_t w) {
   return Codes{{__builtin_bit_cast(half2v, w & 0x000f000fu), __builtin_bit_cast(half2v, w & 0x00f000f0u),
                 __builtin_bit_cast(half2v, y & 0x000f000fu), __builtin_bit_cast(half2v, y & 0x00f000f0u)}};
 }
-// Channel c's unit, as the caller's factors: 2^-24 on even channels, 2^-20 on odd ones.
-constexpr float kTiny = 0x1p-24f, kUnTiny[2] = {0x1p24f, 0x1p20f};
+// Channel c's unit is 2^-24 on even channels, 2^-20 on odd ones; the caller's scales make it 2^-24 on
+// all, in which values are summed (no scale leaves the range).
+constexpr float kTiny = 0x1p-24f, kUnTiny = 0x1p24f;
 
 template <int LPR>
 __device__ __forceinline__ float sum_lanes(float x) {
@@ -73,9 +74,10 @@ __device__ __forceinline__ uint32_t of_quad(uint32_t x, int u) {
 // joined at the end by exchanges between lanes.  Rows are loaded one step ahead of the arithmetic, ids
 // another one.  What belongs to a slot and not to a channel - its page and address, and with QG (groups
 // of a multiple of 32 channels) its scale and base - is fetched by one lane of every four and passed on
-// by lane moves: 11 loads a step instead of 24.  K is taken as values (one multiply-add a code, then
-// one a query head); of V the codes are summed with p * scale, the bases apart.  As in the matrix form,
-// the running maximum is only followed when a logit passes it by 8.
+// by lane moves: 11 loads a step instead of 24.  K and V are taken as values (one multiply-add a code,
+// then one a query head).  Summing V's codes with p * scale and the bases apart spares V's first one,
+// but the two sums cancel: 32-bit outputs were 3 times as far off as the formula in 32 bits.  As in the
+// matrix form, the running maximum is only followed when a logit passes it by 8.
 // SL = 1 is for rows of at most 16 slots: no join, and with all query heads of a head in the item
 // the probabilities stay in registers and the item writes its weights itself.
 // Bound by the vector instructions: 10 million of a wave in the 22.6 us of 16 rows of 8 heads (128
@@ -126,7 +128,7 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
   }
   int a0 = h * a.g + gc * GC, gn = a.g - gc * GC < GC ? a.g - gc * GC : GC;
 
-  float q[GC][W][8], o[GC][W][8], ob[GC][W], m[GC], l[GC], xs[kKeep][GC];
+  float q[GC][W][8], o[GC][W][8], m[GC], l[GC], xs[kKeep][GC];
   const int ps = a.c.pshift, mask = (1 << ps) - 1;
   const bool wide = a.table.bytes == 8;
   const char *tab;  // the row's
@@ -204,7 +206,6 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
       for (int k = 0; k < W; ++k) {
         const uint32_t kw = QG ? of_quad(t.km[0][k], u) : t.km[QG ? 0 : u][k];
         const uint32_t km = live[k] ? kw : 0u;
-        // values in units of 2^-24: no scale leaves the range
         const float ks[2] = {scale_of(km), scale_of(km) * 0x1p-4f}, kb = base_of(km) * kTiny;
         const Codes kc = codes_of(t.kq[u][k]);
         float kv[8];
@@ -217,7 +218,7 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
       }
 #pragma unroll
       for (int g = 0; g < GC; ++g) {
-        const float x0 = sum_lanes<LPR>(s[g]) * kUnTiny[0];
+        const float x0 = sum_lanes<LPR>(s[g]) * kUnTiny;
         x[g][u] = ok ? x0 : -INFINITY;
       }
     }
@@ -246,11 +247,9 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
         m[g] = top;
         l[g] *= f;
 #pragma unroll
-        for (int k = 0; k < W; ++k) {
-          ob[g][k] *= f;
+        for (int k = 0; k < W; ++k)
 #pragma unroll
           for (int i = 0; i < 8; ++i) o[g][k][i] *= f;
-        }
       }
       const float ms = m[g] == -INFINITY ? 0.f : m[g];
 #pragma unroll
@@ -265,16 +264,15 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
       for (int k = 0; k < W; ++k) {
         const uint32_t vw = QG ? of_quad(t.vm[0][k], u) : t.vm[QG ? 0 : u][k];
         const uint32_t vm = live[k] && u < t.n && !((t.bad >> u) & 1) ? vw : 0u;
-        const float vs = scale_of(vm), vb = base_of(vm);
+        const float vs[2] = {scale_of(vm), scale_of(vm) * 0x1p-4f}, vb = base_of(vm) * kTiny;
         const Codes vc = codes_of(t.vq[u][k]);
+        float vv[8];
 #pragma unroll
-        for (int g = 0; g < GC; ++g) {
-          const float ps = x[g][u] * vs;
-          ob[g][k] = __builtin_fmaf(x[g][u], vb, ob[g][k]);
+        for (int i = 0; i < 8; ++i) vv[i] = __builtin_fmaf((float)vc.p[i & 3][i >> 2], vs[i & 1], vb);
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            o[g][k][i] = __builtin_fmaf((float)vc.p[i & 3][i >> 2], ps, o[g][k][i]);
-        }
+        for (int g = 0; g < GC; ++g)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[g][k][i] = __builtin_fmaf(x[g][u], vv[i], o[g][k][i]);
       }
   };
 #pragma unroll 1
@@ -299,7 +297,6 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
           q[g][k][i] *= a.scale2;
           o[g][k][i] = 0.f;
         }
-        ob[g][k] = 0.f;
       }
       m[g] = -INFINITY;
       l[g] = 0.f;
@@ -338,7 +335,7 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
         for (int k = 0; k < W; ++k)
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            o[g][k][i] = __builtin_fmaf(o[g][k][i], kUnTiny[i & 1], ob[g][k]);
+            o[g][k][i] *= kUnTiny;
 #pragma unroll
         for (int s = LPR; s < kItem; s <<= 1) {
           const float mo = __shfl_xor(m[g], s, 64);

@@ -187,6 +187,33 @@ def test_infinite_logits_are_no_empty_row(cap, g):
     assert bool(((ones - 1).abs() <= (cap + 8) * U).all())  # a mean of ones
 
 
+@pytest.mark.parametrize("dim, group", [(64, 64), (40, 40), (96, 32), (128, 32), (24, 8), (256, 128)])
+@pytest.mark.parametrize("g", [1, 2, 3, 4, 6])
+@pytest.mark.parametrize("rows, cap", [(70, 15), (30, 200), (5, 600), (3, 3000), (600, 1000)])
+def test_values_of_zero_sum_to_zero(dim, group, g, rows, cap):
+    """32-bit outputs are sums of p * v with v = scale * code + base taken first: where every slot's v is
+    exactly 0 (here scale * 5 - 5 * scale), so is the sum, however large scale and base are.  The
+    scales are k / 8, k up to 25: 5 k has 7 bits, so bases are exact too."""
+    gen = torch.Generator().manual_seed(cap + g)
+    heads, pages = 2, max(cap, 64)
+    ng = dim // group
+    codes = torch.randint(0, 16, (pages, heads, 1, dim), generator=gen).to(torch.uint8)
+    codes[..., ::3] = 5
+    s = torch.randint(1, 26, (pages, heads, 1, ng), generator=gen) / 8
+    vs = torch.stack([s, -5 * s], -1).to(torch.bfloat16)
+    kc, ks = ref.quantise(torch.randn(pages, heads, 1, dim, generator=gen), group)
+    cache = dgs.classes.StateCache.wrap(ref.pack(kc).cuda(), ks.cuda(), ref.pack(codes).cuda(),
+                                        vs.cuda())
+    q = torch.randn(rows, heads * g, dim, generator=gen).cuda()
+    table = torch.randint(0, pages, (rows, cap), generator=gen).cuda()
+    lens = torch.randint(1, cap + 1, (rows,), generator=gen).cuda()
+    got = cache.attend(q, table, lens)
+    assert bool((got[..., ::3] == 0).all()), float(got[..., ::3].abs().max())
+    rest = torch.ones(dim, dtype=torch.bool)
+    rest[::3] = False
+    assert bool((got[..., rest.cuda()] != 0).any())
+
+
 def test_streams_keep_their_own_weights():
     gen = torch.Generator().manual_seed(0)
     cache = full_cache(256, 16, 2, 128, 64)
