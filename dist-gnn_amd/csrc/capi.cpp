@@ -711,6 +711,9 @@ StateView state_view(const dgs_state_cache *c) {
             "state cache: head_dim must be a multiple of 8 up to 256");
   DGS_CHECK(c->group > 0 && c->group % 8 == 0 && c->head_dim % c->group == 0,
             "state cache: group must be a multiple of 8 that divides head_dim");
+  // a slot's channels and groups are counted in 32 bits
+  DGS_CHECK((int64_t)c->heads * c->head_dim <= (int64_t(1) << 30),
+            "state cache: heads * head_dim must be at most 2^30");
   DGS_CHECK(c->k_codes && c->k_scales && c->v_codes && c->v_scales, "state cache: null buffer");
   DGS_CHECK((((uintptr_t)c->k_codes | (uintptr_t)c->k_scales | (uintptr_t)c->v_codes |
               (uintptr_t)c->v_scales) % 16) == 0,

@@ -133,6 +133,7 @@ class StateCache:
                  "head_dim must be a multiple of 8 up to 256")
         _require(group > 0 and group % 8 == 0 and head_dim % group == 0,
                  "group must be a multiple of 8 that divides head_dim")
+        _require(heads * head_dim <= 2 ** 30, "heads * head_dim must be at most 2^30")
 
     # read-only: the library holds their addresses
     k_codes = property(lambda self: self._buffers[0])
@@ -224,10 +225,10 @@ class StateCache:
         """Attention of q [rows, q_heads, head_dim] (one query token a row; q_heads a multiple of
         heads, neighbouring query heads share a head) over the first lens[i] slots of table row i
         -> [rows, q_heads, head_dim]; a row of length 0, or with all its pages outside the cache,
-        gives zeros.  scale: 1 / sqrt(head_dim) by default.  weights (float32 [rows, heads, >= pages * page_size], updated in place):
-        weights[i, h, j] = decay * weights[i, h, j] + the probabilities of head h's query heads,
-        for j < lens[i].  Several query tokens of one sequence are several rows with the same
-        table row, each with the length that it may see."""
+        gives zeros.  scale: 1 / sqrt(head_dim) by default.  weights (float32 [rows, heads, >= pages *
+        page_size], updated in place): weights[i, h, j] = decay * weights[i, h, j] + the probabilities
+        of head h's query heads, for j < lens[i].  Several query tokens of one sequence are several
+        rows with the same table row, each with the length that it may see."""
         if q.dim() != 3 or q.shape[2] != self.head_dim:
             raise RuntimeError(f"q must be [rows, q_heads, {self.head_dim}]")
         rows, q_heads = q.shape[0], q.shape[1]

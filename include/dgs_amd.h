@@ -337,10 +337,11 @@ int dgs_feature_server_destroy(dgs_feature_server *s);
  *   codes  uint8    [pages, heads, page_size, head_dim / 2]   two channels a byte, the even one low
  *   scales bfloat16 [pages, heads, page_size, head_dim / group, 2]   scale s, base b
  * value = s * code + b.  head_dim: a multiple of 8 up to 256; group: a multiple of 8 that divides
- * it.  The four buffers are contiguous, 16-byte aligned device memory.  A flat slot is
- * page * page_size + offset.  A page, slot or length outside the cache or its table is left out (or
- * clamped) by the kernel, and the next gather or state entry point (or dgs_check_async_errors)
- * raises.  No function here synchronises or allocates; all can be captured into a graph.
+ * it; heads * head_dim: at most 2^30.  The four buffers are contiguous, 16-byte aligned device
+ * memory.  A flat slot is page * page_size + offset.  A page, slot or length outside the cache or its
+ * table is left out (or clamped) by the kernel, and the next gather or state entry point (or
+ * dgs_check_async_errors) raises.  No function here synchronises or allocates; all can be captured
+ * into a graph.
  * ---------------------------------------------------------------------------------- */
 #define DGS_STATE_F32 0
 #define DGS_STATE_BF16 1
@@ -370,9 +371,10 @@ int dgs_state_read(const dgs_state_cache *c, const int64_t *slots, int64_t n, in
                    void *k_out, void *v_out, void *stream);
 /* out[i, a] = sum_j softmax_j(scale * q[i, a] . K[j, h]) V[j, h], j over the first lens[i] slots of
  * table row i, h = a / (q_heads / heads); lens[i] = 0 gives zeros, and so does a row all of whose
- * pages lie outside the cache (its weights only decay).  q [rows, q_heads, head_dim] with strides, out contiguous, both of `dtype`.  weights (float [rows, heads, weights_cols],
- * weights_cols >= width * page_size, or NULL): weights[i, h, j] = decay * weights[i, h, j] + the
- * sum of head h's query heads' probabilities, for j < lens[i]; decay 0 does not read them. */
+ * pages lie outside the cache (its weights only decay).  q [rows, q_heads, head_dim] with strides,
+ * out contiguous, both of `dtype`.  weights (float [rows, heads, weights_cols], weights_cols >= width
+ * * page_size, or NULL): weights[i, h, j] = decay * weights[i, h, j] + the sum of head h's query
+ * heads' probabilities, for j < lens[i]; decay 0 does not read them. */
 int dgs_state_attend_workspace(const dgs_state_cache *c, int64_t rows, int q_heads, int64_t width,
                                int with_weights, int dtype, int64_t *bytes);
 int dgs_state_attend(const dgs_state_cache *c, const void *q, int dtype, int64_t rows,
