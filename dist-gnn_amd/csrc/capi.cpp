@@ -743,6 +743,10 @@ IdArray id_array(const void *p, int bytes, const char *what) {
 void check_width(int64_t width, const char *what) {
   DGS_CHECK(width >= 0 && width < (int64_t(1) << 30), std::string(what) + ": bad table width");
 }
+// Whether two arrays share memory (their sizes fit 63 bits).
+bool share(const void *a, int64_t na, const void *b, int64_t nb) {
+  return a && b && (uintptr_t)a < (uintptr_t)b + (uint64_t)nb && (uintptr_t)b < (uintptr_t)a + (uint64_t)na;
+}
 void check_rows16(const void *p, int64_t s0, int64_t s1, StateType t, const char *what) {
   const int64_t e = t == kStateF32 ? 4 : 2;
   DGS_CHECK(p, std::string(what) + " is null");
@@ -899,10 +903,19 @@ int dgs_evict_rows(void *const *stores, const int64_t *row_bytes, int nstores, i
     if (rows == 0) return;
     e.lens = id_array(lens, lens_bytes, "lens");
     DGS_CHECK(lens_out, "evict: null lens_out");
+    DGS_CHECK(rows < (int64_t(1) << 31) && rows * heads < (int64_t(1) << 31) &&
+                  cols < (int64_t(1) << 30),
+              "evict: too many rows or columns");
+    // other workgroups of a row still read what one has written
+    DGS_CHECK(!share(lens, rows * lens_bytes, lens_out, rows * lens_bytes),
+              "evict: lens_out must be another array than lens");
     if (cols > 0) {
       if (width > 0) e.table = id_array(table, table_bytes, "table");
       DGS_CHECK(weights && weights_out && positions_out, "evict: null weights or positions");
-      DGS_CHECK(weights != weights_out && positions != positions_out,
+      const int64_t nb = rows * heads * cols * 4;
+      DGS_CHECK(!share(weights, nb, weights_out, nb) && !share(positions, nb, positions_out, nb) &&
+                    !share(weights, nb, positions_out, nb) && !share(positions, nb, weights_out, nb) &&
+                    !share(weights_out, nb, positions_out, nb),
                 "evict: the outputs must be other arrays than the inputs");
     }
     e.nstores = nstores;

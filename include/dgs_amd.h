@@ -388,8 +388,9 @@ int dgs_state_attend(const dgs_state_cache *c, const void *q, int dtype, int64_t
  * The i-th dropped slot below budget receives the row of the i-th kept slot at or past it, in every
  * store ([pages, heads, page_size, row_bytes] device memory, at most 8; in place).  weights (float)
  * and positions (int32 or NULL: position = slot) are [rows, heads, cols], cols >= width * page_size;
- * the *_out arrays (others than the inputs) receive them for the slots that stay, 0 and -1 behind;
- * lens_out (of lens' type) = min(n, budget).  Table rows must not share pages that move. */
+ * the *_out arrays (none may share memory with an input or another one) receive them for the slots
+ * that stay, 0 and -1 behind; lens_out (of lens' type, another array) = min(n, budget).  Table rows
+ * must not share pages that move. */
 int dgs_evict_workspace(int64_t rows, int heads, int64_t cols, int64_t budget, int64_t *bytes);
 int dgs_evict_rows(void *const *stores, const int64_t *row_bytes, int nstores, int64_t pages,
                    int heads, int64_t page_size, const float *weights, const int32_t *positions,

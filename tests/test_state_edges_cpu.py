@@ -25,3 +25,19 @@ def test_slots_of_too_many_channels_are_refused(heads, dim):
     last(lib.dgs_state_attend_workspace(ref, 1, heads, 1, 0, 0, ctypes.byref(n)), b"2^30")
     most = _CCache(4096, 4096, 4096, 4096, 1, 1, 2 ** 30 // dim, dim, dim)
     assert lib.dgs_state_read(ctypes.addressof(most), None, 0, 0, None, None, None) == 0
+
+
+def test_eviction_into_its_own_lengths_is_refused():
+    """The heads of a row read its length while the first of them writes the new one."""
+    rows, heads, cols = 2, 2, 64
+    for lens, bytes_, out in ((4096, 4, 4096), (4096, 8, 4096), (4096, 8, 4104), (4104, 4, 4100)):
+        last(lib.dgs_evict_rows(None, None, 0, 4, heads, 16, 1 << 20, None, 1 << 21, 1 << 22, rows, cols,
+                                1 << 23, 4, 4, lens, bytes_, out, 8, 0, 0, None, 0, None), b"lens_out")
+    many = rows * heads * cols * 4
+    w, p, wo, po = (1 << k for k in (20, 21, 22, 23))
+    for bad in ((w, p, w, po), (w, p, wo, p), (w, p, w + 4, po), (w, p, wo, p - many + 4), (w, p, wo, wo),
+                (w, p, p, po), (w, None, wo, w - 4), (w, p, wo, w)):
+        last(lib.dgs_evict_rows(None, None, 0, 4, heads, 16, *bad, rows, cols, 1 << 24, 4, 4, 4096, 4, 8192,
+                                8, 0, 0, None, 0, None), b"other arrays")
+    last(lib.dgs_evict_rows(None, None, 0, 4, 2 ** 30, 16, w, p, wo, po, 2, cols, 1 << 24, 4, 4, 4096, 4,
+                            8192, 8, 0, 0, None, 0, None), b"too many rows")
