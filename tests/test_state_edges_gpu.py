@@ -214,6 +214,34 @@ def test_values_of_zero_sum_to_zero(dim, group, g, rows, cap):
     assert bool((got[..., rest.cuda()] != 0).any())
 
 
+@pytest.mark.parametrize("page, cap", [(1, 48), (16, 48), (1, 2000), (16, 2000)])
+def test_large_queries_that_cancel(page, cap):
+    """The matrix form multiplies q by codes that stand 16 too high and takes the offset out again.  Two
+    channels of +-2^18 with equal codes lie in different products; q (16 + c) and its sums are whole
+    numbers below 2^24, the scale is a power of two and the base 0: every logit is exact, and the weights
+    are off by the softmax alone.  (An offset of 128 would make the logits off by 1 / 32.)"""
+    gen = torch.Generator().manual_seed(cap)
+    dim, slots = 64, 4096
+    codes = torch.randint(0, 16, (slots // page, 1, page, dim), generator=gen).to(torch.uint8)
+    codes[..., 63] = codes[..., 0]
+    ks = torch.tensor([1 / 64, 0.0]).to(torch.bfloat16).expand(slots // page, 1, page, 1, 2)
+    vc, vs = ref.quantise(torch.randn(slots // page, 1, page, dim, generator=gen), 64)
+    cache = dgs.classes.StateCache.wrap(ref.pack(codes).cuda(), ks.contiguous().cuda(),
+                                        ref.pack(vc).cuda(), vs.cuda())
+    q = torch.randint(-3, 4, (5, 4, dim), generator=gen).float()
+    q[..., 0], q[..., 63] = 2.0 ** 18, -2.0 ** 18
+    q = q.bfloat16().cuda()
+    table = torch.randint(0, slots // page, (5, cap // page), generator=gen).cuda()
+    lens = torch.tensor([cap, cap - 1, 33, 1, cap // 2]).cuda()
+    w = torch.zeros(5, 1, cap, device="cuda")
+    cache.attend(q, table, lens, scale=1.0, weights=w, decay=0.0)
+    _, prob, _, _, _ = ref.attend(q, cache, table, lens, 1.0)
+    largest = 62 * 3 * 15 / 64
+    rel = 2 * (2.0 ** -23 + 3 * U * (largest + 1) + 64 * U)
+    err = (w.cpu().double() - prob).abs()
+    assert bool((err <= rel * prob + 8 * U * prob).all()), float((err / prob.clamp(min=1e-30)).max())
+
+
 def test_streams_keep_their_own_weights():
     gen = torch.Generator().manual_seed(0)
     cache = full_cache(256, 16, 2, 128, 64)
