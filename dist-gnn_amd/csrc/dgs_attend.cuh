@@ -33,7 +33,7 @@ struct AttendArgs {
   int64_t weights_cols;
   float decay;
   void *out;
-  GatherGuard gd;
+  StateGuard gd;
 };
 
 // The matrix form for channel groups of 32, 64 or 128 and head_dim / group of 1, 2 or 4

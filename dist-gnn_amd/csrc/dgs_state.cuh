@@ -94,13 +94,15 @@ __device__ __forceinline__ void store8(void *p, int64_t elem, const float (&x)[8
   }
 }
 
-// Range guard of one state-cache launch.
-inline GatherGuard state_guard(int64_t kind, int64_t bound) {
-  GatherGuard g;
-  g.nrows = (uint64_t)bound;
+// Where a state-cache launch reports ids and lengths outside their bounds.
+struct StateGuard {
+  int64_t *err = nullptr;
+  int64_t tag = 0;
+};
+inline StateGuard state_guard() {
+  StateGuard g;
   g.err = async_err_dev();
   g.tag = (int64_t)async_err_next_tag();
-  g.kind = kind;
   return g;
 }
 

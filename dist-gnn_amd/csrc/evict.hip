@@ -36,7 +36,7 @@ struct EvictArgs {
   int64_t room;  // holes a (row, head) can have
   int32_t *moves;  // [rows * heads], the number of moves
   int32_t *holes, *movers;  // [rows * heads, room]
-  GatherGuard gd;
+  StateGuard gd;
 };
 
 // Inclusive sum over the lanes of a wave by lane moves: within rows of 16, then the rows' last lanes.
@@ -734,7 +734,7 @@ void evict_rows(const EvictCall &e, void *ws, int64_t ws_bytes, hipStream_t st) 
   EvictArgs a{};
   a.e = e;
   a.room = evict_room(e);
-  a.gd = state_guard(kAsyncErrSlot, e.pages);
+  a.gd = state_guard();
   if (few_moves(e)) {
     plan<true>(a, st);
     return;

@@ -773,7 +773,7 @@ void state_attend(const StateView &c, const AttendCall &call, void *ws, int64_t 
   a.weights_cols = call.weights_cols;
   a.decay = call.decay;
   a.out = call.out;
-  a.gd = state_guard(kAsyncErrSlot, c.pages);
+  a.gd = state_guard();
   if (p.matrix) {
     (c.group == 32 ? attend_matrix_32 : c.group == 64 ? attend_matrix_64 : attend_matrix_128)(
         a, p.waves, call.type, st);

@@ -76,7 +76,7 @@ struct WriteArgs {
   IdArray table, lens;
   int64_t width;
   int64_t *slots_out;
-  GatherGuard gd;
+  StateGuard gd;
 };
 
 // The flat slot of token t (-1: skipped; an id outside the cache is reported and skipped).
@@ -186,7 +186,7 @@ template <int TYPE>
 __global__ __launch_bounds__(kThreads) void k_state_read(StateView c, const int64_t *slots,
                                                          uint32_t pieces, FastDivU32 per_row,
                                                          FastDivU32 heads, void *out_k, void *out_v,
-                                                         GatherGuard gd) {
+                                                         StateGuard gd) {
   constexpr int kCh = TYPE == kStateF32 ? 4 : 8;
   const int kv = blockIdx.y, ng = c.dim / c.group;
   const uint8_t *codes = kv ? c.vc : c.kc;
@@ -289,7 +289,7 @@ void launch_write(WriteArgs a, StateType type, hipStream_t st) {
 }
 template <int TYPE>
 void launch_read(const StateView &c, const int64_t *slots, int64_t n, void *k_out, void *v_out,
-                 const GatherGuard &gd, hipStream_t st) {
+                 const StateGuard &gd, hipStream_t st) {
   constexpr int kCh = TYPE == kStateF32 ? 4 : 8;
   const uint32_t pieces = (uint32_t)(n * c.heads * (c.dim / kCh));
   const dim3 grid((unsigned)ceil_div(pieces, kThreads * kRU), 2);
@@ -307,7 +307,7 @@ void state_write(const StateView &c, const StateRows &x, StateType type, int64_t
   a.x = x;
   a.n = n;
   a.slots = slots;
-  a.gd = state_guard(kAsyncErrSlot, c.pages);
+  a.gd = state_guard();
   launch_write(a, type, st);
 }
 
@@ -322,14 +322,14 @@ void state_append(const StateView &c, const StateRows &x, StateType type, int64_
   a.lens = lens;
   a.width = width;
   a.slots_out = slots_out;
-  a.gd = state_guard(kAsyncErrSlot, c.pages);
+  a.gd = state_guard();
   launch_write(a, type, st);
 }
 
 void state_read(const StateView &c, const int64_t *slots, int64_t n, StateType type, void *k_out,
                 void *v_out, hipStream_t st) {
   if (n <= 0) return;
-  const GatherGuard gd = state_guard(kAsyncErrSlot, c.pages);
+  const StateGuard gd = state_guard();
   const int64_t step = tokens_a_launch(c);
   const int64_t row = (int64_t)c.heads * c.dim * (type == kStateF32 ? 4 : 2);
   for (int64_t t = 0; t < n; t += step) {
