@@ -461,6 +461,7 @@ uint64_t async_err_next_tag() {
   t_last_tag = async_err().tag.fetch_add(1) + 1;
   return t_last_tag;
 }
+uint64_t async_err_next_state_tag() { return async_err().tag.fetch_add(1) + 1; }
 uint64_t async_err_last_tag() { return t_last_tag; }
 
 void check_async_errors() {

@@ -102,7 +102,7 @@ struct StateGuard {
 inline StateGuard state_guard() {
   StateGuard g;
   g.err = async_err_dev();
-  g.tag = (int64_t)async_err_next_tag();
+  g.tag = (int64_t)async_err_next_state_tag();
   return g;
 }
 

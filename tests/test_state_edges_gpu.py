@@ -263,3 +263,22 @@ def test_streams_keep_their_own_weights():
                     cache.attend(q, table, lens, weights=w, decay=0.5)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_the_last_gather_is_no_state_call():
+    """A loader tells its batches by the tag of this thread's last gather."""
+    cache = full_cache(8, 16, 2, 64, 64)
+    dgs.ops._CAPI_cuda_index_select(torch.arange(8.0).cuda().view(8, 1), torch.tensor([3]).cuda())
+    tag = dgs.ops._last_gather_tag()
+    assert tag > 0
+    slots = torch.arange(4).cuda()
+    k, v = cache.read(slots)
+    cache.write(k, v, slots)
+    table = torch.arange(8).view(1, 8).cuda()
+    cache.append(k[:1], v[:1], table, slots[:1])
+    w = torch.zeros(1, 2, 128, device="cuda")
+    cache.attend(k[:1], table, slots[1:2], weights=w)
+    cache.evict(w, None, table, slots[3:], 2)
+    assert dgs.ops._last_gather_tag() == tag
+    dgs.ops._CAPI_cuda_index_select(torch.arange(8.0).cuda().view(8, 1), torch.tensor([3]).cuda())
+    assert dgs.ops._last_gather_tag() > tag
