@@ -59,20 +59,24 @@ __device__ __forceinline__ int64_t row_length(const AttendArgs &a, int64_t row, 
   return len;
 }
 
-// Whether every page of a row's first `len` slots lies outside the cache, where a sum of probabilities
-// is 0: only then it is inverted to 0, so that the output is zeros and the weights get nothing (logits
-// that are all -infinity give NaN, as the formula does).  The lanes of a wave look together, or each for
-// itself (kTogether = 1, rows of a few slots).
+// A sum of probabilities is 0 where no slot is left, because every page lies outside the cache: the
+// output is zeros then and the weights get nothing.  It is 0 too where every logit is -infinity, which
+// has no softmax (NaN).  The maximum tells them apart: -infinity where no slot is left, kNoSoftmax,
+// which every finite logit passes by far, where there is one.
+constexpr float kNoSoftmax = -3.4028235e38f;
+__device__ __forceinline__ float inverse_sum(float m, float l) { return m == -INFINITY ? 0.f : 1.f / l; }
+// Whether one of the slots [first, last) of a row lies in the cache.  The lanes of a wave look together,
+// or each for itself (kTogether = 1, rows of a few slots).
 template <int kTogether>
-__device__ __forceinline__ bool none_left(const AttendArgs &a, int64_t row, int64_t len) {
-  const int64_t n = (len + (int64_t(1) << a.c.pshift) - 1) >> a.c.pshift;
+__device__ __forceinline__ bool some_left(const AttendArgs &a, int64_t row, int first, int last) {
+  const int end = (int)((last + (int64_t(1) << a.c.pshift) - 1) >> a.c.pshift);
 #pragma unroll 1
-  for (int64_t p0 = 0; p0 < n; p0 += kTogether) {
-    const int64_t p = p0 + (kTogether > 1 ? threadIdx.x & 63 : 0);
-    const bool in = p < n && (uint64_t)a.table[row * a.width + p] < (uint64_t)a.c.pages;
-    if (kTogether > 1 ? __any(in) : in) return false;
+  for (int p0 = first >> a.c.pshift; p0 < end; p0 += kTogether) {
+    const int p = p0 + (kTogether > 1 ? (int)(threadIdx.x & 63) : 0);
+    const bool in = p < end && (uint64_t)a.table[row * a.width + p] < (uint64_t)a.c.pages;
+    if (kTogether > 1 ? __any(in) : in) return true;
   }
-  return true;
+  return false;
 }
 
 __device__ __forceinline__ void store_out(int type, void *out, int64_t elem, const float (&x)[8]) {
@@ -711,8 +715,8 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
         const bool whole = run.tile == 0 && last == len;
         l = over_columns(l);
         const int64_t part = (run.row * pairs + run.pair + blockIdx.x * waves + wave) * gs + n;
-        float inv = 1.f;
-        if (whole) inv = __any(l == 0.f) && none_left<64>(a, run.row, len) ? 0.f : 1.f / l;
+        if (__any(l == 0.f) && some_left<64>(a, run.row, j1, last)) m = l == 0.f ? kNoSoftmax : m;
+        const float inv = whole ? inverse_sum(m, l) : 1.f;
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
           const float c = over_columns(cb[g]);
@@ -747,6 +751,7 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
   __syncthreads();  // the corners become the joining area:
   // [waves][16] maxima, [waves][16] sums, [waves][gn][kD] outputs
   l = over_columns(l);
+  if (j1 < last && __any(l == 0.f) && some_left<64>(a, run.row, 0, len)) m = l == 0.f ? kNoSoftmax : m;
   float *s_m = s_mem, *s_l = s_mem + waves * 16, *s_o = s_mem + waves * 32;
   if (q4 == 0) s_m[wave * 16 + n] = m;
   __syncthreads();
@@ -766,30 +771,21 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
     }
   }
   __syncthreads();
-  bool none = len == 0;
-  if (!none) {
-    float ls = 0.f;
-    for (int w = 0; w < waves; ++w) ls += s_l[w * 16 + n];
-    if (__any(ls == 0.f)) none = none_left<64>(a, run.row, len);
-  }
   for (int i = threadIdx.x; i < gn * (kD / 8); i += blockDim.x) {
     const int hd = i / (kD / 8), ch = (i % (kD / 8)) * 8;
-    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, ls = 0.f;
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, ls = 0.f, mm = -INFINITY;
     for (int w = 0; w < waves; ++w) {
+      mm = fmaxf(mm, s_m[w * 16 + hd]);
       ls += s_l[w * 16 + hd];
       const float *src = s_o + (w * gn + hd) * kD + ch;
 #pragma unroll
       for (int y = 0; y < 8; ++y) acc[y] += src[y];
     }
-    const float inv = none ? 0.f : 1.f / ls;
+    const float inv = inverse_sum(mm, ls);
 #pragma unroll
     for (int y = 0; y < 8; ++y) acc[y] *= inv;
     store_out(type, a.out, (qh0 + hd) * kD + ch, acc);
-    if (a.part_ml && ch == 0) {
-      float mm = -INFINITY;
-      for (int w = 0; w < waves; ++w) mm = fmaxf(mm, s_m[w * 16 + hd]);
-      a.part_ml[(run.row * pairs + run.pair) * gs + hd] = make_float2(mm, ls);
-    }
+    if (a.part_ml && ch == 0) a.part_ml[(run.row * pairs + run.pair) * gs + hd] = make_float2(mm, ls);
   }
   if (!a.logits || a.part_ml) return;
   // The row and all its query heads are this workgroup's: it adds the weights from the logits
@@ -804,7 +800,7 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
         ls += s_l[w * 16 + g];
       }
     mh[g] = g < gn ? (mm == -INFINITY ? 0.f : mm) : INFINITY;  // no head: exp2(-inf) * 0
-    ih[g] = g < gn && !none ? 1.f / ls : 0.f;
+    ih[g] = g < gn ? inverse_sum(mm, ls) : 0.f;
   }
   const float *lg = a.logits + qh0 * a.cap;
   float *wr = a.weights + (run.row * a.c.heads + h) * a.weights_cols;

@@ -324,11 +324,11 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
     // a pair that a wave of the stream form holds whole is finished here
     const bool whole = STREAM ? first == 0 && last == len : a.splits == 1;
     if (!STREAM || first < last) {
-      bool none = false;  // some query head has no slot left
+      bool zero = false;  // a query head's sum is 0
 #pragma unroll
       for (int g = 0; g < GC; ++g)
-        if (g < gn) none |= SL == 1 ? l[g] == 0.f : __all(l[g] == 0.f);
-      if (whole && none) none = none_left<SL == 1 ? 1 : 64>(a, row, len);
+        if (g < gn) zero |= SL == 1 ? l[g] == 0.f : __all(l[g] == 0.f);
+      if (zero) zero = some_left<SL == 1 ? 1 : 64>(a, row, first, last);
 #pragma unroll
       for (int g = 0; g < GC; ++g) {
 #pragma unroll
@@ -349,11 +349,12 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
             for (int i = 0; i < 8; ++i)
               o[g][k][i] = o[g][k][i] * f + __shfl_xor(o[g][k][i], s, 64) * fo;
         }
+        if (zero && l[g] == 0.f) m[g] = kNoSoftmax;
         if (g >= gn || sl != 0) continue;
         const int64_t qh = row * a.q_heads + a0 + g;
         const int64_t part = STREAM ? (row * run.pairs + run.pair + item) * (a.g < GC ? a.g : GC) + g
                                     : qh * a.splits + split;
-        const float inv = none ? 0.f : 1.f / l[g];
+        const float inv = inverse_sum(m[g], l[g]);
 #pragma unroll
         for (int k = 0; k < W; ++k) {
           if (!live[k]) continue;
@@ -432,12 +433,11 @@ __device__ __forceinline__ Parts parts_of(const AttendArgs &a, int64_t row, int 
   }
   return Parts{part * gs + n % t, gs, parts};
 }
-// The maximum and 1 / sum of kG query heads of a row over their parts (head g's `step` g behind), on
-// every lane of the wave; heads at or past g_end repeat the first.  64 / kG lanes take a head's parts.
+// The maximum and 1 / sum of kG query heads over their parts (head g's `step` g behind), on every
+// lane of the wave; heads at or past g_end repeat the first.  64 / kG lanes take a head's parts.
 template <int kG>
-__device__ __forceinline__ void join_ml(const AttendArgs &a, int64_t row, int64_t len,
-                                        const Parts &p, int64_t step, int g_end,
-                                        float2 (&out)[kG]) {
+__device__ __forceinline__ void join_ml(const AttendArgs &a, const Parts &p, int64_t step,
+                                        int g_end, float2 (&out)[kG]) {
   constexpr int kL = 64 / kG;
   const int lane = threadIdx.x & 63, g = lane / kL, s0 = lane % kL;
   const float2 *ml = a.part_ml + p.part + (g < g_end ? g * step : 0);
@@ -446,7 +446,8 @@ __device__ __forceinline__ void join_ml(const AttendArgs &a, int64_t row, int64_
   for (int s = s0 + kL; s < p.n; s += kL) m = fmaxf(m, ml[(int64_t)s * p.stride].x);
 #pragma unroll
   for (int o = 1; o < kL; o <<= 1) m = fmaxf(m, over(m, o));
-  m = m == -INFINITY ? 0.f : m;
+  const bool none = m == -INFINITY;
+  m = none ? 0.f : m;
   float l = own.y * __builtin_amdgcn_exp2f(own.x - m);
   for (int s = s0 + kL; s < p.n; s += kL) {
     const float2 x = ml[(int64_t)s * p.stride];
@@ -454,7 +455,7 @@ __device__ __forceinline__ void join_ml(const AttendArgs &a, int64_t row, int64_
   }
 #pragma unroll
   for (int o = 1; o < kL; o <<= 1) l += over(l, o);
-  l = __any(l == 0.f) && none_left<64>(a, row, len) ? 0.f : 1.f / l;
+  l = none ? 0.f : 1.f / l;
 #pragma unroll
   for (int k = 0; k < kG; ++k)
     out[k] = make_float2(
@@ -469,7 +470,7 @@ __device__ __forceinline__ void join_ml(const AttendArgs &a, int64_t row, int64_
 // lengths, parts and maxima, loads that wait for each other; without weights 6 us.
 constexpr int kSpan = 1024;
 template <int TYPE>
-__global__ __launch_bounds__(kThreads, 4) void k_attend_finish(AttendArgs a, int64_t outs, int lpr,
+__global__ __launch_bounds__(kThreads) void k_attend_finish(AttendArgs a, int64_t outs, int lpr,
                                                             int spans, int64_t waves) {
   const int64_t id = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
   if (id >= waves) return;
@@ -485,7 +486,7 @@ __global__ __launch_bounds__(kThreads, 4) void k_attend_finish(AttendArgs a, int
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (len > 0) {
       float2 joined[1];
-      join_ml<1>(a, row, len, p, 0, 1, joined);
+      join_ml<1>(a, p, 0, 1, joined);
       const float2 ml = joined[0];
       if (w < words)
         for (int s0 = part; s0 < p.n; s0 += 4 * parts) {  // four parts in flight
@@ -534,7 +535,7 @@ __global__ __launch_bounds__(kThreads, 4) void k_attend_finish(AttendArgs a, int
     if (a.splits || (g0 > 0 && g0 % a.together == 0)) p = parts_of(a, row, head0 + g0, len);
     const Parts pg{p.part + (a.splits ? 0 : g0 % a.together), p.stride, p.n};
     float2 ml[kG];
-    join_ml<kG>(a, row, len, pg, a.splits ? a.splits : 1, a.g - g0, ml);
+    join_ml<kG>(a, pg, a.splits ? a.splits : 1, a.g - g0, ml);
 #pragma unroll
     for (int r = 0; r < kRuns; ++r) {
       if (j0 + r * kI * 64 >= len) break;
