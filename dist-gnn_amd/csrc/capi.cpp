@@ -843,6 +843,7 @@ int dgs_state_attend(const dgs_state_cache *c, const void *q, int dtype, int64_t
     DGS_CHECK((width << view.pshift) < (int64_t(1) << 30), "attend: rows of 2^30 slots");
     DGS_CHECK(q_heads > 0 && q_heads % view.heads == 0,
               "attend: q_heads must be a multiple of the cache's heads");
+    DGS_CHECK(scale > -0x1p100 && scale < 0x1p100, "attend: scale must lie between -2^100 and 2^100");
     if (rows == 0) return;
     check_rows16(q, q_row, q_head, a.type, "q");
     check_rows16(out, 0, 0, a.type, "out");

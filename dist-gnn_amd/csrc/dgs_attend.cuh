@@ -15,7 +15,7 @@ struct AttendArgs {
   int q_heads, g;  // g = query heads per head
   IdArray table, lens;
   int64_t width;
-  float scale2;  // scale * log2 e
+  float scale2;  // scale * log2 e, below 2^101
   // How the work is cut.  A "pair" is a row and up to `together` query heads of one head (matrix form
   // 16, vector form 4).  With `stream` waves, the pairs' tiles of 2^shift slots lie in a line that is
   // cut evenly over the waves; else the matrix form takes a workgroup a pair and the vector form
@@ -208,10 +208,11 @@ constexpr int kMatrixShift = 5, kMatrixCost = 6, kMatrixLeast = 4;
 //    mask-or a pair.  V's become 0x4300 | c = 128 + c, which spares one shift in four; the offset's sums,
 //    and their rounding, are 8 times as large, which K cannot have: the attention weights of 16-bit
 //    queries would be off by 4e-7 instead of 6e-8 (V's go into a 16-bit output).
-//  - x = K q: rows are slots, columns query heads, k channels; one product chain per channel group,
-//    r_g = sum 16 q (16 + c) / 16.  Then x = sum_g s_g r_g + sum_g (b_g - 16 s_g) Q_g with Q_g = sum q over
+//  - x = K q / 16: rows are slots, columns query heads, k channels; one product chain per channel group,
+//    r_g = sum q (16 + c) / 16.  Then x = sum_g s_g r_g + sum_g (b_g / 16 - s_g) Q_g with Q_g = sum q over
 //    the group; the second sum is one more product whose slot operand is the stored (s, b) words
-//    themselves and whose other operand holds -16 Q_g and Q_g in three bfloat16 terms (24 bits).
+//    themselves and whose other operand holds -Q_g and Q_g / 16 in three bfloat16 terms (24 bits).  The
+//    scale follows the sums, so that large queries only overflow where their sums do.
 //  - The result leaves eight slots of a query head in a lane, of which only GR = 4, 8 or 16 columns
 //    are query heads.  With fewer than 16, the other columns' lanes take over their share of the
 //    slots (lane 4 b + h of a row of 16 takes slots 2 b and 2 b + 1 of head h), with one lane move
@@ -350,7 +351,7 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
   int last = STREAM ? run.last(kMatrixShift, kMatrixCost) : len;
   // logits grow with x: a negative scale is taken into q, and so is 0 (masked slots are -inf)
   const float sign = a.scale2 < 0.f ? -1.f : (a.scale2 == 0.f ? 0.f : 1.f);
-  const float scale2 = a.scale2 == 0.f ? 1.f : fabsf(a.scale2);
+  const float scale2 = a.scale2 == 0.f ? 1.f : 16.f * fabsf(a.scale2);
   uint32_t magic_k = 0x3f803f80u, magic_v = 0x43004300u;
   asm volatile("" : "+v"(magic_k), "+v"(magic_v));
 
@@ -664,7 +665,6 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
       for (int i = 0; i < 8; ++i) {
         x[i] *= sign;
         qsum[c / kGC] += x[i];
-        x[i] *= 16.f;
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -675,7 +675,7 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
                                     x[4 + i] - __uint_as_float(hi & 0xffff0000u));
       }
     }
-    // quarter 0 holds the first bfloat16 terms of (-16 Q_g, Q_g), 1 the second, 2 the third
+    // quarter 0 holds the first bfloat16 terms of (-Q_g, Q_g / 16), 1 the second, 2 the third
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       qm.u[g] = 0;
@@ -686,7 +686,7 @@ __global__ __launch_bounds__(NG * GROUP == 256 ? 256 : 512, NG * GROUP == 256 ? 
         const float t0 = (float)(__bf16)s, t1 = (float)(__bf16)(s - t0);
         const float t2 = (s - t0) - t1;
         const float t = q4 == 0 ? t0 : (q4 == 1 ? t1 : (q4 == 2 ? t2 : 0.f));
-        qm.u[g] = pack_bf16(-16.f * t, t);
+        qm.u[g] = pack_bf16(-t, t * 0.0625f);
       }
     }
 

@@ -4,7 +4,7 @@
 // query head a reads the K and V rows of head a / G, G = q_heads / heads:
 //   x_j = scale * q . k_j,  p_j = exp(x_j - max x) / sum exp(x - max x),  out = sum_j p_j v_j.
 // One pass over the slots with the running maximum m and sum l of the softmax, in 32 bits and
-// base 2 (scale * log2 e goes into q).  Long rows are split into chunks of slots whose (m, l,
+// base 2 (scale * log2 e follows q . k).  Long rows are split into chunks of slots whose (m, l,
 // sum p v) go through the workspace; the finishing kernel joins them.  When the caller keeps
 // attention weights, the logits of every slot go through the workspace too and the finishing
 // kernel adds the G heads' probabilities in head order: no atomics, so results do not vary.
@@ -118,6 +118,7 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
   }
   const int words = a.c.dim >> 3;
   const int ng = a.c.dim / a.c.group;
+  const float scale = a.scale2 * kUnTiny;  // of the sums, after them: only those can overflow
   bool live[W];
   int w[W], grp[W];  // my words of a row, and their groups
 #pragma unroll
@@ -218,7 +219,7 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
       }
 #pragma unroll
       for (int g = 0; g < GC; ++g) {
-        const float x0 = sum_lanes<LPR>(s[g]) * kUnTiny;
+        const float x0 = sum_lanes<LPR>(s[g]) * scale;
         x[g][u] = ok ? x0 : -INFINITY;
       }
     }
@@ -294,7 +295,6 @@ __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          q[g][k][i] *= a.scale2;
           o[g][k][i] = 0.f;
         }
       }

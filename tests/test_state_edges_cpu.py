@@ -41,3 +41,10 @@ def test_eviction_into_its_own_lengths_is_refused():
                                 8, 0, 0, None, 0, None), b"other arrays")
     last(lib.dgs_evict_rows(None, None, 0, 4, 2 ** 30, 16, w, p, wo, po, 2, cols, 1 << 24, 4, 4, 4096, 4,
                             8192, 8, 0, 0, None, 0, None), b"too many rows")
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 100, -2.0 ** 100, 1e300, float("inf"), float("nan")])
+def test_scales_past_the_sums_range_are_refused(scale):
+    c = _CCache(4096, 4096, 4096, 4096, 4, 8, 2, 64, 32)
+    last(lib.dgs_state_attend(ctypes.addressof(c), 4096, 0, 1, 2, 128, 64, 4096, 4, 1, 4096, 4, scale, None,
+                              0, 1.0, 4096, None, 0, None), b"scale")

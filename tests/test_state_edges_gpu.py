@@ -187,6 +187,42 @@ def test_infinite_logits_are_no_empty_row(cap, g):
     assert bool(((ones - 1).abs() <= (cap + 8) * U).all())  # a mean of ones
 
 
+@pytest.mark.parametrize("page", [1, 16])
+@pytest.mark.parametrize("cap", [16, 256, 2048, 40000])
+@pytest.mark.parametrize("g", [1, 3])
+def test_infinite_logits_beside_finite_ones(page, cap, g):
+    """Slots whose logits overflow to -infinity, slots on pages outside and slots of logit 0, in runs that
+    different parts of a row take: the last share the row evenly."""
+    dim, pages = 64, 64
+    half = pages // 2  # pages of keys of 1, then of 0
+    codes = torch.full((pages, 1, page, dim // 2), 0x11, dtype=torch.uint8)
+    codes[half:] = 0
+    scales = torch.tensor([1.0, 0.0]).to(torch.bfloat16).expand(pages, 1, page, 1, 2).contiguous()
+    cache = dgs.classes.StateCache.wrap(codes.cuda(), scales.cuda(), codes.flip(0).contiguous().cuda(),
+                                        scales.clone().cuda())  # values of 0, then of 1
+    width = cap // page
+    table = torch.zeros(4, width, dtype=torch.int64)
+    table[0] = torch.where(torch.arange(width) >= width - max(1, width // 4), half, 0)  # finite at the end
+    table[1, 0], table[1, 1:], table[1, width // 2:] = half + 1, 3, pages  # and at the front, bad ones behind
+    table[2] = torch.where(torch.arange(width) < width - 1, pages, 1)  # only -infinity is left
+    table[3] = pages
+    q = torch.full((4, g, dim), -3e38, device="cuda")
+    w = torch.zeros(4, 1, cap, device="cuda")
+    lens = torch.full((4,), cap).cuda()
+    if width == 1:
+        table[1, 0] = half + 1
+    got = cache.attend(q, table.cuda(), lens, scale=1.0, weights=w)
+    raises_next("page or slot")
+    share = (table[:2] >= half) & (table[:2] < pages)
+    prob = share.repeat_interleave(page, 1).double()
+    prob = g * prob / prob.sum(1, keepdim=True)
+    # sums of cap equal terms and of their parts
+    assert bool(((w[:2, 0].cpu().double() - prob).abs() <= 8 * (cap + 8) * U * prob).all())
+    assert bool(((got[:2].cpu().double() - 1).abs() <= 8 * (cap + 8) * U).all())
+    assert bool(got[2].isnan().all()) and bool(w[2].isnan().all())
+    assert not got[3].any() and not w[3].any()
+
+
 @pytest.mark.parametrize("dim, group", [(64, 64), (40, 40), (96, 32), (128, 32), (24, 8), (256, 128)])
 @pytest.mark.parametrize("g", [1, 2, 3, 4, 6])
 @pytest.mark.parametrize("rows, cap", [(70, 15), (30, 200), (5, 600), (3, 3000), (600, 1000)])
@@ -240,6 +276,36 @@ def test_large_queries_that_cancel(page, cap):
     rel = 2 * (2.0 ** -23 + 3 * U * (largest + 1) + 64 * U)
     err = (w.cpu().double() - prob).abs()
     assert bool((err <= rel * prob + 8 * U * prob).all()), float((err / prob.clamp(min=1e-30)).max())
+
+
+@pytest.mark.parametrize("dtype, top", [("f32", 3e38), ("bf16", 3e38), ("f16", 65504.0)])
+@pytest.mark.parametrize("page, cap", [(1, 16), (16, 64), (16, 2048)])
+def test_queries_near_the_types_largest_value(dtype, top, page, cap):
+    """A query of +-top in two channels whose keys are alike cancels; the scale makes a small factor of
+    what a third adds: logits of top * scale * code, which is 1 / 4 * code."""
+    gen = torch.Generator().manual_seed(cap)
+    dim, pages = 64, 4096 // page
+    codes = torch.zeros(pages, 1, page, dim, dtype=torch.uint8)
+    codes[..., 5] = torch.randint(0, 16, (pages, 1, page), generator=gen).to(torch.uint8)
+    ks = torch.tensor([1.0, 0.0]).to(torch.bfloat16).expand(pages, 1, page, 1, 2).contiguous()
+    vc, vs = ref.quantise(torch.randn(pages, 1, page, dim, generator=gen), 64)
+    cache = dgs.classes.StateCache.wrap(ref.pack(codes).cuda(), ks.cuda(), ref.pack(vc).cuda(), vs.cuda())
+    big = torch.tensor(top).to(TYPES[dtype])
+    q = torch.zeros(2, 2, dim, dtype=TYPES[dtype])
+    q[..., 5], q[:, 1, 9] = big / 16, -big / 16  # sums of codes up to 15 stay in range
+    if dtype != "bf16":
+        q[0, 0, 5] = big if dtype == "f16" else big / 16
+    table = torch.randint(0, pages, (2, cap // page), generator=gen)
+    lens = torch.tensor([cap, cap // 2 + 1])
+    scale = 4 / float(big)  # logits of up to 15 * 4 (f16: 64)
+    w = torch.zeros(2, 1, cap, device="cuda")
+    out, prob, size, steps, vmax = ref.attend(q, cache, table, lens, scale)
+    got = cache.attend(q.cuda(), table.cuda(), lens.cuda(), scale=scale, weights=w)
+    rel = prob_error(dim, size, steps, dtype == "f32")
+    off = (2 * rel * vmax)[..., None]
+    tol = off + torch.finfo(q.dtype).eps / 2 * (out.abs() + off) + (2.0 ** -25 if dtype == "f16" else 0)
+    assert bool(((got.cpu().double() - out).abs() <= tol).all())
+    assert bool(((w.cpu().double() - prob).abs() <= 2 * rel.amax(1)[:, None, None] * prob + 8 * U).all())
 
 
 def test_streams_keep_their_own_weights():
