@@ -747,6 +747,9 @@ void check_width(int64_t width, const char *what) {
 bool share(const void *a, int64_t na, const void *b, int64_t nb) {
   return a && b && (uintptr_t)a < (uintptr_t)b + (uint64_t)nb && (uintptr_t)b < (uintptr_t)a + (uint64_t)na;
 }
+void check_workspace(const void *p, const char *what) {
+  DGS_CHECK((uintptr_t)p % 16 == 0, std::string(what) + ": the workspace must be 16-byte aligned");
+}
 void check_rows16(const void *p, int64_t s0, int64_t s1, StateType t, const char *what) {
   const int64_t e = t == kStateF32 ? 4 : 2;
   DGS_CHECK(p, std::string(what) + " is null");
@@ -862,6 +865,7 @@ int dgs_state_attend(const dgs_state_cache *c, const void *q, int dtype, int64_t
     a.weights_cols = weights_cols;
     a.decay = (float)decay;
     a.out = out;
+    check_workspace(workspace, "attend");
     check_async_errors();
     state_attend(view, a, workspace, workspace_bytes, S(stream));
   });
@@ -938,6 +942,7 @@ int dgs_evict_rows(void *const *stores, const int64_t *row_bytes, int nstores, i
     e.budget = budget;
     e.sinks = sinks;
     e.recent = recent;
+    check_workspace(workspace, "evict");
     check_async_errors();
     evict_rows(e, workspace, workspace_bytes, S(stream));
   });

@@ -340,8 +340,9 @@ int dgs_feature_server_destroy(dgs_feature_server *s);
  * it; heads * head_dim: at most 2^30.  The four buffers are contiguous, 16-byte aligned device
  * memory.  A flat slot is page * page_size + offset.  A page, slot or length outside the cache or its
  * table is left out (or clamped) by the kernel, and the next gather or state entry point (or
- * dgs_check_async_errors) raises.  No function here synchronises or allocates; all can be captured
- * into a graph.
+ * dgs_check_async_errors) raises.  Workspaces are 16-byte aligned device memory of the size that the
+ * *_workspace function gives.  No function here synchronises or allocates; all can be captured into a
+ * graph.
  * ---------------------------------------------------------------------------------- */
 #define DGS_STATE_F32 0
 #define DGS_STATE_BF16 1

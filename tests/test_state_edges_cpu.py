@@ -48,3 +48,13 @@ def test_scales_past_the_sums_range_are_refused(scale):
     c = _CCache(4096, 4096, 4096, 4096, 4, 8, 2, 64, 32)
     last(lib.dgs_state_attend(ctypes.addressof(c), 4096, 0, 1, 2, 128, 64, 4096, 4, 1, 4096, 4, scale, None,
                               0, 1.0, 4096, None, 0, None), b"scale")
+
+
+@pytest.mark.parametrize("off", [1, 4, 8])
+def test_misaligned_workspaces_are_refused(off):
+    """Parts are stored 16 bytes at a time."""
+    c = _CCache(4096, 4096, 4096, 4096, 4, 8, 2, 64, 32)
+    last(lib.dgs_state_attend(ctypes.addressof(c), 4096, 0, 1, 2, 128, 64, 4096, 4, 1000, 4096, 4, 1.0, None,
+                              0, 1.0, 4096, 8192 + off, 1 << 30, None), b"attend: the workspace")
+    last(lib.dgs_evict_rows(None, None, 0, 4, 2, 16, 1 << 20, None, 1 << 21, 1 << 22, 2, 2000, 1 << 24, 4, 4,
+                            4096, 4, 8192, 300, 0, 0, 16384 + off, 1 << 30, None), b"evict: the workspace")
