@@ -197,7 +197,7 @@ struct Run {
 };
 // Matrix form: tiles of 32 slots, and 6 units for a pair (three loads that wait for each other, the
 // query, the write of its part: as long as some tiles.  64 rows of 1 to 8192 slots with weights:
-// 112 us without, 91 us at 2 units, 77 at 4, 76 at 6 and 8).
+// 98 us without, 78 us at 2 units, 63 to 65 at 4, 6 and 8).
 constexpr int kMatrixShift = 5, kMatrixCost = 6, kMatrixLeast = 4;
 
 // Matrix form, for 16-bit queries.  One wave takes up to 16 query heads of a head (the columns left
@@ -221,8 +221,10 @@ constexpr int kMatrixShift = 5, kMatrixCost = 6, kMatrixLeast = 4;
 //    heads, k slots (which slot counts as which k is free, so the layout of x is the layout of p).
 //    a_g = p s_g is rounded to two bfloat16 terms (17 bits: one term's 2^-9 would show in the
 //    output), and the 128 sum a_g that the codes' offset adds is taken out with the same rounded
-//    terms, through a product with a constant operand.  sum p b_g is summed in 32 bits.  The pairs
-//    of slots that a register of V holds are made with v_perm_b32.
+//    terms, through a product with a constant operand.  sum p b_g is summed in 32 bits and added at the
+//    end: an output is off by up to 2^-17 of its group's largest value, which 16 bits hide except where
+//    values cancel (32-bit queries take the vector form).  The pairs of slots that a register of V holds
+//    are made with v_perm_b32.
 //  - m only follows the maximum when a logit passes it by 8 (in base 2): p stays below 2^8, and
 //    the rescaling is a rare branch.
 //  - Rows come in 16 bytes a lane, two tiles ahead in registers, and pass through the wave's own

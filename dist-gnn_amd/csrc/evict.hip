@@ -12,9 +12,9 @@
 // and stay in registers as keys (32 bits, larger is better; rows past 32768 slots read them again
 // each time); the budget-th best key by counting digits; then ties, holes and movers are numbered
 // in slot order by scans over lanes and waves.  What lies below the budget is copied as it passes and the
-// holes are overwritten afterwards.  16 rows of 8 heads of 20000 to 32768 slots to 4096: 35 us, of which
-// 13 read and write the arrays and 8 count digits; a workgroup a (row, head) leaves half of the card
-// idle there.
+// holes are overwritten afterwards.  16 rows of 8 heads of 20000 to 32768 slots to 4096: 34 us, more than half
+// of which its waves wait (profiles/state_cache_counters.txt); a workgroup a (row, head) leaves half of the
+// card idle there.
 // The moves are a kernel of their own, over all stores; where there can only be a few (a cache
 // that takes single tokens) the plan's workgroup does them.
 #include "dgs_block.cuh"

@@ -80,9 +80,9 @@ __device__ __forceinline__ uint32_t of_quad(uint32_t x, int u) {
 // matrix form, the running maximum is only followed when a logit passes it by 8.
 // SL = 1 is for rows of at most 16 slots: no join, and with all query heads of a head in the item
 // the probabilities stay in registers and the item writes its weights itself.
-// Bound by the vector instructions: 10 million of a wave in the 22.6 us of 16 rows of 8 heads (128
-// channels, 32-bit, 1 to 8192 slots) keep the SIMDs busy for 17; the sampled neighbours' rows (40960
-// rows of 0 to 15 slots, 4 heads of 32 channels) take 32 us, 21 of them in instructions.
+// Bound by the vector instructions (profiles/state_cache_counters.txt): 16 rows of 8 heads (128 channels,
+// 32-bit, 1 to 8192 slots) 9.6 million of a wave, which keep the SIMDs busy for 15.6 of 23.6 us; the
+// sampled neighbours' rows (40960 rows of 0 to 15 slots, 4 heads of 32 channels) 13.4 million, 21.7 of 32.4.
 template <int LPR, int W, int SL, int GC, bool QG, bool STREAM>
 __global__ __launch_bounds__(kThreads) void k_attend_vec(AttendArgs a, int type,
                                                          FastDivU32 splits, FastDivU32 gchunks,
@@ -466,8 +466,8 @@ __device__ __forceinline__ void join_ml(const AttendArgs &a, const Parts &p, int
 // Joins the parts of the rows' query heads and adds the weights; every wave works alone.  The
 // first `outs` waves take 8 `lpr` channels of a query head's output each (eight channels a lane, the
 // lanes' groups taking every n-th part), the others 1024 slots of a (row, head)'s weights.  64 rows of
-// 8 heads, 32 query heads, 1 to 8192 slots (50 MB of logits and weights): 15.5 us, a third of them the
-// lengths, parts and maxima, loads that wait for each other; without weights 6 us.
+// 8 heads, 32 query heads, 1 to 8192 slots (50 MB of logits and weights): 15.6 us, before whose rows come
+// the lengths, parts and maxima, loads that wait for each other; 8 rows without weights 6 us.
 constexpr int kSpan = 1024;
 template <int TYPE>
 __global__ __launch_bounds__(kThreads) void k_attend_finish(AttendArgs a, int64_t outs, int lpr,
@@ -568,8 +568,9 @@ __global__ __launch_bounds__(kThreads) void k_attend_finish(AttendArgs a, int64_
 }
 
 // The vector form's line: tiles are its steps, and a pair costs two of them (16 rows of 8 heads of 128
-// channels, 1 to 8192 slots, 32-bit: 29 us; 32 to 37 us at 4 to 6 where rows are short).  4096 waves are
-// the four a SIMD that the registers of two query heads leave; 5120 and 8192 are no faster.
+// channels, 1 to 8192 slots, 32-bit: 30 us, 32 at 4 and 30 at 6; 64 rows of 1 to 700: 30, 30, 35; 700 rows of
+// 1 to 1000: 100, 108, 114).  4096 waves are the four a SIMD that the registers of two query heads leave;
+// 8192 are no faster (30, 30 and 102).
 constexpr int kVecWaves = 4096, kVecCost = 2, kVecLeast = 1;
 // Waves below which the joining takes narrower slices of channels.
 constexpr int kJoinWaves = 1024;
@@ -628,8 +629,8 @@ AttendPlan plan_attend(const StateView &c, const AttendCall &a) {
     return p;
   }
   // Rows that can be longer than 512 slots are cut evenly, as in the matrix form: 16 rows of 8 heads,
-  // 1 to 8192 slots, 32-bit: 29 us against 45 in equal chunks; 300 rows of 1 to 2000: 115, 152;
-  // 4 rows of 500 to 700: 20.0, 18.6; 700 rows of 5 to 300: 52, 36.
+  // 1 to 8192 slots, 32-bit: 30 us against 48 in equal chunks; 300 rows of 1 to 2000, two query heads a head:
+  // 100, 130; 4 rows of 500 to 700: 19, 19; 700 rows of 5 to 300, 4 heads of 64: 41, 30.
   p.stream = p.cap > 512 && a.rows <= kStreamRows &&
                      a.rows * ceil_div(p.cap, 8) < (int64_t(1) << 30)
                  ? kVecWaves
@@ -665,9 +666,9 @@ int pow2_at_least(int x) {
 // How a row's words lie in lanes.  Two or three words a lane make less work of a slot (its softmax and
 // addresses are shared by more channels, and 10 or 12 words fill their lanes), but steps of more slots,
 // so not where slots are few or rows short, and not with the registers of three query heads: 16 rows
-// of 8 heads, 1 to 8192 slots, of 256 channels 45 to 40 us, of 96 with two query heads a head 37 to 33;
-// 700 rows of 1 to 1000 slots, 128 channels, 109 to 97; but 37 rows of 12 heads of 80 channels, 0 to
-// 1531 slots, 28 to 31, and 5000 rows of 20 to 40 slots 96 to 200.
+// of 8 heads, 1 to 8192 slots, of 256 channels 48 to 42 us, of 96 with two query heads a head 37 to 32;
+// 700 rows of 1 to 1000 slots, 128 channels, 109 to 100; but 37 rows of 12 heads of 80 channels, 0 to
+// 1531 slots, 29 to 31, and 5000 rows of 20 to 40 slots, 96 channels, 96 to 200.
 struct VecShape {
   int lanes, words;
 };
@@ -790,7 +791,7 @@ void state_attend(const StateView &c, const AttendCall &call, void *ws, int64_t 
   const int64_t qh = call.rows * call.q_heads;
   // lanes of a part in the joining: few query heads have many parts each, which narrow slices take
   // more at a time: 32 query heads of 256 parts 11 us, 20 with 128 channels a wave; where there are
-  // many heads it only makes waves (64 rows of 32: 67 us in all, 74 at 16384)
+  // many heads it only makes waves (64 rows of 32: 64 us in all, 70 at 16384)
   int lpr = pow2_at_least(c.dim >> 3);
   while (lpr > 4 && qh * ceil_div(c.dim >> 3, lpr) < kJoinWaves) lpr >>= 1;
   const int64_t outs = p.splits > 1 || p.stream ? qh * ceil_div(c.dim >> 3, lpr) : 0;

@@ -5,7 +5,7 @@ It stands beside the feature server as a cache of rows: with pages of one slot a
 node and a table row holds a seed's sampled neighbours; with larger pages a table row is a
 sequence.  Serving only: no gradients flow through a cache (tensors that require grad are refused).
 All calls run on the current stream of their tensors' device, neither synchronise nor allocate
-outside torch's allocator, and can be captured into a graph.  An id or length outside the cache or
+outside torch's allocator (but for the report words, once a process), and can be captured into a graph.  An id or length outside the cache or
 its table is left out or clamped by the kernel, and the next gather or state call (or
 dgs.ops._check_async_errors) raises.
 """
@@ -295,10 +295,11 @@ def evict_rows(stores, weights, positions, table, lens, budget, sinks=0, recent=
     Every (row, head) with n = lens[row] > budget slots keeps the `budget` slots that come first by
     (protected, weight descending, slot ascending).  A slot is protected when its position is below
     `sinks` or among the `recent` highest (position >= highest + 1 - recent); sinks + recent may
-    not exceed budget.  A NaN weight counts as the lowest.  The i-th dropped slot below budget
+    not exceed budget (positions may repeat: of more protected slots than stay the heaviest do).
+    A NaN weight counts as the lowest.  The i-th dropped slot below budget
     receives the row of the i-th kept slot at or past it, in every tensor of `stores` ([pages,
     heads, page_size, ...], contiguous, any type; in place, at most 8).  Rows whose pages move must
-    not share them.
+    not share them: this is for sequences; tables of sampled neighbours share their nodes' pages.
 
     weights: float32 [rows, heads, cols], positions: int32 of that shape or None (position = slot),
     cols >= table.shape[1] * page_size.  Returns new (weights, positions, lens): the kept slots'

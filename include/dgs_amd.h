@@ -341,8 +341,8 @@ int dgs_feature_server_destroy(dgs_feature_server *s);
  * memory.  A flat slot is page * page_size + offset.  A page, slot or length outside the cache or its
  * table is left out (or clamped) by the kernel, and the next gather or state entry point (or
  * dgs_check_async_errors) raises.  Workspaces are 16-byte aligned device memory of the size that the
- * *_workspace function gives.  No function here synchronises or allocates; all can be captured into a
- * graph.
+ * *_workspace function gives.  No function here synchronises or allocates (but for the report words,
+ * which the first call of a process makes); all can be captured into a graph.
  * ---------------------------------------------------------------------------------- */
 #define DGS_STATE_F32 0
 #define DGS_STATE_BF16 1
@@ -375,7 +375,7 @@ int dgs_state_read(const dgs_state_cache *c, const int64_t *slots, int64_t n, in
  * pages lie outside the cache (its weights only decay).  q [rows, q_heads, head_dim] with strides,
  * out contiguous, both of `dtype`.  weights (float [rows, heads, weights_cols], weights_cols >= width
  * * page_size, or NULL): weights[i, h, j] = decay * weights[i, h, j] + the sum of head h's query
- * heads' probabilities, for j < lens[i]; decay 0 does not read them. */
+ * heads' probabilities, for j < lens[i]; decay 0 does not read them.  -2^100 < scale < 2^100. */
 int dgs_state_attend_workspace(const dgs_state_cache *c, int64_t rows, int q_heads, int64_t width,
                                int with_weights, int dtype, int64_t *bytes);
 int dgs_state_attend(const dgs_state_cache *c, const void *q, int dtype, int64_t rows,
@@ -385,7 +385,8 @@ int dgs_state_attend(const dgs_state_cache *c, const void *q, int dtype, int64_t
                      void *workspace, int64_t workspace_bytes, void *stream);
 /* Per (row, head) of a paged cache with n = lens[row] > budget slots, keeps the `budget` slots that
  * come first by (protected, weight descending, slot ascending); protected: position < sinks or
- * position >= highest + 1 - recent (sinks + recent <= budget); a NaN weight counts as the lowest.
+ * position >= highest + 1 - recent (sinks + recent <= budget; positions may repeat, and of more
+ * protected slots than stay the heaviest do); a NaN weight counts as the lowest.
  * The i-th dropped slot below budget receives the row of the i-th kept slot at or past it, in every
  * store ([pages, heads, page_size, row_bytes] device memory, at most 8; in place).  weights (float)
  * and positions (int32 or NULL: position = slot) are [rows, heads, cols], cols >= width * page_size;
