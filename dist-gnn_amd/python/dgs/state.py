@@ -5,9 +5,9 @@ It stands beside the feature server as a cache of rows: with pages of one slot a
 node and a table row holds a seed's sampled neighbours; with larger pages a table row is a
 sequence.  Serving only: no gradients flow through a cache (tensors that require grad are refused).
 All calls run on the current stream of their tensors' device, neither synchronise nor allocate
-outside torch's allocator (but for the report words, once a process), and can be captured into a graph.  An id or length outside the cache or
-its table is left out or clamped by the kernel, and the next gather or state call (or
-dgs.ops._check_async_errors) raises.
+outside torch's allocator (but for the report words, once a process), and can be captured into a
+graph.  An id or length outside the cache or its table is left out or clamped by the kernel, and the
+next gather or state call (or dgs.ops._check_async_errors) raises.
 """
 import contextlib
 import ctypes
